@@ -64,6 +64,10 @@ extern "C" {
 #define MH_GUIDANCE_CFG 0u       /* batch 2: items 0 = uncond, 1 = cond */
 #define MH_GUIDANCE_COND_ONLY 1u /* batch 1: cond */
 
+/* Pairs of a rotated head (MhRope): channels 2i, 2i + 1, or i, i + pairs. */
+#define MH_ROPE_INTERLEAVED 0u
+#define MH_ROPE_HALVES 1u
+
 typedef struct MhContext MhContext;
 typedef struct MhEvent MhEvent;
 typedef struct MhUNet MhUNet;
@@ -443,6 +447,132 @@ int32_t mh_cross_lambda_row_sums(MhContext *ctx, const float *q, const float *e,
 int32_t mh_gemm_nt(MhContext *ctx, const float *a, uint64_t lda, const void *b, uint32_t b_dtype, uint64_t ldb,
                    uint32_t m, uint32_t n, uint32_t k, const float *bias, const float *residual, float *c,
                    uint64_t ldc, uint32_t row_group);
+
+/* ---- transformers over image and video tokens, adapters ----
+ *
+ * No counterpart in the reference, whose UNet mixes tokens with the lambda layers
+ * above. Heads of tokens are stored [row][head][channel], a row's heads next to
+ * each other, rows `ld` elements apart (ld >= heads * d: queries, keys and values
+ * of one projection are read where they lie), dtype MH_DTYPE_F32 or MH_DTYPE_F16
+ * for all tensors of a call; vectors, means and statistics are f32. Pointers are
+ * aligned to their element; 16-byte aligned bases with ld and d multiples of 8 take
+ * the wide loads. Arrays of lengths, positions, blocks and slots are device int32;
+ * lengths are clamped to 0 .. the tensor's tokens. */
+
+/* Rotary positions over 1 to 4 axes (time, height, width, ...). Axis a turns the
+ * next axis_dims[a] channels of a head (even, summing to at most d; channels behind
+ * them pass through), pair i of all of them by
+ *   positions[row % pos_rows][axis] * freq[i] radians,
+ * (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos); inverse 1: by the negative angle,
+ * which undoes it and is its transpose. Angles are reduced in f64: positions of any
+ * size keep f32 accuracy. freq is device f64 [sum(axis_dims) / 2]. */
+typedef struct MhRope {
+    const int32_t *positions; /* [pos_rows][axes] */
+    uint64_t pos_rows;        /* >= 1; one item's positions serve every item of a batch */
+    const double *freq;
+    uint32_t axes;
+    uint32_t axis_dims[4];
+    uint32_t pairing; /* MH_ROPE_* */
+    uint32_t inverse;
+    uint32_t reserved; /* 0 */
+} MhRope;
+
+/* On the host: freq [sum(axis_dims) / 2] = theta^(-2j / axis_dims[a]) for pair j of
+ * each axis a in turn, for the caller to scale and upload. */
+int32_t mh_rope_frequencies(double theta, uint32_t axes, const uint32_t *axis_dims, double *freq);
+
+/* out = x turned, rows < 2^31. out may be x with the same ld (in place), or share
+ * rows with it in other columns; any other overlap is refused. */
+int32_t mh_rope_axes(MhContext *ctx, const void *x, uint32_t dtype, uint64_t rows, uint32_t heads, uint32_t d,
+                     uint64_t ld_x, const MhRope *rope, void *out, uint64_t ld_out);
+
+/* Every head of q and k divided by its root mean square and turned in one pass:
+ * y = rope(x / sqrt(mean(x^2) + eps) * gamma), gamma_q / gamma_k [d] or NULL (ones),
+ * f32 statistics for f16 rows, f64 for f32 rows, one rounding. q_out may be q and
+ * k_out k (same ld); other overlaps as for mh_rope_axes. */
+int32_t mh_qk_norm_rope(MhContext *ctx, const void *q, uint64_t ld_q, uint32_t heads_q, const void *k, uint64_t ld_k,
+                        uint32_t heads_k, uint32_t dtype, uint64_t rows, uint32_t d, const float *gamma_q,
+                        const float *gamma_k, float eps, const MhRope *rope, void *q_out, uint64_t ld_qo, void *k_out,
+                        uint64_t ld_ko);
+
+/* Sparse attention over blocks: n items of q_tokens queries and kv_tokens keys and
+ * values (item i's row t at row i * tokens + t), heads_q a multiple of heads_kv
+ * (query head h reads key head h / (heads_q / heads_kv)). Queries are taken q_block
+ * at a time, all of them and all heads of a key head attending to the same `top`
+ * blocks of kv_block keys (16, 32, 64 or 128). q_len / kv_len [n] or NULL: rows and
+ * keys at or above them are not there. causal: query i sees keys up to
+ * i + kv_len - q_len. q_block 1 is the form for single tokens. */
+typedef struct MhBlockShape {
+    uint32_t n, q_tokens, kv_tokens;
+    uint32_t heads_q, heads_kv, d; /* d <= 256 */
+    uint32_t q_block;              /* 1 .. 1024 */
+    uint32_t kv_block;
+    uint32_t top; /* 1 .. 1024 */
+    uint32_t causal;
+    const int32_t *q_len, *kv_len;
+} MhBlockShape;
+
+/* means [n][ceil(tokens / block)][heads][d] f32: each block's mean over its tokens
+ * below len[item] (NULL: tokens). Blocks without such a token, and those that end at
+ * or below first[item] (NULL: 0), are left as they were: after new tokens are written
+ * to a cache, first = the length before brings its means up to date. block 1 .. 1024. */
+int32_t mh_block_means(MhContext *ctx, const void *x, uint32_t dtype, uint32_t n, uint32_t tokens, uint32_t heads,
+                       uint32_t d, uint64_t ld, const int32_t *first, const int32_t *len, uint32_t block,
+                       float *means);
+
+/* blocks [n][ceil(q_tokens / q_block)][heads_kv][top]: for each block of queries and
+ * key head, the `top` blocks of keys with the largest product of their mean
+ * (k_means, from mh_block_means) with the mean query over the block's rows below
+ * q_len and the key head's query heads; ascending, -1 behind the last (where fewer
+ * can be seen, all of them; for rows at or above q_len none). Products in f64; ties
+ * go to the lower index, NaN is lowest. causal: blocks of the queries' own tokens
+ * come before all others, and `top` has to hold them. At most 8192 blocks of keys. */
+int32_t mh_block_select(MhContext *ctx, const void *q, uint32_t dtype, uint64_t ld_q, const MhBlockShape *shape,
+                        const float *k_means, int32_t *blocks);
+
+/* Scratch of mh_block_attention for this shape on this context (0: none needed). */
+int32_t mh_block_attention_scratch(MhContext *ctx, const MhBlockShape *shape, uint64_t *bytes);
+
+/* out [n][q_tokens][heads_q][d] = softmax(scale q . k) v over the keys of the listed
+ * blocks (as mh_block_select writes them, in any order: indices outside the item's
+ * blocks are skipped, one listed twice counts once), in one pass with f32 scores and
+ * sums; scale > 0. Rows that see no key are zero, rows at or above q_len are left as
+ * they were; what lies at keys a row does not see (NaN among it) does not reach it.
+ * f16 tensors: f16 products. f32 tensors: f32 products, or on FAST contexts products
+ * of operands rounded to f16. Lists are split over workgroups where rows are few, and
+ * the parts joined through scratch (mh_block_attention_scratch bytes, 16-byte
+ * aligned); NULL takes the context's workspace, which is refused while the stream is
+ * being captured into a graph. out overlaps no input. */
+int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const void *k, uint64_t ld_k, const void *v,
+                           uint64_t ld_v, uint32_t dtype, const MhBlockShape *shape, const int32_t *blocks, float scale,
+                           void *out, uint64_t ld_out, void *scratch, uint64_t scratch_bytes);
+
+/* Low-rank adapters of a projection [c_out][c_in]: a [slots][rank][c_in],
+ * b [slots][c_out][rank] (dtype MH_DTYPE_*), scale [slots] f32; one of lower rank
+ * fills the rest with zeros. rank 1 .. 256. */
+typedef struct MhAdapters {
+    const void *a, *b;
+    const float *scale;
+    uint32_t dtype, slots, rank;
+    uint32_t reserved; /* 0 */
+} MhAdapters;
+
+/* Scratch of mh_conv1x1_lora for these sizes on this context. */
+int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, uint32_t rank, uint64_t *bytes);
+
+/* mh_conv1x1_forward with an adapter per request: out = x . W^T + bias (+ residual),
+ * and for rows whose s = slot[row / rows_per_slot] is 0 .. slots - 1 (others, -1 by
+ * convention, have none)
+ *   out += scale[s] (x . a[s]^T) . b[s]^T.
+ * rows_per_slot: h * w where each image of a batch is a request, 1 for single tokens
+ * or rows of mixed requests; slot has ceil(rows / rows_per_slot) entries. The adapters'
+ * products are f32 on EXACT and FAST contexts. scratch as for mh_block_attention
+ * (mh_conv1x1_lora_scratch bytes); the projection itself uses the context's workspace
+ * as mh_conv1x1_forward does. */
+int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t c_in, const void *weight,
+                        uint32_t weight_dtype, uint32_t c_out, const float *bias, const float *residual,
+                        const MhAdapters *adapters, const int32_t *slot, uint64_t rows_per_slot, float *out,
+                        void *scratch, uint64_t scratch_bytes);
 
 /* ---- UNet (src/unet) ---- */
 

@@ -114,6 +114,16 @@ SIGNATURES = {
     "mh_cross_lambda": (_i32, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp]),
     "mh_cross_lambda_row_sums": (_i32, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp]),
     "mh_gemm_nt": (_i32, [_vp, _vp, _u64, _vp, _u32, _u64, _u32, _u32, _u32, _vp, _vp, _vp, _u64, _u32]),
+    "mh_rope_frequencies": (_i32, [ctypes.c_double, _u32, _vp, _vp]),
+    "mh_rope_axes": (_i32, [_vp, _vp, _u32, _u64, _u32, _u32, _u64, _vp, _vp, _u64]),
+    "mh_qk_norm_rope": (_i32, [_vp, _vp, _u64, _u32, _vp, _u64, _u32, _u32, _u64, _u32, _vp, _vp, _f32, _vp, _vp, _u64,
+                               _vp, _u64]),
+    "mh_block_means": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, _u64, _vp, _vp, _u32, _vp]),
+    "mh_block_select": (_i32, [_vp, _vp, _u32, _u64, _vp, _vp, _vp]),
+    "mh_block_attention_scratch": (_i32, [_vp, _vp, ctypes.POINTER(_u64)]),
+    "mh_block_attention": (_i32, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _u64]),
+    "mh_conv1x1_lora_scratch": (_i32, [_vp, _u64, _u32, _u32, ctypes.POINTER(_u64)]),
+    "mh_conv1x1_lora": (_i32, [_vp, _vp, _u64, _u32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _u64, _vp, _vp, _u64]),
     "mh_unet_create": (_i32, [_vp, _vp, _u32, ctypes.POINTER(_vp)]),
     "mh_unet_destroy": (None, [_vp]),
     "mh_unet_forward": (_i32, [_vp, _vp, _u32, _u32, _vp]),
@@ -181,6 +191,30 @@ class DenoiseParams(ctypes.Structure):
                 ("spacing", ctypes.c_uint32), ("solver", ctypes.c_uint32), ("cfg_steps", ctypes.c_int32),
                 ("reserved", ctypes.c_uint32)]
 
+
+class Rope(ctypes.Structure):
+    """include/moebius_hip.h MhRope."""
+    _fields_ = [("positions", ctypes.c_void_p), ("pos_rows", ctypes.c_uint64), ("freq", ctypes.c_void_p),
+                ("axes", ctypes.c_uint32), ("axis_dims", ctypes.c_uint32 * 4), ("pairing", ctypes.c_uint32),
+                ("inverse", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
+class BlockShape(ctypes.Structure):
+    """include/moebius_hip.h MhBlockShape."""
+    _fields_ = [("n", ctypes.c_uint32), ("q_tokens", ctypes.c_uint32), ("kv_tokens", ctypes.c_uint32),
+                ("heads_q", ctypes.c_uint32), ("heads_kv", ctypes.c_uint32), ("d", ctypes.c_uint32),
+                ("q_block", ctypes.c_uint32), ("kv_block", ctypes.c_uint32), ("top", ctypes.c_uint32),
+                ("causal", ctypes.c_uint32), ("q_len", ctypes.c_void_p), ("kv_len", ctypes.c_void_p)]
+
+
+class AdapterSet(ctypes.Structure):
+    """include/moebius_hip.h MhAdapters."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("dtype", ctypes.c_uint32), ("slots", ctypes.c_uint32), ("rank", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+ROPE_PAIRING = {"interleaved": 0, "halves": 1}
 
 MODEL_UNET = 0
 MODEL_VAE = 1

@@ -1,0 +1,603 @@
+// Attention over selected blocks of keys: one pass with a running maximum and sum.
+//
+// For the rows r of a block of queries (query r / G, head hk G + r % G, G query heads
+// per key head: all of them share the list) and the keys j of the listed blocks:
+//   s_j = c q . k_j (c = scale log2 e),  m = max s_j,  p_j = 2^(s_j - m),  o = sum p_j v_j / sum p_j
+// in tiles of KT keys: m' = max(m, tile), o and the sum scaled by 2^(m - m').
+//
+// A wave takes 32 rows. It forms S^T = K . Q^T, so that a lane holds one row's scores
+// (32x32 instructions: column = lane % 32), the maximum and the sum of a row stay in the
+// lane but for one exchange with lane +- 32, and the scores are already the B operand of
+// O^T = V^T . P^T: its lane half h wants eight keys of sixteen, and holds eight, keys
+// 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3; V is staged with its keys in that order. WR waves
+// share a tile of keys, WK groups of waves take every WK-th tile and join in LDS.
+//
+// Half: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated as the
+// f16 GEMMs round operands; P rounded to f16, at most 1 with a relative 2^-11 each, which
+// a sum over keys averages. Else f32 products (v_mfma_f32_32x32x2_f32). Scores, maxima,
+// sums and outputs are f32 in both.
+#pragma once
+
+#include <type_traits>
+
+#include "attention.hpp"
+
+namespace mh {
+namespace battn {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
+
+struct Args {
+    const void *q, *k, *v;
+    void *out;
+    int64_t ldq, ldk, ldv, ldo;
+    const int32_t *blocks, *q_len, *kv_len;
+    float *part;  // split partials, NULL: none
+    float c;      // scale . log2 e
+    int n, q_tokens, kv_tokens, hk, g, d, qb, kb_log, nq, top, row_tiles, splits, work;
+    bool causal;
+};
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Floats of one wave's partial: the sums of DT x 16 registers and the row's maximum and sum.
+constexpr int part_floats(int dt) { return (dt * 16 + 2) * 64; }
+
+template <bool HALF, int DT, int WR>
+struct Tiling {
+    static constexpr int kDP = DT * 32;
+    static constexpr int kKT = HALF && DT <= 4 && WR >= 2 ? 64 : 32;  // keys per tile
+    static constexpr int kES = HALF ? 2 : 4;              // bytes of a staged value
+    static constexpr int kKS = kDP + (HALF ? 8 : 4);      // staged key row (values)
+    static constexpr int kVS = HALF ? kKT : kDP + 8;      // staged value row (half: a channel's keys)
+    static constexpr int kVRows = HALF ? kDP : kKT;
+    static constexpr int kKBytes = kKT * kKS * kES, kVBytes = kVRows * kVS * kES;
+    static constexpr int kStage = kKBytes + kVBytes;      // one key group's tile
+    // key groups: four waves together, fewer where their tiles exceed the LDS of a CU (160 KiB)
+    static constexpr int kWK = 4 / WR * kStage <= 144 * 1024 ? 4 / WR : 2 / WR;
+    static_assert(kWK >= 1 && kWK * kStage <= 144 * 1024, "tiles exceed the LDS");
+    static constexpr int kThreads = 64 * WR * kWK;
+    static constexpr int kJoin = WR * part_floats(DT) * 4;
+    static constexpr int kLds = kStage * kWK > kJoin || kWK == 1 ? kStage * kWK : kJoin;
+};
+
+// Eight consecutive values of a row.
+template <typename T>
+struct Run8 {
+    typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+    static constexpr int kN = int(sizeof(T)) / 2;  // 16-byte loads
+    V v[kN];
+    template <bool VEC>
+    __device__ __forceinline__ void load(const T *p, int valid) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) v[i] = reinterpret_cast<const V *>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i / (8 / kN)][i % (8 / kN)] = i < valid ? p[i] : T(0);
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = V(T(0));
+    }
+    __device__ __forceinline__ T at(int i) const { return v[i / (8 / kN)][i % (8 / kN)]; }
+    __device__ __forceinline__ halfx8 half() const {
+        halfx8 h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                h[i] = at(i);
+            } else {
+                const float x = at(i);
+                h[i] = static_cast<_Float16>(__builtin_fabsf(x) > 65504.0f ? __builtin_copysignf(65504.0f, x) : x);
+            }
+        }
+        return h;
+    }
+    __device__ __forceinline__ bool finite() const {
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ok = ok && __builtin_fabsf(float(at(i))) < __builtin_huge_valf();
+        return ok;
+    }
+};
+
+// Column of the 8-key runs of channel `dim` in the staged V^T: the eight (four) runs of a
+// channel are exchanged so that neither the lanes of a read (consecutive channels) nor
+// those of a write (every eighth channel) meet in a bank.
+template <int KT>
+__device__ __forceinline__ int vt_run(int dim, int run) {
+    return run ^ (((dim >> (KT == 64 ? 1 : 2)) ^ (dim >> 3)) & (KT / 8 - 1));
+}
+
+// Key of accumulator register i in lane half h (32 x 32 results: row of the tile).
+__device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
+
+template <typename T, bool HALF, bool VEC, int DT, int WR>
+__global__ __launch_bounds__(256) void block_attention_kernel(Args a) {
+    using L = Tiling<HALF, DT, WR>;
+    constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP;
+    constexpr int NT = 64 * WR;                       // threads that stage one tile
+    constexpr int KU = (KT * DP / 8 + NT - 1) / NT;   // runs of 8 channels of K per thread
+    constexpr int VU = (KT / 4 * DP / 8 + NT - 1) / NT;  // units of 4 keys x 8 channels of V
+    extern __shared__ __align__(16) char smem[];
+    __shared__ int32_t list[kMaxTop];  // first token of every block to visit
+    __shared__ int list_n, bad[WK];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % WR, wk = wave / WR, ttid = tid % NT;
+    const int col = lane & 31, h = lane >> 5;
+
+    // Work items (item, key head, block of queries, rows, split) in this order: workgroup i
+    // runs on XCD i % 8, and each XCD takes one contiguous eighth, few heads' keys.
+    const int per_xcd = (a.work + 7) / 8;
+    int w = int(blockIdx.x % 8) * per_xcd + int(blockIdx.x / 8);
+    if (int(blockIdx.x / 8) >= per_xcd || w >= a.work) return;
+    const int work = w;
+    const int split = w % a.splits;
+    w /= a.splits;
+    const int rt = w % a.row_tiles;
+    w /= a.row_tiles;
+    const int qb = w % a.nq;
+    w /= a.nq;
+    const int hk = w % a.hk, item = w / a.hk;
+    const int q_len = a.q_len ? min(max(a.q_len[item], 0), a.q_tokens) : a.q_tokens;
+    const int kv_len = a.kv_len ? min(max(a.kv_len[item], 0), a.kv_tokens) : a.kv_tokens;
+    const int i0 = qb * a.qb, i1 = min(i0 + a.qb, q_len);
+    const int rows = (i1 - i0) * a.g, r0 = rt * WR * 32;
+    if (r0 >= rows) return;
+    const int kb = 1 << a.kb_log;
+    const int off = kv_len - q_len;
+    // the last token that the rows of this workgroup may see
+    const int last = a.causal ? min(kv_len, off + i0 + (min(rows, r0 + WR * 32) - 1) / a.g + 1) - 1 : kv_len - 1;
+
+    // The list without what is outside, behind `last` or listed before, by the first wave.
+    if (wave == 0) {
+        const int32_t *src = a.blocks + ((int64_t(item) * a.nq + qb) * a.hk + hk) * a.top;
+        bool ascending = true;
+        for (int i = lane; i < a.top; i += 64) {
+            const int e = src[i], before = i ? src[i - 1] : -1;
+            ascending = ascending && (e < 0 || i == 0 || (before >= 0 && e > before));
+        }
+        ascending = __all(ascending);
+        int n = 0;
+        for (int i = lane; i < (a.top + 63) / 64 * 64; i += 64) {
+            const int e = i < a.top ? src[i] : -1;
+            bool ok = e >= 0 && e <= (last >> a.kb_log) && last >= 0;
+            if (ok && !ascending)
+                for (int j = 0; j < i; ++j) ok = ok && src[j] != e;
+            const uint64_t all = __ballot(ok);
+            if (ok) list[n + __popcll(all & ((uint64_t(1) << lane) - 1))] = e << a.kb_log;
+            n += __popcll(all);
+        }
+        if (lane == 0) list_n = n;
+        if (lane < WK) bad[lane] = 0;
+    }
+
+    // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of chunk c (f32: 8 c + 4 h .. + 3).
+    const int row = r0 + wr * 32 + col;
+    const bool row_ok = row < rows;
+    const int qi = i0 + (row_ok ? row : 0) / a.g, qe = hk * a.g + (row_ok ? row : 0) % a.g;
+    const T *qp = static_cast<const T *>(a.q) + (int64_t(item) * a.q_tokens + qi) * a.ldq + int64_t(qe) * a.d;
+    halfx8 qh[HALF ? DT * 2 : 1];
+    float qf[HALF ? 1 : DT * 16];
+    if constexpr (HALF) {
+#pragma unroll
+        for (int c = 0; c < DT * 2; ++c) {
+            const int ch = c * 16 + h * 8;
+            Run8<T> r;
+            r.zero();
+            if (ch < a.d) r.template load<VEC>(qp + ch, a.d - ch);
+            qh[c] = r.half();
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < DT * 4; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int ch = c * 8 + h * 4 + j;
+                qf[c * 4 + j] = ch < a.d ? float(qp[ch]) : 0.0f;
+            }
+    }
+    const int lim = a.causal ? min(kv_len, off + qi + 1) : kv_len;  // this lane's row sees tokens below it
+    // the tokens that every row of the wave sees
+    const int lim_all = a.causal ? min(kv_len, off + i0 + (r0 + wr * 32) / a.g + 1) : kv_len;
+
+    char *const kst = smem + wk * L::kStage, *const vst = kst + L::kKBytes;
+    // Channels behind d of the staged keys: zeros, which the loads never overwrite.
+    if (a.d < DP)
+        for (int i = ttid; i < KT * (DP / 8); i += NT) {
+            const int ch = i % (DP / 8) * 8;
+            if (ch + 8 > a.d) {
+                char *p = kst + (i / (DP / 8) * L::kKS + ch) * L::kES;
+                reinterpret_cast<floatx4 *>(p)[0] = floatx4{0, 0, 0, 0};
+                if constexpr (!HALF) reinterpret_cast<floatx4 *>(p)[1] = floatx4{0, 0, 0, 0};
+            }
+        }
+    __syncthreads();
+
+    // This split's share of the list, whole tiles of keys.
+    const int n_all = list_n;
+    const int unit = max(1, KT >> a.kb_log);
+    const int share = ((n_all + a.splits - 1) / a.splits + unit - 1) / unit * unit;
+    const int l0 = min(split * share, n_all), l1 = min(l0 + share, n_all);
+    const int keys = (l1 - l0) << a.kb_log;
+    const int tiles = (keys + KT - 1) / KT;
+    const T *kp = static_cast<const T *>(a.k) + int64_t(item) * a.kv_tokens * a.ldk + int64_t(hk) * a.d;
+    const T *vp = static_cast<const T *>(a.v) + int64_t(item) * a.kv_tokens * a.ldv + int64_t(hk) * a.d;
+
+    // Token of key j of this split; past its end none. Loads of tokens there are not
+    // (behind the list or kv_len) read the last one instead and are not used.
+    auto token = [&](int j) { return j < keys ? list[l0 + (j >> a.kb_log)] + (j & (kb - 1)) : 0x7fffffff; };
+    Run8<T> kr[KU], vr[VU][4];
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
+            if (i / (DP / 8) < KT && ch < a.d)
+                kr[u].template load<VEC>(kp + int64_t(min(token(tile * KT + j), kv_len - 1)) * a.ldk + ch, a.d - ch);
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int i = ttid + u * NT, j = i / (DP / 8) * 4, ch = i % (DP / 8) * 8;
+            if (j < KT && ch < a.d) {
+                const int t0 = token(tile * KT + j);  // four keys lie in one block
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    vr[u][e].template load<VEC>(vp + int64_t(min(t0 == 0x7fffffff ? t0 : t0 + e, kv_len - 1)) * a.ldv + ch,
+                                                a.d - ch);
+            }
+        }
+    };
+    auto stage = [&](int tile) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
+            if (i / (DP / 8) < KT && ch < a.d) {
+                if constexpr (HALF) {
+                    *reinterpret_cast<halfx8 *>(kst + (j * L::kKS + ch) * 2) = kr[u].half();
+                } else {
+                    float *p = reinterpret_cast<float *>(kst) + j * L::kKS + ch;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<floatx4 *>(p + 4 * e) = floatx4{float(kr[u].at(4 * e)), float(kr[u].at(4 * e + 1)),
+                                                                          float(kr[u].at(4 * e + 2)),
+                                                                          float(kr[u].at(4 * e + 3))};
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int i = ttid + u * NT, j = i / (DP / 8) * 4, ch = i % (DP / 8) * 8;
+            if (j < KT && ch < a.d) {
+                const int t0 = token(tile * KT + j);
+                if (t0 > kv_len - 4) {  // values of tokens that there are not: zeros, whatever lies there
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (t0 >= kv_len || t0 + e >= kv_len) vr[u][e].zero();
+                }
+                if (a.causal) {
+                    bool ok = true;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ok = ok && vr[u][e].finite();
+                    if (!ok) bad[wk] = 1;
+                }
+                if constexpr (HALF) {
+                    halfx8 hv[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) hv[e] = vr[u][e].half();
+                    // keys 4 m .. 4 m + 3 of sixteen: lane half m % 2, its first or second four
+                    const int m = (j >> 2) & 3, run = (j >> 4) * 2 + (m & 1);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int dim = ch + k;
+                        *reinterpret_cast<halfx4 *>(vst + (dim * KT + vt_run<KT>(dim, run) * 8 + (m >> 1) * 4) * 2) =
+                            halfx4{hv[0][k], hv[1][k], hv[2][k], hv[3][k]};
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float *p = reinterpret_cast<float *>(vst) + (j + e) * L::kVS + ch;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            *reinterpret_cast<floatx4 *>(p + 4 * k) =
+                                floatx4{float(vr[u][e].at(4 * k)), float(vr[u][e].at(4 * k + 1)),
+                                        float(vr[u][e].at(4 * k + 2)), float(vr[u][e].at(4 * k + 3))};
+                    }
+                }
+            }
+        }
+    };
+
+    floatx16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m = kNegInf, l = 0.0f;
+
+    const int steps = (tiles + WK - 1) / WK;
+    if (wk < tiles) fetch(wk);
+    for (int s = 0; s < steps; ++s) {
+        const int tile = s * WK + wk;
+        const bool live = tile < tiles;
+        if (s) __syncthreads();  // the tile before has been read
+        if (live) stage(tile);
+        __syncthreads();
+        if (tile + WK < tiles) fetch(tile + WK);
+        if (!live) continue;
+
+        floatx16 sc[SUB];
+#pragma unroll
+        for (int b = 0; b < SUB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[b][i] = 0.0f;
+            if constexpr (HALF) {
+                const char *p = kst + ((b * 32 + col) * L::kKS + h * 8) * 2;
+#pragma unroll
+                for (int c = 0; c < DT * 2; ++c)
+                    if (c * 16 < a.d)
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const halfx8 *>(p + c * 32), qh[c],
+                                                                       sc[b], 0, 0, 0);
+            } else {
+                const float *p = reinterpret_cast<const float *>(kst) + (b * 32 + col) * L::kKS + h * 4;
+#pragma unroll
+                for (int c = 0; c < DT * 4; ++c)
+                    if (c * 8 < a.d) {
+                        const floatx4 kv = *reinterpret_cast<const floatx4 *>(p + c * 8);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[j], qf[c * 4 + j], sc[b], 0, 0, 0);
+                    }
+            }
+        }
+        // Keys that some row of the wave does not see.
+        const bool masked = !__all(token(tile * KT + lane % KT) < lim_all);
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    const int t0 = token(tile * KT + b * 32 + 8 * f + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (t0 >= lim || t0 + e >= lim) sc[b][4 * f + e] = kNegInf;
+                }
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int b = 0; b < SUB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, sc[b][i]);
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+        const float mn = __builtin_fmaxf(m, mx);
+        const float mu = mn == kNegInf ? 0.0f : mn;
+        if (__any(mn > m)) {
+            const float f = __builtin_amdgcn_exp2f(m - mu);  // 0 before the first key
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= f;
+            m = mn;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < SUB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], a.c, -mu));
+                sum += sc[b][i];
+            }
+        l += sum;
+        if (masked && bad[wk]) {
+            // A value that is not finite may lie at a key that a row does not see, and 0 times
+            // it is NaN in the products: row by row, over the keys the row sees.
+            for (int n = 0; n < SUB * 32; ++n) {
+                float p = 0.0f;  // register n / 2 of the lane (even n) or of its other half
+#pragma unroll
+                for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p = n / 2 == b * 16 + i ? sc[b][i] : p;
+                const float other = __shfl_xor(p, 32);
+                if (n & 1) p = other;
+                const int j = n / 32 * 32 + acc_row(n / 2 % 16, h ^ (n & 1));
+                const bool sees = token(tile * KT + j) < lim;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int dim = t * 32 + acc_row(r, h);
+                        float v;
+                        if constexpr (HALF) {
+                            const int mm = (j >> 2) & 3, run = (j >> 4) * 2 + (mm & 1);
+                            v = float(reinterpret_cast<const _Float16 *>(
+                                vst)[dim * KT + vt_run<KT>(dim, run) * 8 + (mm >> 1) * 4 + (j & 3)]);
+                        } else {
+                            v = reinterpret_cast<const float *>(vst)[j * L::kVS + dim];
+                        }
+                        if (sees) o[t][r] = __builtin_fmaf(p, v, o[t][r]);
+                    }
+            }
+        } else if constexpr (HALF) {
+#pragma unroll
+            for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    halfx8 p;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) p[i] = static_cast<_Float16>(sc[b][x * 8 + i]);
+                    const int run = (b * 2 + x) * 2 + h;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const int dim = t * 32 + col;
+                        const halfx8 v = *reinterpret_cast<const halfx8 *>(vst + (dim * KT + vt_run<KT>(dim, run) * 8) * 2);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[t], 0, 0, 0);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float *p = reinterpret_cast<const float *>(vst) + (b * 32 + acc_row(i, h)) * L::kVS + col;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(p[t * 32], sc[b][i], o[t], 0, 0, 0);
+                }
+        }
+    }
+    l += __shfl_xor(l, 32);
+
+    // Groups of waves join: group 0 takes the others' sums one after another.
+    if constexpr (WK > 1) {
+        float *slot = reinterpret_cast<float *>(smem) + wr * part_floats(DT);
+        for (int src = 1; src < WK; ++src) {
+            __syncthreads();
+            if (wk == src) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) slot[(t * 16 + i) * 64 + lane] = o[t][i];
+                slot[DT * 16 * 64 + lane] = m;
+                slot[(DT * 16 + 1) * 64 + lane] = l;
+            }
+            __syncthreads();
+            if (wk == 0) {
+                const float m2 = slot[DT * 16 * 64 + lane], l2 = slot[(DT * 16 + 1) * 64 + lane];
+                const float mn = __builtin_fmaxf(m, m2), mu = mn == kNegInf ? 0.0f : mn;
+                const float f = __builtin_amdgcn_exp2f(m - mu), f2 = __builtin_amdgcn_exp2f(m2 - mu);
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[t][i] = __builtin_fmaf(o[t][i], f, slot[(t * 16 + i) * 64 + lane] * f2);
+                l = __builtin_fmaf(l, f, l2 * f2);
+                m = mn;
+            }
+        }
+        if (wk) return;
+    }
+    if (a.part) {
+        float *p = a.part + (int64_t(work) * WR + wr) * part_floats(DT);
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[(t * 16 + i) * 64 + lane] = o[t][i];
+        p[DT * 16 * 64 + lane] = m;
+        p[(DT * 16 + 1) * 64 + lane] = l;
+        return;
+    }
+    if (!row_ok) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *op = static_cast<T *>(a.out) + (int64_t(item) * a.q_tokens + qi) * a.ldo + int64_t(qe) * a.d;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            const int ch = t * 32 + 8 * f + 4 * h;
+            if constexpr (VEC) {
+                typedef T V4 __attribute__((ext_vector_type(4)));
+                if (ch < a.d) {
+                    V4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(o[t][4 * f + e] * inv);
+                    *reinterpret_cast<V4 *>(op + ch) = v;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (ch + e < a.d) op[ch + e] = static_cast<T>(o[t][4 * f + e] * inv);
+            }
+        }
+}
+
+// Joins the splits of a row tile: a wave per 32 rows and 32 channels, with the lanes'
+// places of the partial sums.
+template <typename T, int DT, int WR>
+__global__ __launch_bounds__(64) void block_attention_join_kernel(Args a) {
+    const int lane = threadIdx.x, col = lane & 31, h = lane >> 5;
+    const int wr = blockIdx.x % WR, t = blockIdx.y;
+    const int base = blockIdx.x / WR;  // (item, key head, block of queries, rows)
+    int w = base;
+    const int rt = w % a.row_tiles;
+    w /= a.row_tiles;
+    const int qb = w % a.nq;
+    w /= a.nq;
+    const int hk = w % a.hk, item = w / a.hk;
+    const int q_len = a.q_len ? min(max(a.q_len[item], 0), a.q_tokens) : a.q_tokens;
+    const int i0 = qb * a.qb, rows = (min(i0 + a.qb, q_len) - i0) * a.g;
+    const int row = (rt * WR + wr) * 32 + col;
+    if (rt * WR * 32 >= rows) return;  // its splits wrote nothing
+    constexpr int PF = part_floats(DT);
+    const float *p = a.part + (int64_t(base) * a.splits * WR + wr) * PF;
+    float m = kNegInf;
+    for (int s = 0; s < a.splits; ++s) m = __builtin_fmaxf(m, p[int64_t(s) * WR * PF + DT * 16 * 64 + lane]);
+    const float mu = m == kNegInf ? 0.0f : m;
+    float l = 0.0f, o[16] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float *ps = p + int64_t(s) * WR * PF;
+        const float f = __builtin_amdgcn_exp2f(ps[DT * 16 * 64 + lane] - mu);
+        l = __builtin_fmaf(ps[(DT * 16 + 1) * 64 + lane], f, l);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __builtin_fmaf(ps[(t * 16 + i) * 64 + lane], f, o[i]);
+    }
+    if (row >= rows) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *op = static_cast<T *>(a.out) + (int64_t(item) * a.q_tokens + i0 + row / a.g) * a.ldo +
+            int64_t(hk * a.g + row % a.g) * a.d;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int ch = t * 32 + acc_row(i, h);
+        if (ch < a.d) op[ch] = static_cast<T>(o[i] * inv);
+    }
+}
+
+template <typename T, bool HALF, bool VEC, int DT, int WR>
+void launch(Context &ctx, const Args &a) {
+    using L = Tiling<HALF, DT, WR>;
+    const void *fn = reinterpret_cast<const void *>(&block_attention_kernel<T, HALF, VEC, DT, WR>);
+    if (L::kLds > 48 * 1024) HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
+    const uint32_t grid = uint32_t((a.work + 7) / 8 * 8);
+    block_attention_kernel<T, HALF, VEC, DT, WR><<<dim3{grid}, dim3{L::kThreads}, L::kLds, ctx.stream>>>(a);
+    MH_LAUNCH_CHECK();
+    if (a.splits > 1) {
+        const dim3 jg{uint32_t(a.work / a.splits * WR), uint32_t((a.d + 31) / 32)};
+        block_attention_join_kernel<T, DT, WR><<<jg, dim3{64}, 0, ctx.stream>>>(a);
+        MH_LAUNCH_CHECK();
+    }
+}
+
+template <typename T, bool HALF, bool VEC, int DT>
+void launch_rows(Context &ctx, const Args &a, int wr) {
+    if (wr == 1) launch<T, HALF, VEC, DT, 1>(ctx, a);
+    else if (wr == 2) launch<T, HALF, VEC, DT, 2>(ctx, a);
+    else launch<T, HALF, VEC, DT, 4>(ctx, a);
+}
+
+// dt: 32-channel tiles of the head as chosen by head_tiles.
+template <typename T, bool HALF>
+void launch_mode(Context &ctx, const Args &a, int wr, int dt, bool vec) {
+    if (vec) {
+        if (dt == 1) launch_rows<T, HALF, true, 1>(ctx, a, wr);
+        else if (dt == 2) launch_rows<T, HALF, true, 2>(ctx, a, wr);
+        else if (dt == 3) launch_rows<T, HALF, true, 3>(ctx, a, wr);
+        else if (dt == 4) launch_rows<T, HALF, true, 4>(ctx, a, wr);
+        else if (dt == 5) launch_rows<T, HALF, true, 5>(ctx, a, wr);
+        else launch_rows<T, HALF, true, 8>(ctx, a, wr);
+    } else {
+        if (dt == 4) launch_rows<T, HALF, false, 4>(ctx, a, wr);
+        else launch_rows<T, HALF, false, 8>(ctx, a, wr);
+    }
+}
+
+void launch_f16(Context &ctx, const Args &a, int wr, int dt, bool vec);
+void launch_f32_half(Context &ctx, const Args &a, int wr, int dt, bool vec);
+void launch_f32(Context &ctx, const Args &a, int wr, int dt, bool vec);
+
+}  // namespace battn
+}  // namespace mh

@@ -1,0 +1,277 @@
+// The blocks of keys that each block of queries attends to.
+//
+// block_means_kernel: m_b = mean of a block's key rows, the state a cache keeps per block.
+// Bound: memory, each key read once.
+//
+// block_select_kernel: score s_b = <q, m_b> with q the mean over the valid queries of a
+// block and over the heads that share a key head; the `top` largest, ties to the lower
+// index; causal: the blocks of the queries' own tokens before all others. The scores
+// decide, so they are f64 sums of f32 products' factors: another order of the sum moves
+// them by 1e-16 of their terms, and the selection does not depend on it. Bound: memory,
+// the queries read once (the products are a 1 / q_block of the attention's).
+//
+// Scores as ordered 64-bit keys in LDS; a wave finds the top-th largest bit by bit from
+// above, counting the keys at or above a candidate with ballots, and stops once exactly
+// `top` are, which takes the exponent's bits and as many as tell the blocks apart.
+#include <algorithm>
+
+#include "attention.hpp"
+
+namespace mh {
+namespace {
+
+template <typename T, int W>
+__device__ __forceinline__ void load_run(const T *p, float (&v)[W]) {
+    if constexpr (W == 1) {
+        v[0] = float(*p);
+    } else {
+        typedef T V __attribute__((ext_vector_type(W)));
+        const V r = *reinterpret_cast<const V *>(p);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = float(r[i]);
+    }
+}
+
+__device__ __forceinline__ int clamp_len(const int32_t *len, int item, int most) {
+    return len ? min(max(len[item], 0), most) : most;
+}
+
+// One workgroup per (item, block, run of 32 column vectors); eight row groups of 32
+// threads, each summing every eighth row, joined in LDS.
+constexpr int kMeanCols = 32, kMeanRows = 8;
+
+template <typename T, int W>
+__global__ __launch_bounds__(256) void block_means_kernel(const T *x, int64_t ld, int tokens, int cols, int block,
+                                                          const int32_t *first, const int32_t *len, float *means) {
+    __shared__ double part[kMeanRows][kMeanCols * W];
+    const int item = blockIdx.z, b = blockIdx.y, nb = gridDim.y;
+    const int n = clamp_len(len, item, tokens);
+    const int r0 = b * block, r1 = min(r0 + block, n);
+    if (r0 >= r1 || (first && r0 + block <= first[item])) return;
+    const int c = threadIdx.x % kMeanCols, rg = threadIdx.x / kMeanCols;
+    const int col = (int(blockIdx.x) * kMeanCols + c) * W;
+    double sum[W] = {};
+    if (col < cols) {
+        const T *p = x + int64_t(item) * tokens * ld + col;
+#pragma unroll 8
+        for (int r = r0 + rg; r < r1; r += kMeanRows) {
+            float v[W];
+            load_run<T, W>(p + int64_t(r) * ld, v);
+#pragma unroll
+            for (int i = 0; i < W; ++i) sum[i] += double(v[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) part[rg][c * W + i] = sum[i];
+    __syncthreads();
+    for (int j = threadIdx.x; j < kMeanCols * W; j += 256) {
+        const int cj = int(blockIdx.x) * kMeanCols * W + j;
+        if (cj >= cols) break;
+        double s = 0;
+#pragma unroll
+        for (int g = 0; g < kMeanRows; ++g) s += part[g][j];
+        means[(int64_t(item) * nb + b) * cols + cj] = float(s / double(r1 - r0));
+    }
+}
+
+struct SelectArgs {
+    const void *q;
+    int64_t ld;
+    const float *means;
+    const int32_t *q_len, *kv_len;
+    int32_t *blocks;
+    int q_tokens, kv_tokens, hk, g, d, qb, kb, nq, nk, top, tiles;
+    bool causal;
+};
+
+constexpr uint64_t kForced = ~uint64_t(0);
+
+// Order-preserving: NaN lowest, then -inf .. +inf (zeros equal), forced blocks above.
+__device__ __forceinline__ uint64_t order_key(double s) {
+    if (s != s) return 0;
+    s += 0.0;
+    const uint64_t b = __builtin_bit_cast(uint64_t, s);
+    return (b >> 63) ? ~b : b | (uint64_t(1) << 63);
+}
+
+// One workgroup per (item, key head, TQ blocks of queries).
+template <typename T, int W, int TQ>
+__global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
+    extern __shared__ uint64_t keys[];  // [TQ][nk]
+    __shared__ float qm[TQ][kMaxHeadDim];
+    const int tile = blockIdx.x % a.tiles;
+    const int hk = (blockIdx.x / a.tiles) % a.hk, item = blockIdx.x / a.tiles / a.hk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int q_len = clamp_len(a.q_len, item, a.q_tokens), kv_len = clamp_len(a.kv_len, item, a.kv_tokens);
+    const int b0 = tile * TQ;
+
+    // Mean query of each block: a wave per block, lanes over (row group, run of channels).
+    const int runs = a.d / W;
+    int span = 1;  // lanes per row: the next power of two
+    while (span < runs && span < 64) span *= 2;
+    const int groups = 64 / span, cl = lane % span, rg = lane / span;
+    for (int t = wave; t < TQ; t += 4) {
+        const int i0 = (b0 + t) * a.qb, i1 = min(i0 + a.qb, q_len);
+        const int rows = max(i1 - i0, 0) * a.g;
+        const T *base = static_cast<const T *>(a.q) + (int64_t(item) * a.q_tokens + i0) * a.ld + int64_t(hk) * a.g * a.d;
+        for (int c0 = cl; c0 < ((runs + span - 1) / span) * span; c0 += span) {
+            double sum[W] = {};
+            if (c0 < runs) {
+#pragma unroll 4
+                for (int r = rg; r < rows; r += groups) {
+                    const int i = r / a.g, e = r - i * a.g;
+                    float v[W];
+                    load_run<T, W>(base + int64_t(i) * a.ld + e * a.d + c0 * W, v);
+#pragma unroll
+                    for (int k = 0; k < W; ++k) sum[k] += double(v[k]);
+                }
+            }
+            for (int m = span; m < 64; m *= 2)
+#pragma unroll
+                for (int k = 0; k < W; ++k) sum[k] += __shfl_xor(sum[k], m);
+            if (rg == 0 && c0 < runs)
+#pragma unroll
+                for (int k = 0; k < W; ++k) qm[t][c0 * W + k] = rows ? float(sum[k] / double(rows)) : 0.0f;
+        }
+    }
+    __syncthreads();
+
+    // Scores: a thread takes a key block and TQ / QS of the query blocks.
+    constexpr int QS = TQ < 4 ? TQ : 4, TT = TQ / QS, CW = 256 / QS;
+    const int qs = tid / CW;
+    const int seen_all = (kv_len + a.kb - 1) / a.kb;
+    for (int b = tid % CW; b < seen_all; b += CW) {
+        const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
+        double s[TT] = {};
+        for (int c = 0; c < a.d; c += 2) {
+            const double m0 = double(m[c]), m1 = c + 1 < a.d ? double(m[c + 1]) : 0.0;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const int tq = qs * TT + t;
+                s[t] = __builtin_fma(double(qm[tq][c]), m0, s[t]);
+                if (c + 1 < a.d) s[t] = __builtin_fma(double(qm[tq][c + 1]), m1, s[t]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) keys[(qs * TT + t) * a.nk + b] = order_key(s[t]);
+    }
+    __syncthreads();
+
+    for (int t = wave; t < TQ; t += 4) {
+        const int qb = b0 + t;
+        if (qb >= a.nq) break;
+        int32_t *out = a.blocks + ((int64_t(item) * a.nq + qb) * a.hk + hk) * a.top;
+        const int i0 = qb * a.qb, i1 = min(i0 + a.qb, q_len);
+        int seen = i1 > i0 ? seen_all : 0, f0 = 0, f1 = 0;  // blocks f0 .. f1 - 1 come first
+        if (a.causal && seen) {
+            const int lo = kv_len - q_len + i0, hi = kv_len - q_len + i1 - 1;
+            seen = hi < 0 ? 0 : hi / a.kb + 1;
+            f0 = max(lo, 0) / a.kb, f1 = seen;
+        }
+        uint64_t *k = keys + t * a.nk;
+        int count = 0;
+        if (seen > a.top) {
+            for (int b = f0 + lane; b < f1; b += 64) k[b] = kForced;
+            __threadfence_block();
+            uint64_t at = 0;  // the largest key with at least `top` keys at or above it
+            int above = seen;
+            for (int bit = 63; bit >= 0 && above != a.top; --bit) {
+                const uint64_t cand = at | (uint64_t(1) << bit);
+                int n = 0;
+                for (int b = lane; b < (seen + 63) / 64 * 64; b += 64)
+                    n += __popcll(__ballot(b < seen && k[b] >= cand));
+                if (n >= a.top) at = cand, above = n;
+            }
+            // above == top: every key at or above; else the lower indices of those equal to it
+            int greater = 0;
+            const bool ties = above != a.top;
+            if (ties)
+                for (int b = lane; b < (seen + 63) / 64 * 64; b += 64)
+                    greater += __popcll(__ballot(b < seen && k[b] > at));
+            int quota = ties ? a.top - greater : seen;
+            for (int b = lane; b < (seen + 63) / 64 * 64; b += 64) {
+                const uint64_t v = b < seen ? k[b] : 0;
+                const uint64_t below = (uint64_t(1) << lane) - 1;
+                const bool gt = b < seen && (ties ? v > at : v >= at);
+                const bool eq = b < seen && ties && v == at;
+                const uint64_t eqs = __ballot(eq);
+                const bool take = gt || (eq && __popcll(eqs & below) < quota);
+                const uint64_t takes = __ballot(take);
+                if (take) out[count + __popcll(takes & below)] = b;
+                count += __popcll(takes);
+                quota -= min(quota, int(__popcll(eqs)));
+            }
+        } else {
+            for (int b = lane; b < seen; b += 64) out[b] = b;
+            count = seen;
+        }
+        for (int i = count + lane; i < a.top; i += 64) out[i] = -1;
+    }
+}
+
+template <typename T, int W>
+void select_w(Context &ctx, SelectArgs &a, int n) {
+    // Blocks of queries per workgroup: up to eight share the reads of the means, as many
+    // as leave the card two workgroups per CU and their keys in 48 KiB of LDS.
+    int tq = 8;
+    while (tq > 1 && (tq > a.nq || int64_t(tq) * a.nk * 8 > 48 * 1024 ||
+                      int64_t(n) * a.hk * ceil_div(a.nq, tq) < 2 * ctx.cu_count))
+        tq /= 2;
+    a.tiles = int(ceil_div(a.nq, tq));
+    const int64_t blocks = int64_t(n) * a.hk * a.tiles;
+    MH_REQUIRE(blocks < (int64_t(1) << 31), "block_select: too many blocks of queries");
+    const uint32_t lds = uint32_t(tq) * a.nk * 8;
+    const dim3 grid{uint32_t(blocks)}, block{256};
+    if (tq == 8) block_select_kernel<T, W, 8><<<grid, block, lds, ctx.stream>>>(a);
+    else if (tq == 4) block_select_kernel<T, W, 4><<<grid, block, lds, ctx.stream>>>(a);
+    else if (tq == 2) block_select_kernel<T, W, 2><<<grid, block, lds, ctx.stream>>>(a);
+    else block_select_kernel<T, W, 1><<<grid, block, lds, ctx.stream>>>(a);
+    MH_LAUNCH_CHECK();
+}
+
+template <typename T>
+bool runs_of(int w, const void *p, int64_t ld, int64_t cols) {
+    return cols % w == 0 && ld % w == 0 && reinterpret_cast<uintptr_t>(p) % (w * sizeof(T)) == 0;
+}
+
+template <typename T>
+void means_t(Context &ctx, HeadRows x, int n, int tokens, int d, const int32_t *first, const int32_t *len, int block,
+             float *means) {
+    constexpr int V = 16 / int(sizeof(T));
+    const int cols = x.heads * d;
+    const bool vec = runs_of<T>(V, x.p, x.ld, cols);
+    const int64_t nb = ceil_div(tokens, block), cg = ceil_div(cols, kMeanCols * (vec ? V : 1));
+    MH_REQUIRE(nb <= 65535 && n <= 65535, "block_means: more than 65535 blocks or items");
+    const dim3 grid{uint32_t(cg), uint32_t(nb), uint32_t(n)}, tb{256};
+    const T *p = static_cast<const T *>(x.p);
+    if (vec) block_means_kernel<T, V><<<grid, tb, 0, ctx.stream>>>(p, x.ld, tokens, cols, block, first, len, means);
+    else block_means_kernel<T, 1><<<grid, tb, 0, ctx.stream>>>(p, x.ld, tokens, cols, block, first, len, means);
+    MH_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+void block_means(Context &ctx, HeadRows x, WeightType type, int n, int tokens, int d, const int32_t *first,
+                 const int32_t *len, int block, float *means) {
+    if (!n || !tokens) return;
+    if (type == kF16) means_t<_Float16>(ctx, x, n, tokens, d, first, len, block, means);
+    else means_t<float>(ctx, x, n, tokens, d, first, len, block, means);
+}
+
+void block_select(Context &ctx, HeadRows q, WeightType type, const BlockShape &s, const float *k_means,
+                  int32_t *blocks) {
+    if (!s.n || !s.q_tokens) return;
+    SelectArgs a{};
+    a.q = q.p, a.ld = q.ld, a.means = k_means, a.q_len = s.q_len, a.kv_len = s.kv_len, a.blocks = blocks;
+    a.q_tokens = s.q_tokens, a.kv_tokens = s.kv_tokens, a.hk = s.heads_kv, a.g = s.heads_q / s.heads_kv, a.d = s.d;
+    a.qb = s.q_block, a.kb = s.kv_block, a.nq = s.q_blocks(), a.nk = s.kv_blocks(), a.top = s.top, a.causal = s.causal;
+    if (type == kF16) {
+        if (runs_of<_Float16>(8, q.p, q.ld, s.d)) select_w<_Float16, 8>(ctx, a, s.n);
+        else select_w<_Float16, 1>(ctx, a, s.n);
+    } else {
+        if (runs_of<float>(4, q.p, q.ld, s.d)) select_w<float, 4>(ctx, a, s.n);
+        else select_w<float, 1>(ctx, a, s.n);
+    }
+}
+
+}  // namespace mh

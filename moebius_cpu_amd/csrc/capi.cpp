@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/moebius_hip.h"
+#include "capi_context.hpp"
 #include "capi_guard.hpp"
 #include "common.hpp"
 #include "denoise.hpp"
@@ -22,11 +23,6 @@
 #include "unet.hpp"
 #include "vae.hpp"
 #include "weights.hpp"
-
-struct MhContext {
-    mh::Context ctx;
-    explicit MhContext(int dev) : ctx(dev) {}
-};
 
 struct MhUNet {
     MhContext *owner;
@@ -55,20 +51,11 @@ struct MhEvent {
 
 namespace {
 
+using mh::capi::C;
+using mh::capi::dim;
 using mh::capi::guard;
 using mh::capi::need;
-
-mh::Context &C(MhContext *c) {
-    if (!c) mh::fail(mh::kInvalidArgument, "context is NULL");
-    HIP_CHECK(hipSetDevice(c->ctx.device));
-    return c->ctx;
-}
-
-mh::WeightType wtype(uint32_t dt) {
-    if (dt == MH_DTYPE_F32) return mh::kF32;
-    if (dt == MH_DTYPE_F16) return mh::kF16;
-    mh::fail(mh::kInvalidArgument, "unknown weight dtype");
-}
+using mh::capi::wtype;
 
 void pad4(const uint32_t *pad, int out[4]) {
     need(pad, "pad");
@@ -80,11 +67,6 @@ void pad4(const uint32_t *pad, int out[4]) {
 
 // Host threads of the imaging entry points (their bytes do not depend on it): one per core, at most 16.
 unsigned host_threads() { return std::min(16u, std::max(1u, std::thread::hardware_concurrency())); }
-
-int dim(uint32_t v, const char *what) {
-    if (v > (1u << 30)) mh::fail(mh::kInvalidArgument, std::string(what) + " too large");
-    return int(v);
-}
 
 }  // namespace
 

@@ -271,6 +271,24 @@ class Conv1x1:
         check(lib().mh_conv1x1_forward(self.ctx.h, x.ptr, x.n, x.h, x.w, x.c, self.weight.ptr, self.weight.dtype,
                                        self.c_out, _ptr(self.bias), _ptr(residual), out.ptr))
 
+    def forward_adapted(self, x: Tensor, adapters, slot: DeviceArray, out: Tensor, residual: Tensor | None = None,
+                        scratch: DeviceArray | None = None):
+        """forward plus the low-rank adapter (adapters.Adapters) that slot names for each item of
+        x, int32 [n], or for each pixel, int32 [n * h * w]; -1: none. No counterpart in the reference."""
+        if x.c != self.c_in or (adapters.c_in, adapters.c_out) != (self.c_in, self.c_out):
+            raise MoebiusError(1, "Conv1x1 input channels")
+        if len(self.weight) != self.c_in * self.c_out:
+            raise MoebiusError(1, "Conv1x1 weight size")
+        if slot.dtype != np.int32 or slot.nbytes // 4 not in (x.n, x.pixels()):
+            raise MoebiusError(1, "slot is int32, one for each item or each pixel")
+        out.set_shape(x.n, x.h, x.w, self.c_out)
+        if residual is not None and residual.shape != out.shape:
+            raise MoebiusError(1, "Conv1x1 residual shape")
+        per = 1 if slot.nbytes // 4 == x.pixels() else x.h * x.w
+        check(lib().mh_conv1x1_lora(self.ctx.h, x.ptr, x.pixels(), x.c, self.weight.ptr, self.weight.dtype, self.c_out,
+                                    _ptr(self.bias), _ptr(residual), ctypes.byref(adapters.c), slot.ptr, max(per, 1),
+                                    out.ptr, _ptr(scratch), 0 if scratch is None else scratch.nbytes))
+
 
 class Affine:
     """Per-item, per-channel GroupNorm affine (src/engine/norm.rs:33-37)."""

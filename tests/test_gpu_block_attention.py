@@ -1,0 +1,507 @@
+"""Block means, the selection of key blocks and the attention over them, against
+the definitions in f64.
+
+Attention tolerances, for a row with scores s_j and values v_j (m = max |v| over
+the keys it sees; all bounds are worst cases of the roundings):
+  - a score is off by (d + 2) u A with u = 2^-24 and A = max_j scale sum |q_i k_ij|
+    (f32 sums of exact or once rounded products), the exponent's argument by 2^-23 B
+    more with B = max |s_j| log2 e, the hardware's exponential by 2^-22, the running
+    rescales and the two sums by (2 tiles + keys) u, all twice (numerator and denominator);
+  - f16 products round each probability by 2^-11;
+  - FAST contexts round q, k and v too: 2 x 2^-11 A per score, twice, and 2^-11 for v;
+  - f16 outputs add half a step.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+
+from moebius_cpu_amd import _lib
+from moebius_cpu_amd import engine as E
+from moebius_cpu_amd._lib import MoebiusError
+from moebius_cpu_amd.attention import (Heads, RopeAxes, block_attention, block_attention_scratch, block_means,
+                                       block_select, qk_norm_rope)
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return E.Context(0)
+
+
+def dev(ctx, a):
+    return E.DeviceArray.from_numpy(ctx, np.ascontiguousarray(a))
+
+
+def lens(ctx, a):
+    return None if a is None else dev(ctx, np.asarray(a, np.int32))
+
+
+def heads(ctx, x, pad=0, offset=0):
+    """x [n][tokens][heads][d] with rows `pad` elements longer, NaN between them."""
+    n, t, h, d = x.shape
+    if not pad and not offset:
+        return Heads(dev(ctx, x), n, t, h, d)
+    flat = np.full(offset + n * t * (h * d + pad), np.nan, x.dtype)
+    rows = np.lib.stride_tricks.as_strided(flat[offset:], (n * t, h * d),
+                                           ((h * d + pad) * x.itemsize, x.itemsize))
+    rows[:] = x.reshape(n * t, h * d)
+    return Heads(dev(ctx, flat), n, t, h, d, ld=h * d + pad, offset=offset)
+
+
+# ---------------------------------------------------------------- means
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("n,tokens,h,d,block,pad,offset", [
+    (1, 1, 1, 1, 16, 0, 0), (2, 130, 3, 40, 64, 0, 0), (1, 1000, 8, 128, 128, 128, 8), (3, 50, 2, 33, 16, 1, 1),
+    (1, 257, 16, 64, 32, 0, 0), (2, 7, 2, 80, 1, 0, 0), (1, 2050, 1, 72, 1024, 0, 0)])
+def test_means(ctx, dtype, n, tokens, h, d, block, pad, offset):
+    """Off by one f32 rounding of the f64 mean (and f64's own, 10^-13 of the largest term)."""
+    r = np.random.default_rng(tokens)
+    x = r.standard_normal((n, tokens, h, d)).astype(dtype)
+    length = r.integers(0, tokens + 1, n)
+    length[0] = tokens
+    for i in range(n):
+        x[i, length[i]:] = np.nan  # behind the length nothing counts
+    nb = -(-tokens // block)
+    means = dev(ctx, np.full((n, nb, h, d), 7, np.float32))
+    block_means(heads(ctx, x, pad, offset), block, means, length=lens(ctx, length))
+    got = means.numpy().astype(np.float64)
+    for i in range(n):
+        for b in range(nb):
+            part = x[i, b * block:min((b + 1) * block, length[i])].astype(np.float64)
+            if len(part):
+                want = part.mean(0)
+                assert np.all(np.abs(got[i, b] - want) <= U * np.abs(want) + 1e-13 * np.abs(part).max())
+            else:
+                assert np.all(got[i, b] == 7)  # left as it was
+
+
+def test_means_of_new_tokens_only(ctx):
+    """first leaves the blocks below it alone; the result is that of the whole pass."""
+    x = np.random.default_rng(0).standard_normal((3, 200, 2, 40)).astype(np.float32)
+    h = heads(ctx, x)
+    whole, step = dev(ctx, np.zeros((3, 7, 2, 40), np.float32)), dev(ctx, np.zeros((3, 7, 2, 40), np.float32))
+    old, new = np.array([0, 64, 95]), np.array([40, 65, 200])
+    block_means(h, 32, whole, length=lens(ctx, new))
+    block_means(h, 32, step, length=lens(ctx, old))
+    marked = step.numpy()
+    marked[1, :2] += 1  # blocks that end at or below `first`
+    marked[2, :2] += 1
+    step.upload(marked)
+    block_means(h, 32, step, length=lens(ctx, new), first=lens(ctx, old))
+    want = whole.numpy()
+    want[1, :2] += 1
+    want[2, :2] += 1
+    assert np.array_equal(step.numpy(), want)
+
+
+def test_lengths_out_of_range_are_clamped(ctx):
+    x = np.random.default_rng(0).standard_normal((2, 40, 1, 8)).astype(np.float32)
+    m = dev(ctx, np.full((2, 3, 1, 8), 5, np.float32))
+    block_means(heads(ctx, x), 16, m, length=lens(ctx, [-3, 2**31 - 1]))
+    assert np.all(m.numpy()[0] == 5)
+    assert np.abs(m.numpy()[1, 2] - x[1, 32:].mean(0)).max() < 1e-6
+
+
+# ---------------------------------------------------------------- selection
+
+def selected(q, means, qb, kb, top, causal, q_len, kv_len):
+    """The definition: f64 scores of the f32 means, a stable order by (forced, score, lower index)."""
+    n, qt, hq, d = q.shape
+    hk, g = means.shape[2], hq // means.shape[2]
+    nq = -(-qt // qb)
+    out = np.full((n, nq, hk, top), -1, np.int32)
+    for i in range(n):
+        ql = qt if q_len is None else q_len[i]
+        kl = kv_len[i]
+        for b in range(nq):
+            rows = q[i, b * qb:min((b + 1) * qb, ql)].astype(np.float64)
+            if not len(rows):
+                continue
+            last = kl - 1
+            if causal:
+                last = min(last, kl - ql + min((b + 1) * qb, ql) - 1)
+            seen = last // kb + 1 if last >= 0 else 0
+            lo = max(kl - ql + b * qb, 0) // kb if causal else seen
+            for h in range(hk):
+                mean = rows[:, h * g:(h + 1) * g].mean((0, 1)).astype(np.float32).astype(np.float64)
+                s = means[i, :seen, h].astype(np.float64) @ mean
+                s = np.where(np.isnan(s), -np.inf, s)
+                keys = sorted(range(seen), key=lambda j: (j < lo, -s[j], j))[:top]
+                out[i, b, h, :len(keys)] = sorted(keys)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("n,qt,kt,hq,hk,d,qb,kb,top,causal", [
+    (1, 1, 40, 1, 1, 8, 1, 16, 2, False), (3, 1, 3000, 8, 2, 128, 1, 16, 20, True), (2, 200, 200, 4, 4, 40, 64, 16, 5, False),
+    (2, 130, 700, 6, 2, 72, 16, 32, 6, True), (1, 1024, 1024, 2, 1, 80, 128, 64, 4, True), (1, 37, 555, 3, 3, 33, 5, 128, 2, True),
+    (2, 300, 90, 2, 2, 64, 32, 16, 7, True), (1, 700, 9000, 1, 1, 256, 1, 32, 64, False), (1, 64, 64, 2, 2, 96, 64, 128, 3, False),
+    (1, 3, 60000, 2, 1, 16, 1, 16, 900, False)])
+def test_select(ctx, dtype, n, qt, kt, hq, hk, d, qb, kb, top, causal):
+    r = np.random.default_rng(kt)
+    q = r.standard_normal((n, qt, hq, d)).astype(dtype)
+    nk = -(-kt // kb)
+    means = r.standard_normal((n, nk, hk, d)).astype(np.float32)
+    kv_len = r.integers(0, kt + 1, n)
+    q_len = r.integers(0, qt + 1, n)
+    kv_len[0], q_len[0] = kt, qt
+    blocks = dev(ctx, np.full((n, -(-qt // qb), hk, top), 77, np.int32))
+    block_select(heads(ctx, q, pad=8, offset=16), dev(ctx, means), kt, blocks, q_block=qb, kv_block=kb, causal=causal,
+                 q_len=lens(ctx, q_len), kv_len=lens(ctx, kv_len))
+    assert np.array_equal(blocks.numpy(), selected(q, means, qb, kb, top, causal, q_len, kv_len))
+
+
+def test_select_ties_nan_and_infinity(ctx):
+    """Equal scores go to the lower index, zeros of either sign are equal, NaN is lowest, infinity highest."""
+    means = np.zeros((1, 200, 1, 8), np.float32)
+    means[0, 3::7, 0, 0] = 1
+    means[0, 5, 0, 0] = np.nan
+    means[0, 6, 0, 0] = -np.inf
+    means[0, 190, 0, 0] = np.inf
+    means[0, 8, 0, 0] = -0.0
+    q = np.zeros((1, 1, 1, 8), np.float32)
+    q[..., 0] = 1
+    for top in (1, 5, 29, 30, 31, 40, 198, 199, 200):
+        blocks = dev(ctx, np.zeros((1, 1, 1, top), np.int32))
+        block_select(heads(ctx, q), dev(ctx, means), 3200, blocks, q_block=1, kv_block=16)
+        s = means[0, :, 0, 0] + 0.0
+        order = sorted(range(200), key=lambda j: (np.isnan(s[j]), -s[j] if not np.isnan(s[j]) else 0, j))[:top]
+        assert blocks.numpy().ravel().tolist() == sorted(order), top
+
+
+def test_select_reads_nothing_behind_the_lengths(ctx):
+    """Means of blocks that there are not, and queries behind q_len, may hold anything."""
+    r = np.random.default_rng(4)
+    q, means = r.standard_normal((1, 64, 2, 40)).astype(np.float32), r.standard_normal((1, 32, 2, 40)).astype(np.float32)
+    got = []
+    for fill in (0.0, np.nan):
+        q[0, 40:], means[0, 10:] = fill, fill
+        blocks = dev(ctx, np.zeros((1, 4, 2, 6), np.int32))
+        block_select(heads(ctx, q), dev(ctx, means), 512, blocks, q_block=16, kv_block=16, q_len=lens(ctx, [40]),
+                     kv_len=lens(ctx, [150]))
+        got.append(blocks.numpy())
+    assert np.array_equal(got[0], got[1])
+    assert (got[0][0, 3] == -1).all() and got[0].max() < 10
+
+
+# ---------------------------------------------------------------- attention
+
+def reference(q, k, v, blocks, scale, qb, kb, causal, q_len, kv_len):
+    """The definition in f64, and what the tolerance of a row goes by: (out, seen keys, A, B, m), rows not there NaN."""
+    n, qt, hq, d = q.shape
+    hk, g = k.shape[2], hq // k.shape[2]
+    out = np.full((n, qt, hq, d), np.nan)
+    tol = np.zeros((n, qt, hq, 4))
+    for i in range(n):
+        ql = qt if q_len is None else min(max(q_len[i], 0), qt)
+        kl = k.shape[1] if kv_len is None else min(max(kv_len[i], 0), k.shape[1])
+        for t in range(ql):
+            for h in range(hq):
+                picked = sorted({int(b) for b in blocks[i, t // qb, h // g] if 0 <= int(b) * kb < kl})
+                keys = [j for b in picked for j in range(b * kb, min((b + 1) * kb, kl)) if not causal or j <= t + kl - ql]
+                if not keys:
+                    out[i, t, h] = 0
+                    continue
+                kk, vv = k[i, keys, h // g].astype(np.float64), v[i, keys, h // g].astype(np.float64)
+                qq = q[i, t, h].astype(np.float64)
+                s = kk @ qq * scale
+                p = np.exp(s - s.max())
+                out[i, t, h] = p @ vv / p.sum()
+                tol[i, t, h] = len(keys), (np.abs(kk) @ np.abs(qq)).max() * scale, np.abs(s).max() * 1.4427, np.abs(vv).max()
+    return out, tol
+
+
+def tolerance(out, tol, d, dtype, fast):
+    keys, A, B, m = (tol[..., i] for i in range(4))
+    e = 2 * ((d + 2) * U * A + 2 * U * B + 4 * U) + (keys + keys / 8) * U
+    if dtype == np.float16 or fast:
+        e = e + 2.0 ** -11
+    if fast:
+        e = e + 2 * 2 * 2.0 ** -11 * A + 2.0 ** -11
+    t = (e * m)[..., None] + 1e-30
+    return t + (np.abs(out) * 2.0 ** -11 + 2.0 ** -25 if dtype == np.float16 else np.abs(out) * U)
+
+
+def lists(r, n, nq, hk, top, nk):
+    """Distinct blocks in any order, some places empty."""
+    out = np.full((n, nq, hk, top), -1, np.int32)
+    for i in np.ndindex(n, nq, hk):
+        pick = r.permutation(nk)[:top]
+        out[i][:len(pick)] = np.sort(pick) if r.random() < 0.5 else pick
+        out[i][r.random(top) < 0.1] = -1
+    return out
+
+
+def run(ctx, q, k, v, blocks, qb, kb, causal=False, q_len=None, kv_len=None, scale=None, pad=0, offset=0, fill=np.nan):
+    """The call on rows `pad` apart; rows that it leaves alone come back as `fill`."""
+    out = heads(ctx, np.full(q.shape, fill, q.dtype), pad, offset)
+    block_attention(heads(ctx, q, pad, offset), heads(ctx, k, pad, offset), heads(ctx, v, pad, offset), dev(ctx, blocks),
+                    out, scale=scale, q_block=qb, kv_block=kb, causal=causal, q_len=lens(ctx, q_len), kv_len=lens(ctx, kv_len))
+    return out.numpy()
+
+
+CASES = [  # n, q, kv, hq, hk, d, qb, kb, top, causal
+    (1, 1, 1, 1, 1, 8, 1, 16, 1, False),        # one token, one key
+    (2, 1, 300, 4, 1, 64, 1, 16, 12, True),     # single tokens, lists split over workgroups
+    (3, 1, 1000, 8, 2, 128, 1, 64, 9, True),
+    (1, 3, 2100, 2, 2, 40, 1, 128, 10, False),
+    (2, 70, 70, 2, 2, 40, 32, 16, 4, False),    # one wave of rows
+    (1, 128, 200, 1, 1, 80, 64, 32, 5, False),  # two
+    (1, 150, 333, 2, 1, 72, 64, 64, 4, True),   # four, ragged
+    (2, 100, 250, 4, 2, 96, 16, 16, 8, True),
+    (1, 260, 260, 1, 1, 128, 128, 64, 3, False),
+    (1, 140, 140, 1, 1, 160, 100, 128, 2, True),  # blocks of queries that are no power of two
+    (1, 40, 200, 3, 1, 256, 16, 32, 4, True),
+    (1, 130, 300, 1, 1, 200, 128, 32, 6, False),
+    (1, 20, 90, 2, 1, 33, 8, 16, 4, True),      # no wide loads
+    (1, 70, 90, 1, 1, 7, 70, 64, 2, False),
+    (1, 10, 100, 2, 2, 130, 4, 16, 5, True),
+    (1, 9, 50, 36, 1, 32, 2, 16, 3, False),     # 72 rows of one key head
+    (1, 5, 64, 70, 2, 16, 5, 16, 3, True),
+]
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32", "fast"])
+@pytest.mark.parametrize("case", CASES)
+def test_attention(ctx, case, kind):
+    n, qt, kt, hq, hk, d, qb, kb, top, causal = case
+    dtype = np.float16 if kind == "f16" else np.float32
+    r = np.random.default_rng(qt * 7 + kt + d)
+    q, k, v = (r.standard_normal(s).astype(dtype) for s in ((n, qt, hq, d), (n, kt, hk, d), (n, kt, hk, d)))
+    kv_len, q_len = r.integers(kt // 2, kt + 1, n), r.integers((qt + 1) // 2, qt + 1, n)
+    kv_len[0], q_len[0] = kt, qt
+    for i in range(n):  # behind the lengths lies anything
+        q[i, q_len[i]:], k[i, kv_len[i]:], v[i, kv_len[i]:] = np.nan, np.nan, np.inf
+    blocks = lists(r, n, -(-qt // qb), hk, top, -(-kt // kb))
+    scale = 1 / np.sqrt(d)
+    pad, offset = (8, 16) if d % 8 == 0 else (1, 3)
+    ctx.set_precision(kind == "fast")
+    try:
+        got = run(ctx, q, k, v, blocks, qb, kb, causal, q_len, kv_len, None, pad, offset, fill=3).astype(np.float64)
+    finally:
+        ctx.set_precision(False)
+    want, tol = reference(q, k, v, blocks, scale, qb, kb, causal, q_len, kv_len)
+    there = ~np.isnan(want)
+    assert np.all(got[~there] == 3)  # rows at or above q_len: left as they were
+    err, bound = np.abs(got - want)[there], tolerance(want, tol, d, dtype, kind == "fast")[there]
+    assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_rows_that_see_nothing_are_zero(ctx, dtype):
+    """No key at all, empty lists, lists of blocks that are not there, causal rows before the first key."""
+    r = np.random.default_rng(0)
+    q, k, v = (r.standard_normal((4, t, 2, 64)).astype(dtype) for t in (40, 96, 96))
+    blocks = lists(r, 4, 3, 2, 6, 6)
+    blocks[1] = -1
+    blocks[2] = np.array([6, 7, -5, 2**31 - 1, -2**31, 1000])
+    got = run(ctx, q, k, v, blocks, 16, 16, True, [40, 40, 40, 40], [0, 96, 96, 10])
+    assert not got[:3].any()
+    assert not got[3, :30].any()  # query i sees keys up to i - 30
+    want, tol = reference(q, k, v, blocks, 1 / 8, 16, 16, True, [40] * 4, [0, 96, 96, 10])
+    assert np.all(np.abs(got[3].astype(np.float64) - want[3]) <= tolerance(want, tol, 64, dtype, False)[3])
+    # no keys in the tensor either
+    none = np.zeros((1, 0, 2, 64), dtype)
+    got = run(ctx, q[:1], none, none, np.zeros((1, 3, 2, 1), np.int32), 16, 16)
+    assert not got.any()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("q_block", [1, 16])
+def test_lists_are_sets(ctx, dtype, q_block):
+    """An index listed twice counts once, in any order; ascending lists and their shuffles of one tile agree in bits."""
+    r = np.random.default_rng(1)
+    q, k, v = (r.standard_normal((1, t, 1, 40)).astype(dtype) for t in (16, 640, 640))
+    nq = 16 // q_block
+    base = np.tile(np.array([3, 7, 20, 39], np.int32), (1, nq, 1, 1))
+    twice = np.tile(np.array([3, 7, 20, 39, -1, 7, 3, 39, 20, 3, 50, -7], np.int32), (1, nq, 1, 1))
+    a, b = run(ctx, q, k, v, base, q_block, 16), run(ctx, q, k, v, twice, q_block, 16)
+    want, tol = reference(q, k, v, base, 1 / np.sqrt(40), q_block, 16, False, None, None)
+    bound = tolerance(want, tol, 40, dtype, False)
+    assert np.all(np.abs(a - want) <= bound) and np.all(np.abs(b - want) <= bound)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("q_block", [1, 16, 64, 128])
+def test_what_a_row_does_not_see_does_not_reach_it(ctx, dtype, q_block):
+    """Causal rows whose tile holds keys and values of later tokens that are NaN or infinite."""
+    r = np.random.default_rng(2)
+    q, k, v = (r.standard_normal((1, 128, 2, 48)).astype(dtype) for _ in range(3))
+    blocks = np.tile(np.arange(4, dtype=np.int32), (1, -(-128 // q_block), 2, 1))
+    clean, tol = reference(q, k, v, blocks, 1 / np.sqrt(48), q_block, 32, True, None, None)
+    v[0, 70, 0, 5], v[0, 100, :, :], k[0, 90] = np.inf, np.nan, np.nan
+    got = run(ctx, q, k, v, blocks, q_block, 32, True).astype(np.float64)
+    bound = tolerance(clean, tol, 48, dtype, False)
+    ok = np.abs(got - clean) <= bound
+    assert ok[0, :70].all()
+    assert ok[0, 70:90, 0, :5].all() and ok[0, 70:90, 0, 6:].all() and np.isposinf(got[0, 70:90, 0, 5]).all()
+    assert ok[0, 70:90, 1].all()
+    assert np.isnan(got[0, 90:]).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_blocks_not_listed_are_not_read(ctx, dtype):
+    r = np.random.default_rng(3)
+    q, k, v = (r.standard_normal((1, t, 1, 64)).astype(dtype) for t in (64, 512, 512))
+    blocks = np.array([1, 4, 6], np.int32).reshape(1, 1, 1, 3)
+    a = run(ctx, q, k, v, blocks, 64, 64)
+    mask = np.ones(512, bool)
+    for b in (1, 4, 6):
+        mask[b * 64:(b + 1) * 64] = False
+    k[0, mask], v[0, mask] = np.nan, np.nan
+    assert np.array_equal(run(ctx, q, k, v, blocks, 64, 64), a)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_large_and_infinite_scores(ctx, dtype):
+    """Scores of thousands keep the softmax finite; equal scores give the mean; a masked lowest value gives nothing."""
+    q, k, v = np.zeros((1, 4, 1, 8), dtype), np.zeros((1, 64, 1, 8), dtype), np.zeros((1, 64, 1, 8), dtype)
+    v[0, :, 0, 0] = np.arange(64)
+    q[0, 1, 0, 0], k[0, 17, 0, 0] = 200, 200     # one score of 40 000 above the others
+    q[0, 2, 0, 1], k[0, 33, 0, 1] = 200, -200    # one far below
+    q[0, 3, 0, 2], k[0, 50:, 0, 2] = -1, np.finfo(dtype).max if dtype == np.float16 else 1e30
+    got = run(ctx, q, k, v, np.arange(4, dtype=np.int32).reshape(1, 1, 1, 4), 4, 16, scale=1.0)[0, :, 0, 0]
+    for g, want in zip(got, (31.5, 17.0, (2016 - 33) / 63, 24.5)):
+        assert abs(float(g) - want) <= want * (2.0 ** -10 if dtype == np.float16 else 1e-6)
+
+
+def test_row_results_do_not_depend_on_the_batch(ctx):
+    """The same item alone and among others, and the same call twice: the same bits."""
+    r = np.random.default_rng(6)
+    q, k, v = (r.standard_normal((3, t, 2, 64)).astype(np.float16) for t in (64, 320, 320))
+    blocks = lists(r, 3, 1, 2, 4, 5)
+    a = run(ctx, q, k, v, blocks, 64, 64)
+    assert np.array_equal(a, run(ctx, q, k, v, blocks, 64, 64))
+
+
+def test_scratch_is_checked(ctx):
+    r = np.random.default_rng(7)
+    q, k, v = (heads(ctx, r.standard_normal((1, t, 2, 64)).astype(np.float16)) for t in (1, 2048, 2048))
+    out, blocks = Heads(E.DeviceArray(ctx, (1, 1, 2, 64), "f2"), 1, 1, 2, 64), dev(ctx, np.arange(32, dtype=np.int32).reshape(1, 1, 2, 16))
+    size = block_attention_scratch(q, k, blocks, 1, 64)
+    assert size > 0
+    with pytest.raises(MoebiusError, match="smaller"):
+        block_attention(q, k, v, blocks, out, q_block=1, scratch=E.DeviceArray(ctx, (size - 1,), np.uint8))
+    block_attention(q, k, v, blocks, out, q_block=1, scratch=E.DeviceArray(ctx, (size,), np.uint8))
+    a = out.numpy()
+    block_attention(q, k, v, blocks, out, q_block=1)
+    assert np.array_equal(out.numpy(), a)
+
+
+def _capture(ctx, calls):
+    """The calls captured from the context's stream into a graph: (launch, destroy)."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    stream = ctypes.c_void_p(_lib.lib().mh_context_stream(ctx.h))
+    graph, execg = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0  # relaxed
+    try:
+        calls()
+    finally:
+        ended = hip.hipStreamEndCapture(stream, ctypes.byref(graph))
+    assert ended == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(execg), graph, None, None, 0) == 0
+    return (lambda: hip.hipGraphLaunch(execg, stream)), (lambda: (hip.hipGraphExecDestroy(execg), hip.hipGraphDestroy(graph)))
+
+
+def test_a_layer_step_captured_and_replayed(ctx):
+    """Norm and rotation, means, selection and attention of single tokens as one run, eager and as
+    two graphs with scratch of their own, replayed in turn among eager calls; against the definitions."""
+    r = np.random.default_rng(8)
+    n, kt, hq, hk, d, kb, top = 2, 1024, 4, 2, 64, 32, 8
+    rope = RopeAxes(ctx, (16, 24, 24))
+    g = dev(ctx, (1 + 0.1 * r.standard_normal(d)).astype(np.float32))
+    cache_v = heads(ctx, r.standard_normal((n, kt, hk, d)).astype(np.float16))
+    ql, kl = lens(ctx, [1, 1]), lens(ctx, [1000, 513])
+
+    def state(seed):
+        r = np.random.default_rng(seed)
+        x = r.standard_normal((n, hq + hk, d)).astype(np.float16)
+        buf = dev(ctx, x)
+        st = dict(q=Heads(buf, n, 1, hq, d, ld=(hq + hk) * d), kn=Heads(buf, n, 1, hk, d, ld=(hq + hk) * d, offset=hq * d),
+                  pos=dev(ctx, r.integers(0, 1000, (n, 3)).astype(np.int32)), k=heads(ctx, r.standard_normal((n, kt, hk, d)).astype(np.float16)),
+                  qo=Heads(E.DeviceArray(ctx, (n, 1, hq, d), "f2"), n, 1, hq, d), ko=Heads(E.DeviceArray(ctx, (n, 1, hk, d), "f2"), n, 1, hk, d),
+                  means=dev(ctx, np.zeros((n, kt // kb, hk, d), np.float32)), blocks=dev(ctx, np.zeros((n, 1, hk, top), np.int32)),
+                  out=Heads(E.DeviceArray(ctx, (n, 1, hq, d), "f2"), n, 1, hq, d))
+        st["scratch"] = E.DeviceArray(ctx, (block_attention_scratch(st["qo"], st["k"], st["blocks"], 1, kb),), np.uint8)
+        return st
+
+    def step(st, scratch):
+        qk_norm_rope(st["q"], st["kn"], g, g, 1e-6, st["pos"], rope, st["qo"], st["ko"])
+        block_means(st["k"], kb, st["means"], length=kl)
+        block_select(st["qo"], st["means"], kt, st["blocks"], q_block=1, kv_block=kb, causal=True, q_len=ql, kv_len=kl)
+        block_attention(st["qo"], st["k"], cache_v, st["blocks"], st["out"], q_block=1, kv_block=kb, causal=True, q_len=ql,
+                        kv_len=kl, scratch=scratch)
+
+    states = [state(1), state(2)]
+    wants = []
+    for st in states:
+        step(st, None)
+        q, k, blocks = st["qo"].numpy(), st["k"].numpy(), st["blocks"].numpy()
+        assert np.array_equal(blocks, selected(q, st["means"].numpy(), 1, kb, top, True, [1, 1], [1000, 513]))
+        want, tol = reference(q, k, cache_v.numpy(), blocks, 1 / 8, 1, kb, True, [1, 1], [1000, 513])
+        got = st["out"].numpy()
+        assert np.all(np.abs(got - want) <= tolerance(want, tol, d, np.float16, False))
+        wants.append(got)
+    with pytest.raises(MoebiusError, match="captured call needs scratch"):
+        _capture(ctx, lambda: step(states[0], None))
+    ctx.synchronize()
+    graphs = [_capture(ctx, lambda st=st: step(st, st["scratch"])) for st in states]
+    for turn in range(4):
+        for st in states:
+            st["out"].buf.upload(np.zeros((n, 1, hq, d), np.float16))
+        for launch, _ in graphs:
+            assert launch() == 0
+        if turn % 2:
+            block_attention(states[0]["qo"], states[0]["k"], cache_v, states[1]["blocks"], Heads(E.DeviceArray(ctx, (n, 1, hq, d), "f2"), n, 1, hq, d),
+                            q_block=1, kv_block=kb)  # eager work between replays, in the context's own workspace
+        ctx.synchronize()
+        for st, want in zip(states, wants):
+            assert np.array_equal(st["out"].numpy(), want)
+    for _, destroy in graphs:
+        destroy()
+
+
+def test_cache_beyond_32_bit_offsets(ctx):
+    """Blocks at the far end of a cache of more than 2^32 bytes and 2^31 elements."""
+    kt, hk, d, kb = 1_100_000, 16, 128, 128
+    k, v = (E.DeviceArray(ctx, (1, kt, hk, d), "f2") for _ in range(2))
+    r = np.random.default_rng(9)
+    small = r.standard_normal((2, 2 * kb, hk, d)).astype(np.float16)
+    picked = np.array([3, kt // kb - 1], np.int32)
+    for buf, src in ((k, small[0]), (v, small[1])):
+        for i, b in enumerate(picked):
+            part = np.ascontiguousarray(src[i * kb:(i + 1) * kb])
+            _lib.check(_lib.lib().mh_memcpy_h2d(ctx.h, buf.ptr + int(b) * kb * hk * d * 2, part.ctypes.data, part.nbytes))
+    q = r.standard_normal((1, 1, hk, d)).astype(np.float16)
+    blocks = np.tile(picked, (1, 1, hk, 1))
+    out = Heads(E.DeviceArray(ctx, q.shape, "f2"), 1, 1, hk, d)
+    block_attention(heads(ctx, q), Heads(k, 1, kt, hk, d), Heads(v, 1, kt, hk, d), dev(ctx, blocks), out, q_block=1, kv_block=kb)
+    want, tol = reference(q, small[:1], small[1:], np.tile(np.arange(2, dtype=np.int32), (1, 1, hk, 1)), d ** -0.5, 1, kb, False, None, None)
+    assert np.all(np.abs(out.numpy() - want) <= tolerance(want, tol, d, np.float16, False))
+    k.free(), v.free()
+
+
+def test_python_refusals(ctx):
+    z = lambda *s: Heads(E.DeviceArray(ctx, s, "f2"), *s)  # noqa: E731
+    q, k, v, out = z(1, 4, 2, 8), z(1, 32, 1, 8), z(1, 32, 1, 8), z(1, 4, 2, 8)
+    blocks = E.DeviceArray(ctx, (1, 1, 1, 2), "i4")
+    with pytest.raises(MoebiusError, match="blocks are int32"):
+        block_attention(q, k, v, E.DeviceArray(ctx, (1, 2, 1, 2), "i4"), out)
+    with pytest.raises(MoebiusError, match="blocks are int32"):
+        block_attention(q, k, v, E.DeviceArray(ctx, (1, 1, 1, 2)), out)
+    with pytest.raises(MoebiusError, match="differ in shape"):
+        block_attention(q, k, z(1, 31, 1, 8), blocks, out)
+    with pytest.raises(MoebiusError, match="differ in type"):
+        block_attention(q, k, v, blocks, Heads(E.DeviceArray(ctx, (1, 4, 2, 8)), 1, 4, 2, 8))
+    with pytest.raises(MoebiusError, match="kv_len is int32"):
+        block_attention(q, k, v, blocks, out, kv_len=E.DeviceArray(ctx, (2,), "i4"))
+    with pytest.raises(MoebiusError, match="means are f32"):
+        block_select(q, E.DeviceArray(ctx, (1, 2, 1, 8)), 32, blocks, kv_block=64)
+    with pytest.raises(MoebiusError, match="means are f32"):
+        block_means(k, 16, E.DeviceArray(ctx, (1, 1, 1, 8)))

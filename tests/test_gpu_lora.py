@@ -1,0 +1,157 @@
+"""Low-rank adapters beside a shared projection, against f64.
+
+Tolerance: the projection's own (1e-5 of the sum of its terms' sizes in EXACT, as the
+f32 parity tests take; f16 operand roundings 2^-10 of them in FAST), and for the
+adapter (c_in + rank + 8) roundings of 2^-24 of scale sum |b| sum |a x|, worst case."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from moebius_cpu_amd import engine as E
+from moebius_cpu_amd._lib import MoebiusError
+from moebius_cpu_amd.adapters import Adapters
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    return E.Context(0)
+
+
+def reference(x, w, bias, res, a, b, scale, slot, per):
+    """y and its tolerances' scale: the projection's and the adapter's sums of sizes."""
+    x, w, a, b = (t.astype(np.float64) for t in (x, w, a, b))
+    y, base = x @ w.T, np.abs(x) @ np.abs(w).T
+    if bias is not None:
+        y, base = y + bias, base + np.abs(bias)
+    if res is not None:
+        y, base = y + res, base + np.abs(res)
+    low = np.zeros_like(y)
+    for r in range(len(x)):
+        s = slot[r // per]
+        if 0 <= s < len(scale):
+            y[r] += float(scale[s]) * (b[s] @ (a[s] @ x[r]))
+            low[r] = abs(float(scale[s])) * (np.abs(b[s]) @ (np.abs(a[s]) @ np.abs(x[r])))
+    return y, base, low
+
+
+CASES = [  # n, h, w, ci, co, rank, slots, per pixel
+    (1, 1, 1, 64, 64, 8, 1, False), (16, 1, 1, 320, 320, 16, 32, False), (3, 5, 7, 100, 52, 4, 5, False),
+    (1, 1, 40, 1280, 256, 32, 4, True), (2, 16, 16, 320, 640, 64, 2, False), (1, 9, 9, 33, 45, 3, 7, True),
+    (5, 1, 1, 2500, 70, 10, 3, False), (1, 20, 20, 64, 128, 256, 2, True), (1, 3, 11, 16, 4, 100, 3, True),
+    (17, 1, 3, 640, 1100, 7, 40, False),
+]
+
+
+def make(ctx, case, f16, seed=0):
+    n, h, w, ci, co, rank, slots, pixel = case
+    r = np.random.default_rng(seed + ci)
+    store = np.float16 if f16 else np.float32
+    d = dict(x=r.standard_normal((n, h, w, ci)).astype(np.float32), w=(r.standard_normal((co, ci)) / np.sqrt(ci)).astype(store),
+             a=(r.standard_normal((slots, rank, ci)) / np.sqrt(ci)).astype(store), b=(r.standard_normal((slots, co, rank)) * 0.3).astype(store),
+             scale=r.uniform(0.3, 2, slots).astype(np.float32), bias=r.standard_normal(co).astype(np.float32),
+             res=r.standard_normal((n, h, w, co)).astype(np.float32))
+    d["slot"] = r.integers(-1, slots, n * h * w if pixel else n).astype(np.int32)
+    return d
+
+
+def layer(ctx, case, d, f16, bias=True):
+    _, _, _, ci, co, rank, _, _ = case
+    conv = E.Conv1x1(ctx, ci, co, E.Param(ctx, d["w"], f16=f16), d["bias"] if bias else None)
+    return conv, Adapters(ctx, E.Param(ctx, d["a"], f16=f16), E.Param(ctx, d["b"], f16=f16), d["scale"], ci, co, rank)
+
+
+@pytest.mark.parametrize("fast", [False, True])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("extra", [False, True])
+@pytest.mark.parametrize("case", CASES)
+def test_against_the_formula(ctx, case, f16, extra, fast):
+    n, h, w, ci, co, rank, slots, pixel = case
+    d = make(ctx, case, f16)
+    conv, ad = layer(ctx, case, d, f16, extra)
+    out = E.Tensor(ctx, n, h, w, co)
+    ctx.set_precision(fast)
+    try:
+        conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, E.DeviceArray.from_numpy(ctx, d["slot"]), out,
+                             E.Tensor.from_numpy(ctx, d["res"]) if extra else None)
+    finally:
+        ctx.set_precision(False)
+    y, base, low = reference(d["x"].reshape(-1, ci), d["w"], d["bias"] if extra else None,
+                             d["res"].reshape(-1, co) if extra else None, d["a"], d["b"], d["scale"], d["slot"],
+                             1 if pixel else h * w)
+    err = np.abs(out.numpy().reshape(-1, co) - y)
+    bound = (2.0 ** -10 if fast else 1e-5) * base + (ci + rank + 8) * U * low + U * np.abs(y)
+    assert np.all(err <= bound), (err / bound).max()
+
+
+@pytest.mark.parametrize("case", [CASES[1], CASES[3], CASES[5]])
+def test_rows_without_adapter_are_the_projection(ctx, case):
+    """Slots below 0 and at or above the number of adapters: the bits of the projection alone."""
+    n, h, w, ci, co, _, slots, pixel = case
+    d = make(ctx, case, True)
+    conv, ad = layer(ctx, case, d, True)
+    x, plain, out = E.Tensor.from_numpy(ctx, d["x"]), E.Tensor(ctx), E.Tensor(ctx)
+    conv.forward(x, plain)
+    slot = np.where(np.arange(d["slot"].size) % 2, d["slot"], np.where(np.arange(d["slot"].size) % 4, slots, -2**31)).astype(np.int32)
+    conv.forward_adapted(x, ad, E.DeviceArray.from_numpy(ctx, slot), out)
+    rows = np.repeat(slot, 1 if pixel else h * w).reshape(n, h, w)
+    none = (rows < 0) | (rows >= slots)
+    assert none.any() and np.array_equal(out.numpy()[none], plain.numpy()[none])
+    assert not np.array_equal(out.numpy(), plain.numpy())
+
+
+def test_values_that_are_not_finite_stay_with_their_request(ctx):
+    """An adapter of NaN and infinity, and a row of NaN, among rows of other requests in the same tile."""
+    case = (1, 1, 16, 64, 64, 8, 3, True)
+    d = make(ctx, case, False)
+    d["slot"][:] = np.arange(16) % 3
+    conv, ad = layer(ctx, case, d, False)
+    slot, good, out = E.DeviceArray.from_numpy(ctx, d["slot"]), E.Tensor(ctx), E.Tensor(ctx)
+    conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, slot, good)
+    d["a"][1, 2], d["b"][1, :, 3] = np.nan, np.inf
+    d["x"][0, 0, 5] = np.nan
+    conv, ad = layer(ctx, case, d, False)
+    conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, slot, out)
+    bad = (d["slot"] == 1) | (np.arange(16) == 5)
+    got = out.numpy()[0, 0]
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+    # the projection repairs tiles with such sums on other instructions: equal but for its roundings
+    assert np.abs(got - good.numpy()[0, 0])[~bad].max() < 1e-5
+
+
+def test_scratch_and_no_rows(ctx):
+    case = (4, 1, 1, 640, 64, 16, 4, False)
+    d = make(ctx, case, True)
+    conv, ad = layer(ctx, case, d, True)
+    x, slot, a, b = E.Tensor.from_numpy(ctx, d["x"]), E.DeviceArray.from_numpy(ctx, d["slot"]), E.Tensor(ctx), E.Tensor(ctx)
+    size = ad.scratch(4)
+    assert size > 0
+    conv.forward_adapted(x, ad, slot, a)
+    conv.forward_adapted(x, ad, slot, b, scratch=E.DeviceArray(ctx, (size,), np.uint8))
+    assert np.array_equal(a.numpy(), b.numpy())
+    with pytest.raises(MoebiusError, match="smaller"):
+        conv.forward_adapted(x, ad, slot, b, scratch=E.DeviceArray(ctx, (size - 1,), np.uint8))
+    conv.forward_adapted(E.Tensor(ctx, 0, 1, 1, 640), ad, E.DeviceArray(ctx, (0,), "i4"), b)
+    assert b.shape == (0, 1, 1, 64)
+
+
+def test_python_refusals(ctx):
+    case = (2, 2, 2, 32, 16, 4, 2, False)
+    d = make(ctx, case, False)
+    conv, ad = layer(ctx, case, d, False)
+    x, out = E.Tensor.from_numpy(ctx, d["x"]), E.Tensor(ctx)
+    with pytest.raises(MoebiusError, match="slot is int32"):
+        conv.forward_adapted(x, ad, E.DeviceArray(ctx, (3,), "i4"), out)
+    with pytest.raises(MoebiusError, match="slot is int32"):
+        conv.forward_adapted(x, ad, E.DeviceArray(ctx, (2,)), out)
+    with pytest.raises(MoebiusError, match="input channels"):
+        conv.forward_adapted(E.Tensor(ctx, 2, 2, 2, 31), ad, E.DeviceArray(ctx, (2,), "i4"), out)
+    with pytest.raises(MoebiusError, match="adapter size"):
+        Adapters(ctx, ad.a, ad.b, d["scale"], 32, 16, 5)
+    with pytest.raises(MoebiusError, match="storage type"):
+        Adapters(ctx, ad.a, E.Param(ctx, d["b"], f16=True), d["scale"], 32, 16, 4)
+    with pytest.raises(MoebiusError, match="residual shape"):
+        conv.forward_adapted(x, ad, E.DeviceArray(ctx, (2,), "i4"), out, E.Tensor(ctx, 1, 2, 2, 16))
