@@ -9,8 +9,8 @@
 // (32x32 instructions: column = lane % 32), the maximum and the sum of a row stay in the
 // lane but for one exchange with lane +- 32, and the scores are already the B operand of
 // O^T = V^T . P^T: its lane half h wants eight keys of sixteen, and holds eight, keys
-// 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3; V is staged with its keys in that order. WR waves
-// share a tile of keys, WK groups of waves take every WK-th tile and join in LDS.
+// 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3, so V^T is read with its keys in that order. WR
+// waves share a tile of keys, WK groups of waves take every WK-th tile and join in LDS.
 //
 // Half: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated as the
 // f16 GEMMs round operands; P rounded to f16, at most 1 with a relative 2^-11 each, which
@@ -49,12 +49,12 @@ constexpr int part_floats(int dt) { return (dt * 16 + 2) * 64; }
 template <bool HALF, int DT, int WR>
 struct Tiling {
     static constexpr int kDP = DT * 32;
-    static constexpr int kKT = HALF && DT <= 4 && WR >= 2 ? 64 : 32;  // keys per tile
+    static constexpr int kKT = HALF && (DT <= 2 ? WR >= 2 : DT <= 4 && WR == 4) ? 64 : 32;  // keys per tile
     static constexpr int kES = HALF ? 2 : 4;              // bytes of a staged value
-    static constexpr int kKS = kDP + (HALF ? 8 : 4);      // staged key row (values)
-    static constexpr int kVS = HALF ? kKT : kDP + 8;      // staged value row (half: a channel's keys)
-    static constexpr int kVRows = HALF ? kDP : kKT;
-    static constexpr int kKBytes = kKT * kKS * kES, kVBytes = kVRows * kVS * kES;
+    // staged rows (values), padded so that the rows of a read lie on distinct banks
+    static constexpr int kKS = kDP + (HALF ? 8 : 4);
+    static constexpr int kVS = HALF ? kDP + (kDP % 64 ? 0 : 32) : kDP + 8;
+    static constexpr int kKBytes = kKT * kKS * kES, kVBytes = kKT * kVS * kES;
     static constexpr int kStage = kKBytes + kVBytes;      // one key group's tile
     // key groups: four waves together, fewer where their tiles exceed the LDS of a CU (160 KiB)
     static constexpr int kWK = 4 / WR * kStage <= 144 * 1024 ? 4 / WR : 2 / WR;
@@ -106,24 +106,28 @@ struct Run8 {
     }
 };
 
-// Column of the 8-key runs of channel `dim` in the staged V^T: the eight (four) runs of a
-// channel are exchanged so that neither the lanes of a read (consecutive channels) nor
-// those of a write (every eighth channel) meet in a bank.
-template <int KT>
-__device__ __forceinline__ int vt_run(int dim, int run) {
-    return run ^ (((dim >> (KT == 64 ? 1 : 2)) ^ (dim >> 3)) & (KT / 8 - 1));
+// V^T operand of 32 channels and sixteen keys from staged rows of stride VS: a transposed
+// read hands lane i of sixteen the i-th of sixteen channels at four keys, the lanes' own
+// addresses being four channels of key lane / 4 each. Keys 4 h .. 4 h + 3, then 8 more on.
+template <int VS>
+__device__ __forceinline__ halfx8 read_vt(const char *v, int lane) {
+    typedef short shortx4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) shortx4 lds4;
+    const char *p = v + ((4 * (lane >> 5) + ((lane >> 2) & 3)) * VS + ((lane >> 4) & 1) * 16 + (lane & 3) * 4) * 2;
+    const shortx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p));
+    const shortx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 8 * VS * 2));
+    return __builtin_bit_cast(halfx8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // Key of accumulator register i in lane half h (32 x 32 results: row of the tile).
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
 
 template <typename T, bool HALF, bool VEC, int DT, int WR>
-__global__ __launch_bounds__(256) void block_attention_kernel(Args a) {
+__global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 : 1) void block_attention_kernel(Args a) {
     using L = Tiling<HALF, DT, WR>;
     constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP;
     constexpr int NT = 64 * WR;                       // threads that stage one tile
-    constexpr int KU = (KT * DP / 8 + NT - 1) / NT;   // runs of 8 channels of K per thread
-    constexpr int VU = (KT / 4 * DP / 8 + NT - 1) / NT;  // units of 4 keys x 8 channels of V
+    constexpr int KU = (KT * DP / 8 + NT - 1) / NT;   // runs of 8 channels of K, and of V, per thread
     extern __shared__ __align__(16) char smem[];
     __shared__ int32_t list[kMaxTop];  // first token of every block to visit
     __shared__ int list_n, bad[WK];
@@ -233,82 +237,38 @@ __global__ __launch_bounds__(256) void block_attention_kernel(Args a) {
     // Token of key j of this split; past its end none. Loads of tokens there are not
     // (behind the list or kv_len) read the last one instead and are not used.
     auto token = [&](int j) { return j < keys ? list[l0 + (j >> a.kb_log)] + (j & (kb - 1)) : 0x7fffffff; };
-    Run8<T> kr[KU], vr[VU][4];
+    Run8<T> kr[KU], vr[KU];
     auto fetch = [&](int tile) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
             const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
-            if (i / (DP / 8) < KT && ch < a.d)
-                kr[u].template load<VEC>(kp + int64_t(min(token(tile * KT + j), kv_len - 1)) * a.ldk + ch, a.d - ch);
-        }
-#pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            const int i = ttid + u * NT, j = i / (DP / 8) * 4, ch = i % (DP / 8) * 8;
             if (j < KT && ch < a.d) {
-                const int t0 = token(tile * KT + j);  // four keys lie in one block
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    vr[u][e].template load<VEC>(vp + int64_t(min(t0 == 0x7fffffff ? t0 : t0 + e, kv_len - 1)) * a.ldv + ch,
-                                                a.d - ch);
+                const int64_t t = min(token(tile * KT + j), kv_len - 1);
+                kr[u].template load<VEC>(kp + t * a.ldk + ch, a.d - ch);
+                vr[u].template load<VEC>(vp + t * a.ldv + ch, a.d - ch);
             }
+        }
+    };
+    auto put = [&](char *p, const Run8<T> &r) {
+        if constexpr (HALF) {
+            *reinterpret_cast<halfx8 *>(p) = r.half();
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                reinterpret_cast<floatx4 *>(p)[e] = floatx4{float(r.at(4 * e)), float(r.at(4 * e + 1)),
+                                                            float(r.at(4 * e + 2)), float(r.at(4 * e + 3))};
         }
     };
     auto stage = [&](int tile) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
             const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
-            if (i / (DP / 8) < KT && ch < a.d) {
-                if constexpr (HALF) {
-                    *reinterpret_cast<halfx8 *>(kst + (j * L::kKS + ch) * 2) = kr[u].half();
-                } else {
-                    float *p = reinterpret_cast<float *>(kst) + j * L::kKS + ch;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<floatx4 *>(p + 4 * e) = floatx4{float(kr[u].at(4 * e)), float(kr[u].at(4 * e + 1)),
-                                                                          float(kr[u].at(4 * e + 2)),
-                                                                          float(kr[u].at(4 * e + 3))};
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            const int i = ttid + u * NT, j = i / (DP / 8) * 4, ch = i % (DP / 8) * 8;
             if (j < KT && ch < a.d) {
-                const int t0 = token(tile * KT + j);
-                if (t0 > kv_len - 4) {  // values of tokens that there are not: zeros, whatever lies there
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (t0 >= kv_len || t0 + e >= kv_len) vr[u][e].zero();
-                }
-                if (a.causal) {
-                    bool ok = true;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) ok = ok && vr[u][e].finite();
-                    if (!ok) bad[wk] = 1;
-                }
-                if constexpr (HALF) {
-                    halfx8 hv[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) hv[e] = vr[u][e].half();
-                    // keys 4 m .. 4 m + 3 of sixteen: lane half m % 2, its first or second four
-                    const int m = (j >> 2) & 3, run = (j >> 4) * 2 + (m & 1);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int dim = ch + k;
-                        *reinterpret_cast<halfx4 *>(vst + (dim * KT + vt_run<KT>(dim, run) * 8 + (m >> 1) * 4) * 2) =
-                            halfx4{hv[0][k], hv[1][k], hv[2][k], hv[3][k]};
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float *p = reinterpret_cast<float *>(vst) + (j + e) * L::kVS + ch;
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            *reinterpret_cast<floatx4 *>(p + 4 * k) =
-                                floatx4{float(vr[u][e].at(4 * k)), float(vr[u][e].at(4 * k + 1)),
-                                        float(vr[u][e].at(4 * k + 2)), float(vr[u][e].at(4 * k + 3))};
-                    }
-                }
+                // values of tokens that there are not: zeros, whatever lies there
+                if (token(tile * KT + j) >= kv_len) vr[u].zero();
+                if (a.causal && !vr[u].finite()) bad[wk] = 1;
+                put(kst + (j * L::kKS + ch) * L::kES, kr[u]);
+                put(vst + (j * L::kVS + ch) * L::kES, vr[u]);
             }
         }
     };
@@ -412,14 +372,8 @@ __global__ __launch_bounds__(256) void block_attention_kernel(Args a) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int dim = t * 32 + acc_row(r, h);
-                        float v;
-                        if constexpr (HALF) {
-                            const int mm = (j >> 2) & 3, run = (j >> 4) * 2 + (mm & 1);
-                            v = float(reinterpret_cast<const _Float16 *>(
-                                vst)[dim * KT + vt_run<KT>(dim, run) * 8 + (mm >> 1) * 4 + (j & 3)]);
-                        } else {
-                            v = reinterpret_cast<const float *>(vst)[j * L::kVS + dim];
-                        }
+                        typedef std::conditional_t<HALF, _Float16, float> E;
+                        const float v = float(reinterpret_cast<const E *>(vst)[j * L::kVS + dim]);
                         if (sees) o[t][r] = __builtin_fmaf(p, v, o[t][r]);
                     }
             }
@@ -431,11 +385,9 @@ __global__ __launch_bounds__(256) void block_attention_kernel(Args a) {
                     halfx8 p;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) p[i] = static_cast<_Float16>(sc[b][x * 8 + i]);
-                    const int run = (b * 2 + x) * 2 + h;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
-                        const int dim = t * 32 + col;
-                        const halfx8 v = *reinterpret_cast<const halfx8 *>(vst + (dim * KT + vt_run<KT>(dim, run) * 8) * 2);
+                        const halfx8 v = read_vt<L::kVS>(vst + ((b * 32 + x * 16) * L::kVS + t * 32) * 2, lane);
                         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[t], 0, 0, 0);
                     }
                 }
