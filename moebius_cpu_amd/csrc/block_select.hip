@@ -94,11 +94,15 @@ __device__ __forceinline__ uint64_t order_key(double s) {
     return (b >> 63) ? ~b : b | (uint64_t(1) << 63);
 }
 
-// One workgroup per (item, key head, TQ blocks of queries).
-template <typename T, int W, int TQ>
+typedef double doublex4 __attribute__((ext_vector_type(4)));
+
+// One workgroup per (item, key head, TQ blocks of queries); W, MW: the runs in which the
+// queries and the means are read.
+template <typename T, int W, int MW, int TQ>
 __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     extern __shared__ uint64_t keys[];  // [TQ][nk]
-    __shared__ float qm[TQ][kMaxHeadDim];
+    constexpr int kQS = kMaxHeadDim + 4;
+    __shared__ __align__(16) float qm[TQ][kQS];
     const int tile = blockIdx.x % a.tiles;
     const int hk = (blockIdx.x / a.tiles) % a.hk, item = blockIdx.x / a.tiles / a.hk;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -110,6 +114,9 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     int span = 1;  // lanes per row: the next power of two
     while (span < runs && span < 64) span *= 2;
     const int groups = 64 / span, cl = lane % span, rg = lane / span;
+    // Zeros behind d, which the products' last run of sixteen reads.
+    for (int i = tid; i < TQ * 16; i += 256)
+        if (a.d + i % 16 < kQS) qm[i / 16][a.d + i % 16] = 0.0f;
     for (int t = wave; t < TQ; t += 4) {
         const int i0 = (b0 + t) * a.qb, i1 = min(i0 + a.qb, q_len);
         const int rows = max(i1 - i0, 0) * a.g;
@@ -117,7 +124,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
         for (int c0 = cl; c0 < ((runs + span - 1) / span) * span; c0 += span) {
             double sum[W] = {};
             if (c0 < runs) {
-#pragma unroll 4
+#pragma unroll 8
                 for (int r = rg; r < rows; r += groups) {
                     const int i = r / a.g, e = r - i * a.g;
                     float v[W];
@@ -136,24 +143,56 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     }
     __syncthreads();
 
-    // Scores: a thread takes a key block and TQ / QS of the query blocks.
-    constexpr int QS = TQ < 4 ? TQ : 4, TT = TQ / QS, CW = 256 / QS;
-    const int qs = tid / CW;
+    // Scores. One block of queries: sixteen lanes per key block. More: 16 key blocks x 16
+    // query blocks on the f64 matrix instruction (lane: row or column lane % 16, four
+    // channels at 4 (lane / 16); result register i is row 4 i + lane / 16).
     const int seen_all = (kv_len + a.kb - 1) / a.kb;
-    for (int b = tid % CW; b < seen_all; b += CW) {
-        const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
-        double s[TT] = {};
-        for (int c = 0; c < a.d; c += 2) {
-            const double m0 = double(m[c]), m1 = c + 1 < a.d ? double(m[c + 1]) : 0.0;
+    const int l16 = lane & 15, kg = lane >> 4;
+    if constexpr (TQ == 1) {
+        for (int t0 = 0; t0 < seen_all; t0 += 16) {
+            const int b = t0 + wave * 4 + kg;
+            double s = 0;
+            if (b < seen_all) {
+                const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
+                for (int c = l16 * MW; c < a.d; c += 16 * MW) {
+                    float v[MW];
+                    load_run<float, MW>(m + c, v);
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                const int tq = qs * TT + t;
-                s[t] = __builtin_fma(double(qm[tq][c]), m0, s[t]);
-                if (c + 1 < a.d) s[t] = __builtin_fma(double(qm[tq][c + 1]), m1, s[t]);
+                    for (int e = 0; e < MW; ++e) s = __builtin_fma(double(qm[0][c + e]), double(v[e]), s);
+                }
+            }
+#pragma unroll
+            for (int x = 8; x; x >>= 1) s += __shfl_xor(s, x);
+            if (b < seen_all && l16 == 0) keys[b] = order_key(s);
+        }
+    } else {
+        for (int t0 = wave * 16; t0 < seen_all; t0 += 64) {
+            const int b = min(t0 + l16, seen_all - 1);
+            const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
+            const float *q = qm[min(l16, TQ - 1)];
+            doublex4 acc = {0, 0, 0, 0};
+            for (int c = kg * 4; c < (a.d + 15) / 16 * 16; c += 16) {
+                float mv[4], qv[4];
+                if (MW == 4) {
+                    const bool in = c < a.d;
+                    load_run<float, 4>(m + (in ? c : 0), mv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mv[e] = in ? mv[e] : 0.0f;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mv[e] = c + e < a.d ? m[c + e] : 0.0f;
+                }
+                load_run<float, 4>(q + c, qv);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(mv[e]), double(qv[e]), acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = t0 + 4 * i + kg;
+                if (l16 < TQ && r < seen_all) keys[l16 * a.nk + r] = order_key(acc[i]);
             }
         }
-#pragma unroll
-        for (int t = 0; t < TT; ++t) keys[(qs * TT + t) * a.nk + b] = order_key(s[t]);
     }
     __syncthreads();
 
@@ -209,12 +248,12 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     }
 }
 
-template <typename T, int W>
+template <typename T, int W, int MW>
 void select_w(Context &ctx, SelectArgs &a, int n) {
     // Blocks of queries per workgroup: up to eight share the reads of the means, as many
-    // as leave the card two workgroups per CU and their keys in 48 KiB of LDS.
+    // as leave the card two workgroups per CU and their keys in 32 KiB of LDS.
     int tq = 8;
-    while (tq > 1 && (tq > a.nq || int64_t(tq) * a.nk * 8 > 48 * 1024 ||
+    while (tq > 1 && (tq > a.nq || int64_t(tq) * a.nk * 8 > 32 * 1024 ||
                       int64_t(n) * a.hk * ceil_div(a.nq, tq) < 2 * ctx.cu_count))
         tq /= 2;
     a.tiles = int(ceil_div(a.nq, tq));
@@ -222,11 +261,24 @@ void select_w(Context &ctx, SelectArgs &a, int n) {
     MH_REQUIRE(blocks < (int64_t(1) << 31), "block_select: too many blocks of queries");
     const uint32_t lds = uint32_t(tq) * a.nk * 8;
     const dim3 grid{uint32_t(blocks)}, block{256};
-    if (tq == 8) block_select_kernel<T, W, 8><<<grid, block, lds, ctx.stream>>>(a);
-    else if (tq == 4) block_select_kernel<T, W, 4><<<grid, block, lds, ctx.stream>>>(a);
-    else if (tq == 2) block_select_kernel<T, W, 2><<<grid, block, lds, ctx.stream>>>(a);
-    else block_select_kernel<T, W, 1><<<grid, block, lds, ctx.stream>>>(a);
+    if (tq == 8) {
+        block_select_kernel<T, W, MW, 8><<<grid, block, lds, ctx.stream>>>(a);
+    } else if (tq == 4) {
+        block_select_kernel<T, W, MW, 4><<<grid, block, lds, ctx.stream>>>(a);
+    } else if (tq == 2) {
+        block_select_kernel<T, W, MW, 2><<<grid, block, lds, ctx.stream>>>(a);
+    } else {
+        const void *fn = reinterpret_cast<const void *>(&block_select_kernel<T, W, MW, 1>);
+        if (lds > 48 * 1024) HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+        block_select_kernel<T, W, MW, 1><<<grid, block, lds, ctx.stream>>>(a);
+    }
     MH_LAUNCH_CHECK();
+}
+
+template <typename T, int W>
+void select_q(Context &ctx, SelectArgs &a, int n) {
+    if (a.d % 4 == 0 && aligned16(a.means)) select_w<T, W, 4>(ctx, a, n);
+    else select_w<T, W, 1>(ctx, a, n);
 }
 
 template <typename T>
@@ -266,11 +318,11 @@ void block_select(Context &ctx, HeadRows q, WeightType type, const BlockShape &s
     a.q_tokens = s.q_tokens, a.kv_tokens = s.kv_tokens, a.hk = s.heads_kv, a.g = s.heads_q / s.heads_kv, a.d = s.d;
     a.qb = s.q_block, a.kb = s.kv_block, a.nq = s.q_blocks(), a.nk = s.kv_blocks(), a.top = s.top, a.causal = s.causal;
     if (type == kF16) {
-        if (runs_of<_Float16>(8, q.p, q.ld, s.d)) select_w<_Float16, 8>(ctx, a, s.n);
-        else select_w<_Float16, 1>(ctx, a, s.n);
+        if (runs_of<_Float16>(8, q.p, q.ld, s.d)) select_q<_Float16, 8>(ctx, a, s.n);
+        else select_q<_Float16, 1>(ctx, a, s.n);
     } else {
-        if (runs_of<float>(4, q.p, q.ld, s.d)) select_w<float, 4>(ctx, a, s.n);
-        else select_w<float, 1>(ctx, a, s.n);
+        if (runs_of<float>(4, q.p, q.ld, s.d)) select_q<float, 4>(ctx, a, s.n);
+        else select_q<float, 1>(ctx, a, s.n);
     }
 }
 
