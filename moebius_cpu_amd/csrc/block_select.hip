@@ -101,7 +101,7 @@ typedef double doublex4 __attribute__((ext_vector_type(4)));
 template <typename T, int W, int MW, int TQ>
 __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     extern __shared__ uint64_t keys[];  // [TQ][nk]
-    constexpr int kQS = kMaxHeadDim + 4;
+    constexpr int kQS = kMaxHeadDim + 20;  // rows of a read on distinct banks, sixteen zeros behind d
     __shared__ __align__(16) float qm[TQ][kQS];
     const int tile = blockIdx.x % a.tiles;
     const int hk = (blockIdx.x / a.tiles) % a.hk, item = blockIdx.x / a.tiles / a.hk;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     const int groups = 64 / span, cl = lane % span, rg = lane / span;
     // Zeros behind d, which the products' last run of sixteen reads.
     for (int i = tid; i < TQ * 16; i += 256)
-        if (a.d + i % 16 < kQS) qm[i / 16][a.d + i % 16] = 0.0f;
+        qm[i / 16][a.d + i % 16] = 0.0f;
     for (int t = wave; t < TQ; t += 4) {
         const int i0 = (b0 + t) * a.qb, i1 = min(i0 + a.qb, q_len);
         const int rows = max(i1 - i0, 0) * a.g;
@@ -171,21 +171,29 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
             const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
             const float *q = qm[min(l16, TQ - 1)];
             doublex4 acc = {0, 0, 0, 0};
-            for (int c = kg * 4; c < (a.d + 15) / 16 * 16; c += 16) {
-                float mv[4], qv[4];
-                if (MW == 4) {
-                    const bool in = c < a.d;
-                    load_run<float, 4>(m + (in ? c : 0), mv);
+            for (int c0 = 0; c0 < a.d; c0 += 64) {
+                float mv[4][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mv[e] = in ? mv[e] : 0.0f;
-                } else {
+                for (int u = 0; u < 4; ++u) {
+                    const int c = c0 + u * 16 + kg * 4;
+                    if constexpr (MW == 4) {
+                        load_run<float, 4>(m + min(c, a.d - 4), mv[u]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mv[e] = c + e < a.d ? m[c + e] : 0.0f;
+                        for (int e = 0; e < 4; ++e) mv[u][e] = c < a.d ? mv[u][e] : 0.0f;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mv[u][e] = c + e < a.d ? m[c + e] : 0.0f;
+                    }
                 }
-                load_run<float, 4>(q + c, qv);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(mv[e]), double(qv[e]), acc, 0, 0, 0);
+                for (int u = 0; u < 4; ++u) {
+                    if (c0 + u * 16 >= a.d) break;
+                    float qv[4];
+                    load_run<float, 4>(q + c0 + u * 16 + kg * 4, qv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(mv[u][e]), double(qv[e]), acc, 0, 0, 0);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
