@@ -38,8 +38,9 @@ struct LoraArgs {
 // Four values at p + k of a run of n, zeros behind it; VEC: n and p keep every run of four aligned.
 template <bool VEC>
 __device__ __forceinline__ floatx4 load4(const float *p, int k, int n) {
-    if constexpr (VEC) {
-        return k < n ? *reinterpret_cast<const floatx4 *>(p + k) : floatx4{0, 0, 0, 0};
+    if constexpr (VEC) {  // behind n the last run is loaded instead, so that no load waits for a branch
+        const floatx4 v = *reinterpret_cast<const floatx4 *>(p + min(k, n - 4));
+        return k < n ? v : floatx4{0, 0, 0, 0};
     } else {
         floatx4 v;
 #pragma unroll
@@ -51,11 +52,9 @@ template <bool VEC>
 __device__ __forceinline__ floatx4 load4(const _Float16 *p, int k, int n) {
     floatx4 v = {0, 0, 0, 0};
     if constexpr (VEC) {
-        if (k < n) {
-            const halfx4 r = *reinterpret_cast<const halfx4 *>(p + k);
+        const halfx4 r = *reinterpret_cast<const halfx4 *>(p + min(k, n - 4));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = float(r[e]);
-        }
+        for (int e = 0; e < 4; ++e) v[e] = k < n ? float(r[e]) : 0.0f;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -74,7 +73,8 @@ __device__ __forceinline__ int slot_of(const LoraArgs &p, int64_t row) {
     return s < p.slots ? s : -1;
 }
 
-constexpr int kRankTiles = 4;  // 16 ranks each per pass over x
+constexpr int kRankTiles = 4;     // 16 ranks each per pass over x
+constexpr int kShrinkUnroll = 5;  // steps of the long axis whose loads are in flight together
 
 // Workgroup (16 rows, split of the long axis); wave w takes every fourth 16 of its share.
 // Lane l holds row (rank) l % 16 and four values of the long axis at 4 (l / 16).
@@ -99,14 +99,20 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
                 acc[j] = floatx4{0, 0, 0, 0};
                 a[j] = static_cast<const T *>(p.a) + (int64_t(s) * p.rank + min(q0 + j * 16 + r16, p.rank - 1)) * p.ci;
             }
-            for (int k = k0 + wave * 16; k < k1; k += 64) {
-                const floatx4 xv = load4<VEC>(x, k + kg * 4, k1);
+            for (int k = k0 + wave * 16; k < k1; k += 64 * kShrinkUnroll) {
+                floatx4 xv[kShrinkUnroll];
+#pragma unroll
+                for (int u = 0; u < kShrinkUnroll; ++u) xv[u] = load4<VEC>(x, k + u * 64 + kg * 4, k1);
 #pragma unroll
                 for (int j = 0; j < kRankTiles; ++j) {
                     if (q0 + j * 16 < p.rank) {
-                        const floatx4 av = load4<VEC>(a[j], k + kg * 4, k1);
+                        floatx4 av[kShrinkUnroll];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[j] = mfma(av[e], xv[e], acc[j]);
+                        for (int u = 0; u < kShrinkUnroll; ++u) av[u] = load4<VEC>(a[j], k + u * 64 + kg * 4, k1);
+#pragma unroll
+                        for (int u = 0; u < kShrinkUnroll; ++u)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[j] = mfma(av[u][e], xv[u][e], acc[j]);
                     }
                 }
             }
@@ -188,8 +194,97 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
     }
 }
 
+// Few rows (single tokens): each row reads its own adapter anyway, so a wave takes one rank
+// of one row, lanes over the long axis; t [rows][rank_pad].
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void lora_row_shrink_kernel(LoraArgs p) {
+    const int lane = threadIdx.x & 63, q = int(blockIdx.y) * 4 + (threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
+    const int s = slot_of(p, row);
+    if (s < 0 || q >= p.rank) return;
+    const float *x = p.x + row * p.ci;
+    const T *a = static_cast<const T *>(p.a) + (int64_t(s) * p.rank + q) * p.ci;
+    float sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int k = lane * 4; k < p.ci; k += 256) {
+        const floatx4 xv = load4<VEC>(x, k, p.ci), av = load4<VEC>(a, k, p.ci);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(xv[e], av[e], sum[e]);
+    }
+    float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
+    if (lane == 0) p.t[row * p.rank_pad + q] = v;
+}
+
+// The projection and the adapters' second product of 16 rows and 16 columns: eight waves
+// split the long axis (f32 products, eight values of it per lane and step: column or row
+// l % 16, values 8 (l / 16) ..), join in LDS, and 256 threads finish one value each.
+// Bound: the weight, read once per 16 rows.
+constexpr int kRowUnroll = 5;  // steps of 256 values in flight: 1280 at once
+
+template <typename W, typename T, bool VEC>
+__global__ __launch_bounds__(512) void lora_row_project_kernel(LoraArgs p, const W *w, const float *bias,
+                                                               const float *residual) {
+    __shared__ float part[8][4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
+    const int c0 = int(blockIdx.x) * 16;
+    const int64_t r0 = int64_t(blockIdx.y) * 16;
+    const W *wr = w + int64_t(min(c0 + r16, p.co - 1)) * p.ci;
+    const float *x = p.x + min(r0 + r16, p.rows - 1) * p.ci;
+    floatx4 acc = {0, 0, 0, 0};
+    for (int k0 = __builtin_amdgcn_readfirstlane(wave) * 32; k0 < p.ci; k0 += 256 * kRowUnroll) {
+        floatx4 wv[kRowUnroll][2], xv[kRowUnroll][2];
+#pragma unroll
+        for (int u = 0; u < kRowUnroll; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int k = k0 + u * 256 + kg * 8 + 4 * i;
+                wv[u][i] = load4<VEC>(wr, k, p.ci);
+                xv[u][i] = load4<VEC>(x, k, p.ci);
+            }
+#pragma unroll
+        for (int u = 0; u < kRowUnroll; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc = mfma(wv[u][i][e], xv[u][i][e], acc);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][e][lane] = acc[e];
+    __syncthreads();
+    if (tid >= 256) return;
+    // thread: column tid % 16 (register e = % 4 of lane group / 4) of row tid / 16
+    const int c = c0 + (tid & 15);
+    const int64_t row = r0 + (tid >> 4);
+    if (c >= p.co || row >= p.rows) return;
+    const int e = tid & 3, l = ((tid & 15) >> 2) * 16 + (tid >> 4);
+    float v = bias ? bias[c] : 0.0f;
+    if (residual) v += residual[row * p.co + c];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part[i][e][l];
+    v += sum;
+    const int s = slot_of(p, row);
+    if (s >= 0) {
+        const T *b = static_cast<const T *>(p.b) + (int64_t(s) * p.co + c) * p.rank;
+        const float *t = p.t + row * p.rank_pad;
+        float y = 0.0f;
+        for (int k = 0; k < p.rank; ++k) y = __builtin_fmaf(t[k], float(b[k]), y);
+        v = __builtin_fmaf(p.scale[s], y, v);
+    }
+    p.out[row * p.co + c] = v;
+}
+
+// Rows up to which the projection is worth forming beside the adapters (few_rows): both
+// of its passes over 16 rows against the general product's split sums and the two
+// adapter passes over its output.
+constexpr int kFewRows = 64;
+bool few_rows(int64_t rows) { return rows <= kFewRows; }
+
 // Splits of the long axis: two workgroups per CU, at least 128 values each.
 int lora_splits(const Context &ctx, int64_t rows, int c_in) {
+    if (few_rows(rows)) return 1;
     const int64_t tiles = ceil_div(rows, 16);
     const int64_t s = std::min<int64_t>(2 * ctx.cu_count / std::max<int64_t>(tiles, 1), c_in / 128);
     return int(std::max<int64_t>(1, std::min<int64_t>(s, 16)));
@@ -215,6 +310,21 @@ void run(Context &ctx, const LoraArgs &p) {
     MH_LAUNCH_CHECK();
 }
 
+template <typename W, typename T>
+void run_few(Context &ctx, const LoraArgs &p, const void *weight, const float *bias, const float *residual) {
+    const bool va = p.ci % 4 == 0 && aligned16(p.x) && reinterpret_cast<uintptr_t>(p.a) % (4 * sizeof(T)) == 0;
+    const dim3 sg{uint32_t(p.rows), uint32_t(ceil_div(p.rank, 4))};
+    if (va) lora_row_shrink_kernel<T, true><<<sg, dim3{256}, 0, ctx.stream>>>(p);
+    else lora_row_shrink_kernel<T, false><<<sg, dim3{256}, 0, ctx.stream>>>(p);
+    MH_LAUNCH_CHECK();
+    const bool vw = p.ci % 4 == 0 && aligned16(p.x) && reinterpret_cast<uintptr_t>(weight) % (4 * sizeof(W)) == 0;
+    const dim3 pg{uint32_t(ceil_div(p.co, 16)), uint32_t(ceil_div(p.rows, 16))};
+    const W *w = static_cast<const W *>(weight);
+    if (vw) lora_row_project_kernel<W, T, true><<<pg, dim3{512}, 0, ctx.stream>>>(p, w, bias, residual);
+    else lora_row_project_kernel<W, T, false><<<pg, dim3{512}, 0, ctx.stream>>>(p, w, bias, residual);
+    MH_LAUNCH_CHECK();
+}
+
 }  // namespace
 
 size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int rank) {
@@ -223,8 +333,9 @@ size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int rank) {
 
 void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const void *weight, WeightType wt, int c_out,
                   const float *bias, const float *residual, const Lora &l, float *out, void *scratch) {
-    conv1x1(ctx, x, rows, c_in, weight, wt, c_out, bias, residual, out);
     if (!rows) return;
+    const bool few = few_rows(rows);
+    if (!few) conv1x1(ctx, x, rows, c_in, weight, wt, c_out, bias, residual, out);
     LoraArgs p{};
     p.x = x, p.a = l.a, p.b = l.b, p.scale = l.scale, p.slot = l.slot, p.out = out;
     // behind the projection on the stream: its split sums in the workspace are done with
@@ -234,6 +345,14 @@ void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const vo
     p.rank_pad = int(ceil_div(l.rank, 16) * 16);
     p.splits = lora_splits(ctx, rows, c_in);
     p.chunk = int(ceil_div(ceil_div(c_in, p.splits), 64) * 64);
+    if (few) {
+        const bool ah = l.type == kF16;
+        if (wt == kF16 && ah) run_few<_Float16, _Float16>(ctx, p, weight, bias, residual);
+        else if (wt == kF16) run_few<_Float16, float>(ctx, p, weight, bias, residual);
+        else if (ah) run_few<float, _Float16>(ctx, p, weight, bias, residual);
+        else run_few<float, float>(ctx, p, weight, bias, residual);
+        return;
+    }
     if (l.type == kF16) run<_Float16>(ctx, p);
     else run<float>(ctx, p);
 }

@@ -89,7 +89,8 @@ def test_against_the_formula(ctx, case, f16, extra, fast):
 
 @pytest.mark.parametrize("case", [CASES[1], CASES[3], CASES[5]])
 def test_rows_without_adapter_are_the_projection(ctx, case):
-    """Slots below 0 and at or above the number of adapters: the bits of the projection alone."""
+    """Slots below 0 and at or above the number of adapters: the projection alone (few rows have a
+    product of their own, so within its tolerance, not in bits)."""
     n, h, w, ci, co, _, slots, pixel = case
     d = make(ctx, case, True)
     conv, ad = layer(ctx, case, d, True)
@@ -99,7 +100,10 @@ def test_rows_without_adapter_are_the_projection(ctx, case):
     conv.forward_adapted(x, ad, E.DeviceArray.from_numpy(ctx, slot), out)
     rows = np.repeat(slot, 1 if pixel else h * w).reshape(n, h, w)
     none = (rows < 0) | (rows >= slots)
-    assert none.any() and np.array_equal(out.numpy()[none], plain.numpy()[none])
+    _, base, _ = reference(d["x"].reshape(-1, ci), d["w"], d["bias"], None, d["a"], d["b"], d["scale"],
+                           np.full(d["slot"].size, -1), 1 if pixel else h * w)
+    assert none.any()
+    assert np.all((np.abs(out.numpy() - plain.numpy()) <= 1e-5 * base.reshape(n, h, w, co))[none])
     assert not np.array_equal(out.numpy(), plain.numpy())
 
 
