@@ -63,7 +63,10 @@ void block_attention(Context &ctx, const BlockAttention &b, WeightType type, voi
                      vec_rows(b.v.p, b.v.ld, s.d, size) && vec_rows(b.out, b.ld_out, s.d, size);
     battn::Args a{};
     a.q = b.q.p, a.k = b.k.p, a.v = b.v.p, a.out = b.out;
-    a.ldq = b.q.ld, a.ldk = b.k.ld, a.ldv = b.v.ld, a.ldo = b.ld_out;
+    a.ldq = b.q.ld, a.ldo = b.ld_out;
+    MH_REQUIRE(b.k.ld * size < (int64_t(1) << 32) && b.v.ld * size < (int64_t(1) << 32),
+               "block_attention: rows of keys or values 4 GiB apart or more");
+    a.ldk = uint32_t(b.k.ld * size), a.ldv = uint32_t(b.v.ld * size);
     a.blocks = b.blocks, a.q_len = s.q_len, a.kv_len = s.kv_len;
     a.part = p.splits > 1 ? static_cast<float *>(scratch) : nullptr;
     a.c = b.scale * 1.44269504088896340736f;

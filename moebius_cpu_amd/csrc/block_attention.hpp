@@ -33,7 +33,8 @@ typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 struct Args {
     const void *q, *k, *v;
     void *out;
-    int64_t ldq, ldk, ldv, ldo;
+    int64_t ldq, ldo;
+    uint32_t ldk, ldv;  // bytes
     const int32_t *blocks, *q_len, *kv_len;
     float *part;  // split partials, NULL: none
     float c;      // scale . log2 e
@@ -98,11 +99,16 @@ struct Run8 {
         }
         return h;
     }
-    __device__ __forceinline__ bool finite() const {
-        bool ok = true;
+    // Zeros in the place of values that are not finite; whether there were any.
+    __device__ __forceinline__ bool clean() {
+        bool any = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ok = ok && __builtin_fabsf(float(at(i))) < __builtin_huge_valf();
-        return ok;
+        for (int i = 0; i < 8; ++i) {
+            const bool ok = __builtin_fabsf(float(at(i))) < __builtin_huge_valf();
+            any = any || !ok;
+            v[i / (8 / kN)][i % (8 / kN)] = ok ? at(i) : T(0);
+        }
+        return any;
     }
 };
 
@@ -123,14 +129,14 @@ __device__ __forceinline__ halfx8 read_vt(const char *v, int lane) {
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
 
 template <typename T, bool HALF, bool VEC, int DT, int WR>
-__global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 : 1) void block_attention_kernel(Args a) {
+__global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_kernel(Args a) {
     using L = Tiling<HALF, DT, WR>;
     constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP;
     constexpr int NT = 64 * WR;                       // threads that stage one tile
     constexpr int KU = (KT * DP / 8 + NT - 1) / NT;   // runs of 8 channels of K, and of V, per thread
     extern __shared__ __align__(16) char smem[];
     __shared__ int32_t list[kMaxTop];  // first token of every block to visit
-    __shared__ int list_n, bad[WK];
+    __shared__ int list_n, bad;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR, ttid = tid % NT;
@@ -178,8 +184,7 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
             if (ok) list[n + __popcll(all & ((uint64_t(1) << lane) - 1))] = e << a.kb_log;
             n += __popcll(all);
         }
-        if (lane == 0) list_n = n;
-        if (lane < WK) bad[lane] = 0;
+        if (lane == 0) list_n = n, bad = 0;
     }
 
     // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of chunk c (f32: 8 c + 4 h .. + 3).
@@ -208,7 +213,8 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
             }
     }
     const int lim = a.causal ? min(kv_len, off + qi + 1) : kv_len;  // this lane's row sees tokens below it
-    // the tokens that every row of the wave sees
+    // the tokens below which every row of the workgroup, and of the wave, sees all
+    const int lim_first = a.causal ? min(kv_len, off + i0 + r0 / a.g + 1) : kv_len;
     const int lim_all = a.causal ? min(kv_len, off + i0 + (r0 + wr * 32) / a.g + 1) : kv_len;
 
     char *const kst = smem + wk * L::kStage, *const vst = kst + L::kKBytes;
@@ -231,22 +237,35 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
     const int l0 = min(split * share, n_all), l1 = min(l0 + share, n_all);
     const int keys = (l1 - l0) << a.kb_log;
     const int tiles = (keys + KT - 1) / KT;
-    const T *kp = static_cast<const T *>(a.k) + int64_t(item) * a.kv_tokens * a.ldk + int64_t(hk) * a.d;
-    const T *vp = static_cast<const T *>(a.v) + int64_t(item) * a.kv_tokens * a.ldv + int64_t(hk) * a.d;
+    const char *kp = static_cast<const char *>(a.k) + uint64_t(item) * a.kv_tokens * a.ldk + int64_t(hk) * a.d * sizeof(T);
+    const char *vp = static_cast<const char *>(a.v) + uint64_t(item) * a.kv_tokens * a.ldv + int64_t(hk) * a.d * sizeof(T);
 
     // Token of key j of this split; past its end none. Loads of tokens there are not
     // (behind the list or kv_len) read the last one instead and are not used.
-    auto token = [&](int j) { return j < keys ? list[l0 + (j >> a.kb_log)] + (j & (kb - 1)) : 0x7fffffff; };
+    auto token = [&](int j) {
+        const int t = list[l0 + (min(j, keys - 1) >> a.kb_log)] + (j & (kb - 1));
+        return j < keys ? t : 0x7fffffff;
+    };
+    // The next tile's runs, their tokens, and whether a row of the wave does not see some of
+    // its keys. Runs behind d are loaded from the last channels and not staged.
     Run8<T> kr[KU], vr[KU];
+    int tok[KU];
+    bool masked_next = false;
+    constexpr bool kWhole = KT * (DP / 8) % NT == 0;
     auto fetch = [&](int tile) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
-            if (j < KT && ch < a.d) {
-                const int64_t t = min(token(tile * KT + j), kv_len - 1);
-                kr[u].template load<VEC>(kp + t * a.ldk + ch, a.d - ch);
-                vr[u].template load<VEC>(vp + t * a.ldv + ch, a.d - ch);
-            }
+            const int j = (ttid + u * NT) / (DP / 8);
+            tok[u] = kWhole || j < KT ? token(tile * KT + j) : 0x7fffffff;
+        }
+        masked_next = !__all(token(tile * KT + lane % KT) < lim_all);
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int i = ttid + u * NT, ch = i % (DP / 8) * 8;
+            const uint32_t t = min(tok[u], kv_len - 1);
+            const int c = VEC ? min(ch, a.d - 8) : ch;
+            kr[u].template load<VEC>(reinterpret_cast<const T *>(kp + c * int(sizeof(T)) + uint64_t(t) * a.ldk), a.d - c);
+            vr[u].template load<VEC>(reinterpret_cast<const T *>(vp + c * int(sizeof(T)) + uint64_t(t) * a.ldv), a.d - c);
         }
     };
     auto put = [&](char *p, const Run8<T> &r) {
@@ -259,14 +278,18 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
                                                             float(r.at(4 * e + 2)), float(r.at(4 * e + 3))};
         }
     };
-    auto stage = [&](int tile) {
+    auto stage = [&]() {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
             const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
-            if (j < KT && ch < a.d) {
-                // values of tokens that there are not: zeros, whatever lies there
-                if (token(tile * KT + j) >= kv_len) vr[u].zero();
-                if (a.causal && !vr[u].finite()) bad[wk] = 1;
+            if (__any(tok[u] >= lim_first)) {
+                // Values of tokens that there are not: zeros, whatever lies there. Values that
+                // are not finite, of tokens that some row does not see (0 times them is NaN in
+                // the products): zeros too, they are added at the end.
+                if (tok[u] >= kv_len) vr[u].zero();
+                else if (tok[u] >= lim_first && vr[u].clean()) bad = 1;
+            }
+            if ((kWhole || j < KT) && ch < a.d) {
                 put(kst + (j * L::kKS + ch) * L::kES, kr[u]);
                 put(vst + (j * L::kVS + ch) * L::kES, vr[u]);
             }
@@ -286,7 +309,8 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
         const int tile = s * WK + wk;
         const bool live = tile < tiles;
         if (s) __syncthreads();  // the tile before has been read
-        if (live) stage(tile);
+        if (live) stage();
+        const bool masked = masked_next;
         __syncthreads();
         if (tile + WK < tiles) fetch(tile + WK);
         if (!live) continue;
@@ -300,23 +324,19 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
                 const char *p = kst + ((b * 32 + col) * L::kKS + h * 8) * 2;
 #pragma unroll
                 for (int c = 0; c < DT * 2; ++c)
-                    if (c * 16 < a.d)
-                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const halfx8 *>(p + c * 32), qh[c],
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const halfx8 *>(p + c * 32), qh[c],
                                                                        sc[b], 0, 0, 0);
             } else {
                 const float *p = reinterpret_cast<const float *>(kst) + (b * 32 + col) * L::kKS + h * 4;
 #pragma unroll
-                for (int c = 0; c < DT * 4; ++c)
-                    if (c * 8 < a.d) {
-                        const floatx4 kv = *reinterpret_cast<const floatx4 *>(p + c * 8);
+                for (int c = 0; c < DT * 4; ++c) {
+                    const floatx4 kv = *reinterpret_cast<const floatx4 *>(p + c * 8);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            sc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[j], qf[c * 4 + j], sc[b], 0, 0, 0);
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[j], qf[c * 4 + j], sc[b], 0, 0, 0);
+                }
             }
         }
-        // Keys that some row of the wave does not see.
-        const bool masked = !__all(token(tile * KT + lane % KT) < lim_all);
         if (masked) {
 #pragma unroll
             for (int b = 0; b < SUB; ++b)
@@ -354,30 +374,7 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
                 sum += sc[b][i];
             }
         l += sum;
-        if (masked && bad[wk]) {
-            // A value that is not finite may lie at a key that a row does not see, and 0 times
-            // it is NaN in the products: row by row, over the keys the row sees.
-            for (int n = 0; n < SUB * 32; ++n) {
-                float p = 0.0f;  // register n / 2 of the lane (even n) or of its other half
-#pragma unroll
-                for (int b = 0; b < SUB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) p = n / 2 == b * 16 + i ? sc[b][i] : p;
-                const float other = __shfl_xor(p, 32);
-                if (n & 1) p = other;
-                const int j = n / 32 * 32 + acc_row(n / 2 % 16, h ^ (n & 1));
-                const bool sees = token(tile * KT + j) < lim;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int dim = t * 32 + acc_row(r, h);
-                        typedef std::conditional_t<HALF, _Float16, float> E;
-                        const float v = float(reinterpret_cast<const E *>(vst)[j * L::kVS + dim]);
-                        if (sees) o[t][r] = __builtin_fmaf(p, v, o[t][r]);
-                    }
-            }
-        } else if constexpr (HALF) {
+        if constexpr (HALF) {
 #pragma unroll
             for (int b = 0; b < SUB; ++b)
 #pragma unroll
@@ -434,6 +431,21 @@ __global__ __launch_bounds__(256, HALF && (DT <= 3 || (DT == 4 && WR > 1)) ? 2 :
         }
         if (wk) return;
     }
+    // The values that were staged as zeros because they are not finite, for the rows that see them.
+    if (bad)
+        for (int j = 0; j < keys; ++j) {
+            const int t = token(j);
+            if (t < lim_first || t >= lim) continue;
+            const T *v = reinterpret_cast<const T *>(vp + uint64_t(uint32_t(t)) * a.ldv);
+#pragma unroll
+            for (int x = 0; x < DT; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int ch = x * 32 + acc_row(i, h);
+                    const float f = ch < a.d ? float(v[ch]) : 0.0f;
+                    if (!(__builtin_fabsf(f) < __builtin_huge_valf())) o[x][i] += f;
+                }
+        }
     if (a.part) {
         float *p = a.part + (int64_t(work) * WR + wr) * part_floats(DT);
 #pragma unroll
@@ -488,9 +500,11 @@ __global__ __launch_bounds__(64) void block_attention_join_kernel(Args a) {
     constexpr int PF = part_floats(DT);
     const float *p = a.part + (int64_t(base) * a.splits * WR + wr) * PF;
     float m = kNegInf;
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) m = __builtin_fmaxf(m, p[int64_t(s) * WR * PF + DT * 16 * 64 + lane]);
     const float mu = m == kNegInf ? 0.0f : m;
     float l = 0.0f, o[16] = {};
+#pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
         const float *ps = p + int64_t(s) * WR * PF;
         const float f = __builtin_amdgcn_exp2f(ps[DT * 16 * 64 + lane] - mu);
