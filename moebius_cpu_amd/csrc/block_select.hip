@@ -98,8 +98,11 @@ typedef double doublex4 __attribute__((ext_vector_type(4)));
 
 // One workgroup per (item, key head, TQ blocks of queries); W, MW: the runs in which the
 // queries and the means are read.
+constexpr int kSelWaves = 8;
+constexpr int kRegKeys = 8;  // keys per lane that the search holds in registers
+
 template <typename T, int W, int MW, int TQ>
-__global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
+__global__ __launch_bounds__(64 * kSelWaves) void block_select_kernel(SelectArgs a) {
     extern __shared__ uint64_t keys[];  // [TQ][nk]
     constexpr int kQS = kMaxHeadDim + 20;  // rows of a read on distinct banks, sixteen zeros behind d
     __shared__ __align__(16) float qm[TQ][kQS];
@@ -109,23 +112,24 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     const int q_len = clamp_len(a.q_len, item, a.q_tokens), kv_len = clamp_len(a.kv_len, item, a.kv_tokens);
     const int b0 = tile * TQ;
 
-    // Mean query of each block: a wave per block, lanes over (row group, run of channels).
+    // Mean query of each block: kParts waves per block, lanes over (row group, run of channels).
+    constexpr int kParts = kSelWaves / TQ;
+    __shared__ double part[kSelWaves][kMaxHeadDim];
     const int runs = a.d / W;
     int span = 1;  // lanes per row: the next power of two
     while (span < runs && span < 64) span *= 2;
     const int groups = 64 / span, cl = lane % span, rg = lane / span;
     // Zeros behind d, which the products' last run of sixteen reads.
-    for (int i = tid; i < TQ * 16; i += 256)
-        qm[i / 16][a.d + i % 16] = 0.0f;
-    for (int t = wave; t < TQ; t += 4) {
-        const int i0 = (b0 + t) * a.qb, i1 = min(i0 + a.qb, q_len);
-        const int rows = max(i1 - i0, 0) * a.g;
+    for (int i = tid; i < TQ * 16; i += 64 * kSelWaves) qm[i / 16][a.d + i % 16] = 0.0f;
+    {
+        const int t = wave / kParts, i0 = (b0 + t) * a.qb, i1 = min(i0 + a.qb, q_len);
+        const int rows = max(i1 - i0, 0) * a.g, step = groups * kParts;
         const T *base = static_cast<const T *>(a.q) + (int64_t(item) * a.q_tokens + i0) * a.ld + int64_t(hk) * a.g * a.d;
         for (int c0 = cl; c0 < ((runs + span - 1) / span) * span; c0 += span) {
             double sum[W] = {};
             if (c0 < runs) {
 #pragma unroll 8
-                for (int r = rg; r < rows; r += groups) {
+                for (int r = rg * kParts + wave % kParts; r < rows; r += step) {
                     const int i = r / a.g, e = r - i * a.g;
                     float v[W];
                     load_run<T, W>(base + int64_t(i) * a.ld + e * a.d + c0 * W, v);
@@ -138,8 +142,17 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
                 for (int k = 0; k < W; ++k) sum[k] += __shfl_xor(sum[k], m);
             if (rg == 0 && c0 < runs)
 #pragma unroll
-                for (int k = 0; k < W; ++k) qm[t][c0 * W + k] = rows ? float(sum[k] / double(rows)) : 0.0f;
+                for (int k = 0; k < W; ++k) part[wave][c0 * W + k] = sum[k];
         }
+    }
+    __syncthreads();
+    for (int i = tid; i < TQ * a.d; i += 64 * kSelWaves) {
+        const int t = i / a.d, c = i - t * a.d;
+        const int rows = max(min((b0 + t + 1) * a.qb, q_len) - (b0 + t) * a.qb, 0) * a.g;
+        double sum = 0;
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) sum += part[t * kParts + p][c];
+        qm[t][c] = rows ? float(sum / double(rows)) : 0.0f;
     }
     __syncthreads();
 
@@ -149,7 +162,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     const int seen_all = (kv_len + a.kb - 1) / a.kb;
     const int l16 = lane & 15, kg = lane >> 4;
     if constexpr (TQ == 1) {
-        for (int t0 = 0; t0 < seen_all; t0 += 16) {
+        for (int t0 = 0; t0 < seen_all; t0 += 4 * kSelWaves) {
             const int b = t0 + wave * 4 + kg;
             double s = 0;
             if (b < seen_all) {
@@ -166,7 +179,7 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
             if (b < seen_all && l16 == 0) keys[b] = order_key(s);
         }
     } else {
-        for (int t0 = wave * 16; t0 < seen_all; t0 += 64) {
+        for (int t0 = wave * 16; t0 < seen_all; t0 += 16 * kSelWaves) {
             const int b = min(t0 + l16, seen_all - 1);
             const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
             const float *q = qm[min(l16, TQ - 1)];
@@ -204,9 +217,8 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
     }
     __syncthreads();
 
-    for (int t = wave; t < TQ; t += 4) {
-        const int qb = b0 + t;
-        if (qb >= a.nq) break;
+    if (wave < TQ && b0 + wave < a.nq) {
+        const int t = wave, qb = b0 + t;
         int32_t *out = a.blocks + ((int64_t(item) * a.nq + qb) * a.hk + hk) * a.top;
         const int i0 = qb * a.qb, i1 = min(i0 + a.qb, q_len);
         int seen = i1 > i0 ? seen_all : 0, f0 = 0, f1 = 0;  // blocks f0 .. f1 - 1 come first
@@ -222,12 +234,26 @@ __global__ __launch_bounds__(256) void block_select_kernel(SelectArgs a) {
             __threadfence_block();
             uint64_t at = 0;  // the largest key with at least `top` keys at or above it
             int above = seen;
-            for (int bit = 63; bit >= 0 && above != a.top; --bit) {
-                const uint64_t cand = at | (uint64_t(1) << bit);
-                int n = 0;
-                for (int b = lane; b < (seen + 63) / 64 * 64; b += 64)
-                    n += __popcll(__ballot(b < seen && k[b] >= cand));
-                if (n >= a.top) at = cand, above = n;
+            if (seen <= 64 * kRegKeys) {  // keys in registers
+                uint64_t r[kRegKeys];
+#pragma unroll
+                for (int j = 0; j < kRegKeys; ++j) r[j] = lane + j * 64 < seen ? k[lane + j * 64] : 0;
+                for (int bit = 63; bit >= 0 && above != a.top; --bit) {
+                    const uint64_t cand = at | (uint64_t(1) << bit);
+                    int n = 0;
+#pragma unroll
+                    for (int j = 0; j < kRegKeys; ++j)
+                        if (j * 64 < seen) n += __popcll(__ballot(r[j] >= cand));
+                    if (n >= a.top) at = cand, above = n;
+                }
+            } else {
+                for (int bit = 63; bit >= 0 && above != a.top; --bit) {
+                    const uint64_t cand = at | (uint64_t(1) << bit);
+                    int n = 0;
+                    for (int b = lane; b < (seen + 63) / 64 * 64; b += 64)
+                        n += __popcll(__ballot(b < seen && k[b] >= cand));
+                    if (n >= a.top) at = cand, above = n;
+                }
             }
             // above == top: every key at or above; else the lower indices of those equal to it
             int greater = 0;
@@ -268,7 +294,7 @@ void select_w(Context &ctx, SelectArgs &a, int n) {
     const int64_t blocks = int64_t(n) * a.hk * a.tiles;
     MH_REQUIRE(blocks < (int64_t(1) << 31), "block_select: too many blocks of queries");
     const uint32_t lds = uint32_t(tq) * a.nk * 8;
-    const dim3 grid{uint32_t(blocks)}, block{256};
+    const dim3 grid{uint32_t(blocks)}, block{64 * kSelWaves};
     if (tq == 8) {
         block_select_kernel<T, W, MW, 8><<<grid, block, lds, ctx.stream>>>(a);
     } else if (tq == 4) {
