@@ -232,6 +232,8 @@ __global__ __launch_bounds__(512) void lora_row_project_kernel(LoraArgs p, const
     const int64_t r0 = int64_t(blockIdx.y) * 16;
     const W *wr = w + int64_t(min(c0 + r16, p.co - 1)) * p.ci;
     const float *x = p.x + min(r0 + r16, p.rows - 1) * p.ci;
+    const int s = slot_of(p, r0 + (tid >> 4));  // of the row that this thread finishes
+    const float scale = s >= 0 ? p.scale[s] : 0.0f;
     floatx4 acc = {0, 0, 0, 0};
     for (int k0 = __builtin_amdgcn_readfirstlane(wave) * 32; k0 < p.ci; k0 += 256 * kRowUnroll) {
         floatx4 wv[kRowUnroll][2], xv[kRowUnroll][2];
@@ -265,13 +267,27 @@ __global__ __launch_bounds__(512) void lora_row_project_kernel(LoraArgs p, const
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += part[i][e][l];
     v += sum;
-    const int s = slot_of(p, row);
     if (s >= 0) {
         const T *b = static_cast<const T *>(p.b) + (int64_t(s) * p.co + c) * p.rank;
         const float *t = p.t + row * p.rank_pad;
         float y = 0.0f;
-        for (int k = 0; k < p.rank; ++k) y = __builtin_fmaf(t[k], float(b[k]), y);
-        v = __builtin_fmaf(p.scale[s], y, v);
+        if (p.rank % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % (4 * sizeof(T)) == 0) {
+            for (int k = 0; k < p.rank; k += 16) {
+                floatx4 bv[4], tv[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    bv[u] = load4<true>(b, k + 4 * u, p.rank);
+                    tv[u] = load4<true>(t, k + 4 * u, p.rank);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y = __builtin_fmaf(tv[u][i], bv[u][i], y);
+            }
+        } else {
+            for (int k = 0; k < p.rank; ++k) y = __builtin_fmaf(t[k], float(b[k]), y);
+        }
+        v = __builtin_fmaf(scale, y, v);
     }
     p.out[row * p.co + c] = v;
 }
