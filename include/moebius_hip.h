@@ -530,8 +530,9 @@ int32_t mh_block_means(MhContext *ctx, const void *x, uint32_t dtype, uint32_t n
 int32_t mh_block_select(MhContext *ctx, const void *q, uint32_t dtype, uint64_t ld_q, const MhBlockShape *shape,
                         const float *k_means, int32_t *blocks);
 
-/* Scratch of mh_block_attention for this shape on this context (0: none needed). */
-int32_t mh_block_attention_scratch(MhContext *ctx, const MhBlockShape *shape, uint64_t *bytes);
+/* Scratch of mh_block_attention for tensors of this type and shape on this context at
+ * its present precision (0: none needed). */
+int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlockShape *shape, uint64_t *bytes);
 
 /* out [n][q_tokens][heads_q][d] = softmax(scale q . k) v over the keys of the listed
  * blocks (as mh_block_select writes them, in any order: indices outside the item's

@@ -185,5 +185,5 @@ def block_attention_scratch(q: Heads, k: Heads, blocks: DeviceArray, q_block: in
     """Bytes of scratch that block_attention needs for these shapes."""
     s = _shape(q, k.tokens, k.heads, blocks, q_block, kv_block, False, None, None)
     n = ctypes.c_uint64()
-    check(lib().mh_block_attention_scratch(q.ctx.h, ctypes.byref(s), ctypes.byref(n)))
+    check(lib().mh_block_attention_scratch(q.ctx.h, q.code, ctypes.byref(s), ctypes.byref(n)))
     return int(n.value)

@@ -81,9 +81,8 @@ struct BlockAttention {
     int64_t ld_out = 0;
     const int32_t *blocks = nullptr;
     float scale = 0;
-    bool half = false;  // products of f16 operands; false: of f32 ones (f32 storage only)
 };
-size_t block_attention_scratch(const Context &ctx, const BlockShape &s);
+size_t block_attention_scratch(const Context &ctx, const BlockShape &s, WeightType type);
 void block_attention(Context &ctx, const BlockAttention &a, WeightType type, void *scratch);
 
 // ---- low-rank adapters beside a shared projection (lora.hip)

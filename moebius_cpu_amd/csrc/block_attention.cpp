@@ -13,7 +13,7 @@ bool vec_rows(const void *p, int64_t ld, int d, int size) {
 // 32-channel tiles of the instantiated kernels that hold a head of d channels.
 int head_tiles(int d, bool vec) {
     const int t = int(ceil_div(d, 32));
-    if (!vec) return t <= 4 ? 4 : 8;
+    if (!vec) return t <= 4 ? 4 : t == 5 ? 5 : 8;
     return t <= 5 ? t : 8;
 }
 
@@ -27,40 +27,66 @@ int row_waves(const BlockShape &s) {
 struct Plan {
     int wr, row_tiles, splits;
     int64_t items;  // workgroups without the splits
+    bool split;     // f32 operands as two f16 parts
 };
 
 // The list is split over workgroups where the rows alone leave CUs idle, into shares of
-// at least 128 keys.
-Plan plan(const Context &ctx, const BlockShape &s) {
+// at least 128 keys. f32 products are split where the keys and values, which that reads and
+// writes once, are then read at least kSplitReuse times by waves full of rows.
+constexpr int64_t kSplitReuse = 2;
+Plan plan(const Context &ctx, const BlockShape &s, WeightType type, bool half) {
     Plan p;
     p.wr = row_waves(s);
     const int64_t rows = int64_t(std::min(s.q_block, s.q_tokens)) * (s.heads_q / s.heads_kv);
     p.row_tiles = int(ceil_div(rows, p.wr * 32));
     p.items = int64_t(s.n) * s.heads_kv * s.q_blocks() * p.row_tiles;
     const int64_t keys = std::min<int64_t>(int64_t(s.top) * s.kv_block, s.kv_tokens);
-    int64_t splits = p.items >= ctx.cu_count ? 1 : std::min<int64_t>(2 * ctx.cu_count / std::max<int64_t>(p.items, 1), keys / 128);
+    const int64_t splits =
+        p.items >= ctx.cu_count ? 1 : std::min<int64_t>(2 * ctx.cu_count / std::max<int64_t>(p.items, 1), keys / 128);
     p.splits = int(std::max<int64_t>(1, std::min<int64_t>(splits, 64)));
+    p.split = type == kF32 && !half && s.kv_tokens > 0 && battn::split_fits(p.wr, head_tiles(s.d, false)) &&
+              battn::split_fits(p.wr, head_tiles(s.d, true)) &&
+              int64_t(s.q_blocks()) * p.row_tiles * keys >= kSplitReuse * s.kv_tokens;
     return p;
+}
+
+// Scratch: the splits' partial sums, then the parts of keys and of values and their scales.
+struct Layout {
+    size_t part = 0, parts = 0, meta = 0;  // bytes of each (parts: of keys, and of values)
+    size_t total() const { return part + 2 * parts + meta; }
+};
+
+Layout layout(const BlockShape &s, const Plan &p) {
+    auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+    Layout l;
+    if (p.splits > 1)  // the most that any alignment of these sizes needs
+        l.part = up(size_t(p.items) * p.splits * p.wr * battn::part_floats(head_tiles(s.d, false)) * sizeof(float));
+    if (p.split) {
+        const size_t rows = size_t(s.n) * s.kv_blocks() * s.kv_block * s.heads_kv;
+        l.parts = up(rows * 2 * size_t(ceil_div(s.d, 8) * 8) * 2);
+        l.meta = up(size_t(s.n) * s.kv_blocks() * s.heads_kv * sizeof(battn::SplitMeta));
+    }
+    return l;
 }
 
 }  // namespace
 
-size_t block_attention_scratch(const Context &ctx, const BlockShape &s) {
+size_t block_attention_scratch(const Context &ctx, const BlockShape &s, WeightType type) {
     if (!s.n || !s.q_tokens) return 0;
-    const Plan p = plan(ctx, s);
-    if (p.splits == 1) return 0;
-    // the most that any storage and alignment of these sizes needs
-    return size_t(p.items) * p.splits * p.wr * battn::part_floats(head_tiles(s.d, false)) * sizeof(float);
+    return layout(s, plan(ctx, s, type, ctx.precision == Precision::Fast)).total();
 }
 
 void block_attention(Context &ctx, const BlockAttention &b, WeightType type, void *scratch) {
     const BlockShape &s = b.s;
     if (!s.n || !s.q_tokens) return;
-    const Plan p = plan(ctx, s);
+    const bool half = type == kF16 || ctx.precision == Precision::Fast;
+    const Plan p = plan(ctx, s, type, half);
+    const Layout l = layout(s, p);
     MH_REQUIRE(p.items * p.splits < (int64_t(1) << 30), "block_attention: too many blocks of queries");
     const int size = type == kF16 ? 2 : 4;
-    const bool vec = vec_rows(b.q.p, b.q.ld, s.d, size) && vec_rows(b.k.p, b.k.ld, s.d, size) &&
-                     vec_rows(b.v.p, b.v.ld, s.d, size) && vec_rows(b.out, b.ld_out, s.d, size);
+    const bool vec_q = vec_rows(b.q.p, b.q.ld, s.d, size) && vec_rows(b.out, b.ld_out, s.d, size);
+    const bool vec = vec_q && (p.split || (vec_rows(b.k.p, b.k.ld, s.d, size) && vec_rows(b.v.p, b.v.ld, s.d, size)));
+    char *mem = static_cast<char *>(scratch);
     battn::Args a{};
     a.q = b.q.p, a.k = b.k.p, a.v = b.v.p, a.out = b.out;
     a.ldq = b.q.ld, a.ldo = b.ld_out;
@@ -68,16 +94,34 @@ void block_attention(Context &ctx, const BlockAttention &b, WeightType type, voi
                "block_attention: rows of keys or values 4 GiB apart or more");
     a.ldk = uint32_t(b.k.ld * size), a.ldv = uint32_t(b.v.ld * size);
     a.blocks = b.blocks, a.q_len = s.q_len, a.kv_len = s.kv_len;
-    a.part = p.splits > 1 ? static_cast<float *>(scratch) : nullptr;
+    a.part = p.splits > 1 ? reinterpret_cast<float *>(mem) : nullptr;
     a.c = b.scale * 1.44269504088896340736f;
     a.n = s.n, a.q_tokens = s.q_tokens, a.kv_tokens = s.kv_tokens, a.hk = s.heads_kv, a.g = s.heads_q / s.heads_kv;
     a.d = s.d, a.qb = s.q_block, a.nq = s.q_blocks(), a.top = s.top;
     while ((1 << a.kb_log) < s.kv_block) ++a.kb_log;
     a.row_tiles = p.row_tiles, a.splits = p.splits, a.work = int(p.items * p.splits), a.causal = s.causal;
+    a.dk = s.d, a.kv_rows = s.kv_tokens;
     const int dt = head_tiles(s.d, vec);
-    if (type == kF16) battn::launch_f16(ctx, a, p.wr, dt, vec);
-    else if (b.half) battn::launch_f32_half(ctx, a, p.wr, dt, vec);
-    else battn::launch_f32(ctx, a, p.wr, dt, vec);
+    if (p.split) {
+        a.dk = int(ceil_div(s.d, 8) * 8);
+        a.kv_rows = s.kv_blocks() * s.kv_block;
+        a.v0 = b.v.p, a.ldv0 = a.ldv;
+        char *kp = mem + l.part, *vp = kp + l.parts;
+        auto *meta = reinterpret_cast<battn::SplitMeta *>(vp + l.parts);
+        battn::split_kv(ctx, static_cast<const float *>(b.k.p), static_cast<const float *>(b.v.p), b.k.ld, b.v.ld, s.n,
+                        s.kv_tokens, s.heads_kv, s.d, a.dk, s.kv_block, s.kv_len, kp, vp, meta);
+        a.k = kp, a.v = vp, a.meta = meta;
+        const uint64_t row = uint64_t(s.heads_kv) * 2 * a.dk * 2;
+        MH_REQUIRE(row < (uint64_t(1) << 32), "block_attention: rows of keys or values of 4 GiB or more");
+        a.ldk = a.ldv = uint32_t(row);
+        battn::launch_split(ctx, a, p.wr, dt, vec);
+    } else if (type == kF16) {
+        battn::launch_f16(ctx, a, p.wr, dt, vec);
+    } else if (half) {
+        battn::launch_f32_half(ctx, a, p.wr, dt, vec);
+    } else {
+        battn::launch_f32(ctx, a, p.wr, dt, vec);
+    }
 }
 
 }  // namespace mh

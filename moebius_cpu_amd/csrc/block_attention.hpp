@@ -12,10 +12,13 @@
 // 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3, so V^T is read with its keys in that order. WR
 // waves share a tile of keys, WK groups of waves take every WK-th tile and join in LDS.
 //
-// Half: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated as the
+// kHalf: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated as the
 // f16 GEMMs round operands; P rounded to f16, at most 1 with a relative 2^-11 each, which
-// a sum over keys averages. Else f32 products (v_mfma_f32_32x32x2_f32). Scores, maxima,
-// sums and outputs are f32 in both.
+// a sum over keys averages. kF32: f32 products (v_mfma_f32_32x32x2_f32, an eighth of the
+// rate). kSplit: each f32 operand as two f16 parts, x = hi + lo to 2^-24, and the three
+// products above 2^-24 of theirs; queries scaled by a power of two per row, keys and values
+// per block (split_kv), probabilities by 2^14, so that the parts keep all bits of values down
+// to 2^-18 of the largest. Scores, maxima, sums and outputs are f32 in all.
 #pragma once
 
 #include <type_traits>
@@ -30,8 +33,18 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 
+// Products of f16 operands; of f32 ones on the f32 instructions; of f32 ones as three
+// products of operands split in two f16 parts.
+enum Mode { kHalf, kF32, kSplit };
+
+// A block's scales where its keys and values are split: largest exponents, and whether
+// values that are not finite were left out.
+struct SplitMeta {
+    int k_exp, v_exp, v_bad, pad;
+};
+
 struct Args {
-    const void *q, *k, *v;
+    const void *q, *k, *v;  // kSplit: k, v as written by split_kv, rows of two parts of dk values
     void *out;
     int64_t ldq, ldo;
     uint32_t ldk, ldv;  // bytes
@@ -40,21 +53,37 @@ struct Args {
     float c;      // scale . log2 e
     int n, q_tokens, kv_tokens, hk, g, d, qb, kb_log, nq, top, row_tiles, splits, work;
     bool causal;
+    int dk;       // values of a staged row's part: d, or d rounded up to 8 (kSplit)
+    int kv_rows;  // rows per item of k and v
+    const void *v0;        // kSplit: the values themselves, rows ldv0 bytes apart, heads of d
+    uint32_t ldv0;
+    const SplitMeta *meta;  // [n][blocks][hk]
 };
+
+constexpr int kSplitExp = 14;  // split operands are scaled to a largest value of 2^14 .. 2^15
+
+// x 2^e in two f16 parts, x = hi + lo to 2^-24 of it (and 2^-40 of the largest value that e
+// was taken from); a value that is not finite is all in hi.
+__device__ __forceinline__ void split2(float x, int e, _Float16 &hi, _Float16 &lo) {
+    const float y = ldexpf(x, e);
+    hi = static_cast<_Float16>(y);
+    const float r = y - float(hi);
+    lo = static_cast<_Float16>(__builtin_fabsf(y) < __builtin_huge_valf() ? r : 0.0f);
+}
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // Floats of one wave's partial: the sums of DT x 16 registers and the row's maximum and sum.
 constexpr int part_floats(int dt) { return (dt * 16 + 2) * 64; }
 
-template <bool HALF, int DT, int WR>
+template <int MODE, int DT, int WR>
 struct Tiling {
-    static constexpr int kDP = DT * 32;
-    static constexpr int kKT = HALF && (DT <= 2 ? WR >= 2 : DT <= 4 && WR == 4) ? 64 : 32;  // keys per tile
-    static constexpr int kES = HALF ? 2 : 4;              // bytes of a staged value
+    static constexpr int kDP = DT * 32, kCols = MODE == kSplit ? 2 * kDP : kDP;
+    static constexpr int kKT = MODE == kHalf && (DT <= 2 ? WR >= 2 : DT <= 4 && WR == 4) ? 64 : 32;  // keys per tile
+    static constexpr int kES = MODE == kF32 ? 4 : 2;  // bytes of a staged value
     // staged rows (values), padded so that the rows of a read lie on distinct banks
-    static constexpr int kKS = kDP + (HALF ? 8 : 4);
-    static constexpr int kVS = HALF ? kDP + (kDP % 64 ? 0 : 32) : kDP + 8;
+    static constexpr int kKS = kCols + (MODE == kF32 ? 4 : 8);
+    static constexpr int kVS = MODE == kF32 ? kDP + 8 : kCols + (kCols % 64 ? 0 : 32);
     static constexpr int kKBytes = kKT * kKS * kES, kVBytes = kKT * kVS * kES;
     static constexpr int kStage = kKBytes + kVBytes;      // one key group's tile
     // key groups: four waves together, fewer where their tiles exceed the LDS of a CU (160 KiB)
@@ -128,15 +157,18 @@ __device__ __forceinline__ halfx8 read_vt(const char *v, int lane) {
 // Key of accumulator register i in lane half h (32 x 32 results: row of the tile).
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
 
-template <typename T, bool HALF, bool VEC, int DT, int WR>
-__global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_kernel(Args a) {
-    using L = Tiling<HALF, DT, WR>;
-    constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP;
-    constexpr int NT = 64 * WR;                       // threads that stage one tile
-    constexpr int KU = (KT * DP / 8 + NT - 1) / NT;   // runs of 8 channels of K, and of V, per thread
+template <typename T, int MODE, bool VEC, int DT, int WR>
+__global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_attention_kernel(Args a) {
+    using L = Tiling<MODE, DT, WR>;
+    typedef std::conditional_t<MODE == kSplit, _Float16, T> S;  // k and v
+    constexpr bool SPLIT = MODE == kSplit, HALF = MODE != kF32, KVEC = VEC || SPLIT;
+    constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP, RUNS = L::kCols / 8;
+    constexpr int NT = 64 * WR;                      // threads that stage one tile
+    constexpr int KU = (KT * RUNS + NT - 1) / NT;    // runs of 8 channels of K, and of V, per thread
     extern __shared__ __align__(16) char smem[];
     __shared__ int32_t list[kMaxTop];  // first token of every block to visit
-    __shared__ int list_n, bad;
+    __shared__ float k_scale[SPLIT ? kMaxTop : 1], v_scale[SPLIT ? kMaxTop : 1];
+    __shared__ int list_n, bad, v_exp;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR, ttid = tid % NT;
@@ -185,6 +217,24 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
             n += __popcll(all);
         }
         if (lane == 0) list_n = n, bad = 0;
+        if constexpr (SPLIT) {
+            // Powers of two that the blocks' parts were scaled by, the values' against the largest.
+            __threadfence_block();
+            const SplitMeta *meta = a.meta + (int64_t(item) * (a.kv_rows >> a.kb_log)) * a.hk + hk;
+            int top = -1000;
+            bool any = false;
+            for (int i = lane; i < n; i += 64) {
+                const SplitMeta s = meta[int64_t(list[i] >> a.kb_log) * a.hk];
+                top = max(top, s.v_exp);
+                any = any || s.v_bad;
+                k_scale[i] = ldexpf(1.0f, s.k_exp - kSplitExp);
+            }
+            for (int x = 32; x; x >>= 1) top = max(top, __shfl_xor(top, x));
+            for (int i = lane; i < n; i += 64)
+                v_scale[i] = ldexpf(1.0f, meta[int64_t(list[i] >> a.kb_log) * a.hk].v_exp - top + kSplitExp);
+            any = __any(any);
+            if (lane == 0) v_exp = top, bad = any;
+        }
     }
 
     // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of chunk c (f32: 8 c + 4 h .. + 3).
@@ -192,9 +242,35 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
     const bool row_ok = row < rows;
     const int qi = i0 + (row_ok ? row : 0) / a.g, qe = hk * a.g + (row_ok ? row : 0) % a.g;
     const T *qp = static_cast<const T *>(a.q) + (int64_t(item) * a.q_tokens + qi) * a.ldq + int64_t(qe) * a.d;
-    halfx8 qh[HALF ? DT * 2 : 1];
+    halfx8 qh[HALF ? DT * 2 : 1], ql[SPLIT ? DT * 2 : 1];
     float qf[HALF ? 1 : DT * 16];
-    if constexpr (HALF) {
+    float cq = a.c;  // what turns a product into a score
+    if constexpr (SPLIT) {
+        Run8<T> r[DT * 2];
+        float mx = 0.0f;
+#pragma unroll
+        for (int c = 0; c < DT * 2; ++c) {
+            const int ch = c * 16 + h * 8;
+            r[c].zero();
+            if (ch < a.d) r[c].template load<VEC>(qp + ch, a.d - ch);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = __builtin_fabsf(float(r[c].at(i)));
+                mx = v < __builtin_huge_valf() ? __builtin_fmaxf(mx, v) : mx;
+            }
+        }
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+        const int e = mx == 0.0f ? 0 : __builtin_amdgcn_frexp_expf(mx) - 1;
+        cq = ldexpf(a.c, e - kSplitExp);
+#pragma unroll
+        for (int c = 0; c < DT * 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                _Float16 hi, lo;
+                split2(float(r[c].at(i)), kSplitExp - e, hi, lo);
+                qh[c][i] = hi, ql[c][i] = lo;
+            }
+    } else if constexpr (HALF) {
 #pragma unroll
         for (int c = 0; c < DT * 2; ++c) {
             const int ch = c * 16 + h * 8;
@@ -219,13 +295,13 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
 
     char *const kst = smem + wk * L::kStage, *const vst = kst + L::kKBytes;
     // Channels behind d of the staged keys: zeros, which the loads never overwrite.
-    if (a.d < DP)
-        for (int i = ttid; i < KT * (DP / 8); i += NT) {
+    if (a.dk < DP)
+        for (int i = ttid; i < KT * RUNS; i += NT) {
             const int ch = i % (DP / 8) * 8;
-            if (ch + 8 > a.d) {
-                char *p = kst + (i / (DP / 8) * L::kKS + ch) * L::kES;
+            if (ch + 8 > a.dk) {
+                char *p = kst + (i / RUNS * L::kKS + i % RUNS * 8) * L::kES;
                 reinterpret_cast<floatx4 *>(p)[0] = floatx4{0, 0, 0, 0};
-                if constexpr (!HALF) reinterpret_cast<floatx4 *>(p)[1] = floatx4{0, 0, 0, 0};
+                if constexpr (L::kES == 4) reinterpret_cast<floatx4 *>(p)[1] = floatx4{0, 0, 0, 0};
             }
         }
     __syncthreads();
@@ -237,8 +313,9 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
     const int l0 = min(split * share, n_all), l1 = min(l0 + share, n_all);
     const int keys = (l1 - l0) << a.kb_log;
     const int tiles = (keys + KT - 1) / KT;
-    const char *kp = static_cast<const char *>(a.k) + uint64_t(item) * a.kv_tokens * a.ldk + int64_t(hk) * a.d * sizeof(T);
-    const char *vp = static_cast<const char *>(a.v) + uint64_t(item) * a.kv_tokens * a.ldv + int64_t(hk) * a.d * sizeof(T);
+    const int64_t head = int64_t(hk) * (SPLIT ? 2 * a.dk : a.dk) * int64_t(sizeof(S));
+    const char *kp = static_cast<const char *>(a.k) + uint64_t(item) * a.kv_rows * a.ldk + head;
+    const char *vp = static_cast<const char *>(a.v) + uint64_t(item) * a.kv_rows * a.ldv + head;
 
     // Token of key j of this split; past its end none. Loads of tokens there are not
     // (behind the list or kv_len) read the last one instead and are not used.
@@ -248,27 +325,27 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
     };
     // The next tile's runs, their tokens, and whether a row of the wave does not see some of
     // its keys. Runs behind d are loaded from the last channels and not staged.
-    Run8<T> kr[KU], vr[KU];
+    Run8<S> kr[KU], vr[KU];
     int tok[KU];
     bool masked_next = false;
-    constexpr bool kWhole = KT * (DP / 8) % NT == 0;
+    constexpr bool kWhole = KT * RUNS % NT == 0;
     auto fetch = [&](int tile) {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int j = (ttid + u * NT) / (DP / 8);
+            const int j = (ttid + u * NT) / RUNS;
             tok[u] = kWhole || j < KT ? token(tile * KT + j) : 0x7fffffff;
         }
         masked_next = !__all(token(tile * KT + lane % KT) < lim_all);
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int i = ttid + u * NT, ch = i % (DP / 8) * 8;
+            const int run = (ttid + u * NT) % RUNS, ch = run % (DP / 8) * 8;
             const uint32_t t = min(tok[u], kv_len - 1);
-            const int c = VEC ? min(ch, a.d - 8) : ch;
-            kr[u].template load<VEC>(reinterpret_cast<const T *>(kp + c * int(sizeof(T)) + uint64_t(t) * a.ldk), a.d - c);
-            vr[u].template load<VEC>(reinterpret_cast<const T *>(vp + c * int(sizeof(T)) + uint64_t(t) * a.ldv), a.d - c);
+            const int c = (KVEC ? min(ch, a.dk - 8) : ch) + run / (DP / 8) * a.dk;
+            kr[u].template load<KVEC>(reinterpret_cast<const S *>(kp + c * int(sizeof(S)) + uint64_t(t) * a.ldk), a.dk - c);
+            vr[u].template load<KVEC>(reinterpret_cast<const S *>(vp + c * int(sizeof(S)) + uint64_t(t) * a.ldv), a.dk - c);
         }
     };
-    auto put = [&](char *p, const Run8<T> &r) {
+    auto put = [&](char *p, const Run8<S> &r) {
         if constexpr (HALF) {
             *reinterpret_cast<halfx8 *>(p) = r.half();
         } else {
@@ -281,17 +358,19 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
     auto stage = [&]() {
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
-            const int i = ttid + u * NT, j = i / (DP / 8), ch = i % (DP / 8) * 8;
-            if (__any(tok[u] >= lim_first)) {
-                // Values of tokens that there are not: zeros, whatever lies there. Values that
-                // are not finite, of tokens that some row does not see (0 times them is NaN in
-                // the products): zeros too, they are added at the end.
-                if (tok[u] >= kv_len) vr[u].zero();
-                else if (tok[u] >= lim_first && vr[u].clean()) bad = 1;
+            const int i = ttid + u * NT, j = i / RUNS, run = i % RUNS, ch = run % (DP / 8) * 8;
+            if constexpr (!SPLIT) {
+                if (__any(tok[u] >= lim_first)) {
+                    // Values of tokens that there are not: zeros, whatever lies there. Values that
+                    // are not finite, of tokens that some row does not see (0 times them is NaN in
+                    // the products): zeros too, they are added at the end.
+                    if (tok[u] >= kv_len) vr[u].zero();
+                    else if (tok[u] >= lim_first && vr[u].clean()) bad = 1;
+                }
             }
-            if ((kWhole || j < KT) && ch < a.d) {
-                put(kst + (j * L::kKS + ch) * L::kES, kr[u]);
-                put(vst + (j * L::kVS + ch) * L::kES, vr[u]);
+            if ((kWhole || j < KT) && ch < a.dk) {
+                put(kst + (j * L::kKS + run * 8) * L::kES, kr[u]);
+                put(vst + (j * L::kVS + run * 8) * L::kES, vr[u]);
             }
         }
     };
@@ -323,9 +402,15 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
             if constexpr (HALF) {
                 const char *p = kst + ((b * 32 + col) * L::kKS + h * 8) * 2;
 #pragma unroll
-                for (int c = 0; c < DT * 2; ++c)
-                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const halfx8 *>(p + c * 32), qh[c],
-                                                                       sc[b], 0, 0, 0);
+                for (int c = 0; c < DT * 2; ++c) {
+                    const halfx8 kh = *reinterpret_cast<const halfx8 *>(p + c * 32);
+                    if constexpr (SPLIT) {  // the small products first
+                        const halfx8 kl = *reinterpret_cast<const halfx8 *>(p + DP * 2 + c * 32);
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], sc[b], 0, 0, 0);
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], sc[b], 0, 0, 0);
+                    }
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], sc[b], 0, 0, 0);
+                }
             } else {
                 const float *p = reinterpret_cast<const float *>(kst) + (b * 32 + col) * L::kKS + h * 4;
 #pragma unroll
@@ -337,6 +422,18 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
                 }
             }
         }
+        float vs[SPLIT ? 2 * SUB : 1];  // scales of the values of each sixteen keys, times the probabilities' own
+        if constexpr (SPLIT) {
+#pragma unroll
+            for (int x = 0; x < 2 * SUB; ++x) {
+                const int e = l0 + (min(tile * KT + x * 16, keys - 1) >> a.kb_log);
+                const float f = cq * k_scale[e];
+                vs[x] = v_scale[e];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sc[x / 2][x % 2 * 8 + i] *= f;
+            }
+        }
+        const float c = SPLIT ? 1.0f : a.c;
         if (masked) {
 #pragma unroll
             for (int b = 0; b < SUB; ++b)
@@ -353,7 +450,7 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
         for (int b = 0; b < SUB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, sc[b][i]);
-        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * a.c;
+        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * c;
         const float mn = __builtin_fmaxf(m, mx);
         const float mu = mn == kNegInf ? 0.0f : mn;
         if (__any(mn > m)) {
@@ -365,12 +462,21 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
                 for (int i = 0; i < 16; ++i) o[t][i] *= f;
             m = mn;
         }
+        // The fused exponent is off by half a step of m, which is nothing until scores are so large
+        // that the largest key's power would leave the range: their products are rounded first.
+        const bool far = !SPLIT && __any(__builtin_fabsf(mu) > 1048576.0f);
+        if (far)
+#pragma unroll
+            for (int b = 0; b < SUB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[b][i] *= c;
+        const float ce = far ? 1.0f : c;
         float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < SUB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], a.c, -mu));
+                sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], ce, -mu));
                 sum += sc[b][i];
             }
         l += sum;
@@ -379,12 +485,26 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
             for (int b = 0; b < SUB; ++b)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    halfx8 p;
+                    halfx8 p, pl;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) p[i] = static_cast<_Float16>(sc[b][x * 8 + i]);
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (SPLIT) {
+                            const float y = sc[b][x * 8 + i] * vs[b * 2 + x];
+                            p[i] = static_cast<_Float16>(y);
+                            pl[i] = static_cast<_Float16>(y - float(p[i]));
+                        } else {
+                            p[i] = static_cast<_Float16>(sc[b][x * 8 + i]);
+                        }
+                    }
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
-                        const halfx8 v = read_vt<L::kVS>(vst + ((b * 32 + x * 16) * L::kVS + t * 32) * 2, lane);
+                        const char *vb = vst + ((b * 32 + x * 16) * L::kVS + t * 32) * 2;
+                        const halfx8 v = read_vt<L::kVS>(vb, lane);
+                        if constexpr (SPLIT) {
+                            const halfx8 vl = read_vt<L::kVS>(vb + DP * 2, lane);
+                            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, p, o[t], 0, 0, 0);
+                            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[t], 0, 0, 0);
+                        }
                         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[t], 0, 0, 0);
                     }
                 }
@@ -431,12 +551,21 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
         }
         if (wk) return;
     }
+    if constexpr (SPLIT) {  // the scales taken back
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = ldexpf(o[t][i], v_exp - 2 * kSplitExp);
+    }
     // The values that were staged as zeros because they are not finite, for the rows that see them.
-    if (bad)
+    if (bad) {
+        const char *v0 = SPLIT ? static_cast<const char *>(a.v0) + uint64_t(item) * a.kv_tokens * a.ldv0 +
+                                     int64_t(hk) * a.d * int64_t(sizeof(T))
+                               : vp;
         for (int j = 0; j < keys; ++j) {
             const int t = token(j);
-            if (t < lim_first || t >= lim) continue;
-            const T *v = reinterpret_cast<const T *>(vp + uint64_t(uint32_t(t)) * a.ldv);
+            if ((!SPLIT && t < lim_first) || t >= lim) continue;
+            const T *v = reinterpret_cast<const T *>(v0 + uint64_t(uint32_t(t)) * (SPLIT ? a.ldv0 : a.ldv));
 #pragma unroll
             for (int x = 0; x < DT; ++x)
 #pragma unroll
@@ -446,6 +575,7 @@ __global__ __launch_bounds__(256, HALF && DT <= 4 ? 2 : 1) void block_attention_
                     if (!(__builtin_fabsf(f) < __builtin_huge_valf())) o[x][i] += f;
                 }
         }
+    }
     if (a.part) {
         float *p = a.part + (int64_t(work) * WR + wr) * part_floats(DT);
 #pragma unroll
@@ -523,13 +653,13 @@ __global__ __launch_bounds__(64) void block_attention_join_kernel(Args a) {
     }
 }
 
-template <typename T, bool HALF, bool VEC, int DT, int WR>
+template <typename T, int MODE, bool VEC, int DT, int WR>
 void launch(Context &ctx, const Args &a) {
-    using L = Tiling<HALF, DT, WR>;
-    const void *fn = reinterpret_cast<const void *>(&block_attention_kernel<T, HALF, VEC, DT, WR>);
+    using L = Tiling<MODE, DT, WR>;
+    const void *fn = reinterpret_cast<const void *>(&block_attention_kernel<T, MODE, VEC, DT, WR>);
     if (L::kLds > 48 * 1024) HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
     const uint32_t grid = uint32_t((a.work + 7) / 8 * 8);
-    block_attention_kernel<T, HALF, VEC, DT, WR><<<dim3{grid}, dim3{L::kThreads}, L::kLds, ctx.stream>>>(a);
+    block_attention_kernel<T, MODE, VEC, DT, WR><<<dim3{grid}, dim3{L::kThreads}, L::kLds, ctx.stream>>>(a);
     MH_LAUNCH_CHECK();
     if (a.splits > 1) {
         const dim3 jg{uint32_t(a.work / a.splits * WR), uint32_t((a.d + 31) / 32)};
@@ -538,32 +668,42 @@ void launch(Context &ctx, const Args &a) {
     }
 }
 
-template <typename T, bool HALF, bool VEC, int DT>
+template <typename T, int MODE, bool VEC, int DT>
 void launch_rows(Context &ctx, const Args &a, int wr) {
-    if (wr == 1) launch<T, HALF, VEC, DT, 1>(ctx, a);
-    else if (wr == 2) launch<T, HALF, VEC, DT, 2>(ctx, a);
-    else launch<T, HALF, VEC, DT, 4>(ctx, a);
+    if constexpr (MODE != kSplit)
+        if (wr == 1) return launch<T, MODE, VEC, DT, 1>(ctx, a);
+    if (wr == 2) launch<T, MODE, VEC, DT, 2>(ctx, a);
+    else launch<T, MODE, VEC, DT, 4>(ctx, a);
 }
 
 // dt: 32-channel tiles of the head as chosen by head_tiles.
-template <typename T, bool HALF>
+template <typename T, int MODE>
 void launch_mode(Context &ctx, const Args &a, int wr, int dt, bool vec) {
     if (vec) {
-        if (dt == 1) launch_rows<T, HALF, true, 1>(ctx, a, wr);
-        else if (dt == 2) launch_rows<T, HALF, true, 2>(ctx, a, wr);
-        else if (dt == 3) launch_rows<T, HALF, true, 3>(ctx, a, wr);
-        else if (dt == 4) launch_rows<T, HALF, true, 4>(ctx, a, wr);
-        else if (dt == 5) launch_rows<T, HALF, true, 5>(ctx, a, wr);
-        else launch_rows<T, HALF, true, 8>(ctx, a, wr);
+        if (dt == 1) launch_rows<T, MODE, true, 1>(ctx, a, wr);
+        else if (dt == 2) launch_rows<T, MODE, true, 2>(ctx, a, wr);
+        else if (dt == 3) launch_rows<T, MODE, true, 3>(ctx, a, wr);
+        else if (dt == 4) launch_rows<T, MODE, true, 4>(ctx, a, wr);
+        else if (dt == 5) launch_rows<T, MODE, true, 5>(ctx, a, wr);
+        else if constexpr (MODE != kSplit) launch_rows<T, MODE, true, 8>(ctx, a, wr);
     } else {
-        if (dt == 4) launch_rows<T, HALF, false, 4>(ctx, a, wr);
-        else launch_rows<T, HALF, false, 8>(ctx, a, wr);
+        if (dt == 4) launch_rows<T, MODE, false, 4>(ctx, a, wr);
+        else if (dt == 5) launch_rows<T, MODE, false, 5>(ctx, a, wr);
+        else if constexpr (MODE != kSplit) launch_rows<T, MODE, false, 8>(ctx, a, wr);
     }
 }
 
 void launch_f16(Context &ctx, const Args &a, int wr, int dt, bool vec);
 void launch_f32_half(Context &ctx, const Args &a, int wr, int dt, bool vec);
 void launch_f32(Context &ctx, const Args &a, int wr, int dt, bool vec);
+// Row waves and head tiles that launch_split takes.
+inline bool split_fits(int wr, int dt) { return wr >= 2 && dt <= 5; }
+void launch_split(Context &ctx, const Args &a, int wr, int dt, bool vec);
+// k and v [n][kv_tokens] rows (ldk, ldv elements apart) of hk heads of d f32 -> kp, vp
+// [n][blocks kb][hk][2][dk] f16 parts of every block scaled by its own power of two, zeros
+// behind kv_len and d; meta [n][blocks][hk].
+void split_kv(Context &ctx, const float *k, const float *v, int64_t ldk, int64_t ldv, int n, int kv_tokens, int hk,
+              int d, int dk, int kb, const int32_t *kv_len, void *kp, void *vp, SplitMeta *meta);
 
 }  // namespace battn
 }  // namespace mh

@@ -4,7 +4,7 @@
 namespace mh {
 namespace battn {
 
-void launch_f16(Context &ctx, const Args &a, int wr, int dt, bool vec) { launch_mode<_Float16, true>(ctx, a, wr, dt, vec); }
+void launch_f16(Context &ctx, const Args &a, int wr, int dt, bool vec) { launch_mode<_Float16, kHalf>(ctx, a, wr, dt, vec); }
 
 }  // namespace battn
 }  // namespace mh

@@ -4,7 +4,7 @@
 namespace mh {
 namespace battn {
 
-void launch_f32(Context &ctx, const Args &a, int wr, int dt, bool vec) { launch_mode<float, false>(ctx, a, wr, dt, vec); }
+void launch_f32(Context &ctx, const Args &a, int wr, int dt, bool vec) { launch_mode<float, kF32>(ctx, a, wr, dt, vec); }
 
 }  // namespace battn
 }  // namespace mh

@@ -4,7 +4,7 @@
 namespace mh {
 namespace battn {
 
-void launch_f32_half(Context &ctx, const Args &a, int wr, int dt, bool vec) { launch_mode<float, true>(ctx, a, wr, dt, vec); }
+void launch_f32_half(Context &ctx, const Args &a, int wr, int dt, bool vec) { launch_mode<float, kHalf>(ctx, a, wr, dt, vec); }
 
 }  // namespace battn
 }  // namespace mh

@@ -217,11 +217,13 @@ int32_t mh_block_select(MhContext *ctx, const void *q, uint32_t dtype, uint64_t 
     });
 }
 
-int32_t mh_block_attention_scratch(MhContext *ctx, const MhBlockShape *shape, uint64_t *bytes) {
+int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlockShape *shape, uint64_t *bytes) {
     return guard([&] {
         need(bytes, "bytes");
+        const mh::WeightType t = wtype(dtype);
+        const mh::BlockShape s = block_shape(shape);
         mh::Context &c = C(ctx);
-        *bytes = mh::block_attention_scratch(c, block_shape(shape));
+        *bytes = mh::block_attention_scratch(c, s, t);
     });
 }
 
@@ -243,7 +245,7 @@ int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const v
         no_overlap(ki, to, "k and out");
         no_overlap(vi, to, "v and out");
         mh::Context &c = C(ctx);
-        const size_t needed = mh::block_attention_scratch(c, a.s);
+        const size_t needed = mh::block_attention_scratch(c, a.s, t);
         scratch = check_scratch(c, scratch, scratch_bytes, needed);
         if (needed && !scratch) scratch = c.ws.get(needed, c.stream);
         a.q = {q, qi.ld, a.s.heads_q};
@@ -253,7 +255,6 @@ int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const v
         a.ld_out = to.ld;
         a.blocks = blocks;
         a.scale = scale;
-        a.half = t == mh::kF16 || c.precision == mh::Precision::Fast;
         mh::block_attention(c, a, t, scratch);
     });
 }

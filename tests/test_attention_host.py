@@ -166,8 +166,8 @@ def test_scratch_refusals():
     L, n = _lib.lib(), ctypes.c_uint64()
     refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 0, ctypes.byref(n)), "rank")
     refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 8, None), "bytes is NULL")
-    refused(L.mh_block_attention_scratch(None, ctypes.byref(shape()), None), "bytes is NULL")
-    refused(L.mh_block_attention_scratch(None, ctypes.byref(shape()), ctypes.byref(n)), "context is NULL")
+    refused(L.mh_block_attention_scratch(None, 0, ctypes.byref(shape()), None), "bytes is NULL")
+    refused(L.mh_block_attention_scratch(None, 0, ctypes.byref(shape()), ctypes.byref(n)), "context is NULL")
 
 
 def test_frequencies():

@@ -7,6 +7,8 @@ the keys it sees; all bounds are worst cases of the roundings):
     (f32 sums of exact or once rounded products), the exponent's argument by 2^-23 B
     more with B = max |s_j| log2 e, the hardware's exponential by 2^-22, the running
     rescales and the two sums by (2 tiles + keys) u, all twice (numerator and denominator);
+  - f32 products formed from operands in two f16 parts leave 3 u of each product out (two
+    roundings of 2^-24 and the product of the small parts), of a score and of p v;
   - f16 products round each probability by 2^-11;
   - FAST contexts round q, k and v too: 2 x 2^-11 A per score, twice, and 2^-11 for v;
   - f16 outputs add half a step.
@@ -219,7 +221,7 @@ def reference(q, k, v, blocks, scale, qb, kb, causal, q_len, kv_len):
 
 def tolerance(out, tol, d, dtype, fast):
     keys, A, B, m = (tol[..., i] for i in range(4))
-    e = 2 * ((d + 2) * U * A + 2 * U * B + 4 * U) + (keys + keys / 8) * U
+    e = 2 * ((d + 5) * U * A + 2 * U * B + 4 * U) + (keys + keys / 8 + 3) * U
     if dtype == np.float16 or fast:
         e = e + 2.0 ** -11
     if fast:
@@ -264,6 +266,14 @@ CASES = [  # n, q, kv, hq, hk, d, qb, kb, top, causal
     (1, 10, 100, 2, 2, 130, 4, 16, 5, True),
     (1, 9, 50, 36, 1, 32, 2, 16, 3, False),     # 72 rows of one key head
     (1, 5, 64, 70, 2, 16, 5, 16, 3, True),
+    # keys read by many rows: f32 operands in two parts
+    (2, 256, 256, 2, 2, 80, 64, 32, 8, False),
+    (1, 300, 400, 2, 1, 40, 64, 16, 20, True),
+    (1, 128, 500, 4, 2, 128, 64, 64, 8, True),
+    (1, 200, 300, 1, 1, 160, 100, 32, 9, False),
+    (1, 130, 140, 1, 1, 33, 70, 16, 8, True),
+    (2, 256, 300, 1, 1, 64, 128, 128, 3, True),
+    (1, 140, 170, 1, 1, 134, 70, 16, 11, False),
 ]
 
 
@@ -366,9 +376,40 @@ def test_large_and_infinite_scores(ctx, dtype):
     q[0, 1, 0, 0], k[0, 17, 0, 0] = 200, 200     # one score of 40 000 above the others
     q[0, 2, 0, 1], k[0, 33, 0, 1] = 200, -200    # one far below
     q[0, 3, 0, 2], k[0, 50:, 0, 2] = -1, np.finfo(dtype).max if dtype == np.float16 else 1e30
-    got = run(ctx, q, k, v, np.arange(4, dtype=np.int32).reshape(1, 1, 1, 4), 4, 16, scale=1.0)[0, :, 0, 0]
-    for g, want in zip(got, (31.5, 17.0, (2016 - 33) / 63, 24.5)):
-        assert abs(float(g) - want) <= want * (2.0 ** -10 if dtype == np.float16 else 1e-6)
+    wants = (31.5, 17.0, (2016 - 33) / 63, 24.5)
+    listed = np.arange(4, dtype=np.int32).reshape(1, 1, 1, 4)
+    for rows in (1, 16):  # one wave of rows, and keys read by many
+        qq, li = np.tile(q, (1, rows, 1, 1)), np.tile(listed, (1, max(1, rows // 16), 1, 1))
+        got = run(ctx, qq, k, v, li, 4 * rows, 16, scale=1.0)[0, :, 0, 0]
+        for g, want in zip(got, wants * rows):
+            assert abs(float(g) - want) <= want * (2.0 ** -10 if dtype == np.float16 else 1e-6)
+    # scores of 10^9 and more, of which those of the largest key are the largest (f16: 200 x 200 x 10^5)
+    big = 1e5 if dtype == np.float16 else 1e20
+    for rows in (1, 16):
+        qq = np.tile(q[:, 1:2], (1, 4 * rows, 1, 1))
+        got = run(ctx, qq, k, v, listed, 4 * rows, 16, scale=big)[0, :, 0, 0]
+        assert np.array_equal(got, np.full(4 * rows, 17, dtype))
+
+
+@pytest.mark.parametrize("d", [64, 80])
+def test_f32_ranges(ctx, d):
+    """Blocks of keys and values, and rows of queries, of sizes far from each other and from f16's range:
+    the errors stay relative to the products a row forms and to the largest value it sees."""
+    r = np.random.default_rng(d)
+    q, k, v = (r.standard_normal((1, t, 1, d)).astype(np.float32) for t in (192, 192, 192))
+    for b, f in enumerate((1e-30, 1e-6, 1.0, 1e4, 3e8, 1e-42)):
+        k[0, b * 32:(b + 1) * 32] *= np.float32(f)
+        v[0, b * 32:(b + 1) * 32] *= np.float32((1e30, 1e-20, 1e10, 1.0, 0.0, 1e20)[b])
+        q[0, b * 32:(b + 1) * 32] *= np.float32((1.0, 1e-9, 1e-4, 1e3, 1e20, 1e-38)[b])
+    v[0, :, 0, :8] *= np.float32(2.0 ** -20)
+    for blocks in ([0, 1, 2], [1, 2, 3], [3, 4], [5], [1], [2, 5], [4], [1, 5]):
+        li = np.tile(np.array(blocks + [-1] * (6 - len(blocks)), np.int32), (1, 2, 1, 1))
+        got = run(ctx, q, k, v, li, 96, 32, scale=0.125).astype(np.float64)
+        want, tol = reference(q, k, v, li, 0.125, 96, 32, False, None, None)
+        ok = tol[..., 2] < 1e4  # beyond it an exponent's rounding is larger than a score's part
+        bound = tolerance(want, tol, d, np.float32, False)
+        assert ok.any() and np.all((np.abs(got - want) <= bound)[ok]), blocks
+        assert np.isfinite(got).all()
 
 
 def test_row_results_do_not_depend_on_the_batch(ctx):
