@@ -558,8 +558,9 @@ typedef struct MhAdapters {
     uint32_t reserved; /* 0 */
 } MhAdapters;
 
-/* Scratch of mh_conv1x1_lora for these sizes on this context. */
-int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, uint32_t rank, uint64_t *bytes);
+/* Scratch of mh_conv1x1_lora for these sizes on this context at its present precision. */
+int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, uint32_t c_out, uint32_t weight_dtype,
+                                uint32_t rank, uint64_t *bytes);
 
 /* mh_conv1x1_forward with an adapter per request: out = x . W^T + bias (+ residual),
  * and for rows whose s = slot[row / rows_per_slot] is 0 .. slots - 1 (others, -1 by

@@ -122,7 +122,7 @@ SIGNATURES = {
     "mh_block_select": (_i32, [_vp, _vp, _u32, _u64, _vp, _vp, _vp]),
     "mh_block_attention_scratch": (_i32, [_vp, _u32, _vp, ctypes.POINTER(_u64)]),
     "mh_block_attention": (_i32, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _u64]),
-    "mh_conv1x1_lora_scratch": (_i32, [_vp, _u64, _u32, _u32, ctypes.POINTER(_u64)]),
+    "mh_conv1x1_lora_scratch": (_i32, [_vp, _u64, _u32, _u32, _u32, _u32, ctypes.POINTER(_u64)]),
     "mh_conv1x1_lora": (_i32, [_vp, _vp, _u64, _u32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _u64, _vp, _vp, _u64]),
     "mh_unet_create": (_i32, [_vp, _vp, _u32, ctypes.POINTER(_vp)]),
     "mh_unet_destroy": (None, [_vp]),

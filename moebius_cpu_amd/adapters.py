@@ -22,8 +22,10 @@ class Adapters:
             raise MoebiusError(1, "adapter size")
         self.c = _lib.AdapterSet(a.ptr, b.ptr, self.scale.ptr, a.dtype, self.slots, rank, 0)
 
-    def scratch(self, rows: int) -> int:
-        """Bytes of scratch that a call over `rows` rows needs, for calls that are captured into a graph."""
+    def scratch(self, rows: int, weight: Param) -> int:
+        """Bytes of scratch that a call over `rows` rows of a projection by `weight` needs, for calls
+        that are captured into a graph."""
         n = ctypes.c_uint64()
-        check(lib().mh_conv1x1_lora_scratch(self.ctx.h, rows, self.c_in, self.rank, ctypes.byref(n)))
+        check(lib().mh_conv1x1_lora_scratch(self.ctx.h, rows, self.c_in, self.c_out, weight.dtype, self.rank,
+                                            ctypes.byref(n)))
         return int(n.value)

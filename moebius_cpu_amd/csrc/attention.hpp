@@ -100,7 +100,7 @@ struct Lora {
     const int32_t *slot = nullptr;  // [ceil(rows / rows_per_slot)]
     int64_t rows_per_slot = 1;
 };
-size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int rank);
+size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int c_out, WeightType wt, int rank);
 void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const void *weight, WeightType wt, int c_out,
                   const float *bias, const float *residual, const Lora &l, float *out, void *scratch);
 

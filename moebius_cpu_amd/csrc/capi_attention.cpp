@@ -259,13 +259,15 @@ int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const v
     });
 }
 
-int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, uint32_t rank, uint64_t *bytes) {
+int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, uint32_t c_out, uint32_t weight_dtype,
+                                uint32_t rank, uint64_t *bytes) {
     return guard([&] {
         need(bytes, "bytes");
         few_rows(rows);
         if (rank < 1 || rank > uint32_t(mh::kMaxRank)) mh::fail(mh::kInvalidArgument, "rank is 1 .. 256");
+        const mh::WeightType t = wtype(weight_dtype);
         mh::Context &c = C(ctx);
-        *bytes = mh::lora_scratch(c, int64_t(rows), dim(c_in, "c_in"), int(rank));
+        *bytes = mh::lora_scratch(c, int64_t(rows), dim(c_in, "c_in"), dim(c_out, "c_out"), t, int(rank));
     });
 }
 
@@ -307,7 +309,8 @@ int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t 
         const Rows in{reinterpret_cast<const char *>(x), int64_t(rows), int64_t(c_in), int64_t(c_in), 4};
         no_overlap(in, to, "x and out");
         mh::Context &c = C(ctx);
-        const size_t needed = mh::lora_scratch(c, int64_t(rows), dim(c_in, "c_in"), l.rank);
+        const size_t needed = mh::lora_scratch(c, int64_t(rows), dim(c_in, "c_in"), dim(c_out, "c_out"),
+                                               wtype(weight_dtype), l.rank);
         scratch = check_scratch(c, scratch, scratch_bytes, needed);
         mh::conv1x1_lora(c, x, int64_t(rows), int(c_in), weight, wtype(weight_dtype), dim(c_out, "c_out"), bias,
                          residual, l, out, scratch);

@@ -16,62 +16,11 @@
 // their own requests.
 #include <algorithm>
 
-#include "attention.hpp"
+#include "lora.hpp"
 
 namespace mh {
+namespace lora {
 namespace {
-
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
-
-struct LoraArgs {
-    const float *x;
-    const void *a, *b;
-    const float *scale;
-    const int32_t *slot;
-    float *t, *out;
-    int64_t rows, rows_per_slot;
-    int ci, co, rank, slots, splits, rank_pad;  // rank_pad: rank rounded up to 16
-    int chunk;                                  // of the long axis per split, a multiple of 64
-};
-
-// Four values at p + k of a run of n, zeros behind it; VEC: n and p keep every run of four aligned.
-template <bool VEC>
-__device__ __forceinline__ floatx4 load4(const float *p, int k, int n) {
-    if constexpr (VEC) {  // behind n the last run is loaded instead, so that no load waits for a branch
-        const floatx4 v = *reinterpret_cast<const floatx4 *>(p + min(k, n - 4));
-        return k < n ? v : floatx4{0, 0, 0, 0};
-    } else {
-        floatx4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k + e < n ? p[k + e] : 0.0f;
-        return v;
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ floatx4 load4(const _Float16 *p, int k, int n) {
-    floatx4 v = {0, 0, 0, 0};
-    if constexpr (VEC) {
-        const halfx4 r = *reinterpret_cast<const halfx4 *>(p + min(k, n - 4));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k < n ? float(r[e]) : 0.0f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (k + e < n) v[e] = float(p[k + e]);
-    }
-    return v;
-}
-
-__device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ int slot_of(const LoraArgs &p, int64_t row) {
-    if (row >= p.rows) return -1;
-    const int s = p.slot[row / p.rows_per_slot];
-    return s < p.slots ? s : -1;
-}
 
 constexpr int kRankTiles = 4;     // 16 ranks each per pass over x
 constexpr int kShrinkUnroll = 5;  // steps of the long axis whose loads are in flight together
@@ -299,15 +248,15 @@ constexpr int kFewRows = 64;
 bool few_rows(int64_t rows) { return rows <= kFewRows; }
 
 // Splits of the long axis: two workgroups per CU, at least 128 values each.
-int lora_splits(const Context &ctx, int64_t rows, int c_in) {
-    if (few_rows(rows)) return 1;
+int lora_splits(const Context &ctx, int64_t rows, int c_in, bool own) {
+    if (few_rows(rows) || own) return 1;  // their second products read t as it is
     const int64_t tiles = ceil_div(rows, 16);
     const int64_t s = std::min<int64_t>(2 * ctx.cu_count / std::max<int64_t>(tiles, 1), c_in / 128);
     return int(std::max<int64_t>(1, std::min<int64_t>(s, 16)));
 }
 
 template <typename T>
-void run(Context &ctx, const LoraArgs &p) {
+void run_shrink(Context &ctx, const LoraArgs &p) {
     const int64_t tiles = ceil_div(p.rows, 16);
     MH_REQUIRE(tiles < (int64_t(1) << 31), "lora: too many rows");
     const dim3 tb{256};
@@ -316,6 +265,12 @@ void run(Context &ctx, const LoraArgs &p) {
     if (vx) lora_shrink_kernel<T, true><<<sg, tb, 0, ctx.stream>>>(p);
     else lora_shrink_kernel<T, false><<<sg, tb, 0, ctx.stream>>>(p);
     MH_LAUNCH_CHECK();
+}
+
+template <typename T>
+void run_expand(Context &ctx, const LoraArgs &p) {
+    const int64_t tiles = ceil_div(p.rows, 16);
+    const dim3 tb{256};
     const bool vb = p.rank % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % (4 * sizeof(T)) == 0;
     const bool vo = p.co % 4 == 0 && aligned16(p.out);
     const dim3 eg{uint32_t(tiles), uint32_t(ceil_div(p.co, 256))};
@@ -341,36 +296,85 @@ void run_few(Context &ctx, const LoraArgs &p, const void *weight, const float *b
     MH_LAUNCH_CHECK();
 }
 
-}  // namespace
+// Scratch: t, then the parts of x and their exponents, then those of an f32 weight.
+struct Layout {
+    size_t t = 0, x = 0, x_exp = 0, w = 0, w_exp = 0;
+    size_t total() const { return t + x + x_exp + w + w_exp; }
+};
 
-size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int rank) {
-    return size_t(lora_splits(ctx, rows, c_in)) * size_t(rows) * size_t(ceil_div(rank, 16) * 16) * sizeof(float);
+bool use_gemm(const Context &ctx, int64_t rows, int c_in, int c_out) {
+    return !few_rows(rows) && ctx.precision == Precision::Exact && gemm_fits(ctx, rows, c_out, c_in);
+}
+
+Layout layout(const Context &ctx, int64_t rows, int c_in, int c_out, WeightType wt, int rank) {
+    auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+    const size_t cip = size_t(ceil_div(c_in, 32) * 32);
+    Layout l;
+    const bool own = use_gemm(ctx, rows, c_in, c_out);
+    l.t = up(size_t(lora_splits(ctx, rows, c_in, own)) * size_t(rows) * size_t(ceil_div(rank, 16) * 16) * sizeof(float));
+    if (own) {
+        l.x = up(size_t(rows) * 2 * cip * 2);
+        l.x_exp = up(size_t(rows) * 4);
+        if (wt == kF32) {
+            l.w = up(size_t(c_out) * 2 * cip * 2);
+            l.w_exp = up(size_t(c_out) * 4);
+        }
+    }
+    return l;
+}
+
+}  // namespace
+}  // namespace lora
+
+size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int c_out, WeightType wt, int rank) {
+    return rows ? lora::layout(ctx, rows, c_in, c_out, wt, rank).total() : 0;
 }
 
 void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const void *weight, WeightType wt, int c_out,
                   const float *bias, const float *residual, const Lora &l, float *out, void *scratch) {
     if (!rows) return;
-    const bool few = few_rows(rows);
-    if (!few) conv1x1(ctx, x, rows, c_in, weight, wt, c_out, bias, residual, out);
-    LoraArgs p{};
-    p.x = x, p.a = l.a, p.b = l.b, p.scale = l.scale, p.slot = l.slot, p.out = out;
+    const bool few = lora::few_rows(rows), own = lora::use_gemm(ctx, rows, c_in, c_out);
+    if (!few && !own) conv1x1(ctx, x, rows, c_in, weight, wt, c_out, bias, residual, out);
+    const lora::Layout mem = lora::layout(ctx, rows, c_in, c_out, wt, l.rank);
     // behind the projection on the stream: its split sums in the workspace are done with
-    p.t = static_cast<float *>(scratch ? scratch : ctx.ws.get(lora_scratch(ctx, rows, c_in, l.rank), ctx.stream));
+    char *at = static_cast<char *>(scratch ? scratch : ctx.ws.get(mem.total(), ctx.stream));
+    lora::LoraArgs p{};
+    p.x = x, p.a = l.a, p.b = l.b, p.scale = l.scale, p.slot = l.slot, p.out = out;
+    p.t = reinterpret_cast<float *>(at);
     p.rows = rows, p.rows_per_slot = l.rows_per_slot;
     p.ci = c_in, p.co = c_out, p.rank = l.rank, p.slots = l.slots;
     p.rank_pad = int(ceil_div(l.rank, 16) * 16);
-    p.splits = lora_splits(ctx, rows, c_in);
+    p.splits = lora::lora_splits(ctx, rows, c_in, own);
     p.chunk = int(ceil_div(ceil_div(c_in, p.splits), 64) * 64);
+    const bool ah = l.type == kF16;
     if (few) {
-        const bool ah = l.type == kF16;
-        if (wt == kF16 && ah) run_few<_Float16, _Float16>(ctx, p, weight, bias, residual);
-        else if (wt == kF16) run_few<_Float16, float>(ctx, p, weight, bias, residual);
-        else if (ah) run_few<float, _Float16>(ctx, p, weight, bias, residual);
-        else run_few<float, float>(ctx, p, weight, bias, residual);
+        if (wt == kF16 && ah) lora::run_few<_Float16, _Float16>(ctx, p, weight, bias, residual);
+        else if (wt == kF16) lora::run_few<_Float16, float>(ctx, p, weight, bias, residual);
+        else if (ah) lora::run_few<float, _Float16>(ctx, p, weight, bias, residual);
+        else lora::run_few<float, float>(ctx, p, weight, bias, residual);
         return;
     }
-    if (l.type == kF16) run<_Float16>(ctx, p);
-    else run<float>(ctx, p);
+    if (ah) lora::run_shrink<_Float16>(ctx, p);
+    else lora::run_shrink<float>(ctx, p);
+    if (!own) {
+        if (ah) lora::run_expand<_Float16>(ctx, p);
+        else lora::run_expand<float>(ctx, p);
+        return;
+    }
+    lora::GemmArgs g{};
+    g.l = p;
+    g.cip = int(ceil_div(c_in, 32) * 32);
+    auto *xp = reinterpret_cast<_Float16 *>(at + mem.t);
+    auto *xe = reinterpret_cast<int *>(at + mem.t + mem.x);
+    lora::split_rows(ctx, x, rows, c_in, g.cip, xp, xe);
+    g.xp = xp, g.x_exp = xe, g.w = weight, g.bias = bias, g.residual = residual;
+    if (wt == kF32) {
+        auto *wp = reinterpret_cast<_Float16 *>(at + mem.t + mem.x + mem.x_exp);
+        auto *we = reinterpret_cast<int *>(at + mem.t + mem.x + mem.x_exp + mem.w);
+        lora::split_rows(ctx, static_cast<const float *>(weight), c_out, c_in, g.cip, wp, we);
+        g.w = wp, g.w_exp = we;
+    }
+    lora::gemm(ctx, g, wt, l.type);
 }
 
 }  // namespace mh

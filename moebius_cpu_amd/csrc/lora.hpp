@@ -1,0 +1,93 @@
+// Shared by the adapter kernels (lora.hip, lora_gemm.hip): see lora.hip for the mathematics.
+#pragma once
+
+#include "attention.hpp"
+
+namespace mh {
+namespace lora {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
+
+struct LoraArgs {
+    const float *x;
+    const void *a, *b;
+    const float *scale;
+    const int32_t *slot;
+    float *t, *out;
+    int64_t rows, rows_per_slot;
+    int ci, co, rank, slots, splits, rank_pad;  // rank_pad: rank rounded up to 16
+    int chunk;                                  // of the long axis per split, a multiple of 64
+};
+
+// Four values at p + k of a run of n, zeros behind it; VEC: n and p keep every run of four aligned.
+template <bool VEC>
+__device__ __forceinline__ floatx4 load4(const float *p, int k, int n) {
+    if constexpr (VEC) {  // behind n the last run is loaded instead, so that no load waits for a branch
+        const floatx4 v = *reinterpret_cast<const floatx4 *>(p + min(k, n - 4));
+        return k < n ? v : floatx4{0, 0, 0, 0};
+    } else {
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = k + e < n ? p[k + e] : 0.0f;
+        return v;
+    }
+}
+template <bool VEC>
+__device__ __forceinline__ floatx4 load4(const _Float16 *p, int k, int n) {
+    floatx4 v = {0, 0, 0, 0};
+    if constexpr (VEC) {
+        const halfx4 r = *reinterpret_cast<const halfx4 *>(p + min(k, n - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = k < n ? float(r[e]) : 0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (k + e < n) v[e] = float(p[k + e]);
+    }
+    return v;
+}
+
+__device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int slot_of(const LoraArgs &p, int64_t row) {
+    if (row >= p.rows) return -1;
+    const int s = p.slot[row / p.rows_per_slot];
+    return s < p.slots ? s : -1;
+}
+
+// f32 values as two f16 parts, x 2^e = hi + lo to 2^-24 of it (2^-40 of the largest value
+// of what e was taken from, scaled to 2^14 .. 2^15); one that is not finite is all in hi.
+constexpr int kSplitExp = 14;
+__device__ __forceinline__ void split2(float x, int e, _Float16 &hi, _Float16 &lo) {
+    const float y = ldexpf(x, e);
+    hi = static_cast<_Float16>(y);
+    const float r = y - float(hi);
+    lo = static_cast<_Float16>(__builtin_fabsf(y) < __builtin_huge_valf() ? r : 0.0f);
+}
+// NULL counts as aligned.
+__device__ __forceinline__ bool aligned16_dev(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__device__ __forceinline__ int top_exp(float mx) { return mx == 0.0f ? 0 : __builtin_amdgcn_frexp_expf(mx) - 1; }
+
+// The projection with the adapters' second product in its epilogue (lora_gemm.hip).
+struct GemmArgs {
+    LoraArgs l;
+    const void *w;           // [co][ci], or its parts [co][2][cip]
+    const int *w_exp;        // [co] where w is in parts
+    const _Float16 *xp;      // [rows][2][cip]
+    const int *x_exp;        // [rows]
+    const float *bias, *residual;
+    int cip;                 // ci rounded up to 32
+    int tiles_m, tiles_n;    // of columns, of rows
+};
+// x [rows][ci] -> parts [rows][2][cip] (zeros behind ci) and each row's exponent.
+void split_rows(Context &ctx, const float *x, int64_t rows, int ci, int cip, _Float16 *parts, int *exps);
+// Whether that kernel is the faster way for these sizes.
+bool gemm_fits(const Context &ctx, int64_t rows, int c_out, int c_in);
+// weight: wt, or f32 in parts.
+void gemm(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at);
+
+}  // namespace lora
+}  // namespace mh

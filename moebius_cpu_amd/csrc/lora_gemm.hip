@@ -1,0 +1,332 @@
+// The projection of many rows with the adapters' second product in its epilogue.
+//
+// f32 products at the f16 matrix rate: x = hi + lo, two f16 parts that hold 24 bits of
+// values down to 2^-18 of their row's largest (split_rows scales each row by a power of
+// two), so x W^T takes two f16 products where W is stored in f16 and three where it is f32
+// and split alike (lo . lo is below 2^-24 of its product). Sums are f32. An eighth of the
+// f32 instructions' time and a third of six bf16 products'.
+//
+// A workgroup forms BT columns x BT rows, its four waves 2 x 2 quarters, as W . X^T: a lane
+// of a 32x32 result holds one row and four runs of four columns, so a row's scale and its
+// adapter are the lane's own. 32 of the long axis are staged in LDS at a time while the
+// next are loaded. Bound: the matrix instructions; the parts of x are written and read
+// once more than x itself.
+#include <algorithm>
+
+#include "lora.hpp"
+
+namespace mh {
+namespace lora {
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+// A wave per row, its values in registers up to kHold runs of 8 per lane.
+constexpr int kHold = 4;
+template <bool VEC>
+__global__ __launch_bounds__(256) void split_rows_kernel(const float *x, int64_t rows, int ci, int cip, _Float16 *parts,
+                                                         int *exps) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float *src = x + row * ci;
+    _Float16 *dst = parts + row * 2 * cip;
+    floatx4 v[kHold][2];
+    float mx = 0.0f;
+    auto scan = [&](const floatx4 &a) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float f = __builtin_fabsf(a[e]);
+            mx = f < __builtin_huge_valf() ? __builtin_fmaxf(mx, f) : mx;
+        }
+    };
+    const int runs = cip / 8;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            v[i][j] = load4<VEC>(src, (i * 64 + lane) * 8 + j * 4, ci);
+            scan(v[i][j]);
+        }
+    for (int r = kHold * 64 + lane; r < runs; r += 64)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) scan(load4<VEC>(src, r * 8 + j * 4, ci));
+#pragma unroll
+    for (int m = 32; m; m >>= 1) mx = __builtin_fmaxf(mx, __shfl_xor(mx, m));
+    const int e = top_exp(mx);
+    auto put = [&](int r, const floatx4 &a, const floatx4 &b) {
+        halfx8 hi, lo;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            _Float16 p, q;
+            split2(c < 4 ? a[c] : b[c - 4], kSplitExp - e, p, q);
+            hi[c] = p, lo[c] = q;
+        }
+        *reinterpret_cast<halfx8 *>(dst + r * 8) = hi;
+        *reinterpret_cast<halfx8 *>(dst + cip + r * 8) = lo;
+    };
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+        if (i * 64 + lane < runs) put(i * 64 + lane, v[i][0], v[i][1]);
+    for (int r = kHold * 64 + lane; r < runs; r += 64) put(r, load4<VEC>(src, r * 8, ci), load4<VEC>(src, r * 8 + 4, ci));
+    if (lane == 0) exps[row] = e;
+}
+
+// Eight values of a row of n at k, zeros behind it.
+template <bool VEC>
+__device__ __forceinline__ halfx8 load8(const _Float16 *p, int k, int n) {
+    halfx8 v;
+    if constexpr (VEC) {
+        v = *reinterpret_cast<const halfx8 *>(p + min(k, n - 8));
+        const halfx8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
+        v = k < n ? v : zero;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[k + e] : _Float16(0);
+    }
+    return v;
+}
+
+__device__ __forceinline__ floatx16 mfma16(halfx8 a, halfx8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kGK = 32;  // of the long axis per stage
+
+// WP: parts of the weight (1: f16 as stored, rows of ci; 2: rows of 2 cip); VW: its rows
+// allow 16-byte loads; T: the adapters' storage.
+template <int BT, int WP, bool VW, typename T>
+__global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
+    constexpr int S = BT / 64;                        // 32-tiles of a wave in each direction
+    constexpr int XS = 2 * kGK + 8, WS = WP * kGK + 8;  // staged rows (halves), on distinct banks
+    constexpr int XU = BT * 2 * kGK / 8 / 256, WU = BT * WP * kGK / 8 / 256;  // runs per thread
+    __shared__ __align__(16) _Float16 xs[BT * XS], ws[BT * WS];
+    const LoraArgs &p = g.l;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave & 1, wn = wave >> 1, l32 = lane & 31, h = lane >> 5;
+    // Tiles of columns within tiles of rows, a contiguous eighth per XCD: a tile's rows are
+    // read from memory once.
+    const int tiles = g.tiles_m * g.tiles_n, per_xcd = (tiles + 7) / 8;
+    const int w = int(blockIdx.x % 8) * per_xcd + int(blockIdx.x / 8);
+    if (int(blockIdx.x / 8) >= per_xcd || w >= tiles) return;
+    const int c0 = (w % g.tiles_m) * BT;
+    const int64_t r0 = int64_t(w / g.tiles_m) * BT;
+
+    halfx8 xr[XU], wv[WU];
+    auto fetch = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < XU; ++u) {
+            const int i = tid + u * 256, r = i / 8, run = i % 8;  // four runs of hi, four of lo
+            xr[u] = *reinterpret_cast<const halfx8 *>(g.xp + (min(r0 + r, p.rows - 1) * 2 + run / 4) * g.cip + k + run % 4 * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < WU; ++u) {
+            const int i = tid + u * 256, c = min(c0 + i / (4 * WP), p.co - 1), run = i % (4 * WP);
+            const _Float16 *wp = static_cast<const _Float16 *>(g.w);
+            if constexpr (WP == 2)
+                wv[u] = *reinterpret_cast<const halfx8 *>(wp + (int64_t(c) * 2 + run / 4) * g.cip + k + run % 4 * 8);
+            else
+                wv[u] = load8<VW>(wp + int64_t(c) * p.ci, k + run * 8, p.ci);
+        }
+    };
+    floatx16 acc[S][S];
+#pragma unroll
+    for (int m = 0; m < S; ++m)
+#pragma unroll
+        for (int n = 0; n < S; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.0f;
+    fetch(0);
+    for (int k = 0; k < g.cip; k += kGK) {
+        if (k) __syncthreads();
+#pragma unroll
+        for (int u = 0; u < XU; ++u) {
+            const int i = tid + u * 256;
+            *reinterpret_cast<halfx8 *>(xs + i / 8 * XS + i % 8 * 8) = xr[u];
+        }
+#pragma unroll
+        for (int u = 0; u < WU; ++u) {
+            const int i = tid + u * 256;
+            *reinterpret_cast<halfx8 *>(ws + i / (4 * WP) * WS + i % (4 * WP) * 8) = wv[u];
+        }
+        __syncthreads();
+        if (k + kGK < g.cip) fetch(k + kGK);
+#pragma unroll
+        for (int c = 0; c < kGK / 16; ++c) {
+            halfx8 xh[S], xl[S];
+#pragma unroll
+            for (int n = 0; n < S; ++n) {
+                const _Float16 *q = xs + (wn * S * 32 + n * 32 + l32) * XS + c * 16 + h * 8;
+                xh[n] = *reinterpret_cast<const halfx8 *>(q);
+                xl[n] = *reinterpret_cast<const halfx8 *>(q + kGK);
+            }
+#pragma unroll
+            for (int m = 0; m < S; ++m) {
+                const _Float16 *q = ws + (wm * S * 32 + m * 32 + l32) * WS + c * 16 + h * 8;
+                const halfx8 wh = *reinterpret_cast<const halfx8 *>(q);
+                if constexpr (WP == 2) {
+                    const halfx8 wl = *reinterpret_cast<const halfx8 *>(q + kGK);
+#pragma unroll
+                    for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wl, xh[n], acc[m][n]);
+                }
+#pragma unroll
+                for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xl[n], acc[m][n]);
+#pragma unroll
+                for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xh[n], acc[m][n]);
+            }
+        }
+    }
+
+    // Columns 8 f + 4 h + e of a 32-tile are register 4 f + e; the row is lane % 32.
+    const bool vb = p.rank % 8 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0;
+    const bool vo = p.co % 4 == 0 && aligned16_dev(p.out) && aligned16_dev(g.residual);
+#pragma unroll
+    for (int n = 0; n < S; ++n) {
+        const int64_t row = r0 + (wn * S + n) * 32 + l32, row_in = min(row, p.rows - 1);
+        const int xe = g.x_exp[row_in] - kSplitExp;
+#pragma unroll
+        for (int m = 0; m < S; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                int e = xe;
+                if constexpr (WP == 2)
+                    e += g.w_exp[min(c0 + (wm * S + m) * 32 + 8 * (i / 4) + 4 * h + i % 4, p.co - 1)] - kSplitExp;
+                acc[m][n][i] = ldexpf(acc[m][n][i], e);
+            }
+        const int mine = slot_of(p, row);
+        uint32_t todo = uint32_t(__ballot(mine >= 0));
+        if (todo) {
+            const float *t = p.t + row_in * p.rank_pad;
+            int te = 0;
+            if constexpr (sizeof(T) == 2) {  // the row of t in two parts, as x
+                float mx = 0.0f;
+                if (mine >= 0)
+                    for (int k = 0; k < p.rank; k += 16)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float f = k + h * 8 + i < p.rank ? __builtin_fabsf(t[k + h * 8 + i]) : 0.0f;
+                            mx = f < __builtin_huge_valf() ? __builtin_fmaxf(mx, f) : mx;
+                        }
+                mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+                te = top_exp(mx);
+            }
+            while (todo) {
+                const int s = __builtin_amdgcn_readfirstlane(__shfl(mine, __builtin_ctz(todo)));
+                const bool own = mine == s;
+                todo &= ~uint32_t(__ballot(own));
+                floatx16 low[S];
+#pragma unroll
+                for (int m = 0; m < S; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) low[m][i] = 0.0f;
+                const T *b[S];
+#pragma unroll
+                for (int m = 0; m < S; ++m)
+                    b[m] = static_cast<const T *>(p.b) +
+                           (int64_t(s) * p.co + min(c0 + (wm * S + m) * 32 + l32, p.co - 1)) * p.rank;
+                for (int k = 0; k < p.rank; k += 16) {
+                    float tv[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) tv[i] = own && k + h * 8 + i < p.rank ? t[k + h * 8 + i] : 0.0f;
+                    if constexpr (sizeof(T) == 2) {
+                        halfx8 th, tl;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            _Float16 hi, lo;
+                            split2(tv[i], kSplitExp - te, hi, lo);
+                            th[i] = hi, tl[i] = lo;
+                        }
+#pragma unroll
+                        for (int m = 0; m < S; ++m) {
+                            const halfx8 bv = vb ? load8<true>(b[m], k + h * 8, p.rank) : load8<false>(b[m], k + h * 8, p.rank);
+                            low[m] = mfma16(bv, tl, low[m]);
+                            low[m] = mfma16(bv, th, low[m]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int m = 0; m < S; ++m)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float bv = k + h * 8 + i < p.rank ? float(b[m][k + h * 8 + i]) : 0.0f;
+                                low[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(bv, tv[i], low[m], 0, 0, 0);
+                            }
+                    }
+                }
+                const float scale = p.scale[s];
+#pragma unroll
+                for (int m = 0; m < S; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float v = sizeof(T) == 2 ? ldexpf(low[m][i], te - kSplitExp) : low[m][i];
+                        acc[m][n][i] = own ? __builtin_fmaf(scale, v, acc[m][n][i]) : acc[m][n][i];
+                    }
+            }
+        }
+        if (row >= p.rows) continue;
+#pragma unroll
+        for (int m = 0; m < S; ++m)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const int c = c0 + (wm * S + m) * 32 + 8 * f + 4 * h;
+                float *out = p.out + row * p.co + c;
+                const float *res = g.residual ? g.residual + row * p.co + c : nullptr;
+                if (vo && c < p.co) {
+                    floatx4 y = {acc[m][n][4 * f], acc[m][n][4 * f + 1], acc[m][n][4 * f + 2], acc[m][n][4 * f + 3]};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] += g.bias ? g.bias[c + e] : 0.0f;
+                    if (res) y += *reinterpret_cast<const floatx4 *>(res);
+                    *reinterpret_cast<floatx4 *>(out) = y;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < p.co)
+                            out[e] = acc[m][n][4 * f + e] + (g.bias ? g.bias[c + e] : 0.0f) + (res ? res[e] : 0.0f);
+                }
+            }
+    }
+}
+
+template <int BT, int WP, bool VW>
+void launch(Context &ctx, GemmArgs g, WeightType at) {
+    g.tiles_m = int(ceil_div(g.l.co, BT));
+    const int64_t tn = ceil_div(g.l.rows, BT);
+    MH_REQUIRE(tn * g.tiles_m < (int64_t(1) << 30), "lora: too many tiles");
+    g.tiles_n = int(tn);
+    const dim3 grid{uint32_t(ceil_div(tn * g.tiles_m, 8) * 8)}, tb{256};
+    if (at == kF16) lora_gemm_kernel<BT, WP, VW, _Float16><<<grid, tb, 0, ctx.stream>>>(g);
+    else lora_gemm_kernel<BT, WP, VW, float><<<grid, tb, 0, ctx.stream>>>(g);
+    MH_LAUNCH_CHECK();
+}
+
+template <int BT>
+void launch_bt(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
+    if (wt == kF32) return launch<BT, 2, true>(ctx, g, at);
+    if (g.l.ci % 8 == 0 && aligned16(g.w)) launch<BT, 1, true>(ctx, g, at);
+    else launch<BT, 1, false>(ctx, g, at);
+}
+
+int64_t tiles_of(int64_t rows, int c_out, int bt) { return ceil_div(rows, bt) * ceil_div(c_out, bt); }
+
+}  // namespace
+
+void split_rows(Context &ctx, const float *x, int64_t rows, int ci, int cip, _Float16 *parts, int *exps) {
+    const int64_t blocks = ceil_div(rows, 4);
+    MH_REQUIRE(blocks < (int64_t(1) << 31), "lora: too many rows");
+    const dim3 grid{uint32_t(blocks)}, tb{256};
+    if (ci % 4 == 0 && aligned16(x)) split_rows_kernel<true><<<grid, tb, 0, ctx.stream>>>(x, rows, ci, cip, parts, exps);
+    else split_rows_kernel<false><<<grid, tb, 0, ctx.stream>>>(x, rows, ci, cip, parts, exps);
+    MH_LAUNCH_CHECK();
+}
+
+bool gemm_fits(const Context &ctx, int64_t rows, int c_out, int c_in) {
+    return tiles_of(rows, c_out, 64) >= ctx.cu_count / 2;
+}
+
+void gemm(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
+    if (tiles_of(g.l.rows, g.l.co, 128) >= ctx.cu_count) launch_bt<128>(ctx, g, wt, at);
+    else launch_bt<64>(ctx, g, wt, at);
+}
+
+}  // namespace lora
+}  // namespace mh

@@ -164,8 +164,9 @@ def test_lora_refusals(kw, text):
 
 def test_scratch_refusals():
     L, n = _lib.lib(), ctypes.c_uint64()
-    refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 0, ctypes.byref(n)), "rank")
-    refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 8, None), "bytes is NULL")
+    refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 32, 0, 0, ctypes.byref(n)), "rank")
+    refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 32, 0, 8, None), "bytes is NULL")
+    refused(L.mh_conv1x1_lora_scratch(None, 8, 64, 32, 9, 8, ctypes.byref(n)), "dtype")
     refused(L.mh_block_attention_scratch(None, 0, ctypes.byref(shape()), None), "bytes is NULL")
     refused(L.mh_block_attention_scratch(None, 0, ctypes.byref(shape()), ctypes.byref(n)), "context is NULL")
 

@@ -43,6 +43,9 @@ CASES = [  # n, h, w, ci, co, rank, slots, per pixel
     (1, 1, 40, 1280, 256, 32, 4, True), (2, 16, 16, 320, 640, 64, 2, False), (1, 9, 9, 33, 45, 3, 7, True),
     (5, 1, 1, 2500, 70, 10, 3, False), (1, 20, 20, 64, 128, 256, 2, True), (1, 3, 11, 16, 4, 100, 3, True),
     (17, 1, 3, 640, 1100, 7, 40, False),
+    # enough rows and columns for the product of operands in two f16 parts
+    (4, 32, 32, 320, 640, 16, 3, False), (3, 23, 29, 333, 1030, 12, 4, False), (1, 50, 43, 100, 1281, 40, 9, True),
+    (5, 20, 21, 64, 1280, 72, 2, False),
 ]
 
 
@@ -87,7 +90,7 @@ def test_against_the_formula(ctx, case, f16, extra, fast):
     assert np.all(err <= bound), (err / bound).max()
 
 
-@pytest.mark.parametrize("case", [CASES[1], CASES[3], CASES[5]])
+@pytest.mark.parametrize("case", [CASES[1], CASES[3], CASES[5], CASES[-2]])
 def test_rows_without_adapter_are_the_projection(ctx, case):
     """Slots below 0 and at or above the number of adapters: the projection alone (few rows have a
     product of their own, so within its tolerance, not in bits)."""
@@ -107,11 +110,13 @@ def test_rows_without_adapter_are_the_projection(ctx, case):
     assert not np.array_equal(out.numpy(), plain.numpy())
 
 
-def test_values_that_are_not_finite_stay_with_their_request(ctx):
+@pytest.mark.parametrize("case", [(1, 1, 16, 64, 64, 8, 3, True), (1, 1, 100, 64, 64, 8, 3, True),
+                                  (1, 1, 2100, 96, 1280, 8, 5, True)])
+def test_values_that_are_not_finite_stay_with_their_request(ctx, case):
     """An adapter of NaN and infinity, and a row of NaN, among rows of other requests in the same tile."""
-    case = (1, 1, 16, 64, 64, 8, 3, True)
     d = make(ctx, case, False)
-    d["slot"][:] = np.arange(16) % 3
+    rows, slots = case[2], case[6]
+    d["slot"][:] = np.arange(rows) % slots
     conv, ad = layer(ctx, case, d, False)
     slot, good, out = E.DeviceArray.from_numpy(ctx, d["slot"]), E.Tensor(ctx), E.Tensor(ctx)
     conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, slot, good)
@@ -119,11 +124,32 @@ def test_values_that_are_not_finite_stay_with_their_request(ctx):
     d["x"][0, 0, 5] = np.nan
     conv, ad = layer(ctx, case, d, False)
     conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, slot, out)
-    bad = (d["slot"] == 1) | (np.arange(16) == 5)
+    bad = (d["slot"] == 1) | (np.arange(rows) == 5)
     got = out.numpy()[0, 0]
     assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
     # the projection repairs tiles with such sums on other instructions: equal but for its roundings
     assert np.abs(got - good.numpy()[0, 0])[~bad].max() < 1e-5
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_f32_ranges(ctx, f16):
+    """Rows, weights and adapters of sizes far from each other and from f16's range keep f32's errors,
+    relative to the terms of their own sums."""
+    case = (1, 1, 2100, 96, 1280, 8, 3, True)
+    d = make(ctx, case, f16)
+    d["x"] *= (10.0 ** (np.arange(2100) % 61 - 30)).astype(np.float32)[None, None, :, None]
+    d["x"][..., :5] *= np.float32(2.0 ** -15)
+    if not f16:
+        d["w"] *= (10.0 ** (np.arange(1280) % 7 - 3)).astype(np.float32)[:, None]
+        d["a"] *= np.array([1e-12, 1.0, 1e6], np.float32)[:, None, None]
+        d["b"] *= np.array([1e5, 1e-5, 1.0], np.float32)[:, None, None]
+    conv, ad = layer(ctx, case, d, f16, bias=False)
+    out = E.Tensor(ctx)
+    conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, E.DeviceArray.from_numpy(ctx, d["slot"]), out)
+    y, base, low = reference(d["x"].reshape(-1, 96), d["w"], None, None, d["a"], d["b"], d["scale"], d["slot"], 1)
+    err = np.abs(out.numpy().reshape(-1, 1280) - y)
+    bound = 1e-5 * base + (96 + 8 + 8) * U * low + U * np.abs(y) + 1e-45
+    assert np.all(err <= bound), (err / bound).max()
 
 
 def test_scratch_and_no_rows(ctx):
@@ -131,7 +157,7 @@ def test_scratch_and_no_rows(ctx):
     d = make(ctx, case, True)
     conv, ad = layer(ctx, case, d, True)
     x, slot, a, b = E.Tensor.from_numpy(ctx, d["x"]), E.DeviceArray.from_numpy(ctx, d["slot"]), E.Tensor(ctx), E.Tensor(ctx)
-    size = ad.scratch(4)
+    size = ad.scratch(4, conv.weight)
     assert size > 0
     conv.forward_adapted(x, ad, slot, a)
     conv.forward_adapted(x, ad, slot, b, scratch=E.DeviceArray(ctx, (size,), np.uint8))
