@@ -537,7 +537,7 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
 /* out [n][q_tokens][heads_q][d] = softmax(scale q . k) v over the keys of the listed
  * blocks (as mh_block_select writes them, in any order: indices outside the item's
  * blocks are skipped, one listed twice counts once), in one pass with f32 scores and
- * sums; scale > 0. Rows that see no key are zero, rows at or above q_len are left as
+ * sums; scale > 0; rows of k and of v less than 32 MiB apart. Rows that see no key are zero, rows at or above q_len are left as
  * they were; what lies at keys a row does not see (NaN among it) does not reach it.
  * f16 tensors: f16 products. f32 tensors: f32 products, or on FAST contexts products
  * of operands rounded to f16. Lists are split over workgroups where rows are few, and

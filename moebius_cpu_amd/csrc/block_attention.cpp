@@ -90,8 +90,6 @@ void block_attention(Context &ctx, const BlockAttention &b, WeightType type, voi
     battn::Args a{};
     a.q = b.q.p, a.k = b.k.p, a.v = b.v.p, a.out = b.out;
     a.ldq = b.q.ld, a.ldo = b.ld_out;
-    MH_REQUIRE(b.k.ld * size < (int64_t(1) << 32) && b.v.ld * size < (int64_t(1) << 32),
-               "block_attention: rows of keys or values 4 GiB apart or more");
     a.ldk = uint32_t(b.k.ld * size), a.ldv = uint32_t(b.v.ld * size);
     a.blocks = b.blocks, a.q_len = s.q_len, a.kv_len = s.kv_len;
     a.part = p.splits > 1 ? reinterpret_cast<float *>(mem) : nullptr;
@@ -112,7 +110,7 @@ void block_attention(Context &ctx, const BlockAttention &b, WeightType type, voi
                         s.kv_tokens, s.heads_kv, s.d, a.dk, s.kv_block, s.kv_len, kp, vp, meta);
         a.k = kp, a.v = vp, a.meta = meta;
         const uint64_t row = uint64_t(s.heads_kv) * 2 * a.dk * 2;
-        MH_REQUIRE(row < (uint64_t(1) << 32), "block_attention: rows of keys or values of 4 GiB or more");
+        MH_REQUIRE(row < (uint64_t(1) << 25), "block_attention: rows of keys or values of 32 MiB or more");
         a.ldk = a.ldv = uint32_t(row);
         battn::launch_split(ctx, a, p.wr, dt, vec);
     } else if (type == kF16) {

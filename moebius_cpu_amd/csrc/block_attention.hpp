@@ -3,7 +3,7 @@
 // For the rows r of a block of queries (query r / G, head hk G + r % G, G query heads
 // per key head: all of them share the list) and the keys j of the listed blocks:
 //   s_j = c q . k_j (c = scale log2 e),  m = max s_j,  p_j = 2^(s_j - m),  o = sum p_j v_j / sum p_j
-// in tiles of KT keys: m' = max(m, tile), o and the sum scaled by 2^(m - m').
+// in tiles of KT keys: where the tile's maximum passes m, o and the sum are scaled by 2^(m - m').
 //
 // A wave takes 32 rows. It forms S^T = K . Q^T, so that a lane holds one row's scores
 // (32x32 instructions: column = lane % 32), the maximum and the sum of a row stay in the
@@ -17,8 +17,8 @@
 // a sum over keys averages. kF32: f32 products (v_mfma_f32_32x32x2_f32, an eighth of the
 // rate). kSplit: each f32 operand as two f16 parts, x = hi + lo to 2^-24, and the three
 // products above 2^-24 of theirs; queries scaled by a power of two per row, keys and values
-// per block (split_kv), probabilities by 2^14, so that the parts keep all bits of values down
-// to 2^-18 of the largest. Scores, maxima, sums and outputs are f32 in all.
+// per block (split_kv), probabilities by 2^11, so that the parts keep all bits of values down
+// to 2^-18 (2^-13) of the largest. Scores, maxima, sums and outputs are f32 in all.
 #pragma once
 
 #include <type_traits>
@@ -61,6 +61,8 @@ struct Args {
 };
 
 constexpr int kSplitExp = 14;  // split operands are scaled to a largest value of 2^14 .. 2^15
+constexpr int kLazyHalf = 8, kLazySplit = 3;  // powers of two by which a row's maximum may pass its reference
+constexpr int kSplitP = 11;    // split probabilities are scaled to at most 2^(11 + 3)
 
 // x 2^e in two f16 parts, x = hi + lo to 2^-24 of it (and 2^-40 of the largest value that e
 // was taken from); a value that is not finite is all in hi.
@@ -154,6 +156,13 @@ __device__ __forceinline__ halfx8 read_vt(const char *v, int lane) {
     return __builtin_bit_cast(halfx8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The value of lane +- 32.
+__device__ __forceinline__ float other_half(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 // Key of accumulator register i in lane half h (32 x 32 results: row of the tile).
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
 
@@ -162,6 +171,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
     using L = Tiling<MODE, DT, WR>;
     typedef std::conditional_t<MODE == kSplit, _Float16, T> S;  // k and v
     constexpr bool SPLIT = MODE == kSplit, HALF = MODE != kF32, KVEC = VEC || SPLIT;
+    constexpr int kLazy = SPLIT ? kLazySplit : kLazyHalf;
     constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP, RUNS = L::kCols / 8;
     constexpr int NT = 64 * WR;                      // threads that stage one tile
     constexpr int KU = (KT * RUNS + NT - 1) / NT;    // runs of 8 channels of K, and of V, per thread
@@ -231,7 +241,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
             }
             for (int x = 32; x; x >>= 1) top = max(top, __shfl_xor(top, x));
             for (int i = lane; i < n; i += 64)
-                v_scale[i] = ldexpf(1.0f, meta[int64_t(list[i] >> a.kb_log) * a.hk].v_exp - top + kSplitExp);
+                v_scale[i] = ldexpf(1.0f, meta[int64_t(list[i] >> a.kb_log) * a.hk].v_exp - top + kSplitP);
             any = __any(any);
             if (lane == 0) v_exp = top, bad = any;
         }
@@ -396,31 +406,34 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
 
         floatx16 sc[SUB];
 #pragma unroll
-        for (int b = 0; b < SUB; ++b) {
+        for (int b = 0; b < SUB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[b][i] = 0.0f;
-            if constexpr (HALF) {
-                const char *p = kst + ((b * 32 + col) * L::kKS + h * 8) * 2;
+        if constexpr (HALF) {
+            const char *p = kst + (col * L::kKS + h * 8) * 2;
 #pragma unroll
-                for (int c = 0; c < DT * 2; ++c) {
-                    const halfx8 kh = *reinterpret_cast<const halfx8 *>(p + c * 32);
+            for (int c = 0; c < DT * 2; ++c)
+#pragma unroll
+                for (int b = 0; b < SUB; ++b) {
+                    const halfx8 kh = *reinterpret_cast<const halfx8 *>(p + (b * 32 * L::kKS + c * 16) * 2);
                     if constexpr (SPLIT) {  // the small products first
-                        const halfx8 kl = *reinterpret_cast<const halfx8 *>(p + DP * 2 + c * 32);
+                        const halfx8 kl = *reinterpret_cast<const halfx8 *>(p + (b * 32 * L::kKS + DP + c * 16) * 2);
                         sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], sc[b], 0, 0, 0);
                         sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], sc[b], 0, 0, 0);
                     }
                     sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], sc[b], 0, 0, 0);
                 }
-            } else {
-                const float *p = reinterpret_cast<const float *>(kst) + (b * 32 + col) * L::kKS + h * 4;
+        } else {
+            const float *p = reinterpret_cast<const float *>(kst) + col * L::kKS + h * 4;
 #pragma unroll
-                for (int c = 0; c < DT * 4; ++c) {
-                    const floatx4 kv = *reinterpret_cast<const floatx4 *>(p + c * 8);
+            for (int c = 0; c < DT * 4; ++c)
+#pragma unroll
+                for (int b = 0; b < SUB; ++b) {
+                    const floatx4 kv = *reinterpret_cast<const floatx4 *>(p + b * 32 * L::kKS + c * 8);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         sc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[j], qf[c * 4 + j], sc[b], 0, 0, 0);
                 }
-            }
         }
         float vs[SPLIT ? 2 * SUB : 1];  // scales of the values of each sixteen keys, times the probabilities' own
         if constexpr (SPLIT) {
@@ -450,11 +463,12 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
         for (int b = 0; b < SUB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, sc[b][i]);
-        mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32)) * c;
-        const float mn = __builtin_fmaxf(m, mx);
-        const float mu = mn == kNegInf ? 0.0f : mn;
-        if (__any(mn > m)) {
-            const float f = __builtin_amdgcn_exp2f(m - mu);  // 0 before the first key
+        mx = __builtin_fmaxf(mx, other_half(mx)) * c;
+        // The reference m follows the maximum only when that has grown by 2^kLazy: probabilities
+        // stay below 2^kLazy and most tiles leave the sums as they are.
+        if (__any(mx > m + float(kLazy))) {
+            const float mn = __builtin_fmaxf(m, mx);
+            const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));  // 0 before the first key
             l *= f;
 #pragma unroll
             for (int t = 0; t < DT; ++t)
@@ -462,6 +476,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
                 for (int i = 0; i < 16; ++i) o[t][i] *= f;
             m = mn;
         }
+        const float mu = m == kNegInf ? 0.0f : m;
         // The fused exponent is off by half a step of m, which is nothing until scores are so large
         // that the largest key's power would leave the range: their products are rounded first.
         const bool far = !SPLIT && __any(__builtin_fabsf(mu) > 1048576.0f);
@@ -555,7 +570,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] = ldexpf(o[t][i], v_exp - 2 * kSplitExp);
+            for (int i = 0; i < 16; ++i) o[t][i] = ldexpf(o[t][i], v_exp - kSplitExp - kSplitP);
     }
     // The values that were staged as zeros because they are not finite, for the rows that see them.
     if (bad) {

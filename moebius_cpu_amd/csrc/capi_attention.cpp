@@ -240,6 +240,8 @@ int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const v
         const Rows vi = rows_of(v, kv_rows, a.s.heads_kv, a.s.d, ld_v, t, "v");
         const Rows to = rows_of(out, q_rows, a.s.heads_q, a.s.d, ld_out, t, "out");
         if (q_rows) need(blocks, "blocks");
+        if (ki.ld * int64_t(ki.size) >= (1 << 25) || vi.ld * int64_t(vi.size) >= (1 << 25))
+            mh::fail(mh::kInvalidArgument, "rows of k or v 32 MiB apart or more");
         if (!(scale > 0) || !std::isfinite(scale)) mh::fail(mh::kInvalidArgument, "scale is positive and finite");
         no_overlap(qi, to, "q and out");
         no_overlap(ki, to, "k and out");

@@ -113,8 +113,9 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
     const int c0 = (w % g.tiles_m) * BT;
     const int64_t r0 = int64_t(w / g.tiles_m) * BT;
 
-    halfx8 xr[XU], wv[WU];
-    auto fetch = [&](int k) {
+    // Two stages are loaded ahead of the one that is staged.
+    halfx8 xr[2][XU], wv[2][WU];
+    auto fetch = [&](int k, halfx8 (&xr)[XU], halfx8 (&wv)[WU]) {
 #pragma unroll
         for (int u = 0; u < XU; ++u) {
             const int i = tid + u * 256, r = i / 8, run = i % 8;  // four runs of hi, four of lo
@@ -137,8 +138,7 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
         for (int n = 0; n < S; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.0f;
-    fetch(0);
-    for (int k = 0; k < g.cip; k += kGK) {
+    auto step = [&](int k, halfx8 (&xr)[XU], halfx8 (&wv)[WU]) {
         if (k) __syncthreads();
 #pragma unroll
         for (int u = 0; u < XU; ++u) {
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
             *reinterpret_cast<halfx8 *>(ws + i / (4 * WP) * WS + i % (4 * WP) * 8) = wv[u];
         }
         __syncthreads();
-        if (k + kGK < g.cip) fetch(k + kGK);
+        if (k + 2 * kGK < g.cip) fetch(k + 2 * kGK, xr, wv);
 #pragma unroll
         for (int c = 0; c < kGK / 16; ++c) {
             halfx8 xh[S], xl[S];
@@ -176,6 +176,12 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
                 for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xh[n], acc[m][n]);
             }
         }
+    };
+    fetch(0, xr[0], wv[0]);
+    if (kGK < g.cip) fetch(kGK, xr[1], wv[1]);
+    for (int k = 0; k < g.cip; k += 2 * kGK) {
+        step(k, xr[0], wv[0]);
+        if (k + kGK < g.cip) step(k + kGK, xr[1], wv[1]);
     }
 
     // Columns 8 f + 4 h + e of a 32-tile are register 4 f + e; the row is lane % 32.

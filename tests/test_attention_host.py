@@ -130,6 +130,7 @@ def test_attention_shape_refusals(kw, text):
     (dict(v=None), "v is NULL"), (dict(out=None), "out is NULL"), (dict(blocks=None), "blocks is NULL"),
     (dict(out=M), "overlap"), (dict(out=2 * M), "overlap"), (dict(out=3 * M + 64), "overlap"),
     (dict(lds=(255, 128, 128, 256)), "ld is less"), (dict(lds=(256, 127, 128, 256)), "ld is less"),
+    (dict(lds=(256, 1 << 24, 128, 256)), "32 MiB"), (dict(lds=(256, 128, 1 << 24, 256)), "32 MiB"),
     (dict(dtype=9), "dtype"), (dict(k=2 * M + 1), "not aligned"), (dict(), "context is NULL")])
 def test_attention_refusals(kw, text):
     refused(attend(**kw), text)
