@@ -20,7 +20,10 @@ from . import _lib
 from ._lib import MoebiusError, check, lib
 from .engine import Context, DeviceArray, _ptr
 
-_DTYPE = {np.dtype(np.float32): _lib.DTYPE_F32, np.dtype(np.float16): _lib.DTYPE_F16}
+# The calls below are a few microseconds on the host, of single tokens as long as on the
+# device: what a view or a table fixes is worked out when it is made.
+_F32, _I32 = np.dtype(np.float32), np.dtype(np.int32)
+_DTYPE = {_F32: _lib.DTYPE_F32, np.dtype(np.float16): _lib.DTYPE_F16}
 
 
 class Heads:
@@ -41,18 +44,14 @@ class Heads:
         if rows and (offset + (rows - 1) * self.ld + heads * d) * self.dtype.itemsize > buf.nbytes:
             raise MoebiusError(1, "heads exceed their buffer")
         self._offset = int(offset) * self.dtype.itemsize
-
-    @property
-    def ctx(self) -> Context:
-        return self.buf.ctx
+        self.ctx: Context = buf.ctx
+        self.rows = rows
+        self._kind = (self.code, self.d)
+        self._shape = (self.code, self.d, self.n, self.tokens, self.heads)
 
     @property
     def ptr(self) -> int:
         return self.buf.ptr + self._offset
-
-    @property
-    def rows(self) -> int:
-        return self.n * self.tokens
 
     def numpy(self) -> np.ndarray:
         """A copy [n, tokens, heads, d]."""
@@ -64,13 +63,14 @@ class Heads:
         return view.copy().reshape(self.n, self.tokens, self.heads, self.d)
 
 
-def _same(*heads):
-    if len({(h.dtype, h.d) for h in heads}) != 1:
-        raise MoebiusError(1, "heads differ in type or channels")
+def _same(a, *heads):
+    for b in heads:
+        if a._kind != b._kind:
+            raise MoebiusError(1, "heads differ in type or channels")
 
 
 def _int32(a, size, what):
-    if a is not None and (a.dtype != np.int32 or a.nbytes != 4 * size):
+    if a is not None and (a.dtype != _I32 or a.nbytes != 4 * size):
         raise MoebiusError(1, f"{what} is int32 of {size} entries")
 
 
@@ -94,23 +94,26 @@ class RopeAxes:
         if freq.shape != (pairs,):
             raise MoebiusError(1, f"rope: {pairs} frequencies")
         self.freq = DeviceArray.from_numpy(ctx, freq)
+        self._dims = (ctypes.c_uint32 * 4)(*self.axis_dims)
 
     def _args(self, positions: DeviceArray, inverse: bool):
-        axes = len(self.axis_dims)
-        if positions.dtype != np.int32 or len(positions.shape) != 2 or positions.shape[1] != axes:
+        axes, shape = len(self.axis_dims), positions.shape
+        if positions.dtype != _I32 or len(shape) != 2 or shape[1] != axes:
             raise MoebiusError(1, f"positions are int32 [rows][{axes}]")
-        return ctypes.byref(_lib.Rope(positions.ptr, positions.shape[0], self.freq.ptr, axes,
-                                      (ctypes.c_uint32 * 4)(*self.axis_dims), self.pairing, int(inverse), 0))
+        return ctypes.byref(_lib.Rope(positions.ptr, shape[0], self.freq.ptr, axes, self._dims, self.pairing,
+                                      1 if inverse else 0, 0))
 
 
 def rope_axes(x: Heads, positions: DeviceArray, rope: RopeAxes, out: Heads, inverse: bool = False):
     """out = x turned by its rows' positions [pos_rows, axes] (row r by positions[r % pos_rows]);
     out may be x. inverse: by the negative angles."""
     _same(x, out)
-    if (x.rows, x.heads) != (out.rows, out.heads):
+    if x.rows != out.rows or x.heads != out.heads:
         raise MoebiusError(1, "x and out differ in shape")
-    check(lib().mh_rope_axes(x.ctx.h, x.ptr, x.code, x.rows, x.heads, x.d, x.ld, rope._args(positions, inverse),
-                             out.ptr, out.ld))
+    st = lib().mh_rope_axes(x.ctx.h, x.ptr, x.code, x.rows, x.heads, x.d, x.ld, rope._args(positions, inverse), out.ptr,
+                            out.ld)
+    if st:
+        check(st)
 
 
 def qk_norm_rope(q: Heads, k: Heads, gamma_q: DeviceArray | None, gamma_k: DeviceArray | None, eps: float,
@@ -118,14 +121,17 @@ def qk_norm_rope(q: Heads, k: Heads, gamma_q: DeviceArray | None, gamma_k: Devic
     """RMS norm (scales gamma [d], None: ones) of every query and key head, then the rotation,
     in one pass; outputs may be their inputs."""
     _same(q, k, q_out, k_out)
-    if (q.rows, q.heads, k.rows, k.heads) != (q_out.rows, q_out.heads, k_out.rows, k_out.heads) or q.rows != k.rows:
+    rows = q.rows
+    if not (rows == k.rows == q_out.rows == k_out.rows and q.heads == q_out.heads and k.heads == k_out.heads):
         raise MoebiusError(1, "q, k and their outputs differ in shape")
     for g in (gamma_q, gamma_k):
-        if g is not None and (g.dtype != np.float32 or g.nbytes != 4 * q.d):
+        if g is not None and (g.dtype != _F32 or g.nbytes != 4 * q.d):
             raise MoebiusError(1, "gamma is f32 of the head's channels")
-    check(lib().mh_qk_norm_rope(q.ctx.h, q.ptr, q.ld, q.heads, k.ptr, k.ld, k.heads, q.code, q.rows, q.d,
-                                _ptr(gamma_q), _ptr(gamma_k), float(eps), rope._args(positions, False), q_out.ptr,
-                                q_out.ld, k_out.ptr, k_out.ld))
+    st = lib().mh_qk_norm_rope(q.ctx.h, q.ptr, q.ld, q.heads, k.ptr, k.ld, k.heads, q.code, rows, q.d, _ptr(gamma_q),
+                               _ptr(gamma_k), eps, rope._args(positions, False), q_out.ptr, q_out.ld, k_out.ptr,
+                               k_out.ld)
+    if st:
+        check(st)
 
 
 def block_means(x: Heads, block: int, means: DeviceArray, length: DeviceArray | None = None,
@@ -133,7 +139,7 @@ def block_means(x: Heads, block: int, means: DeviceArray, length: DeviceArray | 
     """means [n, ceil(tokens / block), heads, d] f32: every block's mean over its tokens below
     length [n]; blocks at or below first [n] and those behind the length are left as they were."""
     blocks = -(-x.tokens // max(int(block), 1))
-    if means.dtype != np.float32 or means.nbytes != 4 * x.n * blocks * x.heads * x.d:
+    if means.dtype != _F32 or means.nbytes != 4 * x.n * blocks * x.heads * x.d:
         raise MoebiusError(1, "means are f32 [n, blocks, heads, d]")
     _int32(length, x.n, "length")
     _int32(first, x.n, "first")
@@ -142,7 +148,7 @@ def block_means(x: Heads, block: int, means: DeviceArray, length: DeviceArray | 
 
 
 def _shape(q: Heads, kv_tokens, heads_kv, blocks: DeviceArray, q_block, kv_block, causal, q_len, kv_len):
-    if blocks.dtype != np.int32 or len(blocks.shape) != 4 or \
+    if blocks.dtype != _I32 or len(blocks.shape) != 4 or \
             blocks.shape[:3] != (q.n, -(-q.tokens // max(int(q_block), 1)), heads_kv):
         raise MoebiusError(1, "blocks are int32 [n, blocks of queries, key heads, top]")
     _int32(q_len, q.n, "q_len")
@@ -160,7 +166,7 @@ def block_select(q: Heads, means: DeviceArray, kv_tokens: int, blocks: DeviceArr
     heads_kv = blocks.shape[2] if len(blocks.shape) == 4 else 0
     s = _shape(q, kv_tokens, heads_kv, blocks, q_block, kv_block, causal, q_len, kv_len)
     nk = -(-int(kv_tokens) // max(int(kv_block), 1))
-    if means.dtype != np.float32 or means.nbytes != 4 * q.n * nk * heads_kv * q.d:
+    if means.dtype != _F32 or means.nbytes != 4 * q.n * nk * heads_kv * q.d:
         raise MoebiusError(1, "means are f32 [n, blocks, key heads, d]")
     check(lib().mh_block_select(q.ctx.h, q.ptr, q.code, q.ld, ctypes.byref(s), means.ptr, blocks.ptr))
 

@@ -25,11 +25,13 @@ namespace {
 constexpr int kRankTiles = 4;     // 16 ranks each per pass over x
 constexpr int kShrinkUnroll = 5;  // steps of the long axis whose loads are in flight together
 
-// Workgroup (16 rows, split of the long axis); wave w takes every fourth 16 of its share.
+constexpr int kShrinkWaves = 8;
+
+// Workgroup (16 rows, split of the long axis); wave w takes an eighth of its share.
 // Lane l holds row (rank) l % 16 and four values of the long axis at 4 (l / 16).
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
-    __shared__ float part[4][kRankTiles][4][64];
+__global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs p) {
+    __shared__ float part[kShrinkWaves][kRankTiles][4][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
     const int64_t r0 = int64_t(blockIdx.x) * 16;
     const int k0 = int(blockIdx.y) * p.chunk, k1 = min(k0 + p.chunk, p.ci);
@@ -48,16 +50,18 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
                 acc[j] = floatx4{0, 0, 0, 0};
                 a[j] = static_cast<const T *>(p.a) + (int64_t(s) * p.rank + min(q0 + j * 16 + r16, p.rank - 1)) * p.ci;
             }
-            for (int k = k0 + wave * 16; k < k1; k += 64 * kShrinkUnroll) {
+            const int share = ((k1 - k0 + 15) / 16 + kShrinkWaves - 1) / kShrinkWaves * 16, kw = k0 + wave * share;
+            const int ke = min(kw + share, k1);
+            for (int k = kw; k < ke; k += 16 * kShrinkUnroll) {
                 floatx4 xv[kShrinkUnroll];
 #pragma unroll
-                for (int u = 0; u < kShrinkUnroll; ++u) xv[u] = load4<VEC>(x, k + u * 64 + kg * 4, k1);
+                for (int u = 0; u < kShrinkUnroll; ++u) xv[u] = load4<VEC>(x, k + u * 16 + kg * 4, ke);
 #pragma unroll
                 for (int j = 0; j < kRankTiles; ++j) {
                     if (q0 + j * 16 < p.rank) {
                         floatx4 av[kShrinkUnroll];
 #pragma unroll
-                        for (int u = 0; u < kShrinkUnroll; ++u) av[u] = load4<VEC>(a[j], k + u * 64 + kg * 4, k1);
+                        for (int u = 0; u < kShrinkUnroll; ++u) av[u] = load4<VEC>(a[j], k + u * 16 + kg * 4, ke);
 #pragma unroll
                         for (int u = 0; u < kShrinkUnroll; ++u)
 #pragma unroll
@@ -73,12 +77,12 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs p) {
             __syncthreads();
             // wave w joins rank tile w; register e is rank 4 (l / 16) + e of row l % 16
             const int q = q0 + wave * 16 + kg * 4;
-            if (q0 + wave * 16 < p.rank && own && r0 + r16 < p.rows) {
-                floatx4 v;
+            if (wave < kRankTiles && q0 + wave * 16 < p.rank && own && r0 + r16 < p.rows) {
+                floatx4 v = {0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = (part[0][wave][e][lane] + part[1][wave][e][lane]) +
-                           (part[2][wave][e][lane] + part[3][wave][e][lane]);
+                for (int w = 0; w < kShrinkWaves; ++w)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] += part[w][wave][e][lane];
                 *reinterpret_cast<floatx4 *>(p.t + (int64_t(blockIdx.y) * p.rows + r0 + r16) * p.rank_pad + q) = v;
             }
         }
@@ -259,7 +263,7 @@ template <typename T>
 void run_shrink(Context &ctx, const LoraArgs &p) {
     const int64_t tiles = ceil_div(p.rows, 16);
     MH_REQUIRE(tiles < (int64_t(1) << 31), "lora: too many rows");
-    const dim3 tb{256};
+    const dim3 tb{64 * kShrinkWaves};
     const bool vx = p.ci % 4 == 0 && aligned16(p.x) && reinterpret_cast<uintptr_t>(p.a) % (4 * sizeof(T)) == 0;
     const dim3 sg{uint32_t(tiles), uint32_t(p.splits)};
     if (vx) lora_shrink_kernel<T, true><<<sg, tb, 0, ctx.stream>>>(p);
@@ -308,7 +312,7 @@ bool use_gemm(const Context &ctx, int64_t rows, int c_in, int c_out) {
 
 Layout layout(const Context &ctx, int64_t rows, int c_in, int c_out, WeightType wt, int rank) {
     auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
-    const size_t cip = size_t(ceil_div(c_in, 32) * 32);
+    const size_t cip = size_t(ceil_div(c_in, 64) * 64);
     Layout l;
     const bool own = use_gemm(ctx, rows, c_in, c_out);
     l.t = up(size_t(lora_splits(ctx, rows, c_in, own)) * size_t(rows) * size_t(ceil_div(rank, 16) * 16) * sizeof(float));
@@ -363,7 +367,7 @@ void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const vo
     }
     lora::GemmArgs g{};
     g.l = p;
-    g.cip = int(ceil_div(c_in, 32) * 32);
+    g.cip = int(ceil_div(c_in, 64) * 64);
     auto *xp = reinterpret_cast<_Float16 *>(at + mem.t);
     auto *xe = reinterpret_cast<int *>(at + mem.t + mem.x);
     lora::split_rows(ctx, x, rows, c_in, g.cip, xp, xe);

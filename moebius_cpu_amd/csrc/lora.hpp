@@ -54,7 +54,7 @@ __device__ __forceinline__ floatx4 mfma(float a, float b, floatx4 c) {
 
 __device__ __forceinline__ int slot_of(const LoraArgs &p, int64_t row) {
     if (row >= p.rows) return -1;
-    const int s = p.slot[row / p.rows_per_slot];
+    const int s = p.slot[uint32_t(row) / uint32_t(p.rows_per_slot)];  // both below 2^31
     return s < p.slots ? s : -1;
 }
 
@@ -79,7 +79,7 @@ struct GemmArgs {
     const _Float16 *xp;      // [rows][2][cip]
     const int *x_exp;        // [rows]
     const float *bias, *residual;
-    int cip;                 // ci rounded up to 32
+    int cip;                 // ci rounded up to 64
     int tiles_m, tiles_n;    // of columns, of rows
 };
 // x [rows][ci] -> parts [rows][2][cip] (zeros behind ci) and each row's exponent.

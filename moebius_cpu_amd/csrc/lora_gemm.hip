@@ -8,7 +8,7 @@
 //
 // A workgroup forms BT columns x BT rows, its four waves 2 x 2 quarters, as W . X^T: a lane
 // of a 32x32 result holds one row and four runs of four columns, so a row's scale and its
-// adapter are the lane's own. 32 of the long axis are staged in LDS at a time while the
+// adapter are the lane's own. 64 of the long axis are staged in LDS at a time while the
 // next are loaded. Bound: the matrix instructions; the parts of x are written and read
 // once more than x itself.
 #include <algorithm>
@@ -92,15 +92,25 @@ __device__ __forceinline__ floatx16 mfma16(halfx8 a, halfx8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-constexpr int kGK = 32;  // of the long axis per stage
+// Eight ranks of a row of t (padded to sixteens), zeros behind the last and where not wanted.
+__device__ __forceinline__ void read_t(const float *t, int k, int rank, bool want, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const floatx4 r = *reinterpret_cast<const floatx4 *>(t + k + 4 * j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * j + e] = want && k + 4 * j + e < rank ? r[e] : 0.0f;
+    }
+}
+
+constexpr int kGK = 64;  // of the long axis per stage
 
 // WP: parts of the weight (1: f16 as stored, rows of ci; 2: rows of 2 cip); VW: its rows
 // allow 16-byte loads; T: the adapters' storage.
 template <int BT, int WP, bool VW, typename T>
-__global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
+__global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArgs g) {
     constexpr int S = BT / 64;                        // 32-tiles of a wave in each direction
     constexpr int XS = 2 * kGK + 8, WS = WP * kGK + 8;  // staged rows (halves), on distinct banks
-    constexpr int XU = BT * 2 * kGK / 8 / 256, WU = BT * WP * kGK / 8 / 256;  // runs per thread
+    constexpr int R = kGK / 8, XU = BT * 2 * R / 256, WU = BT * WP * R / 256;  // runs of 8 per part, per thread
     __shared__ __align__(16) _Float16 xs[BT * XS], ws[BT * WS];
     const LoraArgs &p = g.l;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -113,24 +123,41 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
     const int c0 = (w % g.tiles_m) * BT;
     const int64_t r0 = int64_t(w / g.tiles_m) * BT;
 
-    // Two stages are loaded ahead of the one that is staged.
-    halfx8 xr[2][XU], wv[2][WU];
-    auto fetch = [&](int k, halfx8 (&xr)[XU], halfx8 (&wv)[WU]) {
+    // A thread's runs: the same place of rows 256 / (2 R) (columns 256 / (WP R)) apart, as
+    // offsets from the tile's first, which the step moves on. The runs of hi, then of lo.
+    static_assert(256 % (2 * R) == 0, "runs");
+    halfx8 xr[XU], wv[WU];
+    uint32_t xo[XU], wo[WU];
+    const int xrun = tid % (2 * R), wrun = tid % (WP * R);
 #pragma unroll
-        for (int u = 0; u < XU; ++u) {
-            const int i = tid + u * 256, r = i / 8, run = i % 8;  // four runs of hi, four of lo
-            xr[u] = *reinterpret_cast<const halfx8 *>(g.xp + (min(r0 + r, p.rows - 1) * 2 + run / 4) * g.cip + k + run % 4 * 8);
-        }
+    for (int u = 0; u < XU; ++u) {
+        const int r = int(min(int64_t(tid / (2 * R) + u * (256 / (2 * R))), p.rows - 1 - r0));
+        xo[u] = uint32_t((r * 2 + xrun / R) * g.cip + xrun % R * 8) * 2;
+    }
+#pragma unroll
+    for (int u = 0; u < WU; ++u) {
+        const int c = min(tid / (WP * R) + u * (256 / (WP * R)), p.co - 1 - c0);
+        wo[u] = uint32_t(WP == 2 ? (c * 2 + wrun / R) * g.cip + wrun % R * 8 : c * p.ci) * 2;
+    }
+    const char *xb = reinterpret_cast<const char *>(g.xp + r0 * 2 * g.cip);
+    const char *wb = static_cast<const char *>(g.w) + int64_t(c0) * (WP == 2 ? 2 * g.cip : p.ci) * 2;
+    auto fetch = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < XU; ++u) xr[u] = *reinterpret_cast<const halfx8 *>(xb + k * 2 + xo[u]);
 #pragma unroll
         for (int u = 0; u < WU; ++u) {
-            const int i = tid + u * 256, c = min(c0 + i / (4 * WP), p.co - 1), run = i % (4 * WP);
-            const _Float16 *wp = static_cast<const _Float16 *>(g.w);
-            if constexpr (WP == 2)
-                wv[u] = *reinterpret_cast<const halfx8 *>(wp + (int64_t(c) * 2 + run / 4) * g.cip + k + run % 4 * 8);
-            else
-                wv[u] = load8<VW>(wp + int64_t(c) * p.ci, k + run * 8, p.ci);
+            if constexpr (WP == 2) wv[u] = *reinterpret_cast<const halfx8 *>(wb + k * 2 + wo[u]);
+            else wv[u] = load8<VW>(reinterpret_cast<const _Float16 *>(wb + wo[u]), k + wrun * 8, p.ci);
         }
     };
+    // The adapters of this lane's rows and the exponents of their parts.
+    int slot[S], xe[S];
+#pragma unroll
+    for (int n = 0; n < S; ++n) {
+        const int64_t row = r0 + (wn * S + n) * 32 + l32;
+        slot[n] = slot_of(p, row);
+        xe[n] = g.x_exp[min(row, p.rows - 1)] - kSplitExp;
+    }
     floatx16 acc[S][S];
 #pragma unroll
     for (int m = 0; m < S; ++m)
@@ -138,20 +165,21 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
         for (int n = 0; n < S; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.0f;
-    auto step = [&](int k, halfx8 (&xr)[XU], halfx8 (&wv)[WU]) {
+    fetch(0);
+    for (int k = 0; k < g.cip; k += kGK) {
         if (k) __syncthreads();
 #pragma unroll
         for (int u = 0; u < XU; ++u) {
             const int i = tid + u * 256;
-            *reinterpret_cast<halfx8 *>(xs + i / 8 * XS + i % 8 * 8) = xr[u];
+            *reinterpret_cast<halfx8 *>(xs + i / (2 * R) * XS + i % (2 * R) * 8) = xr[u];
         }
 #pragma unroll
         for (int u = 0; u < WU; ++u) {
             const int i = tid + u * 256;
-            *reinterpret_cast<halfx8 *>(ws + i / (4 * WP) * WS + i % (4 * WP) * 8) = wv[u];
+            *reinterpret_cast<halfx8 *>(ws + i / (WP * R) * WS + i % (WP * R) * 8) = wv[u];
         }
         __syncthreads();
-        if (k + 2 * kGK < g.cip) fetch(k + 2 * kGK, xr, wv);
+        if (k + kGK < g.cip) fetch(k + kGK);
 #pragma unroll
         for (int c = 0; c < kGK / 16; ++c) {
             halfx8 xh[S], xl[S];
@@ -176,12 +204,6 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
                 for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xh[n], acc[m][n]);
             }
         }
-    };
-    fetch(0, xr[0], wv[0]);
-    if (kGK < g.cip) fetch(kGK, xr[1], wv[1]);
-    for (int k = 0; k < g.cip; k += 2 * kGK) {
-        step(k, xr[0], wv[0]);
-        if (k + kGK < g.cip) step(k + kGK, xr[1], wv[1]);
     }
 
     // Columns 8 f + 4 h + e of a 32-tile are register 4 f + e; the row is lane % 32.
@@ -190,30 +212,31 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
 #pragma unroll
     for (int n = 0; n < S; ++n) {
         const int64_t row = r0 + (wn * S + n) * 32 + l32, row_in = min(row, p.rows - 1);
-        const int xe = g.x_exp[row_in] - kSplitExp;
 #pragma unroll
         for (int m = 0; m < S; ++m)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                int e = xe;
+                int e = xe[n];
                 if constexpr (WP == 2)
                     e += g.w_exp[min(c0 + (wm * S + m) * 32 + 8 * (i / 4) + 4 * h + i % 4, p.co - 1)] - kSplitExp;
                 acc[m][n][i] = ldexpf(acc[m][n][i], e);
             }
-        const int mine = slot_of(p, row);
+        const int mine = slot[n];
         uint32_t todo = uint32_t(__ballot(mine >= 0));
         if (todo) {
             const float *t = p.t + row_in * p.rank_pad;
             int te = 0;
             if constexpr (sizeof(T) == 2) {  // the row of t in two parts, as x
                 float mx = 0.0f;
-                if (mine >= 0)
-                    for (int k = 0; k < p.rank; k += 16)
+                for (int k = 0; k < p.rank; k += 16) {
+                    float tv[8];
+                    read_t(t, k + h * 8, p.rank, mine >= 0, tv);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float f = k + h * 8 + i < p.rank ? __builtin_fabsf(t[k + h * 8 + i]) : 0.0f;
-                            mx = f < __builtin_huge_valf() ? __builtin_fmaxf(mx, f) : mx;
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        const float f = __builtin_fabsf(tv[i]);
+                        mx = f < __builtin_huge_valf() ? __builtin_fmaxf(mx, f) : mx;
+                    }
+                }
                 mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
                 te = top_exp(mx);
             }
@@ -233,8 +256,7 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
                            (int64_t(s) * p.co + min(c0 + (wm * S + m) * 32 + l32, p.co - 1)) * p.rank;
                 for (int k = 0; k < p.rank; k += 16) {
                     float tv[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) tv[i] = own && k + h * 8 + i < p.rank ? t[k + h * 8 + i] : 0.0f;
+                    read_t(t, k + h * 8, p.rank, own, tv);
                     if constexpr (sizeof(T) == 2) {
                         halfx8 th, tl;
 #pragma unroll
@@ -279,8 +301,9 @@ __global__ __launch_bounds__(256, 2) void lora_gemm_kernel(GemmArgs g) {
                 const float *res = g.residual ? g.residual + row * p.co + c : nullptr;
                 if (vo && c < p.co) {
                     floatx4 y = {acc[m][n][4 * f], acc[m][n][4 * f + 1], acc[m][n][4 * f + 2], acc[m][n][4 * f + 3]};
+                    if (g.bias)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] += g.bias ? g.bias[c + e] : 0.0f;
+                        for (int e = 0; e < 4; ++e) y[e] += g.bias[c + e];
                     if (res) y += *reinterpret_cast<const floatx4 *>(res);
                     *reinterpret_cast<floatx4 *>(out) = y;
                 } else {

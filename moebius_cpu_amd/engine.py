@@ -172,6 +172,9 @@ class DeviceArray:
             pass
 
 
+_I32 = np.dtype(np.int32)
+
+
 def _ptr(t):
     return None if t is None else t.ptr
 
@@ -279,7 +282,7 @@ class Conv1x1:
             raise MoebiusError(1, "Conv1x1 input channels")
         if len(self.weight) != self.c_in * self.c_out:
             raise MoebiusError(1, "Conv1x1 weight size")
-        if slot.dtype != np.int32 or slot.nbytes // 4 not in (x.n, x.pixels()):
+        if slot.dtype != _I32 or slot.nbytes // 4 not in (x.n, x.pixels()):
             raise MoebiusError(1, "slot is int32, one for each item or each pixel")
         out.set_shape(x.n, x.h, x.w, self.c_out)
         if residual is not None and residual.shape != out.shape:
