@@ -317,7 +317,7 @@ Layout layout(const Context &ctx, int64_t rows, int c_in, int c_out, WeightType 
     const bool own = use_gemm(ctx, rows, c_in, c_out);
     l.t = up(size_t(lora_splits(ctx, rows, c_in, own)) * size_t(rows) * size_t(ceil_div(rank, 16) * 16) * sizeof(float));
     if (own) {
-        l.x = up(size_t(rows) * 2 * cip * 2);
+        l.x = up(size_t(padded_rows(rows)) * 2 * cip * 2);
         l.x_exp = up(size_t(rows) * 4);
         if (wt == kF32) {
             l.w = up(size_t(c_out) * 2 * cip * 2);
@@ -358,9 +358,9 @@ void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const vo
         else lora::run_few<float, float>(ctx, p, weight, bias, residual);
         return;
     }
-    if (ah) lora::run_shrink<_Float16>(ctx, p);
-    else lora::run_shrink<float>(ctx, p);
     if (!own) {
+        if (ah) lora::run_shrink<_Float16>(ctx, p);
+        else lora::run_shrink<float>(ctx, p);
         if (ah) lora::run_expand<_Float16>(ctx, p);
         else lora::run_expand<float>(ctx, p);
         return;
@@ -370,7 +370,12 @@ void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const vo
     g.cip = int(ceil_div(c_in, 64) * 64);
     auto *xp = reinterpret_cast<_Float16 *>(at + mem.t);
     auto *xe = reinterpret_cast<int *>(at + mem.t + mem.x);
-    lora::split_rows(ctx, x, rows, c_in, g.cip, xp, xe);
+    if (ah) {
+        lora::split_shrink(ctx, p, g.cip, xp, xe);
+    } else {
+        lora::run_shrink<float>(ctx, p);
+        lora::split_rows(ctx, x, rows, c_in, g.cip, xp, xe);
+    }
     g.xp = xp, g.x_exp = xe, g.w = weight, g.bias = bias, g.residual = residual;
     if (wt == kF32) {
         auto *wp = reinterpret_cast<_Float16 *>(at + mem.t + mem.x + mem.x_exp);

@@ -84,6 +84,10 @@ struct GemmArgs {
 };
 // x [rows][ci] -> parts [rows][2][cip] (zeros behind ci) and each row's exponent.
 void split_rows(Context &ctx, const float *x, int64_t rows, int ci, int cip, _Float16 *parts, int *exps);
+// The same of p.x and, for f16 adapters, p.t of every row that has one.
+void split_shrink(Context &ctx, const LoraArgs &p, int cip, _Float16 *parts, int *exps);
+// Rows that the parts of x have room for.
+inline int64_t padded_rows(int64_t rows) { return ceil_div(rows, 128) * 128; }
 // Whether that kernel is the faster way for these sizes.
 bool gemm_fits(const Context &ctx, int64_t rows, int c_out, int c_in);
 // weight: wt, or f32 in parts.

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void split_rows_kernel(const float *x, int64_t
     if (lane == 0) exps[row] = e;
 }
 
-// Eight values of a row of n at k, zeros behind it.
+// Eight values of a row of n at k, zeros behind it (VEC: n and p allow 16-byte loads).
 template <bool VEC>
 __device__ __forceinline__ halfx8 load8(const _Float16 *p, int k, int n) {
     halfx8 v;
@@ -90,6 +90,113 @@ __device__ __forceinline__ halfx8 load8(const _Float16 *p, int k, int n) {
 
 __device__ __forceinline__ floatx16 mfma16(halfx8 a, halfx8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+typedef floatx4 accx4;
+
+// split_rows and the adapters' first product of 16 rows in one pass over x, for adapters
+// stored in f16: t = 2^-e (hi A^T + lo A^T) on v_mfma_f32_16x16x32_f16. Eight waves share
+// the long axis, 32 values of 16 rows per step (lane: row l % 16, values 8 (l / 16) ..),
+// kUnits steps in registers between the row's maximum and its parts; longer rows are read
+// again. Bound: memory, x read and its parts written.
+constexpr int kUnits = 5, kPassWaves = 8, kPass = kUnits * kPassWaves * 32;
+
+template <bool VEC>
+__global__ __launch_bounds__(64 * kPassWaves) void split_shrink_kernel(LoraArgs p, int cip, _Float16 *parts, int *exps) {
+    __shared__ float wave_max[kPassWaves][16];
+    __shared__ float part[kPassWaves][4][64];
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t r0 = int64_t(blockIdx.x) * 16, row = r0 + r16;
+    const int mine = slot_of(p, row);
+    const float *x = p.x + min(row, p.rows - 1) * p.ci;
+    const int passes = (cip + kPass - 1) / kPass;
+    floatx4 v[kUnits][2];
+    auto load = [&](int pass) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                v[u][j] = load4<VEC>(x, pass * kPass + (wave * kUnits + u) * 32 + kg * 8 + j * 4, p.ci);
+    };
+    float mx = 0.0f;
+    for (int pass = passes - 1; pass >= 0; --pass) {
+        load(pass);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float f = __builtin_fabsf(v[u][i / 4][i % 4]);
+                mx = f < __builtin_huge_valf() ? __builtin_fmaxf(mx, f) : mx;
+            }
+    }
+    mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
+    mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+    if (lane < 16) wave_max[wave][lane] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPassWaves; ++w) mx = __builtin_fmaxf(mx, wave_max[w][r16]);
+    const int e = top_exp(mx);
+    if (tid < 16 && row < p.rows) exps[row] = e;
+
+    const uint32_t rows16 = uint32_t(__ballot(mine >= 0)) & 0xFFFFu;
+    // Adapters one after another, ranks sixteen at a time; the parts are written by the first round.
+    uint32_t todo = rows16;
+    bool first = true;
+    do {
+        const int s = todo ? __builtin_amdgcn_readfirstlane(__shfl(mine, __builtin_ctz(todo))) : -1;
+        const bool own = s >= 0 && mine == s;
+        todo &= ~uint32_t(__ballot(own));
+        for (int q0 = 0; q0 < p.rank; q0 += 16) {
+            accx4 acc = {0, 0, 0, 0};
+            const _Float16 *a = static_cast<const _Float16 *>(p.a) + (int64_t(max(s, 0)) * p.rank + min(q0 + r16, p.rank - 1)) * p.ci;
+            for (int pass = 0; pass < passes; ++pass) {
+                if (passes > 1) load(pass);
+                halfx8 av[kUnits];
+                if (s >= 0)
+#pragma unroll
+                    for (int u = 0; u < kUnits; ++u)
+                        av[u] = load8<VEC>(a, pass * kPass + (wave * kUnits + u) * 32 + kg * 8, p.ci);
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) {
+                    const int k = pass * kPass + (wave * kUnits + u) * 32 + kg * 8;
+                    halfx8 hi, lo;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        _Float16 h, l;
+                        split2(v[u][i / 4][i % 4], kSplitExp - e, h, l);
+                        hi[i] = h, lo[i] = l;
+                    }
+                    if (first && row < p.rows && k < cip) {
+                        _Float16 *dst = parts + row * 2 * cip + k;
+                        *reinterpret_cast<halfx8 *>(dst) = hi;
+                        *reinterpret_cast<halfx8 *>(dst + cip) = lo;
+                    }
+                    if (s >= 0) {
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u], lo, acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u], hi, acc, 0, 0, 0);
+                    }
+                }
+            }
+            first = false;
+            if (s < 0) break;
+            __syncthreads();  // the sums before have been read
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i];
+            __syncthreads();
+            // register i is rank 4 (l / 16) + i of row l % 16
+            if (wave == 0 && own) {
+                floatx4 t = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < kPassWaves; ++w)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[i] += part[w][i][lane];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] = ldexpf(t[i], e - kSplitExp);
+                *reinterpret_cast<floatx4 *>(p.t + row * p.rank_pad + q0 + kg * 4) = t;
+            }
+        }
+    } while (todo);
 }
 
 // Eight ranks of a row of t (padded to sixteens), zeros behind the last and where not wanted.
@@ -127,13 +234,11 @@ __global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArg
     // offsets from the tile's first, which the step moves on. The runs of hi, then of lo.
     static_assert(256 % (2 * R) == 0, "runs");
     halfx8 xr[XU], wv[WU];
-    uint32_t xo[XU], wo[WU];
+    uint32_t wo[WU];
     const int xrun = tid % (2 * R), wrun = tid % (WP * R);
-#pragma unroll
-    for (int u = 0; u < XU; ++u) {
-        const int r = int(min(int64_t(tid / (2 * R) + u * (256 / (2 * R))), p.rows - 1 - r0));
-        xo[u] = uint32_t((r * 2 + xrun / R) * g.cip + xrun % R * 8) * 2;
-    }
+    // (the parts of x hold whole tiles of rows)
+    const uint32_t xo = uint32_t((tid / (2 * R) * 2 + xrun / R) * g.cip + xrun % R * 8) * 2;
+    const uint32_t xstep = uint32_t(256 / (2 * R)) * 2 * uint32_t(g.cip) * 2;
 #pragma unroll
     for (int u = 0; u < WU; ++u) {
         const int c = min(tid / (WP * R) + u * (256 / (WP * R)), p.co - 1 - c0);
@@ -143,7 +248,7 @@ __global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArg
     const char *wb = static_cast<const char *>(g.w) + int64_t(c0) * (WP == 2 ? 2 * g.cip : p.ci) * 2;
     auto fetch = [&](int k) {
 #pragma unroll
-        for (int u = 0; u < XU; ++u) xr[u] = *reinterpret_cast<const halfx8 *>(xb + k * 2 + xo[u]);
+        for (int u = 0; u < XU; ++u) xr[u] = *reinterpret_cast<const halfx8 *>(xb + k * 2 + u * xstep + xo);
 #pragma unroll
         for (int u = 0; u < WU; ++u) {
             if constexpr (WP == 2) wv[u] = *reinterpret_cast<const halfx8 *>(wb + k * 2 + wo[u]);
@@ -345,6 +450,16 @@ void split_rows(Context &ctx, const float *x, int64_t rows, int ci, int cip, _Fl
     const dim3 grid{uint32_t(blocks)}, tb{256};
     if (ci % 4 == 0 && aligned16(x)) split_rows_kernel<true><<<grid, tb, 0, ctx.stream>>>(x, rows, ci, cip, parts, exps);
     else split_rows_kernel<false><<<grid, tb, 0, ctx.stream>>>(x, rows, ci, cip, parts, exps);
+    MH_LAUNCH_CHECK();
+}
+
+void split_shrink(Context &ctx, const LoraArgs &p, int cip, _Float16 *parts, int *exps) {
+    const int64_t blocks = ceil_div(p.rows, 16);
+    MH_REQUIRE(blocks < (int64_t(1) << 31), "lora: too many rows");
+    const dim3 grid{uint32_t(blocks)}, tb{64 * kPassWaves};
+    if (p.ci % 8 == 0 && aligned16(p.x) && aligned16(p.a))
+        split_shrink_kernel<true><<<grid, tb, 0, ctx.stream>>>(p, cip, parts, exps);
+    else split_shrink_kernel<false><<<grid, tb, 0, ctx.stream>>>(p, cip, parts, exps);
     MH_LAUNCH_CHECK();
 }
 
