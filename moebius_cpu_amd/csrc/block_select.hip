@@ -94,8 +94,6 @@ __device__ __forceinline__ uint64_t order_key(double s) {
     return (b >> 63) ? ~b : b | (uint64_t(1) << 63);
 }
 
-typedef double doublex4 __attribute__((ext_vector_type(4)));
-
 // One workgroup per (item, key head, TQ blocks of queries); W, MW: the runs in which the
 // queries and the means are read.
 constexpr int kSelWaves = 8;
@@ -111,6 +109,28 @@ __global__ __launch_bounds__(64 * kSelWaves) void block_select_kernel(SelectArgs
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int q_len = clamp_len(a.q_len, item, a.q_tokens), kv_len = clamp_len(a.kv_len, item, a.kv_tokens);
     const int b0 = tile * TQ;
+    const int seen_all = (kv_len + a.kb - 1) / a.kb;
+    const int l16 = lane & 15, kg = lane >> 4;
+    // The first means that the scores take are loaded before the queries.
+    const int t_first = __builtin_amdgcn_readfirstlane(wave) * 16;
+    float mv[4][4];
+    auto load_means = [&](int t0, int c0) {
+        const int b = min(t0 + l16, seen_all - 1);
+        const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + u * 16 + kg * 4;
+            if constexpr (MW == 4) {
+                load_run<float, 4>(m + min(c, a.d - 4), mv[u]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mv[u][e] = c < a.d ? mv[u][e] : 0.0f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mv[u][e] = c + e < a.d ? m[c + e] : 0.0f;
+            }
+        }
+    };
+    if (TQ > 1 && t_first < seen_all) load_means(t_first, 0);
 
     // Mean query of each block: kParts waves per block, lanes over (row group, run of channels).
     constexpr int kParts = kSelWaves / TQ;
@@ -156,11 +176,10 @@ __global__ __launch_bounds__(64 * kSelWaves) void block_select_kernel(SelectArgs
     }
     __syncthreads();
 
-    // Scores. One block of queries: sixteen lanes per key block. More: 16 key blocks x 16
-    // query blocks on the f64 matrix instruction (lane: row or column lane % 16, four
-    // channels at 4 (lane / 16); result register i is row 4 i + lane / 16).
-    const int seen_all = (kv_len + a.kb - 1) / a.kb;
-    const int l16 = lane & 15, kg = lane >> 4;
+    // Scores. One block of queries: sixteen lanes per key block. More: 16 key blocks x 4 query
+    // blocks on the f64 matrix instruction of four 4 x 4 products (lane: key block lane % 16,
+    // query block lane % 4, four channels at 4 (lane / 16); its result is of key block
+    // 4 (lane / 4 % 4) + lane / 16), the next means loaded meanwhile.
     if constexpr (TQ == 1) {
         for (int t0 = 0; t0 < seen_all; t0 += 4 * kSelWaves) {
             const int b = t0 + wave * 4 + kg;
@@ -179,40 +198,40 @@ __global__ __launch_bounds__(64 * kSelWaves) void block_select_kernel(SelectArgs
             if (b < seen_all && l16 == 0) keys[b] = order_key(s);
         }
     } else {
-        for (int t0 = wave * 16; t0 < seen_all; t0 += 16 * kSelWaves) {
-            const int b = min(t0 + l16, seen_all - 1);
-            const float *m = a.means + ((int64_t(item) * a.nk + b) * a.hk + hk) * a.d;
-            const float *q = qm[min(l16, TQ - 1)];
-            doublex4 acc = {0, 0, 0, 0};
-            for (int c0 = 0; c0 < a.d; c0 += 64) {
-                float mv[4][4];
+        constexpr int QG = TQ / 4 ? TQ / 4 : 1;
+        double acc[QG] = {};
+        int t0 = t_first, c0 = 0;
+        while (t0 < seen_all) {
+            float cur[4][4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int c = c0 + u * 16 + kg * 4;
-                    if constexpr (MW == 4) {
-                        load_run<float, 4>(m + min(c, a.d - 4), mv[u]);
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mv[u][e] = c < a.d ? mv[u][e] : 0.0f;
-                    } else {
+                for (int e = 0; e < 4; ++e) cur[u][e] = mv[u][e];
+            const bool last = c0 + 64 >= a.d;
+            const int t_next = last ? t0 + 16 * kSelWaves : t0, c_next = last ? 0 : c0 + 64;
+            if (t_next < seen_all) load_means(t_next, c_next);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mv[u][e] = c + e < a.d ? m[c + e] : 0.0f;
-                    }
-                }
+            for (int u = 0; u < 4; ++u) {
+                if (c0 + u * 16 >= a.d) break;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (c0 + u * 16 >= a.d) break;
+                for (int x = 0; x < QG; ++x) {
                     float qv[4];
-                    load_run<float, 4>(q + c0 + u * 16 + kg * 4, qv);
+                    load_run<float, 4>(qm[min(x * 4 + (lane & 3), TQ - 1)] + c0 + u * 16 + kg * 4, qv);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(double(mv[u][e]), double(qv[e]), acc, 0, 0, 0);
+                        acc[x] = __builtin_amdgcn_mfma_f64_4x4x4f64(double(cur[u][e]), double(qv[e]), acc[x], 0, 0, 0);
                 }
             }
+            if (last) {
+                const int r = t0 + (lane >> 2 & 3) * 4 + kg;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = t0 + 4 * i + kg;
-                if (l16 < TQ && r < seen_all) keys[l16 * a.nk + r] = order_key(acc[i]);
+                for (int x = 0; x < QG; ++x) {
+                    const int t = x * 4 + (lane & 3);
+                    if (t < TQ && r < seen_all) keys[t * a.nk + r] = order_key(acc[x]);
+                    acc[x] = 0;
+                }
             }
+            t0 = t_next, c0 = c_next;
         }
     }
     __syncthreads();
