@@ -67,6 +67,8 @@ def _same(a, *heads):
     for b in heads:
         if a._kind != b._kind:
             raise MoebiusError(1, "heads differ in type or channels")
+        if a.ctx is not b.ctx:
+            raise MoebiusError(1, "heads of different contexts")
 
 
 def _int32(a, size, what):

@@ -221,6 +221,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
             const int e = i < a.top ? src[i] : -1;
             bool ok = e >= 0 && e <= (last >> a.kb_log) && last >= 0;
             if (ok && !ascending)
+#pragma unroll 8
                 for (int j = 0; j < i; ++j) ok = ok && src[j] != e;
             const uint64_t all = __ballot(ok);
             if (ok) list[n + __popcll(all & ((uint64_t(1) << lane) - 1))] = e << a.kb_log;
@@ -592,6 +593,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
         }
     }
     if (a.part) {
+        if (!row_ok) return;
         float *p = a.part + (int64_t(work) * WR + wr) * part_floats(DT);
 #pragma unroll
         for (int t = 0; t < DT; ++t)
@@ -641,7 +643,7 @@ __global__ __launch_bounds__(64) void block_attention_join_kernel(Args a) {
     const int q_len = a.q_len ? min(max(a.q_len[item], 0), a.q_tokens) : a.q_tokens;
     const int i0 = qb * a.qb, rows = (min(i0 + a.qb, q_len) - i0) * a.g;
     const int row = (rt * WR + wr) * 32 + col;
-    if (rt * WR * 32 >= rows) return;  // its splits wrote nothing
+    if (rt * WR * 32 >= rows || row >= rows) return;  // its splits wrote nothing
     constexpr int PF = part_floats(DT);
     const float *p = a.part + (int64_t(base) * a.splits * WR + wr) * PF;
     float m = kNegInf;
@@ -657,7 +659,6 @@ __global__ __launch_bounds__(64) void block_attention_join_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = __builtin_fmaf(ps[(t * 16 + i) * 64 + lane], f, o[i]);
     }
-    if (row >= rows) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T *op = static_cast<T *>(a.out) + (int64_t(item) * a.q_tokens + i0 + row / a.g) * a.ldo +
             int64_t(hk * a.g + row % a.g) * a.d;

@@ -36,7 +36,7 @@ __device__ __forceinline__ int clamp_len(const int32_t *len, int item, int most)
     return len ? min(max(len[item], 0), most) : most;
 }
 
-// One workgroup per (item, block, run of 32 column vectors); eight row groups of 32
+// One workgroup per (item, block, run of 32 column vectors), these innermost; eight row groups of 32
 // threads, each summing every eighth row, joined in LDS.
 constexpr int kMeanCols = 32, kMeanRows = 8;
 
@@ -44,12 +44,13 @@ template <typename T, int W>
 __global__ __launch_bounds__(256) void block_means_kernel(const T *x, int64_t ld, int tokens, int cols, int block,
                                                           const int32_t *first, const int32_t *len, float *means) {
     __shared__ double part[kMeanRows][kMeanCols * W];
-    const int item = blockIdx.z, b = blockIdx.y, nb = gridDim.y;
+    const uint32_t cg = (uint32_t(cols) + kMeanCols * W - 1) / (kMeanCols * W), at = blockIdx.x / cg;
+    const int nb = (tokens + block - 1) / block, item = int(at / uint32_t(nb)), b = int(at % uint32_t(nb));
     const int n = clamp_len(len, item, tokens);
     const int r0 = b * block, r1 = min(r0 + block, n);
     if (r0 >= r1 || (first && r0 + block <= first[item])) return;
     const int c = threadIdx.x % kMeanCols, rg = threadIdx.x / kMeanCols;
-    const int col = (int(blockIdx.x) * kMeanCols + c) * W;
+    const int col0 = int(blockIdx.x % cg) * kMeanCols * W, col = col0 + c * W;
     double sum[W] = {};
     if (col < cols) {
         const T *p = x + int64_t(item) * tokens * ld + col;
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(256) void block_means_kernel(const T *x, int64_t ld
     for (int i = 0; i < W; ++i) part[rg][c * W + i] = sum[i];
     __syncthreads();
     for (int j = threadIdx.x; j < kMeanCols * W; j += 256) {
-        const int cj = int(blockIdx.x) * kMeanCols * W + j;
+        const int cj = col0 + j;
         if (cj >= cols) break;
         double s = 0;
 #pragma unroll
@@ -346,8 +347,8 @@ void means_t(Context &ctx, HeadRows x, int n, int tokens, int d, const int32_t *
     const int cols = x.heads * d;
     const bool vec = runs_of<T>(V, x.p, x.ld, cols);
     const int64_t nb = ceil_div(tokens, block), cg = ceil_div(cols, kMeanCols * (vec ? V : 1));
-    MH_REQUIRE(nb <= 65535 && n <= 65535, "block_means: more than 65535 blocks or items");
-    const dim3 grid{uint32_t(cg), uint32_t(nb), uint32_t(n)}, tb{256};
+    MH_REQUIRE(cg * nb < (int64_t(1) << 31) / n, "block_means: too many blocks");
+    const dim3 grid{uint32_t(cg * nb * n)}, tb{256};
     const T *p = static_cast<const T *>(x.p);
     if (vec) block_means_kernel<T, V><<<grid, tb, 0, ctx.stream>>>(p, x.ld, tokens, cols, block, first, len, means);
     else block_means_kernel<T, 1><<<grid, tb, 0, ctx.stream>>>(p, x.ld, tokens, cols, block, first, len, means);

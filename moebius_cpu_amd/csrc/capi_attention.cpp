@@ -88,8 +88,19 @@ mh::RopeTable rope_table(const MhRope *r, uint32_t d) {
     return t;
 }
 
+// Arrays of 4-byte elements (NULL counts as aligned).
+void aligned4(const void *p, const char *what) {
+    if (reinterpret_cast<uintptr_t>(p) % 4)
+        mh::fail(mh::kInvalidArgument, std::string(what) + " is not aligned to its type");
+}
+
 void few_rows(uint64_t rows) {
     if (rows >= (uint64_t(1) << 31)) mh::fail(mh::kInvalidArgument, "2^31 rows or more");
+}
+
+// (offsets within a tile of a projection are 32 bits)
+void few_channels(uint32_t c_in, uint32_t c_out) {
+    if (std::max(c_in, c_out) > (1u << 22)) mh::fail(mh::kInvalidArgument, "Conv1x1: more than 2^22 channels");
 }
 
 mh::BlockShape block_shape(const MhBlockShape *s) {
@@ -102,6 +113,7 @@ mh::BlockShape block_shape(const MhBlockShape *s) {
     b.heads_q = dim(s->heads_q, "heads_q");
     b.heads_kv = dim(s->heads_kv, "heads_kv");
     if (b.heads_q % b.heads_kv) mh::fail(mh::kInvalidArgument, "heads_q is not a multiple of heads_kv");
+    if (b.heads_q / b.heads_kv > 65536) mh::fail(mh::kInvalidArgument, "more than 65536 query heads per key head");
     if (s->d > uint32_t(mh::kMaxHeadDim)) mh::fail(mh::kInvalidArgument, "heads of more than 256 channels");
     b.d = int(s->d);
     if (s->q_block < 1 || s->q_block > 1024) mh::fail(mh::kInvalidArgument, "q_block is 1 .. 1024");
@@ -175,6 +187,8 @@ int32_t mh_qk_norm_rope(MhContext *ctx, const void *q, uint64_t ld_q, uint32_t h
         const Rows qo = rows_of(q_out, rows, heads_q, d, ld_qo, t, "q_out");
         const Rows ko = rows_of(k_out, rows, heads_k, d, ld_ko, t, "k_out");
         if (!(eps >= 0) || !std::isfinite(eps)) mh::fail(mh::kInvalidArgument, "eps is finite and not negative");
+        aligned4(gamma_q, "gamma_q");
+        aligned4(gamma_k, "gamma_k");
         const mh::RopeTable table = rope_table(rope, d);
         same_or_apart(qi, qo, "q and q_out");
         same_or_apart(ki, ko, "k and k_out");
@@ -196,6 +210,9 @@ int32_t mh_block_means(MhContext *ctx, const void *x, uint32_t dtype, uint32_t n
         const Rows in = rows_of(x, rows, heads, d, ld, t, "x");
         if (block < 1 || block > 1024) mh::fail(mh::kInvalidArgument, "block is 1 .. 1024");
         if (rows) need(means, "means");
+        aligned4(first, "first");
+        aligned4(len, "len");
+        aligned4(means, "means");
         mh::Context &c = C(ctx);
         mh::block_means(c, {x, in.ld, int(heads)}, t, int(n), int(tokens), int(d), first, len, int(block), means);
     });
@@ -209,6 +226,8 @@ int32_t mh_block_select(MhContext *ctx, const void *q, uint32_t dtype, uint64_t 
         const Rows in = rows_of(q, uint64_t(s.n) * s.q_tokens, s.heads_q, s.d, ld_q, t, "q");
         if (in.rows) need(blocks, "blocks");
         if (in.rows && s.kv_tokens) need(k_means, "k_means");
+        aligned4(blocks, "blocks");
+        aligned4(k_means, "k_means");
         if (s.kv_blocks() > mh::kMaxKeyBlocks) mh::fail(mh::kInvalidArgument, "more than 8192 blocks of keys");
         if (s.causal && s.top < std::min(s.kv_blocks(), (s.q_block + s.kv_block - 2) / s.kv_block + 1))
             mh::fail(mh::kInvalidArgument, "top does not hold the blocks of the queries' own tokens");
@@ -240,6 +259,7 @@ int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const v
         const Rows vi = rows_of(v, kv_rows, a.s.heads_kv, a.s.d, ld_v, t, "v");
         const Rows to = rows_of(out, q_rows, a.s.heads_q, a.s.d, ld_out, t, "out");
         if (q_rows) need(blocks, "blocks");
+        aligned4(blocks, "blocks");
         if (ki.ld * int64_t(ki.size) >= (1 << 25) || vi.ld * int64_t(vi.size) >= (1 << 25))
             mh::fail(mh::kInvalidArgument, "rows of k or v 32 MiB apart or more");
         if (!(scale > 0) || !std::isfinite(scale)) mh::fail(mh::kInvalidArgument, "scale is positive and finite");
@@ -268,6 +288,7 @@ int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, ui
         few_rows(rows);
         if (rank < 1 || rank > uint32_t(mh::kMaxRank)) mh::fail(mh::kInvalidArgument, "rank is 1 .. 256");
         const mh::WeightType t = wtype(weight_dtype);
+        few_channels(c_in, c_out);
         mh::Context &c = C(ctx);
         *bytes = mh::lora_scratch(c, int64_t(rows), dim(c_in, "c_in"), dim(c_out, "c_out"), t, int(rank));
     });
@@ -289,6 +310,7 @@ int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t 
         if (c_in == 0 || c_out == 0) mh::fail(mh::kInvalidArgument, "Conv1x1: empty channel axis");
         if (rows_per_slot == 0 || rows_per_slot >= (uint64_t(1) << 31))
             mh::fail(mh::kInvalidArgument, "rows_per_slot is 1 .. 2^31 - 1");
+        few_channels(c_in, c_out);
         mh::Lora l;
         l.type = wtype(adapters->dtype);
         if (adapters->rank < 1 || adapters->rank > uint32_t(mh::kMaxRank))
@@ -304,12 +326,21 @@ int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t 
         if (reinterpret_cast<uintptr_t>(adapters->a) % size_of(l.type) ||
             reinterpret_cast<uintptr_t>(adapters->b) % size_of(l.type))
             mh::fail(mh::kInvalidArgument, "adapters are not aligned to their type");
+        for (const void *q : {static_cast<const void *>(x), static_cast<const void *>(out), static_cast<const void *>(bias),
+                              static_cast<const void *>(residual), static_cast<const void *>(slot),
+                              static_cast<const void *>(adapters->scale)})
+            aligned4(q, "x, out, bias, residual, slot or scale");
+        if (reinterpret_cast<uintptr_t>(weight) % size_of(wtype(weight_dtype)))
+            mh::fail(mh::kInvalidArgument, "weight is not aligned to its type");
         l.a = adapters->a, l.b = adapters->b, l.scale = adapters->scale;
         l.slot = slot;
         l.rows_per_slot = int64_t(rows_per_slot);
         const Rows to{reinterpret_cast<const char *>(out), int64_t(rows), int64_t(c_out), int64_t(c_out), 4};
         const Rows in{reinterpret_cast<const char *>(x), int64_t(rows), int64_t(c_in), int64_t(c_in), 4};
         no_overlap(in, to, "x and out");
+        Rows res = to;
+        res.p = reinterpret_cast<const char *>(residual);
+        if (residual) same_or_apart(res, to, "residual and out");
         mh::Context &c = C(ctx);
         const size_t needed = mh::lora_scratch(c, int64_t(rows), dim(c_in, "c_in"), dim(c_out, "c_out"),
                                                wtype(weight_dtype), l.rank);

@@ -53,9 +53,9 @@ def test_rope_refusals(kw, text):
 
 
 def qk_call(q=A16, k=A16 + 0x10000, qo=A16 + 0x20000, ko=A16 + 0x30000, lds=(32, 16, 32, 16), heads=(2, 1), d=16, rows=4,
-            eps=1e-6, dtype=0, r=None):
+            eps=1e-6, dtype=0, r=None, gammas=(None, None)):
     r = rope() if r is None else r
-    return _lib.lib().mh_qk_norm_rope(None, q, lds[0], heads[0], k, lds[1], heads[1], dtype, rows, d, None, None, eps,
+    return _lib.lib().mh_qk_norm_rope(None, q, lds[0], heads[0], k, lds[1], heads[1], dtype, rows, d, *gammas, eps,
                                       ctypes.byref(r), qo, lds[2], ko, lds[3])
 
 
@@ -64,6 +64,7 @@ def qk_call(q=A16, k=A16 + 0x10000, qo=A16 + 0x20000, ko=A16 + 0x30000, lds=(32,
     (dict(heads=(0, 1)), "no heads"), (dict(heads=(2, 0)), "no heads"), (dict(qo=A16 + 0x10000), "overlap"),
     (dict(ko=A16), "overlap"), (dict(ko=A16 + 0x20000), "overlap"), (dict(k=None), "k is NULL"),
     (dict(dtype=7), "dtype"), (dict(rows=1 << 31), "2^31"), (dict(r=rope(axis_dims=(16, 16, 0, 0))), "exceed"),
+    (dict(gammas=(A16 + 2, None)), "gamma_q is not aligned"), (dict(gammas=(None, A16 + 1)), "gamma_k is not aligned"),
     (dict(), "context is NULL"), (dict(qo=A16, ko=A16 + 0x10000), "context is NULL"),
     # queries and keys of one projection turned where they lie
     (dict(k=A16 + 32 * 4, qo=A16, ko=A16 + 32 * 4, lds=(64, 64, 64, 64)), "context is NULL"),
@@ -83,7 +84,8 @@ SHAPES = [(dict(heads_q=3), "multiple"), (dict(heads_kv=0), "no heads"), (dict(h
           (dict(d=0), "no heads"), (dict(d=257), "256 channels"), (dict(q_block=0), "q_block"),
           (dict(q_block=1025), "q_block"), (dict(kv_block=0), "kv_block"), (dict(kv_block=48), "kv_block"),
           (dict(kv_block=256), "kv_block"), (dict(top=0), "top is"), (dict(top=1025), "top is"),
-          (dict(q_len=A16 + 2), "not aligned"), (dict(n=1 << 31), "too large")]
+          (dict(q_len=A16 + 2), "not aligned"), (dict(n=1 << 31), "too large"),
+          (dict(heads_q=65537, heads_kv=1, d=1), "65536")]
 
 
 @pytest.mark.parametrize("kw,text", SHAPES + [
@@ -108,6 +110,8 @@ def test_select_null_arguments():
     refused(L.mh_block_select(None, A16, 0, 256, None, A16, A16), "shape is NULL")
     refused(L.mh_block_select(None, A16, 0, 255, ctypes.byref(s), A16, A16), "ld is less")
     refused(L.mh_block_select(None, A16, 3, 256, ctypes.byref(s), A16, A16), "dtype")
+    refused(L.mh_block_select(None, A16, 0, 256, ctypes.byref(s), A16 + 2, A16), "k_means is not aligned")
+    refused(L.mh_block_select(None, A16, 0, 256, ctypes.byref(s), A16, A16 + 2), "blocks is not aligned")
 
 
 M = 1 << 24
@@ -131,25 +135,29 @@ def test_attention_shape_refusals(kw, text):
     (dict(out=M), "overlap"), (dict(out=2 * M), "overlap"), (dict(out=3 * M + 64), "overlap"),
     (dict(lds=(255, 128, 128, 256)), "ld is less"), (dict(lds=(256, 127, 128, 256)), "ld is less"),
     (dict(lds=(256, 1 << 24, 128, 256)), "32 MiB"), (dict(lds=(256, 128, 1 << 24, 256)), "32 MiB"),
-    (dict(dtype=9), "dtype"), (dict(k=2 * M + 1), "not aligned"), (dict(), "context is NULL")])
+    (dict(dtype=9), "dtype"), (dict(k=2 * M + 1), "not aligned"), (dict(blocks=A16 + 1), "blocks is not aligned"),
+    (dict(), "context is NULL")])
 def test_attention_refusals(kw, text):
     refused(attend(**kw), text)
 
 
 @pytest.mark.parametrize("kw,text", [(dict(block=0), "block is"), (dict(block=1025), "block is"), (dict(x=None), "x is NULL"),
                                      (dict(means=None), "means is NULL"), (dict(ld=63), "ld is less"),
-                                     (dict(heads=0), "no heads"), (dict(dtype=5), "dtype"), (dict(), "context is NULL")])
+                                     (dict(heads=0), "no heads"), (dict(dtype=5), "dtype"),
+                                     (dict(first=A16 + 2), "first is not"), (dict(len=A16 + 2), "len is not"),
+                                     (dict(means=A16 + 2), "means is not"), (dict(), "context is NULL")])
 def test_means_refusals(kw, text):
     a = dict(x=A16, dtype=0, n=1, tokens=10, heads=1, d=64, ld=64, first=None, len=None, block=16, means=A16)
     a.update(kw)
     refused(_lib.lib().mh_block_means(None, *a.values()), text)
 
 
-def lora_call(ad=None, x=M, out=2 * M, w=3 * M, slot=A16, rows=8, ci=64, co=32, per=1, **kw):
+def lora_call(ad=None, x=M, out=2 * M, w=3 * M, slot=A16, rows=8, ci=64, co=32, per=1, bias=None, res=None,
+              **kw):
     a = dict(a=4 * M, b=5 * M, scale=A16, dtype=0, slots=2, rank=8, reserved=0)
     a.update(kw)
     s = _lib.AdapterSet(*(a[f] for f, _ in _lib.AdapterSet._fields_)) if ad is None else ad
-    return _lib.lib().mh_conv1x1_lora(None, x, rows, ci, w, 0, co, None, None, ctypes.byref(s), slot, per, out, None, 0)
+    return _lib.lib().mh_conv1x1_lora(None, x, rows, ci, w, 0, co, bias, res, ctypes.byref(s), slot, per, out, None, 0)
 
 
 @pytest.mark.parametrize("kw,text", [
@@ -158,7 +166,10 @@ def lora_call(ad=None, x=M, out=2 * M, w=3 * M, slot=A16, rows=8, ci=64, co=32, 
     (dict(a=4 * M + 2), "not aligned"), (dict(x=None), "x is NULL"), (dict(out=None), "out is NULL"),
     (dict(w=None), "weight is NULL"), (dict(slot=None), "slot is NULL"), (dict(per=0), "rows_per_slot"),
     (dict(rows=1 << 31), "2^31"), (dict(ci=0), "empty channel"), (dict(co=0), "empty channel"),
-    (dict(out=M + 256), "overlap"), (dict(), "context is NULL"), (dict(slots=0, a=None, b=None), "context is NULL")])
+    (dict(out=M + 256), "overlap"), (dict(res=2 * M + 64), "overlap"), (dict(res=2 * M), "context is NULL"),
+    (dict(w=3 * M + 2), "weight is not aligned"), (dict(ci=(1 << 22) + 1), "2^22 channels"), (dict(co=(1 << 22) + 1), "2^22 channels"),
+    *((dict([(f, A16 + 2)]), "x, out, bias") for f in ("x", "out", "bias", "res", "slot", "scale")),
+    (dict(), "context is NULL"), (dict(slots=0, a=None, b=None), "context is NULL")])
 def test_lora_refusals(kw, text):
     refused(lora_call(**kw), text)
 
