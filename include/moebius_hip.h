@@ -537,8 +537,9 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
 /* out [n][q_tokens][heads_q][d] = softmax(scale q . k) v over the keys of the listed
  * blocks (as mh_block_select writes them, in any order: indices outside the item's
  * blocks are skipped, one listed twice counts once), in one pass with f32 scores and
- * sums; scale > 0; rows of k and of v less than 32 MiB apart. Rows that see no key are zero, rows at or above q_len are left as
- * they were; what lies at keys a row does not see (NaN among it) does not reach it.
+ * sums; scale > 0; rows of k and of v less than 32 MiB apart. Rows that see no key are
+ * zero, rows at or above q_len are left as they were; what lies at keys a row does not
+ * see (NaN among it) does not reach it.
  * f16 tensors: f16 products. f32 tensors: f32 products, or on FAST contexts products
  * of operands rounded to f16. Lists are split over workgroups where rows are few, and
  * the parts joined through scratch (mh_block_attention_scratch bytes, 16-byte
@@ -567,10 +568,13 @@ int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, ui
  * convention, have none)
  *   out += scale[s] (x . a[s]^T) . b[s]^T.
  * rows_per_slot: h * w where each image of a batch is a request, 1 for single tokens
- * or rows of mixed requests; slot has ceil(rows / rows_per_slot) entries. The adapters'
- * products are f32 on EXACT and FAST contexts. scratch as for mh_block_attention
- * (mh_conv1x1_lora_scratch bytes); the projection itself uses the context's workspace
- * as mh_conv1x1_forward does. */
+ * or rows of mixed requests; slot has ceil(rows / rows_per_slot) entries. residual may
+ * be out; no other overlap with out. Sums are f32. EXACT: f32 products up to 64 rows;
+ * beyond, products of x (and of an f32 weight) in two f16 parts, which hold a value to
+ * 2^-24 of itself or 2^-40 of the largest of its row, whichever is more. FAST: beyond 64
+ * rows the projection's operands are rounded to f16, scaled by their row's largest; the
+ * adapters' products are as in EXACT. scratch as for mh_block_attention
+ * (mh_conv1x1_lora_scratch bytes). At most 2^22 channels. */
 int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t c_in, const void *weight,
                         uint32_t weight_dtype, uint32_t c_out, const float *bias, const float *residual,
                         const MhAdapters *adapters, const int32_t *slot, uint64_t rows_per_slot, float *out,

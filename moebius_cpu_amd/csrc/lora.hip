@@ -1,13 +1,12 @@
 // Low-rank adapters of many requests beside a shared 1x1 projection:
 //   y = x W^T + bias + residual + scale_s (x A_s^T) B_s^T,  s the row's adapter.
 //
-// The projection is the library's GEMM. The adapters take two passes of f32 products
-// (v_mfma_f32_16x16x4_f32, f16 adapters widened exactly) in EXACT and FAST contexts
-// alike: at rank r they are r (c_in + c_out) of the projection's c_in c_out operations,
-// so memory bounds them, x read once more and out read and written once.
-//   shrink: t = x A_s^T [rows][rank], the long axis split over the waves of a workgroup,
-//           joined in LDS, and over workgroups where rows are few (partials side by side);
-//   expand: out += scale_s t B_s^T, the partials added up as t is read.
+// The adapters' products are f32 in EXACT and FAST contexts alike: at rank r they are
+// r (c_in + c_out) of the projection's c_in c_out operations. Few rows take two passes of
+// f32 products:
+//   row shrink: t = x A_s^T [rows][rank], a wave per rank of a row;
+//   row project: x W^T in tiles of 16 x 16, finished with bias, residual and scale_s t B_s^T.
+// More rows take the product of lora_gemm.hip behind one pass over x, which forms t as well.
 //
 // A tile of 16 rows takes the adapters its rows name one after another, each product
 // over all 16 rows and kept for its own: rows of one image share one, single tokens of
@@ -24,17 +23,18 @@ namespace {
 
 constexpr int kRankTiles = 4;     // 16 ranks each per pass over x
 constexpr int kShrinkUnroll = 5;  // steps of the long axis whose loads are in flight together
-
 constexpr int kShrinkWaves = 8;
 
-// Workgroup (16 rows, split of the long axis); wave w takes an eighth of its share.
+// Adapters stored in f32: a workgroup takes 16 rows, wave w an eighth of the long axis.
 // Lane l holds row (rank) l % 16 and four values of the long axis at 4 (l / 16).
-template <typename T, bool VEC>
+template <bool VEC>
 __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs p) {
     __shared__ float part[kShrinkWaves][kRankTiles][4][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t r0 = int64_t(blockIdx.x) * 16;
-    const int k0 = int(blockIdx.y) * p.chunk, k1 = min(k0 + p.chunk, p.ci);
+    const int share = ((p.ci + 15) / 16 + kShrinkWaves - 1) / kShrinkWaves * 16;
+    const int k0 = wave * share, ke = min(k0 + share, p.ci);
     const int mine = slot_of(p, r0 + r16);
     const float *x = p.x + min(r0 + r16, p.rows - 1) * p.ci;
     uint32_t todo = uint32_t(__ballot(mine >= 0)) & 0xFFFFu;
@@ -44,15 +44,13 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs
         todo &= ~uint32_t(__ballot(own));
         for (int q0 = 0; q0 < p.rank; q0 += 16 * kRankTiles) {
             floatx4 acc[kRankTiles];
-            const T *a[kRankTiles];
+            const float *a[kRankTiles];
 #pragma unroll
             for (int j = 0; j < kRankTiles; ++j) {
                 acc[j] = floatx4{0, 0, 0, 0};
-                a[j] = static_cast<const T *>(p.a) + (int64_t(s) * p.rank + min(q0 + j * 16 + r16, p.rank - 1)) * p.ci;
+                a[j] = static_cast<const float *>(p.a) + (int64_t(s) * p.rank + min(q0 + j * 16 + r16, p.rank - 1)) * p.ci;
             }
-            const int share = ((k1 - k0 + 15) / 16 + kShrinkWaves - 1) / kShrinkWaves * 16, kw = k0 + wave * share;
-            const int ke = min(kw + share, k1);
-            for (int k = kw; k < ke; k += 16 * kShrinkUnroll) {
+            for (int k = k0; k < ke; k += 16 * kShrinkUnroll) {
                 floatx4 xv[kShrinkUnroll];
 #pragma unroll
                 for (int u = 0; u < kShrinkUnroll; ++u) xv[u] = load4<VEC>(x, k + u * 16 + kg * 4, ke);
@@ -83,65 +81,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(LoraArgs
                 for (int w = 0; w < kShrinkWaves; ++w)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] += part[w][wave][e][lane];
-                *reinterpret_cast<floatx4 *>(p.t + (int64_t(blockIdx.y) * p.rows + r0 + r16) * p.rank_pad + q) = v;
-            }
-        }
-    }
-}
-
-// A wave takes 16 rows and 64 columns; register e of a 16-column tile is column
-// 4 (l / 16) + e of row l % 16, so a lane reads and writes runs of four columns.
-template <typename T, bool VEC, bool VOUT>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs p) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, kg = lane >> 4;
-    const int64_t r0 = int64_t(blockIdx.x) * 16;
-    const int c0 = (int(blockIdx.y) * 4 + wave) * 64;
-    if (c0 >= p.co) return;
-    const int mine = slot_of(p, r0 + r16);
-    uint32_t todo = uint32_t(__ballot(mine >= 0)) & 0xFFFFu;
-    if (!todo) return;
-    const int64_t row = min(r0 + r16, p.rows - 1);
-    float *out = p.out + row * p.co;
-    while (todo) {
-        const int s = __shfl(mine, __builtin_ctz(todo));
-        const bool own = mine == s;
-        todo &= ~uint32_t(__ballot(own));
-        floatx4 acc[4];
-        const T *b[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc[j] = floatx4{0, 0, 0, 0};
-            b[j] = static_cast<const T *>(p.b) + (int64_t(s) * p.co + min(c0 + j * 16 + r16, p.co - 1)) * p.rank;
-        }
-        for (int k = 0; k < p.rank; k += 16) {
-            // rows of other adapters: whatever lies there, selected away below
-            floatx4 tv = {0, 0, 0, 0};
-            if (own)
-                for (int i = 0; i < p.splits; ++i)
-                    tv += *reinterpret_cast<const floatx4 *>(p.t + (int64_t(i) * p.rows + row) * p.rank_pad + k + kg * 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const floatx4 bv = load4<VEC>(b[j], k + kg * 4, p.rank);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[j] = mfma(bv[e], k + kg * 4 + e < p.rank ? tv[e] : 0.0f, acc[j]);
-            }
-        }
-        if (!own) continue;
-        const float scale = p.scale[s];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + j * 16 + kg * 4;
-            if constexpr (VOUT) {
-                if (c < p.co) {
-                    floatx4 v = *reinterpret_cast<const floatx4 *>(out + c);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(scale, acc[j][e], v[e]);
-                    *reinterpret_cast<floatx4 *>(out + c) = v;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < p.co) out[c + e] = __builtin_fmaf(scale, acc[j][e], out[c + e]);
+                *reinterpret_cast<floatx4 *>(p.t + (r0 + r16) * p.rank_pad + q) = v;
             }
         }
     }
@@ -245,43 +185,20 @@ __global__ __launch_bounds__(512) void lora_row_project_kernel(LoraArgs p, const
     p.out[row * p.co + c] = v;
 }
 
-// Rows up to which the projection is worth forming beside the adapters (few_rows): both
-// of its passes over 16 rows against the general product's split sums and the two
-// adapter passes over its output.
-constexpr int kFewRows = 64;
-bool few_rows(int64_t rows) { return rows <= kFewRows; }
-
-// Splits of the long axis: two workgroups per CU, at least 128 values each.
-int lora_splits(const Context &ctx, int64_t rows, int c_in, bool own) {
-    if (few_rows(rows) || own) return 1;  // their second products read t as it is
-    const int64_t tiles = ceil_div(rows, 16);
-    const int64_t s = std::min<int64_t>(2 * ctx.cu_count / std::max<int64_t>(tiles, 1), c_in / 128);
-    return int(std::max<int64_t>(1, std::min<int64_t>(s, 16)));
+// Whether the two passes over few rows are taken: they cost 10 us and 4.7 us more for every
+// 256 tiles of 16 x 16 behind the first (at c_in 1280), the other way two thirds more to
+// begin with. 1280 x 1280, f16 / f32 weight, us against that: 16 rows 9.8 / 9.8 (22 / 30),
+// 96 rows 14.8 / 14.7 (23 / 33), 128 rows 19.5 / 19.7 (23 / 34), 256 rows 30 / 30 (23 / 35);
+// 320 x 320, 256 rows 14.6 / 14.6 (15.8 / 17.8), 512 rows 20.7 / 20.1 (15.8 / 17.9). The first
+// pass reads an adapter per row: rank 256, 640 x 64, 256 rows 31 us (67), 512 rows 48 (50).
+bool few_rows(const Context &ctx, int64_t rows, int c_out, WeightType wt, int rank) {
+    return rows * rank <= 1 << 16 && ceil_div(rows, 16) * ceil_div(c_out, 16) <= (wt == kF32 ? 3 : 2) * ctx.cu_count;
 }
 
-template <typename T>
 void run_shrink(Context &ctx, const LoraArgs &p) {
-    const int64_t tiles = ceil_div(p.rows, 16);
-    MH_REQUIRE(tiles < (int64_t(1) << 31), "lora: too many rows");
-    const dim3 tb{64 * kShrinkWaves};
-    const bool vx = p.ci % 4 == 0 && aligned16(p.x) && reinterpret_cast<uintptr_t>(p.a) % (4 * sizeof(T)) == 0;
-    const dim3 sg{uint32_t(tiles), uint32_t(p.splits)};
-    if (vx) lora_shrink_kernel<T, true><<<sg, tb, 0, ctx.stream>>>(p);
-    else lora_shrink_kernel<T, false><<<sg, tb, 0, ctx.stream>>>(p);
-    MH_LAUNCH_CHECK();
-}
-
-template <typename T>
-void run_expand(Context &ctx, const LoraArgs &p) {
-    const int64_t tiles = ceil_div(p.rows, 16);
-    const dim3 tb{256};
-    const bool vb = p.rank % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % (4 * sizeof(T)) == 0;
-    const bool vo = p.co % 4 == 0 && aligned16(p.out);
-    const dim3 eg{uint32_t(tiles), uint32_t(ceil_div(p.co, 256))};
-    if (vb && vo) lora_expand_kernel<T, true, true><<<eg, tb, 0, ctx.stream>>>(p);
-    else if (vb) lora_expand_kernel<T, true, false><<<eg, tb, 0, ctx.stream>>>(p);
-    else if (vo) lora_expand_kernel<T, false, true><<<eg, tb, 0, ctx.stream>>>(p);
-    else lora_expand_kernel<T, false, false><<<eg, tb, 0, ctx.stream>>>(p);
+    const dim3 grid{uint32_t(ceil_div(p.rows, 16))}, tb{64 * kShrinkWaves};
+    if (p.ci % 4 == 0 && aligned16(p.x) && aligned16(p.a)) lora_shrink_kernel<true><<<grid, tb, 0, ctx.stream>>>(p);
+    else lora_shrink_kernel<false><<<grid, tb, 0, ctx.stream>>>(p);
     MH_LAUNCH_CHECK();
 }
 
@@ -300,29 +217,26 @@ void run_few(Context &ctx, const LoraArgs &p, const void *weight, const float *b
     MH_LAUNCH_CHECK();
 }
 
+// FAST rounds the projection's operands to f16.
+int parts_of(const Context &ctx) { return ctx.precision == Precision::Fast ? 1 : 2; }
+
 // Scratch: t, then the parts of x and their exponents, then those of an f32 weight.
 struct Layout {
     size_t t = 0, x = 0, x_exp = 0, w = 0, w_exp = 0;
     size_t total() const { return t + x + x_exp + w + w_exp; }
 };
 
-bool use_gemm(const Context &ctx, int64_t rows, int c_in, int c_out) {
-    return !few_rows(rows) && ctx.precision == Precision::Exact && gemm_fits(ctx, rows, c_out, c_in);
-}
-
 Layout layout(const Context &ctx, int64_t rows, int c_in, int c_out, WeightType wt, int rank) {
     auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
-    const size_t cip = size_t(ceil_div(c_in, 64) * 64);
     Layout l;
-    const bool own = use_gemm(ctx, rows, c_in, c_out);
-    l.t = up(size_t(lora_splits(ctx, rows, c_in, own)) * size_t(rows) * size_t(ceil_div(rank, 16) * 16) * sizeof(float));
-    if (own) {
-        l.x = up(size_t(padded_rows(rows)) * 2 * cip * 2);
-        l.x_exp = up(size_t(rows) * 4);
-        if (wt == kF32) {
-            l.w = up(size_t(c_out) * 2 * cip * 2);
-            l.w_exp = up(size_t(c_out) * 4);
-        }
+    l.t = up(size_t(rows) * size_t(ceil_div(rank, 16) * 16) * sizeof(float));
+    if (few_rows(ctx, rows, c_out, wt, rank)) return l;
+    const size_t row = size_t(parts_of(ctx)) * padded_channels(c_in) * sizeof(_Float16);
+    l.x = up(size_t(padded_rows(rows)) * row);
+    l.x_exp = up(size_t(rows) * sizeof(int));
+    if (wt == kF32) {
+        l.w = up(size_t(c_out) * row);
+        l.w_exp = up(size_t(c_out) * sizeof(int));
     }
     return l;
 }
@@ -337,10 +251,7 @@ size_t lora_scratch(const Context &ctx, int64_t rows, int c_in, int c_out, Weigh
 void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const void *weight, WeightType wt, int c_out,
                   const float *bias, const float *residual, const Lora &l, float *out, void *scratch) {
     if (!rows) return;
-    const bool few = lora::few_rows(rows), own = lora::use_gemm(ctx, rows, c_in, c_out);
-    if (!few && !own) conv1x1(ctx, x, rows, c_in, weight, wt, c_out, bias, residual, out);
     const lora::Layout mem = lora::layout(ctx, rows, c_in, c_out, wt, l.rank);
-    // behind the projection on the stream: its split sums in the workspace are done with
     char *at = static_cast<char *>(scratch ? scratch : ctx.ws.get(mem.total(), ctx.stream));
     lora::LoraArgs p{};
     p.x = x, p.a = l.a, p.b = l.b, p.scale = l.scale, p.slot = l.slot, p.out = out;
@@ -348,42 +259,36 @@ void conv1x1_lora(Context &ctx, const float *x, int64_t rows, int c_in, const vo
     p.rows = rows, p.rows_per_slot = l.rows_per_slot;
     p.ci = c_in, p.co = c_out, p.rank = l.rank, p.slots = l.slots;
     p.rank_pad = int(ceil_div(l.rank, 16) * 16);
-    p.splits = lora::lora_splits(ctx, rows, c_in, own);
-    p.chunk = int(ceil_div(ceil_div(c_in, p.splits), 64) * 64);
     const bool ah = l.type == kF16;
-    if (few) {
+    if (lora::few_rows(ctx, rows, c_out, wt, l.rank)) {
         if (wt == kF16 && ah) lora::run_few<_Float16, _Float16>(ctx, p, weight, bias, residual);
         else if (wt == kF16) lora::run_few<_Float16, float>(ctx, p, weight, bias, residual);
         else if (ah) lora::run_few<float, _Float16>(ctx, p, weight, bias, residual);
         else lora::run_few<float, float>(ctx, p, weight, bias, residual);
         return;
     }
-    if (!own) {
-        if (ah) lora::run_shrink<_Float16>(ctx, p);
-        else lora::run_shrink<float>(ctx, p);
-        if (ah) lora::run_expand<_Float16>(ctx, p);
-        else lora::run_expand<float>(ctx, p);
-        return;
-    }
+    const int nparts = lora::parts_of(ctx);
     lora::GemmArgs g{};
     g.l = p;
-    g.cip = int(ceil_div(c_in, 64) * 64);
+    g.cip = lora::padded_channels(c_in);
     auto *xp = reinterpret_cast<_Float16 *>(at + mem.t);
     auto *xe = reinterpret_cast<int *>(at + mem.t + mem.x);
-    if (ah) {
-        lora::split_shrink(ctx, p, g.cip, xp, xe);
-    } else {
-        lora::run_shrink<float>(ctx, p);
-        lora::split_rows(ctx, x, rows, c_in, g.cip, xp, xe);
-    }
     g.xp = xp, g.x_exp = xe, g.w = weight, g.bias = bias, g.residual = residual;
+    lora::SplitRows xs, ws;
+    if (ah) {
+        lora::split_shrink(ctx, p, g.cip, nparts, xp, xe);
+    } else {
+        lora::run_shrink(ctx, p);
+        xs = {x, rows, xp, xe};
+    }
     if (wt == kF32) {
         auto *wp = reinterpret_cast<_Float16 *>(at + mem.t + mem.x + mem.x_exp);
         auto *we = reinterpret_cast<int *>(at + mem.t + mem.x + mem.x_exp + mem.w);
-        lora::split_rows(ctx, static_cast<const float *>(weight), c_out, c_in, g.cip, wp, we);
+        ws = {static_cast<const float *>(weight), c_out, wp, we};
         g.w = wp, g.w_exp = we;
     }
-    lora::gemm(ctx, g, wt, l.type);
+    if (xs.rows || ws.rows) lora::split_rows(ctx, xs, ws, c_in, g.cip, nparts);
+    lora::gemm(ctx, g, nparts, wt, l.type);
 }
 
 }  // namespace mh

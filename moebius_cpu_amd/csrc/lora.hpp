@@ -16,8 +16,7 @@ struct LoraArgs {
     const int32_t *slot;
     float *t, *out;
     int64_t rows, rows_per_slot;
-    int ci, co, rank, slots, splits, rank_pad;  // rank_pad: rank rounded up to 16
-    int chunk;                                  // of the long axis per split, a multiple of 64
+    int ci, co, rank, slots, rank_pad;  // rank_pad: rank rounded up to 16
 };
 
 // Four values at p + k of a run of n, zeros behind it; VEC: n and p keep every run of four aligned.
@@ -74,24 +73,29 @@ __device__ __forceinline__ int top_exp(float mx) { return mx == 0.0f ? 0 : __bui
 // The projection with the adapters' second product in its epilogue (lora_gemm.hip).
 struct GemmArgs {
     LoraArgs l;
-    const void *w;           // [co][ci], or its parts [co][2][cip]
+    const void *w;           // [co][ci], or its parts [co][nparts][cip]
     const int *w_exp;        // [co] where w is in parts
-    const _Float16 *xp;      // [rows][2][cip]
+    const _Float16 *xp;      // [rows][nparts][cip]
     const int *x_exp;        // [rows]
     const float *bias, *residual;
-    int cip;                 // ci rounded up to 64
+    int cip;                 // ci padded (padded_channels)
     int tiles_m, tiles_n;    // of columns, of rows
 };
-// x [rows][ci] -> parts [rows][2][cip] (zeros behind ci) and each row's exponent.
-void split_rows(Context &ctx, const float *x, int64_t rows, int ci, int cip, _Float16 *parts, int *exps);
-// The same of p.x and, for f16 adapters, p.t of every row that has one.
-void split_shrink(Context &ctx, const LoraArgs &p, int cip, _Float16 *parts, int *exps);
-// Rows that the parts of x have room for.
+// Channels and rows that the parts have room for: whole stages and tiles of the product.
+inline int padded_channels(int ci) { return int(ceil_div(ci, 256) * 256); }
 inline int64_t padded_rows(int64_t rows) { return ceil_div(rows, 128) * 128; }
-// Whether that kernel is the faster way for these sizes.
-bool gemm_fits(const Context &ctx, int64_t rows, int c_out, int c_in);
-// weight: wt, or f32 in parts.
-void gemm(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at);
+// Rows [ci] -> parts [nparts][cip] (zeros behind ci) and each row's exponent, of one or two sets.
+struct SplitRows {
+    const float *x = nullptr;
+    int64_t rows = 0;
+    _Float16 *parts = nullptr;
+    int *exps = nullptr;
+};
+void split_rows(Context &ctx, const SplitRows &a, const SplitRows &b, int ci, int cip, int nparts);
+// The same of p.x and, for f16 adapters, p.t of every row that has one.
+void split_shrink(Context &ctx, const LoraArgs &p, int cip, int nparts, _Float16 *parts, int *exps);
+// nparts: 2, or 1 where operands are rounded to f16. An f32 weight is in parts.
+void gemm(Context &ctx, const GemmArgs &g, int nparts, WeightType wt, WeightType at);
 
 }  // namespace lora
 }  // namespace mh

@@ -6,11 +6,17 @@
 // and split alike (lo . lo is below 2^-24 of its product). Sums are f32. An eighth of the
 // f32 instructions' time and a third of six bf16 products'.
 //
-// A workgroup forms BT columns x BT rows, its four waves 2 x 2 quarters, as W . X^T: a lane
+// FAST contexts take one part (operands rounded to f16 after their row's scale).
+//
+// A workgroup forms BT columns x BT rows, four waves the 2 x 2 quarters, as W . X^T: a lane
 // of a 32x32 result holds one row and four runs of four columns, so a row's scale and its
 // adapter are the lane's own. 64 of the long axis are staged in LDS at a time while the
-// next are loaded. Bound: the matrix instructions; the parts of x are written and read
-// once more than x itself.
+// next are loaded; where the tiles are too few to hide those loads in each other, two or
+// four such groups of waves share the long axis. Bound: the matrix instructions; the parts
+// of x are written and read once more than x itself.
+//
+// Measured: 8192 rows, 1280 x 1280, f16 weight, rank 32, residual: 121 us, of it 92 the
+// product (54 GFLOP in two f16 products: 583 TFLOP/s) and 27 the pass over x.
 #include <algorithm>
 
 #include "lora.hpp"
@@ -24,14 +30,17 @@ typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 
 // A wave per row, its values in registers up to kHold runs of 8 per lane.
 constexpr int kHold = 4;
-template <bool VEC>
-__global__ __launch_bounds__(256) void split_rows_kernel(const float *x, int64_t rows, int ci, int cip, _Float16 *parts,
-                                                         int *exps) {
+template <bool VEC, int P>
+__global__ __launch_bounds__(256) void split_rows_kernel(SplitRows s0, SplitRows s1, int ci, int cip) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
+    const int64_t at = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), row = at < s0.rows ? at : at - s0.rows;
+    const SplitRows &s = at < s0.rows ? s0 : s1;
+    if (row >= s.rows) return;
+    const float *x = s.x;
+    _Float16 *parts = s.parts;
+    int *exps = s.exps;
     const float *src = x + row * ci;
-    _Float16 *dst = parts + row * 2 * cip;
+    _Float16 *dst = parts + row * P * cip;
     floatx4 v[kHold][2];
     float mx = 0.0f;
     auto scan = [&](const floatx4 &a) {
@@ -64,7 +73,7 @@ __global__ __launch_bounds__(256) void split_rows_kernel(const float *x, int64_t
             hi[c] = p, lo[c] = q;
         }
         *reinterpret_cast<halfx8 *>(dst + r * 8) = hi;
-        *reinterpret_cast<halfx8 *>(dst + cip + r * 8) = lo;
+        if constexpr (P == 2) *reinterpret_cast<halfx8 *>(dst + cip + r * 8) = lo;
     };
 #pragma unroll
     for (int i = 0; i < kHold; ++i)
@@ -100,11 +109,12 @@ typedef floatx4 accx4;
 // kUnits steps in registers between the row's maximum and its parts; longer rows are read
 // again. Bound: memory, x read and its parts written.
 constexpr int kUnits = 5, kPassWaves = 8, kPass = kUnits * kPassWaves * 32;
+constexpr int kTiles = 2;  // of 16 ranks per round: rank 256 of 512 rows 62 -> 47 us against one
 
-template <bool VEC>
+template <bool VEC, int P>
 __global__ __launch_bounds__(64 * kPassWaves) void split_shrink_kernel(LoraArgs p, int cip, _Float16 *parts, int *exps) {
     __shared__ float wave_max[kPassWaves][16];
-    __shared__ float part[kPassWaves][4][64];
+    __shared__ float part[kPassWaves][kTiles][4][64];
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t r0 = int64_t(blockIdx.x) * 16, row = r0 + r16;
@@ -139,61 +149,86 @@ __global__ __launch_bounds__(64 * kPassWaves) void split_shrink_kernel(LoraArgs 
     const int e = top_exp(mx);
     if (tid < 16 && row < p.rows) exps[row] = e;
 
-    const uint32_t rows16 = uint32_t(__ballot(mine >= 0)) & 0xFFFFu;
-    // Adapters one after another, ranks sixteen at a time; the parts are written by the first round.
-    uint32_t todo = rows16;
+    // The values' parts take their place; those of a row longer than a pass are loaded for every round.
+    halfx8 hi[kUnits], lo[kUnits];
+    auto part_values = [&] {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                _Float16 h, l;
+                split2(v[u][i / 4][i % 4], kSplitExp - e, h, l);
+                hi[u][i] = h, lo[u][i] = l;
+            }
+    };
+    if (passes == 1) part_values();
+    // Adapters one after another, ranks kTiles x 16 at a time, the next round's loaded before
+    // this one's sums are joined; the parts are written by the first round.
+    halfx8 av[kTiles][kUnits];
+    auto fetch = [&](int s, int q0, int pass) {
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+            const _Float16 *a = static_cast<const _Float16 *>(p.a) +
+                                (int64_t(s) * p.rank + min(q0 + j * 16 + r16, p.rank - 1)) * p.ci;
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u)
+                av[j][u] = load8<VEC>(a, pass * kPass + (wave * kUnits + u) * 32 + kg * 8, p.ci);
+        }
+    };
+    uint32_t todo = uint32_t(__ballot(mine >= 0)) & 0xFFFFu;
     bool first = true;
     do {
         const int s = todo ? __builtin_amdgcn_readfirstlane(__shfl(mine, __builtin_ctz(todo))) : -1;
         const bool own = s >= 0 && mine == s;
         todo &= ~uint32_t(__ballot(own));
-        for (int q0 = 0; q0 < p.rank; q0 += 16) {
-            accx4 acc = {0, 0, 0, 0};
-            const _Float16 *a = static_cast<const _Float16 *>(p.a) + (int64_t(max(s, 0)) * p.rank + min(q0 + r16, p.rank - 1)) * p.ci;
+        if (s >= 0) fetch(s, 0, 0);
+        for (int q0 = 0; q0 < p.rank; q0 += 16 * kTiles) {
+            accx4 acc[kTiles];
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) acc[j] = accx4{0, 0, 0, 0};
             for (int pass = 0; pass < passes; ++pass) {
-                if (passes > 1) load(pass);
-                halfx8 av[kUnits];
-                if (s >= 0)
-#pragma unroll
-                    for (int u = 0; u < kUnits; ++u)
-                        av[u] = load8<VEC>(a, pass * kPass + (wave * kUnits + u) * 32 + kg * 8, p.ci);
-#pragma unroll
-                for (int u = 0; u < kUnits; ++u) {
-                    const int k = pass * kPass + (wave * kUnits + u) * 32 + kg * 8;
-                    halfx8 hi, lo;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        _Float16 h, l;
-                        split2(v[u][i / 4][i % 4], kSplitExp - e, h, l);
-                        hi[i] = h, lo[i] = l;
-                    }
-                    if (first && row < p.rows && k < cip) {
-                        _Float16 *dst = parts + row * 2 * cip + k;
-                        *reinterpret_cast<halfx8 *>(dst) = hi;
-                        *reinterpret_cast<halfx8 *>(dst + cip) = lo;
-                    }
-                    if (s >= 0) {
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u], lo, acc, 0, 0, 0);
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u], hi, acc, 0, 0, 0);
-                    }
+                if (passes > 1) {
+                    load(pass);
+                    part_values();
                 }
+                if (first && row < p.rows)
+#pragma unroll
+                    for (int u = 0; u < kUnits; ++u) {
+                        const int k = pass * kPass + (wave * kUnits + u) * 32 + kg * 8;
+                        if (k >= cip) continue;
+                        _Float16 *dst = parts + row * P * cip + k;
+                        *reinterpret_cast<halfx8 *>(dst) = hi[u];
+                        if constexpr (P == 2) *reinterpret_cast<halfx8 *>(dst + cip) = lo[u];
+                    }
+                if (s < 0) continue;
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+                    for (int j = 0; j < kTiles; ++j) {
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][u], lo[u], acc[j], 0, 0, 0);
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][u], hi[u], acc[j], 0, 0, 0);
+                    }
+                if (pass + 1 < passes) fetch(s, q0, pass + 1);
+                else if (q0 + 16 * kTiles < p.rank) fetch(s, q0 + 16 * kTiles, 0);
             }
             first = false;
             if (s < 0) break;
             __syncthreads();  // the sums before have been read
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i];
+            for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][j][i][lane] = acc[j][i];
             __syncthreads();
-            // register i is rank 4 (l / 16) + i of row l % 16
-            if (wave == 0 && own) {
+            // wave j joins rank tile j; register i is rank 4 (l / 16) + i of row l % 16
+            if (wave < kTiles && own && q0 + wave * 16 < p.rank) {
                 floatx4 t = {0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < kPassWaves; ++w)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) t[i] += part[w][i][lane];
+                    for (int i = 0; i < 4; ++i) t[i] += part[w][wave][i][lane];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) t[i] = ldexpf(t[i], e - kSplitExp);
-                *reinterpret_cast<floatx4 *>(p.t + row * p.rank_pad + q0 + kg * 4) = t;
+                *reinterpret_cast<floatx4 *>(p.t + row * p.rank_pad + q0 + wave * 16 + kg * 4) = t;
             }
         }
     } while (todo);
@@ -209,19 +244,20 @@ __device__ __forceinline__ void read_t(const float *t, int k, int rank, bool wan
     }
 }
 
-constexpr int kGK = 64;  // of the long axis per stage
-
-// WP: parts of the weight (1: f16 as stored, rows of ci; 2: rows of 2 cip); VW: its rows
-// allow 16-byte loads; T: the adapters' storage.
-template <int BT, int WP, bool VW, typename T>
-__global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArgs g) {
-    constexpr int S = BT / 64;                        // 32-tiles of a wave in each direction
-    constexpr int XS = 2 * kGK + 8, WS = WP * kGK + 8;  // staged rows (halves), on distinct banks
-    constexpr int R = kGK / 8, XU = BT * 2 * R / 256, WU = BT * WP * R / 256;  // runs of 8 per part, per thread
+// P: parts of x; WPARTS: the weight is in as many, rows of P cip (else f16 as stored, rows
+// of ci); VW: its rows allow 16-byte loads; T: the adapters' storage. KG: groups of four waves that share the long
+// axis.
+template <int BT, int KG, int P, bool WPARTS, bool VW, typename T>
+__global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_gemm_kernel(GemmArgs g) {
+    constexpr int NT = 256 * KG, GK = 64 * KG;  // GK: of the long axis per stage
+    constexpr int WP = WPARTS ? P : 1;
+    constexpr int S = BT / 64;                      // 32-tiles of a wave in each direction
+    constexpr int XS = P * GK + 8, WS = WP * GK + 8;  // staged rows (halves), on distinct banks
+    constexpr int R = GK / 8, XU = BT * P * R / NT, WU = BT * WP * R / NT;  // runs of 8 per part, per thread
     __shared__ __align__(16) _Float16 xs[BT * XS], ws[BT * WS];
     const LoraArgs &p = g.l;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave & 1, wn = wave >> 1, l32 = lane & 31, h = lane >> 5;
+    const int wm = wave & 1, wn = wave >> 1 & 1, kg = wave >> 2, l32 = lane & 31, h = lane >> 5;
     // Tiles of columns within tiles of rows, a contiguous eighth per XCD: a tile's rows are
     // read from memory once.
     const int tiles = g.tiles_m * g.tiles_n, per_xcd = (tiles + 7) / 8;
@@ -230,28 +266,28 @@ __global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArg
     const int c0 = (w % g.tiles_m) * BT;
     const int64_t r0 = int64_t(w / g.tiles_m) * BT;
 
-    // A thread's runs: the same place of rows 256 / (2 R) (columns 256 / (WP R)) apart, as
+    // A thread's runs: the same place of rows NT / (P R) (columns NT / (WP R)) apart, as
     // offsets from the tile's first, which the step moves on. The runs of hi, then of lo.
-    static_assert(256 % (2 * R) == 0, "runs");
+    static_assert(NT % (P * R) == 0, "runs");
     halfx8 xr[XU], wv[WU];
     uint32_t wo[WU];
-    const int xrun = tid % (2 * R), wrun = tid % (WP * R);
+    const int xrun = tid % (P * R), wrun = tid % (WP * R);
     // (the parts of x hold whole tiles of rows)
-    const uint32_t xo = uint32_t((tid / (2 * R) * 2 + xrun / R) * g.cip + xrun % R * 8) * 2;
-    const uint32_t xstep = uint32_t(256 / (2 * R)) * 2 * uint32_t(g.cip) * 2;
+    const uint32_t xo = uint32_t((tid / (P * R) * P + xrun / R) * g.cip + xrun % R * 8) * 2;
+    const uint32_t xstep = uint32_t(NT / (P * R)) * P * uint32_t(g.cip) * 2;
 #pragma unroll
     for (int u = 0; u < WU; ++u) {
-        const int c = min(tid / (WP * R) + u * (256 / (WP * R)), p.co - 1 - c0);
-        wo[u] = uint32_t(WP == 2 ? (c * 2 + wrun / R) * g.cip + wrun % R * 8 : c * p.ci) * 2;
+        const int c = min(tid / (WP * R) + u * (NT / (WP * R)), p.co - 1 - c0);
+        wo[u] = uint32_t(WPARTS ? (c * P + wrun / R) * g.cip + wrun % R * 8 : c * p.ci) * 2;
     }
-    const char *xb = reinterpret_cast<const char *>(g.xp + r0 * 2 * g.cip);
-    const char *wb = static_cast<const char *>(g.w) + int64_t(c0) * (WP == 2 ? 2 * g.cip : p.ci) * 2;
+    const char *xb = reinterpret_cast<const char *>(g.xp + r0 * P * g.cip);
+    const char *wb = static_cast<const char *>(g.w) + int64_t(c0) * (WPARTS ? P * g.cip : p.ci) * 2;
     auto fetch = [&](int k) {
 #pragma unroll
         for (int u = 0; u < XU; ++u) xr[u] = *reinterpret_cast<const halfx8 *>(xb + k * 2 + u * xstep + xo);
 #pragma unroll
         for (int u = 0; u < WU; ++u) {
-            if constexpr (WP == 2) wv[u] = *reinterpret_cast<const halfx8 *>(wb + k * 2 + wo[u]);
+            if constexpr (WPARTS) wv[u] = *reinterpret_cast<const halfx8 *>(wb + k * 2 + wo[u]);
             else wv[u] = load8<VW>(reinterpret_cast<const _Float16 *>(wb + wo[u]), k + wrun * 8, p.ci);
         }
     };
@@ -271,44 +307,62 @@ __global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArg
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.0f;
     fetch(0);
-    for (int k = 0; k < g.cip; k += kGK) {
+    for (int k = 0; k < p.ci; k += GK) {  // (cip is a whole number of stages)
         if (k) __syncthreads();
 #pragma unroll
         for (int u = 0; u < XU; ++u) {
-            const int i = tid + u * 256;
-            *reinterpret_cast<halfx8 *>(xs + i / (2 * R) * XS + i % (2 * R) * 8) = xr[u];
+            const int i = tid + u * NT;
+            *reinterpret_cast<halfx8 *>(xs + i / (P * R) * XS + i % (P * R) * 8) = xr[u];
         }
 #pragma unroll
         for (int u = 0; u < WU; ++u) {
-            const int i = tid + u * 256;
+            const int i = tid + u * NT;
             *reinterpret_cast<halfx8 *>(ws + i / (WP * R) * WS + i % (WP * R) * 8) = wv[u];
         }
         __syncthreads();
-        if (k + kGK < g.cip) fetch(k + kGK);
+        if (k + GK < p.ci) fetch(k + GK);
 #pragma unroll
-        for (int c = 0; c < kGK / 16; ++c) {
+        for (int c4 = 0; c4 < 4; ++c4) {
+            const int c = kg * 4 + c4;
             halfx8 xh[S], xl[S];
 #pragma unroll
             for (int n = 0; n < S; ++n) {
                 const _Float16 *q = xs + (wn * S * 32 + n * 32 + l32) * XS + c * 16 + h * 8;
                 xh[n] = *reinterpret_cast<const halfx8 *>(q);
-                xl[n] = *reinterpret_cast<const halfx8 *>(q + kGK);
+                if constexpr (P == 2) xl[n] = *reinterpret_cast<const halfx8 *>(q + GK);
             }
 #pragma unroll
             for (int m = 0; m < S; ++m) {
                 const _Float16 *q = ws + (wm * S * 32 + m * 32 + l32) * WS + c * 16 + h * 8;
                 const halfx8 wh = *reinterpret_cast<const halfx8 *>(q);
                 if constexpr (WP == 2) {
-                    const halfx8 wl = *reinterpret_cast<const halfx8 *>(q + kGK);
+                    const halfx8 wl = *reinterpret_cast<const halfx8 *>(q + GK);
 #pragma unroll
                     for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wl, xh[n], acc[m][n]);
                 }
+                if constexpr (P == 2)
 #pragma unroll
-                for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xl[n], acc[m][n]);
+                    for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xl[n], acc[m][n]);
 #pragma unroll
                 for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xh[n], acc[m][n]);
             }
         }
+    }
+
+    if constexpr (KG > 1) {  // the groups' sums, one after another
+        static_assert(sizeof(xs) >= 4 * S * S * 16 * 64 * sizeof(float), "sums");
+        float *sum = reinterpret_cast<float *>(xs) + (wave & 3) * S * S * 16 * 64 + lane;
+        for (int q = 1; q < KG; ++q) {
+            __syncthreads();
+            if (kg == q)
+#pragma unroll
+                for (int i = 0; i < S * S * 16; ++i) sum[i * 64] = acc[i / 16 / S][i / 16 % S][i % 16];
+            __syncthreads();
+            if (kg == 0)
+#pragma unroll
+                for (int i = 0; i < S * S * 16; ++i) acc[i / 16 / S][i / 16 % S][i % 16] += sum[i * 64];
+        }
+        if (kg) return;
     }
 
     // Columns 8 f + 4 h + e of a 32-tile are register 4 f + e; the row is lane % 32.
@@ -322,7 +376,7 @@ __global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArg
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 int e = xe[n];
-                if constexpr (WP == 2)
+                if constexpr (WPARTS)
                     e += g.w_exp[min(c0 + (wm * S + m) * 32 + 8 * (i / 4) + 4 * h + i % 4, p.co - 1)] - kSplitExp;
                 acc[m][n][i] = ldexpf(acc[m][n][i], e);
             }
@@ -421,55 +475,69 @@ __global__ __launch_bounds__(256, WP == 1 ? 3 : 2) void lora_gemm_kernel(GemmArg
     }
 }
 
-template <int BT, int WP, bool VW>
+template <int BT, int KG, int P, bool WPARTS, bool VW>
 void launch(Context &ctx, GemmArgs g, WeightType at) {
     g.tiles_m = int(ceil_div(g.l.co, BT));
     const int64_t tn = ceil_div(g.l.rows, BT);
     MH_REQUIRE(tn * g.tiles_m < (int64_t(1) << 30), "lora: too many tiles");
     g.tiles_n = int(tn);
-    const dim3 grid{uint32_t(ceil_div(tn * g.tiles_m, 8) * 8)}, tb{256};
-    if (at == kF16) lora_gemm_kernel<BT, WP, VW, _Float16><<<grid, tb, 0, ctx.stream>>>(g);
-    else lora_gemm_kernel<BT, WP, VW, float><<<grid, tb, 0, ctx.stream>>>(g);
+    const dim3 grid{uint32_t(ceil_div(tn * g.tiles_m, 8) * 8)}, tb{256 * KG};
+    if (at == kF16) lora_gemm_kernel<BT, KG, P, WPARTS, VW, _Float16><<<grid, tb, 0, ctx.stream>>>(g);
+    else lora_gemm_kernel<BT, KG, P, WPARTS, VW, float><<<grid, tb, 0, ctx.stream>>>(g);
     MH_LAUNCH_CHECK();
 }
 
-template <int BT>
-void launch_bt(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
-    if (wt == kF32) return launch<BT, 2, true>(ctx, g, at);
-    if (g.l.ci % 8 == 0 && aligned16(g.w)) launch<BT, 1, true>(ctx, g, at);
-    else launch<BT, 1, false>(ctx, g, at);
+template <int BT, int KG, int P>
+void launch_parts(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
+    if (wt == kF32) launch<BT, KG, P, true, true>(ctx, g, at);
+    else if (g.l.ci % 8 == 0 && aligned16(g.w)) launch<BT, KG, P, false, true>(ctx, g, at);
+    else launch<BT, KG, P, false, false>(ctx, g, at);
 }
 
-int64_t tiles_of(int64_t rows, int c_out, int bt) { return ceil_div(rows, bt) * ceil_div(c_out, bt); }
+template <int P>
+void launch_tiles(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
+    // 2048 rows of 1280 x 1280: 41 us with one group of tiles of 64, 44 with two; 1024 rows
+    // 33 and 30.5; 128 rows 29, 25 and with four groups 23, but 15.8 and 16.4 where the long
+    // axis is 320.
+    auto tiles = [&](int bt) { return ceil_div(g.l.rows, bt) * ceil_div(g.l.co, bt); };
+    if (tiles(128) >= ctx.cu_count) launch_parts<128, 1, P>(ctx, g, wt, at);
+    else if (tiles(64) >= 2 * ctx.cu_count) launch_parts<64, 1, P>(ctx, g, wt, at);
+    else if (tiles(64) >= ctx.cu_count || g.l.ci < 1024) launch_parts<64, 2, P>(ctx, g, wt, at);
+    else launch_parts<64, 4, P>(ctx, g, wt, at);
+}
+
+template <int P>
+void launch_split_rows(Context &ctx, const SplitRows &a, const SplitRows &b, int ci, int cip) {
+    const dim3 grid{uint32_t(ceil_div(a.rows + b.rows, 4))}, tb{256};
+    if (ci % 4 == 0 && aligned16(a.x) && aligned16(b.x)) split_rows_kernel<true, P><<<grid, tb, 0, ctx.stream>>>(a, b, ci, cip);
+    else split_rows_kernel<false, P><<<grid, tb, 0, ctx.stream>>>(a, b, ci, cip);
+    MH_LAUNCH_CHECK();
+}
+
+template <int P>
+void launch_split_shrink(Context &ctx, const LoraArgs &p, int cip, _Float16 *parts, int *exps) {
+    const dim3 grid{uint32_t(ceil_div(p.rows, 16))}, tb{64 * kPassWaves};
+    if (p.ci % 8 == 0 && aligned16(p.x) && aligned16(p.a))
+        split_shrink_kernel<true, P><<<grid, tb, 0, ctx.stream>>>(p, cip, parts, exps);
+    else split_shrink_kernel<false, P><<<grid, tb, 0, ctx.stream>>>(p, cip, parts, exps);
+    MH_LAUNCH_CHECK();
+}
 
 }  // namespace
 
-void split_rows(Context &ctx, const float *x, int64_t rows, int ci, int cip, _Float16 *parts, int *exps) {
-    const int64_t blocks = ceil_div(rows, 4);
-    MH_REQUIRE(blocks < (int64_t(1) << 31), "lora: too many rows");
-    const dim3 grid{uint32_t(blocks)}, tb{256};
-    if (ci % 4 == 0 && aligned16(x)) split_rows_kernel<true><<<grid, tb, 0, ctx.stream>>>(x, rows, ci, cip, parts, exps);
-    else split_rows_kernel<false><<<grid, tb, 0, ctx.stream>>>(x, rows, ci, cip, parts, exps);
-    MH_LAUNCH_CHECK();
+void split_rows(Context &ctx, const SplitRows &a, const SplitRows &b, int ci, int cip, int nparts) {
+    if (nparts == 1) launch_split_rows<1>(ctx, a, b, ci, cip);
+    else launch_split_rows<2>(ctx, a, b, ci, cip);
 }
 
-void split_shrink(Context &ctx, const LoraArgs &p, int cip, _Float16 *parts, int *exps) {
-    const int64_t blocks = ceil_div(p.rows, 16);
-    MH_REQUIRE(blocks < (int64_t(1) << 31), "lora: too many rows");
-    const dim3 grid{uint32_t(blocks)}, tb{64 * kPassWaves};
-    if (p.ci % 8 == 0 && aligned16(p.x) && aligned16(p.a))
-        split_shrink_kernel<true><<<grid, tb, 0, ctx.stream>>>(p, cip, parts, exps);
-    else split_shrink_kernel<false><<<grid, tb, 0, ctx.stream>>>(p, cip, parts, exps);
-    MH_LAUNCH_CHECK();
+void split_shrink(Context &ctx, const LoraArgs &p, int cip, int nparts, _Float16 *parts, int *exps) {
+    if (nparts == 1) launch_split_shrink<1>(ctx, p, cip, parts, exps);
+    else launch_split_shrink<2>(ctx, p, cip, parts, exps);
 }
 
-bool gemm_fits(const Context &ctx, int64_t rows, int c_out, int c_in) {
-    return tiles_of(rows, c_out, 64) >= ctx.cu_count / 2;
-}
-
-void gemm(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
-    if (tiles_of(g.l.rows, g.l.co, 128) >= ctx.cu_count) launch_bt<128>(ctx, g, wt, at);
-    else launch_bt<64>(ctx, g, wt, at);
+void gemm(Context &ctx, const GemmArgs &g, int nparts, WeightType wt, WeightType at) {
+    if (nparts == 1) launch_tiles<1>(ctx, g, wt, at);
+    else launch_tiles<2>(ctx, g, wt, at);
 }
 
 }  // namespace lora

@@ -11,6 +11,7 @@ import pytest
 from moebius_cpu_amd import engine as E
 from moebius_cpu_amd._lib import MoebiusError
 from moebius_cpu_amd.adapters import Adapters
+from tests.graph_capture import capture
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -46,6 +47,9 @@ CASES = [  # n, h, w, ci, co, rank, slots, per pixel
     # enough rows and columns for the product of operands in two f16 parts
     (4, 32, 32, 320, 640, 16, 3, False), (3, 23, 29, 333, 1030, 12, 4, False), (1, 50, 43, 100, 1281, 40, 9, True),
     (5, 20, 21, 64, 1280, 72, 2, False), (2, 20, 25, 1400, 1300, 24, 3, False),
+    # its tiles, and the groups of waves that share the long axis
+    (1, 27, 30, 1100, 320, 12, 3, True), (2, 19, 23, 2600, 330, 40, 3, False), (1, 27, 30, 333, 321, 33, 5, True),
+    (1, 64, 65, 72, 1100, 20, 4, True), (1, 4100, 1, 33, 1030, 16, 2, True), (1, 20, 20, 40, 600, 256, 2, True),
 ]
 
 
@@ -185,3 +189,53 @@ def test_python_refusals(ctx):
         Adapters(ctx, ad.a, E.Param(ctx, d["b"], f16=True), d["scale"], 32, 16, 4)
     with pytest.raises(MoebiusError, match="residual shape"):
         conv.forward_adapted(x, ad, E.DeviceArray(ctx, (2,), "i4"), out, E.Tensor(ctx, 1, 2, 2, 16))
+
+
+@pytest.mark.parametrize("fast", [False, True])
+@pytest.mark.parametrize("case", [(4, 1, 1, 640, 64, 16, 4, False), (2, 20, 20, 640, 640, 16, 4, False),
+                                  (40, 5, 5, 96, 700, 8, 9, True)])
+def test_captured_and_replayed(ctx, case, fast):
+    """Two graphs of one projection with scratch of their own, replayed among eager calls in the
+    context's workspace; without scratch a captured call is refused."""
+    n, h, w, ci, co, rank, slots, pixel = case
+    d = make(ctx, case, False)
+    conv, ad = layer(ctx, case, d, False)
+    slot = E.DeviceArray.from_numpy(ctx, d["slot"])
+    xs = [E.Tensor.from_numpy(ctx, d["x"]), E.Tensor.from_numpy(ctx, d["x"][..., ::-1])]
+    res = E.Tensor.from_numpy(ctx, d["res"])
+    outs, eager = [E.Tensor(ctx, n, h, w, co) for _ in xs], E.Tensor(ctx)
+    ctx.set_precision(fast)
+    try:
+        wants = []
+        for x in xs:
+            conv.forward_adapted(x, ad, slot, eager, res)
+            wants.append(eager.numpy())
+        scratch = [E.DeviceArray(ctx, (ad.scratch(n * h * w, conv.weight),), np.uint8) for _ in xs]
+        with pytest.raises(MoebiusError, match="captured call needs scratch"):
+            capture(ctx, lambda: conv.forward_adapted(xs[0], ad, slot, outs[0], res))
+        graphs = [capture(ctx, lambda i=i: conv.forward_adapted(xs[i], ad, slot, outs[i], res, scratch[i])) for i in range(2)]
+        for turn in range(4):
+            for o in outs:
+                o.upload(np.zeros((n, h, w, co), np.float32))
+            for launch, _ in graphs:
+                launch()
+            conv.forward_adapted(xs[turn % 2], ad, slot, eager, res)
+            ctx.synchronize()
+            for o, want in zip(outs, wants):
+                assert np.array_equal(o.numpy(), want)
+            assert np.array_equal(eager.numpy(), wants[turn % 2])
+        for _, destroy in graphs:
+            destroy()
+    finally:
+        ctx.set_precision(False)
+
+
+@pytest.mark.parametrize("case", [(3, 1, 5, 64, 64, 8, 3, True), (2, 25, 25, 64, 640, 8, 3, False)])
+def test_residual_in_place(ctx, case):
+    d = make(ctx, case, True)
+    conv, ad = layer(ctx, case, d, True)
+    x, slot = E.Tensor.from_numpy(ctx, d["x"]), E.DeviceArray.from_numpy(ctx, d["slot"])
+    res, out = E.Tensor.from_numpy(ctx, d["res"]), E.Tensor(ctx)
+    conv.forward_adapted(x, ad, slot, out, res)
+    conv.forward_adapted(x, ad, slot, res, res)
+    assert np.array_equal(res.numpy(), out.numpy())
