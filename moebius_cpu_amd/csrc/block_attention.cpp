@@ -18,7 +18,9 @@ int head_tiles(int d, bool vec) {
 }
 
 // Waves of 32 rows that share a tile of keys: as many as the rows of a block of queries
-// fill, up to four.
+// fill, up to four. 24 heads of 64, 8192 rows in blocks of 128, 2048 keys each: four 142 us,
+// two 165; 8 heads, 4096 rows in blocks of 64, 1024 keys: two 20.6, one 31.7, four 27.8; in
+// blocks of 32: one 30.7, two 34.0.
 int row_waves(const BlockShape &s) {
     const int64_t rows = int64_t(std::min(s.q_block, s.q_tokens)) * (s.heads_q / s.heads_kv);
     return rows > 64 ? 4 : rows > 32 ? 2 : 1;
@@ -30,9 +32,18 @@ struct Plan {
     bool split;     // f32 operands as two f16 parts
 };
 
-// The list is split over workgroups where the rows alone leave CUs idle, into shares of
-// at least 128 keys. f32 products are split where the keys and values, which that reads and
-// writes once, are then read at least kSplitReuse times by waves full of rows.
+// The list is split over workgroups where the rows alone leave CUs idle: into a power of
+// two of shares (equal ones of most lists), of 256 keys, or of 128 where that leaves CUs
+// idle, up to two workgroups per CU. Single tokens, 8 heads of 128, f16, caches that are
+// not in the L2, us without splits, with this rule, with half and with twice as many: 1 item
+// of 4096 keys 95, 17.6, 22, 18.3; 4 of 2048 46, 19.1, 21.9, 20.7; 8 of 2048 47, 24.6, 24.9,
+// 31; 16 of 2048 52.8, 35.9, 37.4, 40.1; 1 of 512 15.1, 12.1, 13.7, 12.1; 4 of 256 10.9
+// without, 12.6 with two; 40 of 2048 76.3 without, 88.7 with two.
+//
+// f32 products are split where the keys and values, which that reads and writes once, are
+// then read at least kSplitReuse times by waves full of rows: 4096 keys, 8 heads of 80, read
+// once 36.9 us (31.2 on the f32 instructions), twice 41.2 (47.3), four times 41.3 (59.1),
+// sixteen times 72 (158).
 constexpr int64_t kSplitReuse = 2;
 Plan plan(const Context &ctx, const BlockShape &s, WeightType type, bool half) {
     Plan p;
@@ -41,9 +52,12 @@ Plan plan(const Context &ctx, const BlockShape &s, WeightType type, bool half) {
     p.row_tiles = int(ceil_div(rows, p.wr * 32));
     p.items = int64_t(s.n) * s.heads_kv * s.q_blocks() * p.row_tiles;
     const int64_t keys = std::min<int64_t>(int64_t(s.top) * s.kv_block, s.kv_tokens);
-    const int64_t splits =
-        p.items >= ctx.cu_count ? 1 : std::min<int64_t>(2 * ctx.cu_count / std::max<int64_t>(p.items, 1), keys / 128);
-    p.splits = int(std::max<int64_t>(1, std::min<int64_t>(splits, 64)));
+    p.splits = 1;
+    if (p.items < ctx.cu_count && keys >= 512) {
+        const int64_t items = std::max<int64_t>(p.items, 1), cus = ctx.cu_count;
+        const int64_t most = std::min<int64_t>(2 * cus / items, std::max<int64_t>(keys / 256, std::min<int64_t>(4, cus / items)));
+        while (2 * p.splits <= most) p.splits *= 2;
+    }
     p.split = type == kF32 && !half && s.kv_tokens > 0 && battn::split_fits(p.wr, head_tiles(s.d, false)) &&
               battn::split_fits(p.wr, head_tiles(s.d, true)) &&
               int64_t(s.q_blocks()) * p.row_tiles * keys >= kSplitReuse * s.kv_tokens;

@@ -294,7 +294,8 @@ void launch_w(Context &ctx, RopeArgs &a) {
     a.units = a.rot_units + (a.d - 2 * a.pairs) / W;
     const int gl = a.units <= 8 ? 8 : a.units <= 16 ? 16 : a.units <= 32 ? 32 : 64;
     // Heads per lane group: all of them share the unit's cosines, but the card wants
-    // about 16 waves on every CU first.
+    // about 16 waves on every CU first. 24 heads of 128, 16384 rows, f16: 1 56.9 us, 2 35.5,
+    // 4 or more 32; 8 heads, 64 rows: 5 us each way.
     const int most = std::max(a.heads[0], a.heads[1]);
     const int64_t want = int64_t(ctx.cu_count) * 16 * 64;
     a.per = int(std::max<int64_t>(1, std::min<int64_t>(most, int64_t(a.rows) * (a.heads[0] + a.heads[1]) * gl / want)));

@@ -25,6 +25,7 @@ from moebius_cpu_amd import engine as E
 from moebius_cpu_amd._lib import MoebiusError
 from moebius_cpu_amd.attention import (Heads, RopeAxes, block_attention, block_attention_scratch, block_means,
                                        block_select, qk_norm_rope)
+from tests.graph_capture import capture
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -433,21 +434,19 @@ def test_scratch_is_checked(ctx):
     a = out.numpy()
     block_attention(q, k, v, blocks, out, q_block=1)
     assert np.array_equal(out.numpy(), a)
-
-
-def _capture(ctx, calls):
-    """The calls captured from the context's stream into a graph: (launch, destroy)."""
-    hip = ctypes.CDLL("libamdhip64.so")
-    stream = ctypes.c_void_p(_lib.lib().mh_context_stream(ctx.h))
-    graph, execg = ctypes.c_void_p(), ctypes.c_void_p()
-    assert hip.hipStreamBeginCapture(stream, 2) == 0  # relaxed
-    try:
-        calls()
-    finally:
-        ended = hip.hipStreamEndCapture(stream, ctypes.byref(graph))
-    assert ended == 0
-    assert hip.hipGraphInstantiate(ctypes.byref(execg), graph, None, None, 0) == 0
-    return (lambda: hip.hipGraphLaunch(execg, stream)), (lambda: (hip.hipGraphExecDestroy(execg), hip.hipGraphDestroy(graph)))
+    with pytest.raises(MoebiusError, match="captured call needs scratch"):
+        capture(ctx, lambda: block_attention(q, k, v, blocks, out, q_block=1))
+    ctx.synchronize()
+    few = dev(ctx, np.arange(4, dtype=np.int32).reshape(1, 1, 2, 2))  # lists that are not split need none
+    assert block_attention_scratch(q, k, few, 1, 64) == 0
+    launch, destroy = capture(ctx, lambda: block_attention(q, k, v, few, out, q_block=1))
+    block_attention(q, k, v, few, out, q_block=1)
+    a = out.numpy()
+    out.buf.upload(np.zeros_like(a))
+    launch()
+    ctx.synchronize()
+    assert np.array_equal(out.numpy(), a)
+    destroy()
 
 
 def test_a_layer_step_captured_and_replayed(ctx):
@@ -489,15 +488,12 @@ def test_a_layer_step_captured_and_replayed(ctx):
         got = st["out"].numpy()
         assert np.all(np.abs(got - want) <= tolerance(want, tol, d, np.float16, False))
         wants.append(got)
-    with pytest.raises(MoebiusError, match="captured call needs scratch"):
-        _capture(ctx, lambda: step(states[0], None))
-    ctx.synchronize()
-    graphs = [_capture(ctx, lambda st=st: step(st, st["scratch"])) for st in states]
+    graphs = [capture(ctx, lambda st=st: step(st, st["scratch"])) for st in states]
     for turn in range(4):
         for st in states:
             st["out"].buf.upload(np.zeros((n, 1, hq, d), np.float16))
         for launch, _ in graphs:
-            assert launch() == 0
+            launch()
         if turn % 2:
             block_attention(states[0]["qo"], states[0]["k"], cache_v, states[1]["blocks"], Heads(E.DeviceArray(ctx, (n, 1, hq, d), "f2"), n, 1, hq, d),
                             q_block=1, kv_block=kb)  # eager work between replays, in the context's own workspace
