@@ -8,15 +8,16 @@
 //
 // FAST contexts take one part (operands rounded to f16 after their row's scale).
 //
-// A workgroup forms BT columns x BT rows, four waves the 2 x 2 quarters, as W . X^T: a lane
+// A workgroup forms BM columns x BN rows, four waves the 2 x 2 quarters, as W . X^T: a lane
 // of a 32x32 result holds one row and four runs of four columns, so a row's scale and its
 // adapter are the lane's own. 64 of the long axis are staged in LDS at a time while the
 // next are loaded; where the tiles are too few to hide those loads in each other, two or
 // four such groups of waves share the long axis. Bound: the matrix instructions; the parts
 // of x are written and read once more than x itself.
 //
-// Measured: 8192 rows, 1280 x 1280, f16 weight, rank 32, residual: 121 us, of it 92 the
-// product (54 GFLOP in two f16 products: 583 TFLOP/s) and 27 the pass over x.
+// Measured: 8192 rows, 1280 x 1280, f16 weight, rank 32, residual: 118 us, of it 88 the
+// product (54 GFLOP in two f16 products: 611 TFLOP/s; 75 us without residual and adapters)
+// and 24 the pass over x.
 #include <algorithm>
 
 #include "lora.hpp"
@@ -245,16 +246,16 @@ __device__ __forceinline__ void read_t(const float *t, int k, int rank, bool wan
 }
 
 // P: parts of x; WPARTS: the weight is in as many, rows of P cip (else f16 as stored, rows
-// of ci); VW: its rows allow 16-byte loads; T: the adapters' storage. KG: groups of four waves that share the long
-// axis.
-template <int BT, int KG, int P, bool WPARTS, bool VW, typename T>
-__global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_gemm_kernel(GemmArgs g) {
+// of ci); VW: its rows allow 16-byte loads; T: the adapters' storage; KG: groups of four waves that share the
+// long axis.
+template <int BM, int BN, int KG, int P, bool WPARTS, bool VW, typename T>
+__global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS || BM > 128 ? 2 : 3) void lora_gemm_kernel(GemmArgs g) {
     constexpr int NT = 256 * KG, GK = 64 * KG;  // GK: of the long axis per stage
     constexpr int WP = WPARTS ? P : 1;
-    constexpr int S = BT / 64;                      // 32-tiles of a wave in each direction
+    constexpr int SM = BM / 64, SN = BN / 64;       // 32-tiles of a wave: of columns, of rows
     constexpr int XS = P * GK + 8, WS = WP * GK + 8;  // staged rows (halves), on distinct banks
-    constexpr int R = GK / 8, XU = BT * P * R / NT, WU = BT * WP * R / NT;  // runs of 8 per part, per thread
-    __shared__ __align__(16) _Float16 xs[BT * XS], ws[BT * WS];
+    constexpr int R = GK / 8, XU = BN * P * R / NT, WU = BM * WP * R / NT;  // runs of 8 per part, per thread
+    __shared__ __align__(16) _Float16 xs[BN * XS], ws[BM * WS];
     const LoraArgs &p = g.l;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave & 1, wn = wave >> 1 & 1, kg = wave >> 2, l32 = lane & 31, h = lane >> 5;
@@ -263,8 +264,8 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
     const int tiles = g.tiles_m * g.tiles_n, per_xcd = (tiles + 7) / 8;
     const int w = int(blockIdx.x % 8) * per_xcd + int(blockIdx.x / 8);
     if (int(blockIdx.x / 8) >= per_xcd || w >= tiles) return;
-    const int c0 = (w % g.tiles_m) * BT;
-    const int64_t r0 = int64_t(w / g.tiles_m) * BT;
+    const int c0 = (w % g.tiles_m) * BM;
+    const int64_t r0 = int64_t(w / g.tiles_m) * BN;
 
     // A thread's runs: the same place of rows NT / (P R) (columns NT / (WP R)) apart, as
     // offsets from the tile's first, which the step moves on. The runs of hi, then of lo.
@@ -292,18 +293,18 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
         }
     };
     // The adapters of this lane's rows and the exponents of their parts.
-    int slot[S], xe[S];
+    int slot[SN], xe[SN];
 #pragma unroll
-    for (int n = 0; n < S; ++n) {
-        const int64_t row = r0 + (wn * S + n) * 32 + l32;
+    for (int n = 0; n < SN; ++n) {
+        const int64_t row = r0 + (wn * SN + n) * 32 + l32;
         slot[n] = slot_of(p, row);
         xe[n] = g.x_exp[min(row, p.rows - 1)] - kSplitExp;
     }
-    floatx16 acc[S][S];
+    floatx16 acc[SM][SN];
 #pragma unroll
-    for (int m = 0; m < S; ++m)
+    for (int m = 0; m < SM; ++m)
 #pragma unroll
-        for (int n = 0; n < S; ++n)
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[m][n][i] = 0.0f;
     fetch(0);
@@ -324,43 +325,43 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
             const int c = kg * 4 + c4;
-            halfx8 xh[S], xl[S];
+            halfx8 xh[SN], xl[SN];
 #pragma unroll
-            for (int n = 0; n < S; ++n) {
-                const _Float16 *q = xs + (wn * S * 32 + n * 32 + l32) * XS + c * 16 + h * 8;
+            for (int n = 0; n < SN; ++n) {
+                const _Float16 *q = xs + (wn * SN * 32 + n * 32 + l32) * XS + c * 16 + h * 8;
                 xh[n] = *reinterpret_cast<const halfx8 *>(q);
                 if constexpr (P == 2) xl[n] = *reinterpret_cast<const halfx8 *>(q + GK);
             }
 #pragma unroll
-            for (int m = 0; m < S; ++m) {
-                const _Float16 *q = ws + (wm * S * 32 + m * 32 + l32) * WS + c * 16 + h * 8;
+            for (int m = 0; m < SM; ++m) {
+                const _Float16 *q = ws + (wm * SM * 32 + m * 32 + l32) * WS + c * 16 + h * 8;
                 const halfx8 wh = *reinterpret_cast<const halfx8 *>(q);
                 if constexpr (WP == 2) {
                     const halfx8 wl = *reinterpret_cast<const halfx8 *>(q + GK);
 #pragma unroll
-                    for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wl, xh[n], acc[m][n]);
+                    for (int n = 0; n < SN; ++n) acc[m][n] = mfma16(wl, xh[n], acc[m][n]);
                 }
                 if constexpr (P == 2)
 #pragma unroll
-                    for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xl[n], acc[m][n]);
+                    for (int n = 0; n < SN; ++n) acc[m][n] = mfma16(wh, xl[n], acc[m][n]);
 #pragma unroll
-                for (int n = 0; n < S; ++n) acc[m][n] = mfma16(wh, xh[n], acc[m][n]);
+                for (int n = 0; n < SN; ++n) acc[m][n] = mfma16(wh, xh[n], acc[m][n]);
             }
         }
     }
 
     if constexpr (KG > 1) {  // the groups' sums, one after another
-        static_assert(sizeof(xs) >= 4 * S * S * 16 * 64 * sizeof(float), "sums");
-        float *sum = reinterpret_cast<float *>(xs) + (wave & 3) * S * S * 16 * 64 + lane;
+        static_assert(sizeof(xs) >= 4 * SM * SN * 16 * 64 * sizeof(float), "sums");
+        float *sum = reinterpret_cast<float *>(xs) + (wave & 3) * SM * SN * 16 * 64 + lane;
         for (int q = 1; q < KG; ++q) {
             __syncthreads();
             if (kg == q)
 #pragma unroll
-                for (int i = 0; i < S * S * 16; ++i) sum[i * 64] = acc[i / 16 / S][i / 16 % S][i % 16];
+                for (int i = 0; i < SM * SN * 16; ++i) sum[i * 64] = acc[i / 16 / SN][i / 16 % SN][i % 16];
             __syncthreads();
             if (kg == 0)
 #pragma unroll
-                for (int i = 0; i < S * S * 16; ++i) acc[i / 16 / S][i / 16 % S][i % 16] += sum[i * 64];
+                for (int i = 0; i < SM * SN * 16; ++i) acc[i / 16 / SN][i / 16 % SN][i % 16] += sum[i * 64];
         }
         if (kg) return;
     }
@@ -369,15 +370,15 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
     const bool vb = p.rank % 8 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0;
     const bool vo = p.co % 4 == 0 && aligned16_dev(p.out) && aligned16_dev(g.residual);
 #pragma unroll
-    for (int n = 0; n < S; ++n) {
-        const int64_t row = r0 + (wn * S + n) * 32 + l32, row_in = min(row, p.rows - 1);
+    for (int n = 0; n < SN; ++n) {
+        const int64_t row = r0 + (wn * SN + n) * 32 + l32, row_in = min(row, p.rows - 1);
 #pragma unroll
-        for (int m = 0; m < S; ++m)
+        for (int m = 0; m < SM; ++m)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 int e = xe[n];
                 if constexpr (WPARTS)
-                    e += g.w_exp[min(c0 + (wm * S + m) * 32 + 8 * (i / 4) + 4 * h + i % 4, p.co - 1)] - kSplitExp;
+                    e += g.w_exp[min(c0 + (wm * SM + m) * 32 + 8 * (i / 4) + 4 * h + i % 4, p.co - 1)] - kSplitExp;
                 acc[m][n][i] = ldexpf(acc[m][n][i], e);
             }
         const int mine = slot[n];
@@ -403,16 +404,16 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
                 const int s = __builtin_amdgcn_readfirstlane(__shfl(mine, __builtin_ctz(todo)));
                 const bool own = mine == s;
                 todo &= ~uint32_t(__ballot(own));
-                floatx16 low[S];
+                floatx16 low[SM];
 #pragma unroll
-                for (int m = 0; m < S; ++m)
+                for (int m = 0; m < SM; ++m)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) low[m][i] = 0.0f;
-                const T *b[S];
+                const T *b[SM];
 #pragma unroll
-                for (int m = 0; m < S; ++m)
+                for (int m = 0; m < SM; ++m)
                     b[m] = static_cast<const T *>(p.b) +
-                           (int64_t(s) * p.co + min(c0 + (wm * S + m) * 32 + l32, p.co - 1)) * p.rank;
+                           (int64_t(s) * p.co + min(c0 + (wm * SM + m) * 32 + l32, p.co - 1)) * p.rank;
                 for (int k = 0; k < p.rank; k += 16) {
                     float tv[8];
                     read_t(t, k + h * 8, p.rank, own, tv);
@@ -425,14 +426,14 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
                             th[i] = hi, tl[i] = lo;
                         }
 #pragma unroll
-                        for (int m = 0; m < S; ++m) {
+                        for (int m = 0; m < SM; ++m) {
                             const halfx8 bv = vb ? load8<true>(b[m], k + h * 8, p.rank) : load8<false>(b[m], k + h * 8, p.rank);
                             low[m] = mfma16(bv, tl, low[m]);
                             low[m] = mfma16(bv, th, low[m]);
                         }
                     } else {
 #pragma unroll
-                        for (int m = 0; m < S; ++m)
+                        for (int m = 0; m < SM; ++m)
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const float bv = k + h * 8 + i < p.rank ? float(b[m][k + h * 8 + i]) : 0.0f;
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
                 }
                 const float scale = p.scale[s];
 #pragma unroll
-                for (int m = 0; m < S; ++m)
+                for (int m = 0; m < SM; ++m)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float v = sizeof(T) == 2 ? ldexpf(low[m][i], te - kSplitExp) : low[m][i];
@@ -452,10 +453,10 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
         }
         if (row >= p.rows) continue;
 #pragma unroll
-        for (int m = 0; m < S; ++m)
+        for (int m = 0; m < SM; ++m)
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
-                const int c = c0 + (wm * S + m) * 32 + 8 * f + 4 * h;
+                const int c = c0 + (wm * SM + m) * 32 + 8 * f + 4 * h;
                 float *out = p.out + row * p.co + c;
                 const float *res = g.residual ? g.residual + row * p.co + c : nullptr;
                 if (vo && c < p.co) {
@@ -475,35 +476,46 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS ? 2 : 3) void lora_g
     }
 }
 
-template <int BT, int KG, int P, bool WPARTS, bool VW>
+template <int BM, int BN, int KG, int P, bool WPARTS, bool VW>
 void launch(Context &ctx, GemmArgs g, WeightType at) {
-    g.tiles_m = int(ceil_div(g.l.co, BT));
-    const int64_t tn = ceil_div(g.l.rows, BT);
+    g.tiles_m = int(ceil_div(g.l.co, BM));
+    const int64_t tn = ceil_div(g.l.rows, BN);
     MH_REQUIRE(tn * g.tiles_m < (int64_t(1) << 30), "lora: too many tiles");
     g.tiles_n = int(tn);
     const dim3 grid{uint32_t(ceil_div(tn * g.tiles_m, 8) * 8)}, tb{256 * KG};
-    if (at == kF16) lora_gemm_kernel<BT, KG, P, WPARTS, VW, _Float16><<<grid, tb, 0, ctx.stream>>>(g);
-    else lora_gemm_kernel<BT, KG, P, WPARTS, VW, float><<<grid, tb, 0, ctx.stream>>>(g);
+    if (at == kF16) lora_gemm_kernel<BM, BN, KG, P, WPARTS, VW, _Float16><<<grid, tb, 0, ctx.stream>>>(g);
+    else lora_gemm_kernel<BM, BN, KG, P, WPARTS, VW, float><<<grid, tb, 0, ctx.stream>>>(g);
     MH_LAUNCH_CHECK();
 }
 
-template <int BT, int KG, int P>
-void launch_parts(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
-    if (wt == kF32) launch<BT, KG, P, true, true>(ctx, g, at);
-    else if (g.l.ci % 8 == 0 && aligned16(g.w)) launch<BT, KG, P, false, true>(ctx, g, at);
-    else launch<BT, KG, P, false, false>(ctx, g, at);
+bool wide_weight(const GemmArgs &g) { return g.l.ci % 8 == 0 && aligned16(g.w); }
+
+template <int KG, int P>
+void launch_small(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
+    if (wt == kF32) launch<64, 64, KG, P, true, true>(ctx, g, at);
+    else if (wide_weight(g)) launch<64, 64, KG, P, false, true>(ctx, g, at);
+    else launch<64, 64, KG, P, false, false>(ctx, g, at);
 }
 
 template <int P>
 void launch_tiles(Context &ctx, const GemmArgs &g, WeightType wt, WeightType at) {
-    // 2048 rows of 1280 x 1280: 41 us with one group of tiles of 64, 44 with two; 1024 rows
-    // 33 and 30.5; 128 rows 29, 25 and with four groups 23, but 15.8 and 16.4 where the long
-    // axis is 320.
-    auto tiles = [&](int bt) { return ceil_div(g.l.rows, bt) * ceil_div(g.l.co, bt); };
-    if (tiles(128) >= ctx.cu_count) launch_parts<128, 1, P>(ctx, g, wt, at);
-    else if (tiles(64) >= 2 * ctx.cu_count) launch_parts<64, 1, P>(ctx, g, wt, at);
-    else if (tiles(64) >= ctx.cu_count || g.l.ci < 1024) launch_parts<64, 2, P>(ctx, g, wt, at);
-    else launch_parts<64, 4, P>(ctx, g, wt, at);
+    // 8192 rows of 1280 x 1280, the product alone: tiles of 128 x 128 92 us, 192 x 128 88;
+    // the whole call for 4096 rows, where the latter leave CUs idle, 65.5, with tiles of 64
+    // 59. 2048 rows: 41 with one group of waves, 44 with two; 1024 rows 33 and 30.5; 128 rows
+    // 29, 25 and with four groups 23, but 15.8 and 16.4 where the long axis is 320.
+    const int wide = wt == kF32 ? 128 : 192;  // columns of the large tile that registers hold
+    const int64_t tiles = ceil_div(g.l.rows, 64) * ceil_div(g.l.co, 64);
+    if (ceil_div(g.l.rows, 128) * ceil_div(g.l.co, wide) >= ctx.cu_count) {
+        if (wt == kF32) launch<128, 128, 1, P, true, true>(ctx, g, at);
+        else if (wide_weight(g)) launch<192, 128, 1, P, false, true>(ctx, g, at);
+        else launch<192, 128, 1, P, false, false>(ctx, g, at);
+    } else if (tiles >= 2 * ctx.cu_count) {
+        launch_small<1, P>(ctx, g, wt, at);
+    } else if (tiles >= ctx.cu_count || g.l.ci < 1024) {
+        launch_small<2, P>(ctx, g, wt, at);
+    } else {
+        launch_small<4, P>(ctx, g, wt, at);
+    }
 }
 
 template <int P>
