@@ -14,6 +14,7 @@
 // are selected away, not multiplied by zero, so values that are not finite stay with
 // their own requests.
 #include <algorithm>
+#include <type_traits>
 
 #include "lora.hpp"
 
@@ -164,22 +165,23 @@ __global__ __launch_bounds__(512) void lora_row_project_kernel(LoraArgs p, const
         const T *b = static_cast<const T *>(p.b) + (int64_t(s) * p.co + c) * p.rank;
         const float *t = p.t + row * p.rank_pad;
         float y = 0.0f;
-        if (p.rank % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % (4 * sizeof(T)) == 0) {
+        auto second = [&](auto vec) {
+            constexpr bool V = decltype(vec)::value;
             for (int k = 0; k < p.rank; k += 16) {
                 floatx4 bv[4], tv[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    bv[u] = load4<true>(b, k + 4 * u, p.rank);
-                    tv[u] = load4<true>(t, k + 4 * u, p.rank);
+                    bv[u] = load4<V>(b, k + 4 * u, p.rank);
+                    tv[u] = load4<V>(t, k + 4 * u, p.rank);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) y = __builtin_fmaf(tv[u][i], bv[u][i], y);
             }
-        } else {
-            for (int k = 0; k < p.rank; ++k) y = __builtin_fmaf(t[k], float(b[k]), y);
-        }
+        };
+        if (p.rank % 4 == 0 && reinterpret_cast<uintptr_t>(p.b) % (4 * sizeof(T)) == 0) second(std::true_type{});
+        else second(std::false_type{});
         v = __builtin_fmaf(scale, y, v);
     }
     p.out[row * p.co + c] = v;

@@ -19,31 +19,44 @@ struct LoraArgs {
     int ci, co, rank, slots, rank_pad;  // rank_pad: rank rounded up to 16
 };
 
-// Four values at p + k of a run of n, zeros behind it; VEC: n and p keep every run of four aligned.
+// N values at p + k of a run of n, zeros behind it, in one load: behind n - N the last N are
+// loaded instead and shifted, so that no load waits for a branch. VEC: n is a multiple of N
+// and every run aligned; else the load is of the element's alignment (the same instruction),
+// but for runs shorter than N.
+template <int N, bool VEC, typename T>
+__device__ __forceinline__ auto load_run(const T *p, int k, int n) {
+    typedef T V __attribute__((ext_vector_type(N)));
+    typedef T U __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    V v = T(0);
+    if constexpr (VEC) {
+        const V r = *reinterpret_cast<const V *>(p + min(k, n - N));
+        v = k < n ? r : v;
+    } else if (n >= N) {
+        const int at = min(k, n - N), d = k - at;  // values that the run's end is short of
+        const U r = *reinterpret_cast<const U *>(p + at);
+        if constexpr (N * sizeof(T) == 16) {
+            const unsigned __int128 bits = __builtin_bit_cast(unsigned __int128, V(r));
+            v = d < N ? __builtin_bit_cast(V, bits >> (min(d, N - 1) * int(8 * sizeof(T)))) : v;
+        } else {
+            const uint64_t bits = __builtin_bit_cast(uint64_t, V(r));
+            v = d < N ? __builtin_bit_cast(V, bits >> (min(d, N - 1) * int(8 * sizeof(T)))) : v;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = k + e < n ? p[min(k + e, n - 1)] : T(0);
+    }
+    return v;
+}
 template <bool VEC>
 __device__ __forceinline__ floatx4 load4(const float *p, int k, int n) {
-    if constexpr (VEC) {  // behind n the last run is loaded instead, so that no load waits for a branch
-        const floatx4 v = *reinterpret_cast<const floatx4 *>(p + min(k, n - 4));
-        return k < n ? v : floatx4{0, 0, 0, 0};
-    } else {
-        floatx4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k + e < n ? p[k + e] : 0.0f;
-        return v;
-    }
+    return load_run<4, VEC>(p, k, n);
 }
 template <bool VEC>
 __device__ __forceinline__ floatx4 load4(const _Float16 *p, int k, int n) {
-    floatx4 v = {0, 0, 0, 0};
-    if constexpr (VEC) {
-        const halfx4 r = *reinterpret_cast<const halfx4 *>(p + min(k, n - 4));
+    const halfx4 r = load_run<4, VEC>(p, k, n);
+    floatx4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = k < n ? float(r[e]) : 0.0f;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (k + e < n) v[e] = float(p[k + e]);
-    }
+    for (int e = 0; e < 4; ++e) v[e] = float(r[e]);
     return v;
 }
 
@@ -66,8 +79,6 @@ __device__ __forceinline__ void split2(float x, int e, _Float16 &hi, _Float16 &l
     const float r = y - float(hi);
     lo = static_cast<_Float16>(__builtin_fabsf(y) < __builtin_huge_valf() ? r : 0.0f);
 }
-// NULL counts as aligned.
-__device__ __forceinline__ bool aligned16_dev(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 __device__ __forceinline__ int top_exp(float mx) { return mx == 0.0f ? 0 : __builtin_amdgcn_frexp_expf(mx) - 1; }
 
 // The projection with the adapters' second product in its epilogue (lora_gemm.hip).

@@ -83,19 +83,9 @@ __global__ __launch_bounds__(256) void split_rows_kernel(SplitRows s0, SplitRows
     if (lane == 0) exps[row] = e;
 }
 
-// Eight values of a row of n at k, zeros behind it (VEC: n and p allow 16-byte loads).
 template <bool VEC>
 __device__ __forceinline__ halfx8 load8(const _Float16 *p, int k, int n) {
-    halfx8 v;
-    if constexpr (VEC) {
-        v = *reinterpret_cast<const halfx8 *>(p + min(k, n - 8));
-        const halfx8 zero = {0, 0, 0, 0, 0, 0, 0, 0};
-        v = k < n ? v : zero;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = k + e < n ? p[k + e] : _Float16(0);
-    }
-    return v;
+    return load_run<8, VEC>(p, k, n);
 }
 
 __device__ __forceinline__ floatx16 mfma16(halfx8 a, halfx8 b, floatx16 c) {
@@ -368,7 +358,7 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS || BM > 128 ? 2 : 3)
 
     // Columns 8 f + 4 h + e of a 32-tile are register 4 f + e; the row is lane % 32.
     const bool vb = p.rank % 8 == 0 && reinterpret_cast<uintptr_t>(p.b) % 16 == 0;
-    const bool vo = p.co % 4 == 0 && aligned16_dev(p.out) && aligned16_dev(g.residual);
+    typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
     for (int n = 0; n < SN; ++n) {
         const int64_t row = r0 + (wn * SN + n) * 32 + l32, row_in = min(row, p.rows - 1);
@@ -459,13 +449,13 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS || BM > 128 ? 2 : 3)
                 const int c = c0 + (wm * SM + m) * 32 + 8 * f + 4 * h;
                 float *out = p.out + row * p.co + c;
                 const float *res = g.residual ? g.residual + row * p.co + c : nullptr;
-                if (vo && c < p.co) {
+                if (c + 4 <= p.co) {
                     floatx4 y = {acc[m][n][4 * f], acc[m][n][4 * f + 1], acc[m][n][4 * f + 2], acc[m][n][4 * f + 3]};
                     if (g.bias)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y[e] += g.bias[c + e];
-                    if (res) y += *reinterpret_cast<const floatx4 *>(res);
-                    *reinterpret_cast<floatx4 *>(out) = y;
+                    if (res) y += floatx4(*reinterpret_cast<const float4u *>(res));
+                    *reinterpret_cast<float4u *>(out) = y;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
