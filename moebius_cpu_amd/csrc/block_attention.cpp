@@ -20,10 +20,13 @@ int head_tiles(int d, bool vec) {
 // Waves of 32 rows that share a tile of keys: as many as the rows of a block of queries
 // fill, up to four. 24 heads of 64, 8192 rows in blocks of 128, 2048 keys each: four 142 us,
 // two 165; 8 heads, 4096 rows in blocks of 64, 1024 keys: two 20.6, one 31.7, four 27.8; in
-// blocks of 32: one 30.7, two 34.0.
+// blocks of 32: one 30.7, two 34.0. Heads of more than 128 channels take two even where one
+// has no rows, as the registers that stage a tile are then shared by both: 8 heads of 160,
+// 2 x 4096 rows in blocks of 32, 1024 keys 130 us, 230 with one; single tokens of 8 requests,
+// 32 / 8 heads, 2048 keys 28.7 and 39.2; f32 148 and 177 (16 requests).
 int row_waves(const BlockShape &s) {
     const int64_t rows = int64_t(std::min(s.q_block, s.q_tokens)) * (s.heads_q / s.heads_kv);
-    return rows > 64 ? 4 : rows > 32 ? 2 : 1;
+    return rows > 64 ? 4 : rows > 32 || s.d > 128 ? 2 : 1;
 }
 
 struct Plan {
@@ -33,18 +36,24 @@ struct Plan {
 };
 
 // The list is split over workgroups where the rows alone leave CUs idle: into a power of
-// two of shares (equal ones of most lists), of 256 keys, or of 128 where that leaves CUs
-// idle, up to two workgroups per CU. Single tokens, 8 heads of 128, f16, caches that are
-// not in the L2, us without splits, with this rule, with half and with twice as many: 1 item
-// of 4096 keys 95, 17.6, 22, 18.3; 4 of 2048 46, 19.1, 21.9, 20.7; 8 of 2048 47, 24.6, 24.9,
-// 31; 16 of 2048 52.8, 35.9, 37.4, 40.1; 1 of 512 15.1, 12.1, 13.7, 12.1; 4 of 256 10.9
-// without, 12.6 with two; 40 of 2048 76.3 without, 88.7 with two.
+// two of shares (equal ones of most lists), of 256 keys (f32 128), or down to 128 (f32, and
+// where two or four waves of rows share the keys, 64) where that leaves CUs idle, up to two
+// workgroups per CU (f32 one).
+// Single tokens, 8 heads of 128, f16, caches that are not in the L2, us without splits, with
+// this rule, with half and with twice as many: 1 item of 4096 keys 95, 17.6, 22, 18.3; 4 of
+// 2048 46, 19.1, 21.9, 20.7; 8 of 2048 47, 24.6, 24.9, 31; 16 of 2048 52.8, 35.9, 37.4, 40.1;
+// 1 of 512 15.1, 12.1, 13.7, 12.1; 4 of 256 10.9 without, 12.6 with two; 40 of 2048 76.3
+// without, 88.7 with two. f32: 2 of 2048 118, 26.8, 30; 8 of 1024 65, 34, 44, 44; 1 of 256
+// 23.6, 19.9, 20.3. Blocks of 128 rows, 1 head of 160, 296 keys: 19.7, 15, 17.4 (f32 41.5,
+// 29.8, 33.8).
 //
 // f32 products are split where the keys and values, which that reads and writes once, are
 // then read at least kSplitReuse times by waves full of rows: 4096 keys, 8 heads of 80, read
 // once 36.9 us (31.2 on the f32 instructions), twice 41.2 (47.3), four times 41.3 (59.1),
-// sixteen times 72 (158).
-constexpr int64_t kSplitReuse = 2;
+// sixteen times 72 (158). Where one wave's rows are all, kSplitReuseFew times, as half of the
+// row waves then stand idle: 2 heads of 80 of 2 items, 8 times 33 (30.7), 16 times 38 (59.5)
+// and 52 (55), 32 times 76 (90), 128 times 154 (344).
+constexpr int64_t kSplitReuse = 2, kSplitReuseFew = 16;
 Plan plan(const Context &ctx, const BlockShape &s, WeightType type, bool half) {
     Plan p;
     p.wr = row_waves(s);
@@ -53,14 +62,17 @@ Plan plan(const Context &ctx, const BlockShape &s, WeightType type, bool half) {
     p.items = int64_t(s.n) * s.heads_kv * s.q_blocks() * p.row_tiles;
     const int64_t keys = std::min<int64_t>(int64_t(s.top) * s.kv_block, s.kv_tokens);
     p.splits = 1;
-    if (p.items < ctx.cu_count && keys >= 512) {
-        const int64_t items = std::max<int64_t>(p.items, 1), cus = ctx.cu_count;
-        const int64_t most = std::min<int64_t>(2 * cus / items, std::max<int64_t>(keys / 256, std::min<int64_t>(4, cus / items)));
+    const bool f32 = type == kF32 && !half;
+    const int64_t items = std::max<int64_t>(p.items, 1), cus = ctx.cu_count, least = f32 || p.wr > 1 ? 64 : 128;
+    if (items < cus && keys >= 4 * least) {
+        const int64_t most = std::min<int64_t>((f32 ? 1 : 2) * cus / items,
+                                               std::max<int64_t>(keys / (f32 ? 128 : 256), std::min<int64_t>(4, cus / items)));
         while (2 * p.splits <= most) p.splits *= 2;
     }
-    p.split = type == kF32 && !half && s.kv_tokens > 0 && battn::split_fits(p.wr, head_tiles(s.d, false)) &&
-              battn::split_fits(p.wr, head_tiles(s.d, true)) &&
-              int64_t(s.q_blocks()) * p.row_tiles * keys >= kSplitReuse * s.kv_tokens;
+    p.split = f32 && s.kv_tokens > 0 && battn::split_fits(head_tiles(s.d, false)) &&
+              battn::split_fits(head_tiles(s.d, true)) &&
+              int64_t(s.q_blocks()) * p.row_tiles * keys >= (p.wr == 1 ? kSplitReuseFew : kSplitReuse) * s.kv_tokens;
+    if (p.split) p.wr = std::max(p.wr, 2);
     return p;
 }
 

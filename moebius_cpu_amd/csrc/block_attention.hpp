@@ -166,8 +166,13 @@ __device__ __forceinline__ float other_half(float x) {
 // Key of accumulator register i in lane half h (32 x 32 results: row of the tile).
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
 
+// Waves per SIMD that the registers allow.
+constexpr int occupancy(int mode, int dt, int wr) {
+    return mode == kF32 ? 1 : dt <= 4 || (mode == kHalf && dt == 5 && wr >= 2) ? 2 : 1;
+}
+
 template <typename T, int MODE, bool VEC, int DT, int WR>
-__global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_attention_kernel(Args a) {
+__global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attention_kernel(Args a) {
     using L = Tiling<MODE, DT, WR>;
     typedef std::conditional_t<MODE == kSplit, _Float16, T> S;  // k and v
     constexpr bool SPLIT = MODE == kSplit, HALF = MODE != kF32, KVEC = VEC || SPLIT;
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
 
     // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of chunk c (f32: 8 c + 4 h .. + 3).
     const int row = r0 + wr * 32 + col;
-    const bool row_ok = row < rows;
+    const bool row_ok = row < rows, rows_here = r0 + wr * 32 < rows;  // this lane's, any of the wave's
     const int qi = i0 + (row_ok ? row : 0) / a.g, qe = hk * a.g + (row_ok ? row : 0) % a.g;
     const T *qp = static_cast<const T *>(a.q) + (int64_t(item) * a.q_tokens + qi) * a.ldq + int64_t(qe) * a.d;
     halfx8 qh[HALF ? DT * 2 : 1], ql[SPLIT ? DT * 2 : 1];
@@ -403,7 +408,7 @@ __global__ __launch_bounds__(256, MODE != kF32 && DT <= 4 ? 2 : 1) void block_at
         const bool masked = masked_next;
         __syncthreads();
         if (tile + WK < tiles) fetch(tile + WK);
-        if (!live) continue;
+        if (!live || !rows_here) continue;
 
         floatx16 sc[SUB];
 #pragma unroll
@@ -686,7 +691,7 @@ void launch(Context &ctx, const Args &a) {
 
 template <typename T, int MODE, bool VEC, int DT>
 void launch_rows(Context &ctx, const Args &a, int wr) {
-    if constexpr (MODE != kSplit)
+    if constexpr (MODE != kSplit && DT <= 4)  // (as the plan takes them)
         if (wr == 1) return launch<T, MODE, VEC, DT, 1>(ctx, a);
     if (wr == 2) launch<T, MODE, VEC, DT, 2>(ctx, a);
     else launch<T, MODE, VEC, DT, 4>(ctx, a);
@@ -712,8 +717,8 @@ void launch_mode(Context &ctx, const Args &a, int wr, int dt, bool vec) {
 void launch_f16(Context &ctx, const Args &a, int wr, int dt, bool vec);
 void launch_f32_half(Context &ctx, const Args &a, int wr, int dt, bool vec);
 void launch_f32(Context &ctx, const Args &a, int wr, int dt, bool vec);
-// Row waves and head tiles that launch_split takes.
-inline bool split_fits(int wr, int dt) { return wr >= 2 && dt <= 5; }
+// Head tiles that launch_split takes (with two row waves or more).
+inline bool split_fits(int dt) { return dt <= 5; }
 void launch_split(Context &ctx, const Args &a, int wr, int dt, bool vec);
 // k and v [n][kv_tokens] rows (ldk, ldv elements apart) of hk heads of d f32 -> kp, vp
 // [n][blocks kb][hk][2][dk] f16 parts of every block scaled by its own power of two, zeros

@@ -275,6 +275,11 @@ CASES = [  # n, q, kv, hq, hk, d, qb, kb, top, causal
     (1, 130, 140, 1, 1, 33, 70, 16, 8, True),
     (2, 256, 300, 1, 1, 64, 128, 128, 3, True),
     (1, 140, 170, 1, 1, 134, 70, 16, 11, False),
+    # the same with a wave of rows and one without, and lists of few keys split over workgroups
+    (2, 300, 300, 2, 2, 80, 16, 32, 8, False), (1, 640, 320, 1, 1, 160, 32, 64, 5, True),
+    (1, 200, 96, 2, 2, 128, 8, 16, 6, True), (1, 330, 120, 1, 1, 33, 16, 16, 8, True),
+    (1, 3, 290, 2, 1, 96, 128, 32, 10, True), (2, 1, 310, 4, 4, 160, 1, 16, 20, True),
+    (1, 70, 400, 1, 1, 160, 64, 64, 6, False),
 ]
 
 
