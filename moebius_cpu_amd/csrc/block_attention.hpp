@@ -19,6 +19,16 @@
 // products above 2^-24 of theirs; queries scaled by a power of two per row, keys and values
 // per block (split_kv), probabilities by 2^11, so that the parts keep all bits of values down
 // to 2^-18 (2^-13) of the largest. Scores, maxima, sums and outputs are f32 in all.
+//
+// Bound: the matrix instructions and the vector instructions beside them (7 to 8 for each;
+// from registers alone 7 leave the card 1278 TFLOP/s of f16 on random values); latency where
+// rows are few. Measured: 16384 tokens, 16 heads of 128, f16, 2048 keys per row 346 us (795
+// TFLOP/s); 2 x 4096, 8 heads of 80, f32, 1024 keys 128 us, on the f32 instructions 298; 8
+// single tokens, 32 / 8 heads of 128, 2048 of up to 16384 keys 24.7 us. For the first: values
+// read from LDS transposed by ds_read_b64_tr_b16 instead of gathered 1140 -> 473 us; loads
+// without branches and 32-bit offsets 473 -> 375; the maximum's reference moved only when it
+// is passed by 2^8 355 -> 350; two buffers, tiles of 32 keys with three waves per SIMD and
+// products interleaved with exponentials by scheduling groups changed nothing.
 #pragma once
 
 #include <type_traits>
@@ -61,7 +71,9 @@ struct Args {
 };
 
 constexpr int kSplitExp = 14;  // split operands are scaled to a largest value of 2^14 .. 2^15
-constexpr int kLazyHalf = 8, kLazySplit = 3;  // powers of two by which a row's maximum may pass its reference
+// Powers of two by which a row's maximum may pass its reference: probabilities up to 2^8 fit
+// f16, split ones (scaled by 2^11) up to 2^3.
+constexpr int kLazyHalf = 8, kLazySplit = 3;
 constexpr int kSplitP = 11;    // split probabilities are scaled to at most 2^(11 + 3)
 
 // x 2^e in two f16 parts, x = hi + lo to 2^-24 of it (and 2^-40 of the largest value that e

@@ -13,6 +13,12 @@
 // Scores as ordered 64-bit keys in LDS; a wave finds the top-th largest bit by bit from
 // above, counting the keys at or above a candidate with ballots, and stops once exactly
 // `top` are, which takes the exponent's bits and as many as tell the blocks apart.
+//
+// Measured, means and selection together: 2 x 4096 tokens, 8 heads of 80, f32, 16 of 64
+// blocks 18.9 us (5.6 and 14.6 by themselves); 16384 tokens, 16 / 8 heads of 128, f16, 32 of
+// 256 blocks 40 us (7.8 and 28.7). Eight waves per workgroup against four: 63 -> 45 and
+// 27 -> 18.5 us; products on v_mfma_f64_4x4x4 against 16x16x4, most of whose rows are no
+// queries, 45 -> 40 us; on the vector units 154 us.
 #include <algorithm>
 
 #include "attention.hpp"
