@@ -540,8 +540,10 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
  * sums; scale > 0; rows of k and of v less than 32 MiB apart. Rows that see no key are
  * zero, rows at or above q_len are left as they were; what lies at keys a row does not
  * see (NaN among it) does not reach it.
- * f16 tensors: f16 products. f32 tensors: f32 products, or on FAST contexts products
- * of operands rounded to f16. Lists are split over workgroups where rows are few, and
+ * f16 tensors: f16 products. f32 tensors: f32 products, where keys are read often of
+ * operands in two f16 parts (which hold a value to 2^-24 of itself or 2^-36 of the largest
+ * of its query or of the listed blocks, whichever is more), or on FAST contexts products of
+ * operands rounded to f16. Lists are split over workgroups where rows are few, and
  * the parts joined through scratch (mh_block_attention_scratch bytes, 16-byte
  * aligned); NULL takes the context's workspace, which is refused while the stream is
  * being captured into a graph. out overlaps no input. */
