@@ -51,6 +51,9 @@ CASES = [  # n, h, w, ci, co, rank, slots, per pixel
     (1, 27, 30, 1100, 320, 12, 3, True), (2, 19, 23, 2600, 330, 40, 3, False), (1, 27, 30, 333, 321, 33, 5, True),
     (1, 64, 65, 72, 1100, 20, 4, True), (1, 4100, 1, 33, 1030, 16, 2, True), (1, 20, 20, 40, 600, 256, 2, True),
     (1, 75, 74, 72, 1100, 20, 4, True), (1, 5600, 1, 33, 1030, 16, 2, True),
+    # rows and ranks shorter than a load
+    (1, 1, 3, 1, 5, 1, 2, True), (2, 3, 3, 3, 7, 2, 2, False), (1, 40, 40, 3, 700, 2, 3, True), (1, 90, 80, 5, 97, 3, 4, True),
+    (2, 50, 50, 1, 130, 1, 2, False),
 ]
 
 
