@@ -571,11 +571,11 @@ int32_t mh_conv1x1_lora_scratch(MhContext *ctx, uint64_t rows, uint32_t c_in, ui
  *   out += scale[s] (x . a[s]^T) . b[s]^T.
  * rows_per_slot: h * w where each image of a batch is a request, 1 for single tokens
  * or rows of mixed requests; slot has ceil(rows / rows_per_slot) entries. residual may
- * be out; no other overlap with out. Sums are f32. EXACT: f32 products up to 64 rows;
- * beyond, products of x (and of an f32 weight) in two f16 parts, which hold a value to
- * 2^-24 of itself or 2^-40 of the largest of its row, whichever is more. FAST: beyond 64
- * rows the projection's operands are rounded to f16, scaled by their row's largest; the
- * adapters' products are as in EXACT. scratch as for mh_block_attention
+ * be out; no other overlap with out. Sums are f32. Few rows (by
+ * the tiles of 16 x 16 results they make): f32 products. More: products of x (and of an f32
+ * weight) in two f16 parts, which hold a value to 2^-24 of itself or 2^-40 of the largest of
+ * its row, whichever is more; FAST rounds the projection's operands to f16, scaled by their
+ * row's largest, and keeps the adapters' products as in EXACT. scratch as for mh_block_attention
  * (mh_conv1x1_lora_scratch bytes). At most 2^22 channels. */
 int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t c_in, const void *weight,
                         uint32_t weight_dtype, uint32_t c_out, const float *bias, const float *residual,
