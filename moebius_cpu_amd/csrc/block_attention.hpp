@@ -70,6 +70,7 @@ struct Args {
     const SplitMeta *meta;  // [n][blocks][hk]
 };
 
+constexpr int kNoExp = -1000;  // v_exp of blocks without a finite value other than zero: below all others
 constexpr int kSplitExp = 14;  // split operands are scaled to a largest value of 2^14 .. 2^15
 // Powers of two by which a row's maximum may pass its reference: probabilities up to 2^8 fit
 // f16, split ones (scaled by 2^11) up to 2^3.
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
             // Powers of two that the blocks' parts were scaled by, the values' against the largest.
             __threadfence_block();
             const SplitMeta *meta = a.meta + (int64_t(item) * (a.kv_rows >> a.kb_log)) * a.hk + hk;
-            int top = -1000;
+            int top = kNoExp;
             bool any = false;
             for (int i = lane; i < n; i += 64) {
                 const SplitMeta s = meta[int64_t(list[i] >> a.kb_log) * a.hk];

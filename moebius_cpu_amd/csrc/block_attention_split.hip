@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256) void split_kv_kernel(const float *k, const flo
     }
     if (threadIdx.x == 0) {
         SplitMeta *m = meta + (int64_t(item) * blocks + b) * hk + head;
-        if (is_v) m->v_exp = e, m->v_bad = bad;
+        if (is_v) m->v_exp = mx == 0.0f ? kNoExp : e, m->v_bad = bad;
         else m->k_exp = e;
     }
 }

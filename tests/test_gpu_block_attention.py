@@ -547,3 +547,23 @@ def test_python_refusals(ctx):
         block_select(q, E.DeviceArray(ctx, (1, 2, 1, 8)), 32, blocks, kv_block=64)
     with pytest.raises(MoebiusError, match="means are f32"):
         block_means(k, 16, E.DeviceArray(ctx, (1, 1, 1, 8)))
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-8, 1e-20])
+def test_blocks_of_zero_values_leave_small_ones_their_bits(ctx, size):
+    """f32 values of any size beside listed blocks whose values are zero, or zero and infinite."""
+    r = np.random.default_rng(10)
+    q, k, v = (r.standard_normal((1, t, 1, 64)).astype(np.float32) for t in (192, 192, 192))
+    v *= np.float32(size)
+    v[0, 32:64], v[0, 96:128] = 0, 0
+    for blocks in ([0, 1], [1, 2, 4], [1, 3], [0, 1, 2, 3, 4, 5]):
+        li = np.tile(np.array(blocks + [-1] * (6 - len(blocks)), np.int32), (1, 2, 1, 1))
+        want, tol = reference(q, k, v, li, 0.125, 96, 32, False, None, None)
+        bound = tolerance(want, tol, 64, np.float32, False)
+        got = run(ctx, q, k, v, li, 96, 32, scale=0.125)
+        assert np.all(np.abs(got - want) <= bound), (blocks, (np.abs(got - want) / bound).max())
+        inf = v.copy()
+        inf[0, 40, 0, 7] = np.inf  # of block 1, which every list holds
+        got = run(ctx, q, k, inf, li, 96, 32, scale=0.125)
+        assert np.isposinf(got[..., 7]).all()
+        assert np.all(np.delete(np.abs(got - want) <= bound, 7, axis=3)), blocks
