@@ -541,9 +541,10 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
  * zero, rows at or above q_len are left as they were; what lies at keys a row does not
  * see (NaN among it) does not reach it.
  * f16 tensors: f16 products. f32 tensors: f32 products, where keys are read often of
- * operands in two f16 parts (which hold a value to 2^-24 of itself or 2^-36 of the largest
- * of its query or of the listed blocks, whichever is more), or on FAST contexts products of
- * operands rounded to f16. Lists are split over workgroups where rows are few, and
+ * operands in two f16 parts (which hold a value to 2^-24 of itself, of a query or key to
+ * 2^-33 of the largest of that head of its token, in the second product to 2^-36 of the
+ * largest that the row sees, whichever is more), or on FAST contexts products of operands
+ * rounded to f16. Lists are split over workgroups where rows are few, and
  * the parts joined through scratch (mh_block_attention_scratch bytes, 16-byte
  * aligned); NULL takes the context's workspace, which is refused while the stream is
  * being captured into a graph. out overlaps no input. */

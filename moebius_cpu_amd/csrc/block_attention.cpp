@@ -90,7 +90,7 @@ Layout layout(const BlockShape &s, const Plan &p) {
     if (p.split) {
         const size_t rows = size_t(s.n) * s.kv_blocks() * s.kv_block * s.heads_kv;
         l.parts = up(rows * 2 * size_t(ceil_div(s.d, 8) * 8) * 2);
-        l.meta = up(size_t(s.n) * s.kv_blocks() * s.heads_kv * sizeof(battn::SplitMeta));
+        l.meta = up(rows * sizeof(battn::KeyScale));
     }
     return l;
 }
@@ -131,9 +131,9 @@ void block_attention(Context &ctx, const BlockAttention &b, WeightType type, voi
         a.kv_rows = s.kv_blocks() * s.kv_block;
         a.v0 = b.v.p, a.ldv0 = a.ldv;
         char *kp = mem + l.part, *vp = kp + l.parts;
-        auto *meta = reinterpret_cast<battn::SplitMeta *>(vp + l.parts);
+        auto *meta = reinterpret_cast<battn::KeyScale *>(vp + l.parts);
         battn::split_kv(ctx, static_cast<const float *>(b.k.p), static_cast<const float *>(b.v.p), b.k.ld, b.v.ld, s.n,
-                        s.kv_tokens, s.heads_kv, s.d, a.dk, s.kv_block, s.kv_len, kp, vp, meta);
+                        s.kv_tokens, a.kv_rows, s.heads_kv, s.d, a.dk, s.kv_len, kp, vp, meta);
         a.k = kp, a.v = vp, a.meta = meta;
         const uint64_t row = uint64_t(s.heads_kv) * 2 * a.dk * 2;
         MH_REQUIRE(row < (uint64_t(1) << 25), "block_attention: rows of keys or values of 32 MiB or more");

@@ -17,8 +17,10 @@
 // a sum over keys averages. kF32: f32 products (v_mfma_f32_32x32x2_f32, an eighth of the
 // rate). kSplit: each f32 operand as two f16 parts, x = hi + lo to 2^-24, and the three
 // products above 2^-24 of theirs; queries scaled by a power of two per row, keys and values
-// per block (split_kv), probabilities by 2^11, so that the parts keep all bits of values down
-// to 2^-18 (2^-13) of the largest. Scores, maxima, sums and outputs are f32 in all.
+// per sixteen tokens, or per token where those are far apart (KeyScale), probabilities by 2^11
+// and their key's power against the largest that the row has seen, so that the parts keep all
+// bits of queries down to 2^-18, of keys to 2^-12 and of p v to 2^-13 of the largest, and no
+// token that a row does not see takes bits from it. Scores, maxima, sums and outputs are f32 in all.
 //
 // Bound: the matrix instructions and the vector instructions beside them (7 to 8 for each;
 // from registers alone 7 leave the card 1278 TFLOP/s of f16 on random values); latency where
@@ -40,6 +42,7 @@ namespace battn {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 
@@ -47,10 +50,13 @@ typedef _Float16 halfx4 __attribute__((ext_vector_type(4)));
 // products of operands split in two f16 parts.
 enum Mode { kHalf, kF32, kSplit };
 
-// A block's scales where its keys and values are split: largest exponents, and whether
-// values that are not finite were left out.
-struct SplitMeta {
-    int k_exp, v_exp, v_bad, pad;
+// The exponents by which the key and the values of a token are scaled where they are split,
+// the values' twice and 1 more where some that are not finite were left out. Sixteen tokens
+// share theirs, the largest, where all are within 2^kSplitSpread of it; else each has its
+// own, which leaves the others their bits whatever lies at tokens that a row does not see.
+constexpr int kSplitSpread = 6;
+struct KeyScale {
+    int k, v;
 };
 
 struct Args {
@@ -67,15 +73,16 @@ struct Args {
     int kv_rows;  // rows per item of k and v
     const void *v0;        // kSplit: the values themselves, rows ldv0 bytes apart, heads of d
     uint32_t ldv0;
-    const SplitMeta *meta;  // [n][blocks][hk]
+    const KeyScale *meta;  // [n][hk][kv_rows]
 };
 
-constexpr int kNoExp = -1000;  // v_exp of blocks without a finite value other than zero: below all others
+constexpr int kNoExp = -1000;  // exponent of values that are all zero or not finite: below all others
 constexpr int kSplitExp = 14;  // split operands are scaled to a largest value of 2^14 .. 2^15
 // Powers of two by which a row's maximum may pass its reference: probabilities up to 2^8 fit
 // f16, split ones (scaled by 2^11) up to 2^3.
 constexpr int kLazyHalf = 8, kLazySplit = 3;
-constexpr int kSplitP = 11;    // split probabilities are scaled to at most 2^(11 + 3)
+constexpr int kSplitP = 11;    // split probabilities are scaled to at most 2^(11 + 3 + kLazyV)
+constexpr int kLazyV = 1;      // powers of two by which a key's values may pass their reference
 
 // x 2^e in two f16 parts, x = hi + lo to 2^-24 of it (and 2^-40 of the largest value that e
 // was taken from); a value that is not finite is all in hi.
@@ -100,7 +107,7 @@ struct Tiling {
     static constexpr int kKS = kCols + (MODE == kF32 ? 4 : 8);
     static constexpr int kVS = MODE == kF32 ? kDP + 8 : kCols + (kCols % 64 ? 0 : 32);
     static constexpr int kKBytes = kKT * kKS * kES, kVBytes = kKT * kVS * kES;
-    static constexpr int kStage = kKBytes + kVBytes;      // one key group's tile
+    static constexpr int kStage = kKBytes + kVBytes + (MODE == kSplit ? 8 * kKT : 0);  // one key group's tile, its scales
     // key groups: four waves together, fewer where their tiles exceed the LDS of a CU (160 KiB)
     static constexpr int kWK = 4 / WR * kStage <= 144 * 1024 ? 4 / WR : 2 / WR;
     static_assert(kWK >= 1 && kWK * kStage <= 144 * 1024, "tiles exceed the LDS");
@@ -179,8 +186,10 @@ __device__ __forceinline__ float other_half(float x) {
 // Key of accumulator register i in lane half h (32 x 32 results: row of the tile).
 __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + (i % 4); }
 
-// Waves per SIMD that the registers allow.
+// Waves per SIMD that the registers allow (kSplit with four tiles and two row waves does without
+// the second: 49 registers spilled, 245 us against 213 with 8 heads of 128, 2 x 4096 rows).
 constexpr int occupancy(int mode, int dt, int wr) {
+    if (mode == kSplit && dt == 4 && wr == 2) return 1;
     return mode == kF32 ? 1 : dt <= 4 || (mode == kHalf && dt == 5 && wr >= 2) ? 2 : 1;
 }
 
@@ -195,8 +204,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
     constexpr int KU = (KT * RUNS + NT - 1) / NT;    // runs of 8 channels of K, and of V, per thread
     extern __shared__ __align__(16) char smem[];
     __shared__ int32_t list[kMaxTop];  // first token of every block to visit
-    __shared__ float k_scale[SPLIT ? kMaxTop : 1], v_scale[SPLIT ? kMaxTop : 1];
-    __shared__ int list_n, bad, v_exp;
+    __shared__ int list_n, bad;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wk = wave / WR, ttid = tid % NT;
@@ -246,24 +254,6 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
             n += __popcll(all);
         }
         if (lane == 0) list_n = n, bad = 0;
-        if constexpr (SPLIT) {
-            // Powers of two that the blocks' parts were scaled by, the values' against the largest.
-            __threadfence_block();
-            const SplitMeta *meta = a.meta + (int64_t(item) * (a.kv_rows >> a.kb_log)) * a.hk + hk;
-            int top = kNoExp;
-            bool any = false;
-            for (int i = lane; i < n; i += 64) {
-                const SplitMeta s = meta[int64_t(list[i] >> a.kb_log) * a.hk];
-                top = max(top, s.v_exp);
-                any = any || s.v_bad;
-                k_scale[i] = ldexpf(1.0f, s.k_exp - kSplitExp);
-            }
-            for (int x = 32; x; x >>= 1) top = max(top, __shfl_xor(top, x));
-            for (int i = lane; i < n; i += 64)
-                v_scale[i] = ldexpf(1.0f, meta[int64_t(list[i] >> a.kb_log) * a.hk].v_exp - top + kSplitP);
-            any = __any(any);
-            if (lane == 0) v_exp = top, bad = any;
-        }
     }
 
     // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of chunk c (f32: 8 c + 4 h .. + 3).
@@ -273,7 +263,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
     const T *qp = static_cast<const T *>(a.q) + (int64_t(item) * a.q_tokens + qi) * a.ldq + int64_t(qe) * a.d;
     halfx8 qh[HALF ? DT * 2 : 1], ql[SPLIT ? DT * 2 : 1];
     float qf[HALF ? 1 : DT * 16];
-    float cq = a.c;  // what turns a product into a score
+    int eq = 0;  // SPLIT: the power of two that the row's products lack, but for the key's
     if constexpr (SPLIT) {
         Run8<T> r[DT * 2];
         float mx = 0.0f;
@@ -290,7 +280,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
         }
         mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
         const int e = mx == 0.0f ? 0 : __builtin_amdgcn_frexp_expf(mx) - 1;
-        cq = ldexpf(a.c, e - kSplitExp);
+        eq = e - 2 * kSplitExp;
 #pragma unroll
         for (int c = 0; c < DT * 2; ++c)
 #pragma unroll
@@ -356,6 +346,9 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
     // its keys. Runs behind d are loaded from the last channels and not staged.
     Run8<S> kr[KU], vr[KU];
     int tok[KU];
+    KeyScale ks{};  // of key ttid % KT
+    const KeyScale *meta = SPLIT ? a.meta + (int64_t(item) * a.hk + hk) * a.kv_rows : nullptr;
+    int *const kx = reinterpret_cast<int *>(vst + L::kVBytes), *const vx = kx + KT;
     bool masked_next = false;
     constexpr bool kWhole = KT * RUNS % NT == 0;
     auto fetch = [&](int tile) {
@@ -365,6 +358,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
             tok[u] = kWhole || j < KT ? token(tile * KT + j) : 0x7fffffff;
         }
         masked_next = !__all(token(tile * KT + lane % KT) < lim_all);
+        if constexpr (SPLIT) ks = meta[min(token(tile * KT + ttid % KT), kv_len - 1)];
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
             const int run = (ttid + u * NT) % RUNS, ch = run % (DP / 8) * 8;
@@ -385,6 +379,11 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
         }
     };
     auto stage = [&]() {
+        if constexpr (SPLIT)
+            if (ttid < KT) {
+                kx[ttid] = ks.k, vx[ttid] = ks.v >> 1;
+                if (ks.v & 1) bad = 1;
+            }
 #pragma unroll
         for (int u = 0; u < KU; ++u) {
             const int i = ttid + u * NT, j = i / RUNS, run = i % RUNS, ch = run % (DP / 8) * 8;
@@ -410,6 +409,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
     float m = kNegInf, l = 0.0f;
+    int top = kNoExp;  // SPLIT: the exponent that the row's o is scaled by
 
     const int steps = (tiles + WK - 1) / WK;
     if (wk < tiles) fetch(wk);
@@ -419,6 +419,16 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
         if (s) __syncthreads();  // the tile before has been read
         if (live) stage();
         const bool masked = masked_next;
+        // SPLIT: the exponents of each sixteen keys and values, unless each has its own or they
+        // count by what a row sees.
+        int ke[2] = {}, ve[2] = {};
+        bool each = false;
+        if constexpr (SPLIT) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                ke[x] = __builtin_amdgcn_readlane(ks.k, 16 * x), ve[x] = __builtin_amdgcn_readlane(ks.v, 16 * x) >> 1;
+            each = masked || !__all(ks.k == (col < 16 ? ke[0] : ke[1]) && ks.v >> 1 == (col < 16 ? ve[0] : ve[1]));
+        }
         __syncthreads();
         if (tile + WK < tiles) fetch(tile + WK);
         if (!live || !rows_here) continue;
@@ -454,18 +464,15 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                         sc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[j], qf[c * 4 + j], sc[b], 0, 0, 0);
                 }
         }
-        float vs[SPLIT ? 2 * SUB : 1];  // scales of the values of each sixteen keys, times the probabilities' own
-        if constexpr (SPLIT) {
+        const float c = a.c;
+        if (SPLIT && each) {
 #pragma unroll
-            for (int x = 0; x < 2 * SUB; ++x) {
-                const int e = l0 + (min(tile * KT + x * 16, keys - 1) >> a.kb_log);
-                const float f = cq * k_scale[e];
-                vs[x] = v_scale[e];
+            for (int f = 0; f < 4; ++f) {
+                const intx4 e = reinterpret_cast<const intx4 *>(kx)[2 * f + h];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sc[x / 2][x % 2 * 8 + i] *= f;
+                for (int i = 0; i < 4; ++i) sc[0][4 * f + i] = ldexpf(sc[0][4 * f + i], e[i] + eq);
             }
         }
-        const float c = SPLIT ? 1.0f : a.c;
         if (masked) {
 #pragma unroll
             for (int b = 0; b < SUB; ++b)
@@ -477,6 +484,20 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                         if (t0 >= lim || t0 + e >= lim) sc[b][4 * f + e] = kNegInf;
                 }
         }
+        int tv = max(ve[0], ve[1]);  // the largest exponent of the values that the row sees
+        if (SPLIT && each) {
+            tv = kNoExp;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const intx4 e = reinterpret_cast<const intx4 *>(vx)[2 * f + h];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tv = max(tv, sc[0][4 * f + i] == kNegInf ? kNoExp : e[i]);
+            }
+            tv = max(tv, __builtin_bit_cast(int, other_half(__builtin_bit_cast(float, tv))));
+        } else if (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[0][i] = ldexpf(sc[0][i], ke[i / 8] + eq);
+        }
         float mx = sc[0][0];
 #pragma unroll
         for (int b = 0; b < SUB; ++b)
@@ -484,21 +505,23 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
             for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, sc[b][i]);
         mx = __builtin_fmaxf(mx, other_half(mx)) * c;
         // The reference m follows the maximum only when that has grown by 2^kLazy: probabilities
-        // stay below 2^kLazy and most tiles leave the sums as they are.
-        if (__any(mx > m + float(kLazy))) {
+        // stay below 2^kLazy and most tiles leave the sums as they are. top follows tv alike.
+        if (__any(mx > m + float(kLazy) || (SPLIT && tv > top + kLazyV))) {
             const float mn = __builtin_fmaxf(m, mx);
             const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));  // 0 before the first key
+            const int tn = max(top, tv);
+            const float fo = SPLIT ? ldexpf(f, top - tn) : f;
             l *= f;
 #pragma unroll
             for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] *= f;
-            m = mn;
+                for (int i = 0; i < 16; ++i) o[t][i] *= fo;
+            m = mn, top = tn;
         }
         const float mu = m == kNegInf ? 0.0f : m;
         // The fused exponent is off by half a step of m, which is nothing until scores are so large
         // that the largest key's power would leave the range: their products are rounded first.
-        const bool far = !SPLIT && __any(__builtin_fabsf(mu) > 1048576.0f);
+        const bool far = __any(__builtin_fabsf(mu) > 1048576.0f);
         if (far)
 #pragma unroll
             for (int b = 0; b < SUB; ++b)
@@ -514,6 +537,17 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                 sum += sc[b][i];
             }
         l += sum;
+        if (SPLIT && each) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const intx4 e = reinterpret_cast<const intx4 *>(vx)[2 * f + h];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[0][4 * f + i] = ldexpf(sc[0][4 * f + i], e[i] - top + kSplitP);
+            }
+        } else if (SPLIT) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[0][i] = ldexpf(sc[0][i], ve[i / 8] - top + kSplitP);
+        }
         if constexpr (HALF) {
 #pragma unroll
             for (int b = 0; b < SUB; ++b)
@@ -522,13 +556,9 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                     halfx8 p, pl;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        if constexpr (SPLIT) {
-                            const float y = sc[b][x * 8 + i] * vs[b * 2 + x];
-                            p[i] = static_cast<_Float16>(y);
-                            pl[i] = static_cast<_Float16>(y - float(p[i]));
-                        } else {
-                            p[i] = static_cast<_Float16>(sc[b][x * 8 + i]);
-                        }
+                        const float y = sc[b][x * 8 + i];
+                        p[i] = static_cast<_Float16>(y);
+                        if constexpr (SPLIT) pl[i] = static_cast<_Float16>(y - float(p[i]));
                     }
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
@@ -555,6 +585,13 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
         }
     }
     l += __shfl_xor(l, 32);
+
+    if constexpr (SPLIT) {  // the scales taken back
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = ldexpf(o[t][i], top - kSplitExp - kSplitP);
+    }
 
     // Groups of waves join: group 0 takes the others' sums one after another.
     if constexpr (WK > 1) {
@@ -584,12 +621,6 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
             }
         }
         if (wk) return;
-    }
-    if constexpr (SPLIT) {  // the scales taken back
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] = ldexpf(o[t][i], v_exp - kSplitExp - kSplitP);
     }
     // The values that were staged as zeros because they are not finite, for the rows that see them.
     if (bad) {
@@ -734,10 +765,10 @@ void launch_f32(Context &ctx, const Args &a, int wr, int dt, bool vec);
 inline bool split_fits(int dt) { return dt <= 5; }
 void launch_split(Context &ctx, const Args &a, int wr, int dt, bool vec);
 // k and v [n][kv_tokens] rows (ldk, ldv elements apart) of hk heads of d f32 -> kp, vp
-// [n][blocks kb][hk][2][dk] f16 parts of every block scaled by its own power of two, zeros
-// behind kv_len and d; meta [n][blocks][hk].
-void split_kv(Context &ctx, const float *k, const float *v, int64_t ldk, int64_t ldv, int n, int kv_tokens, int hk,
-              int d, int dk, int kb, const int32_t *kv_len, void *kp, void *vp, SplitMeta *meta);
+// [n][kv_rows][hk][2][dk] f16 parts of every token below kv_len, scaled by its own power of
+// two, zeros behind d; meta [n][hk][kv_rows].
+void split_kv(Context &ctx, const float *k, const float *v, int64_t ldk, int64_t ldv, int n, int kv_tokens, int kv_rows,
+              int hk, int d, int dk, const int32_t *kv_len, void *kp, void *vp, KeyScale *meta);
 
 }  // namespace battn
 }  // namespace mh

@@ -567,3 +567,42 @@ def test_blocks_of_zero_values_leave_small_ones_their_bits(ctx, size):
         got = run(ctx, q, k, inf, li, 96, 32, scale=0.125)
         assert np.isposinf(got[..., 7]).all()
         assert np.all(np.delete(np.abs(got - want) <= bound, 7, axis=3)), blocks
+
+
+@pytest.mark.parametrize("big", [1e8, 1e12, 1e30])
+@pytest.mark.parametrize("d", [48, 33])
+@pytest.mark.parametrize("q_block", [1, 16, 64, 128])
+def test_large_values_of_unseen_keys_do_not_reach_a_row(ctx, q_block, d, big):
+    """Causal f32 rows whose listed blocks hold keys and values of later tokens that are far larger than theirs."""
+    r = np.random.default_rng(11)
+    q, k, v = (r.standard_normal((1, 128, 2, d)).astype(np.float32) for _ in range(3))
+    blocks = np.tile(np.arange(4, dtype=np.int32), (1, -(-128 // q_block), 2, 1))
+    clean, tol = reference(q, k, v, blocks, d ** -0.5, q_block, 32, True, None, None)
+    v[0, 40, 0, 5], v[0, 71:75, 1], v[0, 100] = big, -big, big
+    k[0, 90, 0], k[0, 101, 1, 3] = big, -big
+    got = run(ctx, q, k, v, blocks, q_block, 32, True).astype(np.float64)
+    ok = np.abs(got - clean) <= tolerance(clean, tol, d, np.float32, False)
+    assert ok[0, :40].all() and ok[0, :71, 1].all()
+    # rows that see the large values: within the largest's roundings
+    want, tol = reference(q, k, v, blocks, d ** -0.5, q_block, 32, True, None, None)
+    ok = np.abs(got - want) <= tolerance(want, tol, d, np.float32, False)
+    assert ok[0, :90].all() and ok[0, :101, 1].all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [8, 64, 80, 160])
+@pytest.mark.parametrize("q_block", [1, 64])
+def test_tokens_of_sizes_far_apart(ctx, q_block, d, causal):
+    """f32 keys and values that differ from token to token by more than the sixteen around them share, some
+    of them zero; values grow along the cache, so causal rows see only what is small beside the rest."""
+    r = np.random.default_rng(17)
+    q, k, v = (r.standard_normal((2, t, 2, d)).astype(np.float32) for t in (160, 200, 200))
+    k *= (10.0 ** r.uniform(-9, 0, (2, 200, 2, 1))).astype(np.float32)
+    v *= (10.0 ** (np.arange(200) / 8 - 12)).astype(np.float32)[None, :, None, None]
+    k[:, 5:90:11], v[:, 3:150:13] = 0, 0
+    blocks = lists(r, 2, -(-160 // q_block), 2, 10, 13)
+    got = run(ctx, q, k, v, blocks, q_block, 16, causal, [160, 130], [200, 187])
+    want, tol = reference(q, k, v, blocks, d ** -0.5, q_block, 16, causal, [160, 130], [200, 187])
+    there = ~np.isnan(want)
+    bound = tolerance(want, tol, d, np.float32, False)
+    assert np.all((np.abs(got - want) <= bound)[there]), (np.abs(got - want) / bound)[there].max()
