@@ -606,3 +606,30 @@ def test_tokens_of_sizes_far_apart(ctx, q_block, d, causal):
     there = ~np.isnan(want)
     bound = tolerance(want, tol, d, np.float32, False)
     assert np.all((np.abs(got - want) <= bound)[there]), (np.abs(got - want) / bound)[there].max()
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32", "fast"])
+@pytest.mark.parametrize("q_block", [1, 64, 128])
+def test_keys_of_infinite_score(ctx, q_block, kind):
+    """A key whose score is -inf has no weight, one of +inf or NaN makes its rows NaN."""
+    dtype = np.float16 if kind == "f16" else np.float32
+    r = np.random.default_rng(13)
+    q, k, v = (r.standard_normal((1, 128, 2, 40)).astype(dtype) for _ in range(3))
+    q[..., 2:5] = np.abs(q[..., 2:5]) + 0.5
+    q[0, ::3, :, 2:5] = 1  # exact in f16: low parts of zero
+    blocks = np.tile(np.arange(4, dtype=np.int32), (1, -(-128 // q_block), 2, 1))
+    k[0, 3, 0, 2] = k[0, 70, 0, 3] = k[0, 100:110, 0, 4] = -np.inf
+    k[0, 33, 1, 2], k[0, 33, 1, 3] = -np.inf, -np.inf
+    ctx.set_precision(kind == "fast")
+    try:
+        got = run(ctx, q, k, v, blocks, q_block, 32).astype(np.float64)
+        k2 = k.copy()
+        k2[0, 50, 0, 2], k2[0, 60, 1, 2], k2[0, 61, 1, 3] = np.inf, np.nan, -np.inf
+        bad = run(ctx, q, k2, v, blocks, q_block, 32)
+    finally:
+        ctx.set_precision(False)
+    k[~np.isfinite(k)] = -1e4  # as far below all others as makes no difference
+    want, tol = reference(q, k, v, blocks, 40 ** -0.5, q_block, 32, False, None, None)
+    tol[..., 1:3] = 20  # (the seen keys' own scores: |q| |k| scale stays below)
+    assert np.all(np.abs(got - want) <= tolerance(want, tol, 40, dtype, kind == "fast"))
+    assert np.isnan(bad).all() or kind == "fast" and np.isnan(bad[..., 1, :]).all()
