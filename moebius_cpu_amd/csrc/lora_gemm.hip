@@ -6,6 +6,11 @@
 // and split alike (lo . lo is below 2^-24 of its product). Sums are f32. An eighth of the
 // f32 instructions' time and a third of six bf16 products'.
 //
+// An infinite value is all in its first part. Its products with the second parts of others are
+// NaN (of zeros) or of either sign, those with first parts what the whole products are: sums
+// that are NaN are formed again from first parts alone. 4096 rows, 1280 x 1280, NaN in every row
+// 154 us against 64, infinities in every row and an f32 weight 230 against 86.
+//
 // FAST contexts take one part (operands rounded to f16 after their row's scale).
 //
 // A workgroup forms BM columns x BN rows, four waves the 2 x 2 quarters, as W . X^T: a lane
@@ -94,6 +99,21 @@ __device__ __forceinline__ floatx16 mfma16(halfx8 a, halfx8 b, floatx16 c) {
 
 typedef floatx4 accx4;
 
+// The sums of a 32 x 32 result that are NaN, from `again` where the row counts (want).
+template <typename F>
+__device__ __forceinline__ void redo_nan(floatx16 &acc, bool want, F again) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) any = any || acc[i] != acc[i];
+    if (!__any(any && want)) return;
+    floatx16 sum;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
+    again(sum);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = acc[i] == acc[i] ? acc[i] : sum[i];
+}
+
 // split_rows and the adapters' first product of 16 rows in one pass over x, for adapters
 // stored in f16: t = 2^-e (hi A^T + lo A^T) on v_mfma_f32_16x16x32_f16. Eight waves share
 // the long axis, 32 values of 16 rows per step (lane: row l % 16, values 8 (l / 16) ..),
@@ -174,9 +194,9 @@ __global__ __launch_bounds__(64 * kPassWaves) void split_shrink_kernel(LoraArgs 
         todo &= ~uint32_t(__ballot(own));
         if (s >= 0) fetch(s, 0, 0);
         for (int q0 = 0; q0 < p.rank; q0 += 16 * kTiles) {
-            accx4 acc[kTiles];
+            accx4 acc[kTiles], low[kTiles];
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) acc[j] = accx4{0, 0, 0, 0};
+            for (int j = 0; j < kTiles; ++j) acc[j] = low[j] = accx4{0, 0, 0, 0};
             for (int pass = 0; pass < passes; ++pass) {
                 if (passes > 1) {
                     load(pass);
@@ -196,7 +216,7 @@ __global__ __launch_bounds__(64 * kPassWaves) void split_shrink_kernel(LoraArgs 
                 for (int u = 0; u < kUnits; ++u)
 #pragma unroll
                     for (int j = 0; j < kTiles; ++j) {
-                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][u], lo[u], acc[j], 0, 0, 0);
+                        low[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][u], lo[u], low[j], 0, 0, 0);
                         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[j][u], hi[u], acc[j], 0, 0, 0);
                     }
                 if (pass + 1 < passes) fetch(s, q0, pass + 1);
@@ -208,7 +228,10 @@ __global__ __launch_bounds__(64 * kPassWaves) void split_shrink_kernel(LoraArgs 
 #pragma unroll
             for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) part[wave][j][i][lane] = acc[j][i];
+                for (int i = 0; i < 4; ++i) {
+                    const float both = acc[j][i] + low[j][i];
+                    part[wave][j][i][lane] = both == both ? both : acc[j][i];
+                }
             __syncthreads();
             // wave j joins rank tile j; register i is rank 4 (l / 16) + i of row l % 16
             if (wave < kTiles && own && q0 + wave * 16 < p.rank) {
@@ -362,6 +385,27 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS || BM > 128 ? 2 : 3)
 #pragma unroll
     for (int n = 0; n < SN; ++n) {
         const int64_t row = r0 + (wn * SN + n) * 32 + l32, row_in = min(row, p.rows - 1);
+        if constexpr (P == 2)
+#pragma unroll
+            for (int m = 0; m < SM; ++m)
+                redo_nan(acc[m][n], row < p.rows, [&](floatx16 &sum) {
+                    constexpr int U = 2;
+                    const int c = min((wm * SM + m) * 32 + l32, p.co - 1 - c0);
+                    const _Float16 *x = g.xp + row_in * P * g.cip + h * 8;
+                    const _Float16 *w = reinterpret_cast<const _Float16 *>(wb) + int64_t(c) * (WPARTS ? P * g.cip : p.ci);
+#pragma nounroll
+                    for (int k = 0; k < p.ci; k += 16 * U) {
+                        halfx8 a[U], b[U];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            b[u] = *reinterpret_cast<const halfx8 *>(x + k + 16 * u);
+                            if constexpr (WPARTS) a[u] = *reinterpret_cast<const halfx8 *>(w + k + 16 * u + h * 8);
+                            else a[u] = load8<VW>(w, k + 16 * u + h * 8, p.ci);
+                        }
+#pragma unroll
+                        for (int u = 0; u < U; ++u) sum = mfma16(a[u], b[u], sum);
+                    }
+                });
 #pragma unroll
         for (int m = 0; m < SM; ++m)
 #pragma unroll
@@ -431,6 +475,24 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : WPARTS || BM > 128 ? 2 : 3)
                             }
                     }
                 }
+                if constexpr (sizeof(T) == 2)
+#pragma unroll
+                    for (int m = 0; m < SM; ++m)
+                        redo_nan(low[m], own, [&](floatx16 &sum) {
+#pragma nounroll
+                            for (int k = 0; k < p.rank; k += 16) {
+                                float tv[8];
+                                read_t(t, k + h * 8, p.rank, own, tv);
+                                halfx8 th;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    _Float16 hi, lo;
+                                    split2(tv[i], kSplitExp - te, hi, lo);
+                                    th[i] = hi;
+                                }
+                                sum = mfma16(load8<false>(b[m], k + h * 8, p.rank), th, sum);
+                            }
+                        });
                 const float scale = p.scale[s];
 #pragma unroll
                 for (int m = 0; m < SM; ++m)

@@ -243,3 +243,43 @@ def test_residual_in_place(ctx, case):
     conv.forward_adapted(x, ad, slot, out, res)
     conv.forward_adapted(x, ad, slot, res, res)
     assert np.array_equal(res.numpy(), out.numpy())
+
+
+@pytest.mark.parametrize("fast", [False, True])
+@pytest.mark.parametrize("wf16", [False, True])
+@pytest.mark.parametrize("af16", [False, True])
+@pytest.mark.parametrize("case", [(1, 1, 20, 96, 80, 8, 3, True), (1, 1, 700, 1100, 320, 40, 3, True), (1, 1, 2100, 96, 1280, 8, 3, True),
+                                  (1, 1, 5600, 70, 1030, 20, 3, True), (1, 1, 300, 1300, 650, 256, 2, True)])
+def test_infinite_values(ctx, case, wf16, af16, fast):
+    """Infinities in x, weight and adapters give the formula's infinities, and NaN where it has NaN, however many rows."""
+    rows, ci, co, rank, slots = case[2:7]
+    d = make(ctx, case, False)
+    for name, half in (("w", wf16), ("a", af16), ("b", af16)):
+        d[name] = d[name].astype(np.float16 if half else np.float32)
+        d[name][np.abs(d[name].astype(np.float32)) < 2.0 ** -12] = 2.0 ** -12  # no product of infinity and zero
+        d[name].reshape(-1)[::5] = np.sign(d[name].reshape(-1)[::5]) * 0.5  # low parts of zero
+    d["x"] += np.where(d["x"] < 0, -2.0 ** -6, 2.0 ** -6).astype(np.float32)
+    d["x"][0, 0, ::4] = np.sign(d["x"][0, 0, ::4])
+    d["slot"][:] = np.arange(rows) % (slots + 1) - 1
+    x = d["x"][0, 0]
+    x[2, 7], x[9, 3], x[10, 3], x[10, 4], x[18, 5] = np.inf, -np.inf, np.inf, -np.inf, np.nan
+    x[rows - 1, ci - 1] = np.inf
+    d["w"][5, 1], d["w"][co - 1, ci - 1], d["w"][33, 2] = np.inf, -np.inf, np.nan
+    d["a"][1, 3, 6], d["b"][1, 41, 2], d["b"][0, 2, rank - 1] = -np.inf, np.inf, np.inf
+    conv = E.Conv1x1(ctx, ci, co, E.Param(ctx, d["w"], f16=wf16), d["bias"])
+    ad = Adapters(ctx, E.Param(ctx, d["a"], f16=af16), E.Param(ctx, d["b"], f16=af16), d["scale"], ci, co, rank)
+    out = E.Tensor(ctx)
+    ctx.set_precision(fast)
+    try:
+        conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, E.DeviceArray.from_numpy(ctx, d["slot"]), out)
+    finally:
+        ctx.set_precision(False)
+    got = out.numpy()[0, 0]
+    with np.errstate(invalid="ignore"):
+        y, base, low = reference(x, d["w"], d["bias"], None, d["a"], d["b"], d["scale"], d["slot"], 1)
+    assert 0 < np.isinf(y).sum() and 0 < np.isnan(y).sum() and 0.5 * y.size < np.isfinite(y).sum()
+    assert np.array_equal(np.isnan(got), np.isnan(y))
+    assert np.array_equal(np.isposinf(got), np.isposinf(y)) and np.array_equal(np.isneginf(got), np.isneginf(y))
+    there = np.isfinite(y)
+    bound = (2.0 ** -10 if fast else 1e-5) * base + (ci + rank + 8) * U * low + U * np.abs(y)
+    assert np.all(np.abs(got - y)[there] <= bound[there])
