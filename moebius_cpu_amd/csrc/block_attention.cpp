@@ -129,7 +129,7 @@ void block_attention(Context &ctx, const BlockAttention &b, WeightType type, voi
     if (p.split) {
         a.dk = int(ceil_div(s.d, 8) * 8);
         a.kv_rows = s.kv_blocks() * s.kv_block;
-        a.k0 = b.k.p, a.ldk0 = a.ldk, a.v0 = b.v.p, a.ldv0 = a.ldv;
+        a.v0 = b.v.p, a.ldv0 = a.ldv;
         char *kp = mem + l.part, *vp = kp + l.parts;
         auto *meta = reinterpret_cast<battn::KeyScale *>(vp + l.parts);
         battn::split_kv(ctx, static_cast<const float *>(b.k.p), static_cast<const float *>(b.v.p), b.k.ld, b.v.ld, s.n,

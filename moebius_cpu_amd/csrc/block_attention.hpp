@@ -71,8 +71,8 @@ struct Args {
     bool causal;
     int dk;       // values of a staged row's part: d, or d rounded up to 8 (kSplit)
     int kv_rows;  // rows per item of k and v
-    const void *k0, *v0;   // kSplit: the keys and values themselves, rows ldk0, ldv0 bytes apart, heads of d
-    uint32_t ldk0, ldv0;
+    const void *v0;        // kSplit: the values themselves, rows ldv0 bytes apart, heads of d
+    uint32_t ldv0;
     const KeyScale *meta;  // [n][hk][kv_rows]
 };
 
@@ -94,11 +94,6 @@ __device__ __forceinline__ void split2(float x, int e, _Float16 &hi, _Float16 &l
 }
 
 constexpr float kNegInf = -__builtin_huge_valf();
-
-// x as a sum with infinite or NaN products takes it: its sign where it is finite.
-__device__ __forceinline__ float sign_or_not_finite(float x) {
-    return x == 0.0f || !(__builtin_fabsf(x) < __builtin_huge_valf()) ? x : __builtin_copysignf(1.0f, x);
-}
 
 // Floats of one wave's partial: the sums of DT x 16 registers and the row's maximum and sum.
 constexpr int part_floats(int dt) { return (dt * 16 + 2) * 64; }
@@ -541,31 +536,25 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                 sc[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], ce, -mu));
                 sum += sc[b][i];
             }
-        // An infinite value has a zero second part, whose products are NaN or of the other sign:
-        // keys whose score is -inf by its products of whole values have no weight.
-        if (SPLIT && __any(sum != sum)) {
-            uint32_t nan = 0;
+        // An infinite value is all in its first part; its products with second parts are NaN or of
+        // either sign. Scores that are NaN are -inf, and their keys without weight, where they are by
+        // the first parts alone.
+        if constexpr (SPLIT)
+            if (__any(sum != sum)) {
+                floatx16 s;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) nan |= uint32_t(sc[0][i] != sc[0][i]) << i;
-            const float *k0 = reinterpret_cast<const float *>(
-                static_cast<const char *>(a.k0) + uint64_t(item) * a.kv_tokens * a.ldk0) + int64_t(hk) * a.d;
-#pragma nounroll
-            for (int i = 0; i < 16; ++i)
-                if (nan >> i & 1) {
-                    const int t = token(tile * KT + acc_row(i, h));
-                    const float *x = reinterpret_cast<const float *>(reinterpret_cast<const char *>(k0) + uint64_t(uint32_t(t)) * a.ldk0);
-                    float s = 0.0f;
-#pragma nounroll
-                    for (int e = 0; e < a.d; ++e) s += sign_or_not_finite(x[e]) * sign_or_not_finite(float(qp[e]));
-                    if (s != kNegInf) nan &= ~(1u << i);
+                for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+                const char *p = kst + (col * L::kKS + h * 8) * 2;
+#pragma unroll
+                for (int c = 0; c < DT * 2; ++c)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const halfx8 *>(p + c * 32), qh[c], s, 0, 0, 0);
+                sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[0][i] = sc[0][i] != sc[0][i] && s[i] == kNegInf ? 0.0f : sc[0][i];
+                    sum += sc[0][i];
                 }
-            sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[0][i] = nan >> i & 1 ? 0.0f : sc[0][i];
-                sum += sc[0][i];
             }
-        }
         l += sum;
         if (SPLIT && each) {
 #pragma unroll
