@@ -539,12 +539,13 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
  * blocks are skipped, one listed twice counts once), in one pass with f32 scores and
  * sums; scale > 0; rows of k and of v less than 32 MiB apart. Rows that see no key are
  * zero, rows at or above q_len are left as they were; what lies at keys a row does not
- * see (NaN among it) does not reach it.
- * f16 tensors: f16 products. f32 tensors: f32 products, where keys are read often of
- * operands in two f16 parts (which hold a value to 2^-24 of itself, of a query or key to
- * 2^-33 of the largest of that head of its token, in the second product to 2^-36 of the
- * largest that the row sees, whichever is more), or on FAST contexts products of operands
- * rounded to f16. Lists are split over workgroups where rows are few, and
+ * see (NaN and infinities among it) does not reach it.
+ * f16 tensors: f16 products, of probabilities that are rounded to f16. f32 tensors: f32
+ * products, where keys are read often of operands in two f16 parts (which hold a value to
+ * 2^-24 of itself, of a query or key to 2^-33 of the largest of that head of its token, in
+ * the second product to 2^-36 of the largest that the row sees, whichever is more), or on
+ * FAST contexts f16 products of operands rounded to f16, those beyond its range (infinities
+ * too) to its largest. Lists are split over workgroups where rows are few, and
  * the parts joined through scratch (mh_block_attention_scratch bytes, 16-byte
  * aligned); NULL takes the context's workspace, which is refused while the stream is
  * being captured into a graph. out overlaps no input. */

@@ -12,8 +12,8 @@
 // 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3, so V^T is read with its keys in that order. WR
 // waves share a tile of keys, WK groups of waves take every WK-th tile and join in LDS.
 //
-// kHalf: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated as the
-// f16 GEMMs round operands; P rounded to f16, at most 1 with a relative 2^-11 each, which
+// kHalf: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated (infinities
+// too) as the f16 GEMMs round operands; P rounded to f16, at most 1 with a relative 2^-11 each, which
 // a sum over keys averages. kF32: f32 products (v_mfma_f32_32x32x2_f32, an eighth of the
 // rate). kSplit: each f32 operand as two f16 parts, x = hi + lo to 2^-24, and the three
 // products above 2^-24 of theirs; queries scaled by a power of two per row, keys and values
@@ -150,12 +150,14 @@ struct Run8 {
         }
         return h;
     }
-    // Zeros in the place of values that are not finite; whether there were any.
+    // Zeros in the place of values that are not finite (SATURATED: NaN alone); whether there were any.
+    template <bool SATURATED = false>
     __device__ __forceinline__ bool clean() {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const bool ok = __builtin_fabsf(float(at(i))) < __builtin_huge_valf();
+            const float x = float(at(i));
+            const bool ok = SATURATED ? x == x : __builtin_fabsf(x) < __builtin_huge_valf();
             any = any || !ok;
             v[i / (8 / kN)][i % (8 / kN)] = ok ? at(i) : T(0);
         }
@@ -198,6 +200,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
     using L = Tiling<MODE, DT, WR>;
     typedef std::conditional_t<MODE == kSplit, _Float16, T> S;  // k and v
     constexpr bool SPLIT = MODE == kSplit, HALF = MODE != kF32, KVEC = VEC || SPLIT;
+    constexpr bool SATURATED = MODE == kHalf && sizeof(T) == 4;  // infinite values are finite operands
     constexpr int kLazy = SPLIT ? kLazySplit : kLazyHalf;
     constexpr int KT = L::kKT, WK = L::kWK, SUB = KT / 32, DP = L::kDP, RUNS = L::kCols / 8;
     constexpr int NT = 64 * WR;                      // threads that stage one tile
@@ -393,7 +396,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                     // are not finite, of tokens that some row does not see (0 times them is NaN in
                     // the products): zeros too, they are added at the end.
                     if (tok[u] >= kv_len) vr[u].zero();
-                    else if (tok[u] >= lim_first && vr[u].clean()) bad = 1;
+                    else if (tok[u] >= lim_first && vr[u].template clean<SATURATED>()) bad = 1;
                 }
             }
             if ((kWhole || j < KT) && ch < a.dk) {
@@ -656,7 +659,7 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
                 for (int i = 0; i < 16; ++i) {
                     const int ch = x * 32 + acc_row(i, h);
                     const float f = ch < a.d ? float(v[ch]) : 0.0f;
-                    if (!(__builtin_fabsf(f) < __builtin_huge_valf())) o[x][i] += f;
+                    if (SATURATED ? f != f : !(__builtin_fabsf(f) < __builtin_huge_valf())) o[x][i] += f;
                 }
         }
     }

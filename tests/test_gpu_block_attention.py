@@ -633,3 +633,24 @@ def test_keys_of_infinite_score(ctx, q_block, kind):
     tol[..., 1:3] = 20  # (the seen keys' own scores: |q| |k| scale stays below)
     assert np.all(np.abs(got - want) <= tolerance(want, tol, 40, dtype, kind == "fast"))
     assert np.isnan(bad).all() or kind == "fast" and np.isnan(bad[..., 1, :]).all()
+
+
+@pytest.mark.parametrize("q_block", [1, 16, 128])
+def test_infinite_values_on_fast_contexts(ctx, q_block):
+    """Infinite f32 operands are taken as f16's largest, as finite ones beyond it are, by every row that sees
+    them, whichever rows share its workgroup; NaN stays NaN."""
+    r = np.random.default_rng(14)
+    q, k, v = (r.standard_normal((1, 128, 1, 64)).astype(np.float32) for _ in range(3))
+    blocks = np.tile(np.arange(4, dtype=np.int32), (1, -(-128 // q_block), 1, 1))
+    v[0, 0, 0, 3], v[0, 70, 0, 5], v[0, 100, 0, 6], v[0, 90, 0, 7] = -np.inf, np.inf, 1e9, np.nan
+    k[0, 110, 0, 9] = np.inf
+    clean, tol = reference(q, np.clip(k, -65504, 65504), np.nan_to_num(np.clip(v, -65504, 65504)), blocks, 0.125, q_block, 32, True, None, None)
+    ctx.set_precision(True)
+    try:
+        got = run(ctx, q, k, v, blocks, q_block, 32, True)
+    finally:
+        ctx.set_precision(False)
+    assert np.isnan(got[0, 90:, 0, 7]).all()
+    ok = np.abs(got - clean) <= tolerance(clean, tol, 64, np.float32, True)
+    ok[0, 90:, 0, 7] = True
+    assert ok.all()
