@@ -654,3 +654,48 @@ def test_infinite_values_on_fast_contexts(ctx, q_block):
     ok = np.abs(got - clean) <= tolerance(clean, tol, 64, np.float32, True)
     ok[0, 90:, 0, 7] = True
     assert ok.all()
+
+
+@pytest.mark.parametrize("nk", [5900, 6007, 6100, 6144, 6145, 8192])
+def test_select_of_many_blocks(ctx, nk):
+    """Scores of single queries over as many blocks as the selection takes."""
+    r = np.random.default_rng(nk)
+    q, means = r.standard_normal((1, 1, 1, 8)).astype(np.float32), r.standard_normal((1, nk, 1, 8)).astype(np.float32)
+    blocks = dev(ctx, np.zeros((1, 1, 1, 1000), np.int32))
+    block_select(heads(ctx, q), dev(ctx, means), nk * 16, blocks, q_block=1, kv_block=16)
+    assert np.array_equal(blocks.numpy(), selected(q, means, 1, 16, 1000, False, None, [nk * 16]))
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32", "fast"])
+@pytest.mark.parametrize("case", [CASES[3], CASES[12], CASES[17], CASES[24]])
+def test_items_alone_and_in_a_batch(ctx, case, kind):
+    """Each item of a batch by itself: equal within both sides' roundings (lists are split by the work that there is)."""
+    _, qt, kt, hq, hk, d, qb, kb, top, causal = case
+    dtype = np.float16 if kind == "f16" else np.float32
+    r = np.random.default_rng(15)
+    q, k, v = (r.standard_normal(s).astype(dtype) for s in ((3, qt, hq, d), (3, kt, hk, d), (3, kt, hk, d)))
+    blocks, kl, ql = lists(r, 3, -(-qt // qb), hk, top, -(-kt // kb)), [kt, kt // 2, kt - 1], [qt, qt, max(qt - 1, 1)]
+    want, tol = reference(q, k, v, blocks, d ** -0.5, qb, kb, causal, ql, kl)
+    bound = tolerance(want, tol, d, dtype, kind == "fast")
+    ctx.set_precision(kind == "fast")
+    try:
+        whole = run(ctx, q, k, v, blocks, qb, kb, causal, ql, kl)
+        for i in range(3):
+            one = run(ctx, q[i:i + 1], k[i:i + 1], v[i:i + 1], blocks[i:i + 1], qb, kb, causal, ql[i:i + 1], kl[i:i + 1])
+            there = ~np.isnan(want[i])
+            diff = np.abs(one[0].astype(np.float64) - whole[i])
+            assert np.all(diff[there] <= 2 * bound[i][there])
+    finally:
+        ctx.set_precision(False)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("q_block", [1, 16])
+def test_lists_of_the_same_order_agree_in_bits(ctx, dtype, q_block):
+    """Places that are empty, outside or listed before change nothing of a list, in bits."""
+    r = np.random.default_rng(16)
+    q, k, v = (r.standard_normal((1, t, 1, 40)).astype(dtype) for t in (16, 640, 640))
+    tile = lambda b: np.tile(np.array(b, np.int32), (1, 16 // q_block, 1, 1))  # noqa: E731
+    a = run(ctx, q, k, v, tile([20, 3, 39, 7, -1, -1, -1, -1]), q_block, 16)
+    b = run(ctx, q, k, v, tile([-1, 20, 3, 20, 50, 39, 3, 7]), q_block, 16)
+    assert np.array_equal(a, b)

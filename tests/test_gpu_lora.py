@@ -283,3 +283,24 @@ def test_infinite_values(ctx, case, wf16, af16, fast):
     there = np.isfinite(y)
     bound = (2.0 ** -10 if fast else 1e-5) * base + (ci + rank + 8) * U * low + U * np.abs(y)
     assert np.all(np.abs(got - y)[there] <= bound[there])
+
+
+@pytest.mark.parametrize("fast", [False, True])
+@pytest.mark.parametrize("wf16", [False, True])
+@pytest.mark.parametrize("case", CASES)
+def test_weight_and_adapters_of_different_types(ctx, case, wf16, fast):
+    n, h, w, ci, co, rank, slots, pixel = case
+    d = make(ctx, case, wf16, seed=1)
+    d["a"], d["b"] = (d[t].astype(np.float32 if wf16 else np.float16) for t in "ab")
+    conv = E.Conv1x1(ctx, ci, co, E.Param(ctx, d["w"], f16=wf16), d["bias"])
+    ad = Adapters(ctx, E.Param(ctx, d["a"], f16=not wf16), E.Param(ctx, d["b"], f16=not wf16), d["scale"], ci, co, rank)
+    out = E.Tensor(ctx)
+    ctx.set_precision(fast)
+    try:
+        conv.forward_adapted(E.Tensor.from_numpy(ctx, d["x"]), ad, E.DeviceArray.from_numpy(ctx, d["slot"]), out)
+    finally:
+        ctx.set_precision(False)
+    y, base, low = reference(d["x"].reshape(-1, ci), d["w"], d["bias"], None, d["a"], d["b"], d["scale"], d["slot"], 1 if pixel else h * w)
+    err = np.abs(out.numpy().reshape(-1, co) - y)
+    bound = (2.0 ** -10 if fast else 1e-5) * base + (ci + rank + 8) * U * low + U * np.abs(y)
+    assert np.all(err <= bound), (err / bound).max()
