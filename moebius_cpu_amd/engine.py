@@ -284,9 +284,11 @@ class Conv1x1:
             raise MoebiusError(1, "Conv1x1 weight size")
         if slot.dtype != _I32 or slot.nbytes // 4 not in (x.n, x.pixels()):
             raise MoebiusError(1, "slot is int32, one for each item or each pixel")
-        out.set_shape(x.n, x.h, x.w, self.c_out)
-        if residual is not None and residual.shape != out.shape:
+        if residual is not None and residual.shape != (x.n, x.h, x.w, self.c_out):  # (residual may be out)
             raise MoebiusError(1, "Conv1x1 residual shape")
+        if out is x:
+            raise MoebiusError(1, "x and out overlap")
+        out.set_shape(x.n, x.h, x.w, self.c_out)
         per = 1 if slot.nbytes // 4 == x.pixels() else x.h * x.w
         check(lib().mh_conv1x1_lora(self.ctx.h, x.ptr, x.pixels(), x.c, self.weight.ptr, self.weight.dtype, self.c_out,
                                     _ptr(self.bias), _ptr(residual), ctypes.byref(adapters.c), slot.ptr, max(per, 1),

@@ -304,3 +304,19 @@ def test_weight_and_adapters_of_different_types(ctx, case, wf16, fast):
     err = np.abs(out.numpy().reshape(-1, co) - y)
     bound = (2.0 ** -10 if fast else 1e-5) * base + (ci + rank + 8) * U * low + U * np.abs(y)
     assert np.all(err <= bound), (err / bound).max()
+
+
+def test_refused_calls_leave_their_tensors(ctx):
+    """A residual or an input that is also out, but of another shape, is refused before out is reshaped."""
+    case = (2, 2, 2, 32, 16, 4, 2, False)
+    d = make(ctx, case, False)
+    conv, ad = layer(ctx, case, d, False)
+    x, slot = E.Tensor.from_numpy(ctx, d["x"]), E.DeviceArray.from_numpy(ctx, d["slot"])
+    small = np.ones((1, 2, 2, 16), np.float32)
+    res = E.Tensor.from_numpy(ctx, small)
+    with pytest.raises(MoebiusError, match="residual shape"):
+        conv.forward_adapted(x, ad, slot, res, res)
+    assert res.shape == small.shape and np.array_equal(res.numpy(), small)
+    with pytest.raises(MoebiusError, match="overlap"):
+        conv.forward_adapted(x, ad, slot, x)
+    assert x.shape == d["x"].shape and np.array_equal(x.numpy(), d["x"])
