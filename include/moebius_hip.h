@@ -545,10 +545,11 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
  * 2^-24 of itself, of a query or key to 2^-33 of the largest of that head of its token, in
  * the second product to 2^-36 of the largest that the row sees, whichever is more), or on
  * FAST contexts f16 products of operands rounded to f16, those beyond its range (infinities
- * too) to its largest. Lists are split over workgroups where rows are few, and
- * the parts joined through scratch (mh_block_attention_scratch bytes, 16-byte
- * aligned); NULL takes the context's workspace, which is refused while the stream is
- * being captured into a graph. out overlaps no input. */
+ * too) to its largest. f32 sums of values times probabilities of up to 2^8: values of
+ * 2^119 divided by the number of a row's keys, or more, may give infinities. Lists are
+ * split over workgroups where rows are few, and the parts joined through scratch
+ * (mh_block_attention_scratch bytes, 16-byte aligned); NULL takes the context's workspace,
+ * which is refused while the stream is being captured into a graph. out overlaps no input. */
 int32_t mh_block_attention(MhContext *ctx, const void *q, uint64_t ld_q, const void *k, uint64_t ld_k, const void *v,
                            uint64_t ld_v, uint32_t dtype, const MhBlockShape *shape, const int32_t *blocks, float scale,
                            void *out, uint64_t ld_out, void *scratch, uint64_t scratch_bytes);

@@ -46,7 +46,7 @@ void qk_norm_rope(Context &ctx, HeadRows q, HeadRows k, WeightType type, int64_t
                   const float *gamma_k, float eps, const RopeTable &t, void *q_out, int64_t ld_qo, void *k_out,
                   int64_t ld_ko);
 
-// ---- attention over selected blocks of keys (block_select.hip, block_attention.hip)
+// ---- attention over selected blocks of keys (block_select.hip, block_attention*)
 constexpr int kMaxHeadDim = 256;    // channels of a head that the selection and the attention take
 constexpr int kMaxKeyBlocks = 8192; // key blocks of an item that the selection orders
 constexpr int kMaxTop = 1024;       // selected blocks per block of queries
@@ -88,10 +88,9 @@ void block_attention(Context &ctx, const BlockAttention &a, WeightType type, voi
 // ---- low-rank adapters beside a shared projection (lora.hip)
 constexpr int kMaxRank = 256;
 
-// out [rows][c_out] = x . W^T + bias + residual (conv1x1), and then, for every row whose
-// slot[row / rows_per_slot] is one of 0 .. slots - 1,
-//   out += scale[slot] (x . a[slot]^T) . b[slot]^T,  a [slots][rank][c_in], b [slots][c_out][rank].
-// Other rows are the projection alone. scratch: lora_scratch bytes, 16-byte aligned.
+// out [rows][c_out] = x . W^T + bias + residual + scale[s] (x . a[s]^T) . b[s]^T, written once, for
+// every row whose s = slot[row / rows_per_slot] is one of 0 .. slots - 1; a [slots][rank][c_in],
+// b [slots][c_out][rank]. Other rows are the projection alone. scratch: lora_scratch bytes, 16-byte aligned.
 struct Lora {
     const void *a = nullptr, *b = nullptr;
     WeightType type = kF32;

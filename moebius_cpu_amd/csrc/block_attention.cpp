@@ -49,10 +49,10 @@ struct Plan {
 //
 // f32 products are split where the keys and values, which that reads and writes once, are
 // then read at least kSplitReuse times by waves full of rows: 4096 keys, 8 heads of 80, read
-// once 36.9 us (31.2 on the f32 instructions), twice 41.2 (47.3), four times 41.3 (59.1),
-// sixteen times 72 (158). Where one wave's rows are all, kSplitReuseFew times, as half of the
-// row waves then stand idle: 2 heads of 80 of 2 items, 8 times 33 (30.7), 16 times 38 (59.5)
-// and 52 (55), 32 times 76 (90), 128 times 154 (344).
+// once 30.4 us (25.0 on the f32 instructions), twice 34.6 (33.5), four times 43.5 (49.5),
+// sixteen times 69 (149). Where one wave's rows are all, kSplitReuseFew times, as half of the
+// row waves then stand idle: 2 heads of 80 of 2 items, 8 times 36.5 (31.6), 16 times 39.7 (60.2)
+// and 57.7 (56.0), 32 times 88 (90), 128 times 170 (345).
 constexpr int64_t kSplitReuse = 2, kSplitReuseFew = 16;
 Plan plan(const Context &ctx, const BlockShape &s, WeightType type, bool half) {
     Plan p;

@@ -13,8 +13,10 @@
 // waves share a tile of keys, WK groups of waves take every WK-th tile and join in LDS.
 //
 // kHalf: f16 products (v_mfma_f32_32x32x16_f16), f32 storage rounded and saturated (infinities
-// too) as the f16 GEMMs round operands; P rounded to f16, at most 1 with a relative 2^-11 each, which
-// a sum over keys averages. kF32: f32 products (v_mfma_f32_32x32x2_f32, an eighth of the
+// too) as the f16 GEMMs round operands; P rounded to f16 while its sum keeps f32, off by at most
+// 2^-11 each, which a sum over keys averages (outputs of f16 tensors then lie 2.6e-4 to 2.9e-4 of
+// the largest from 64 bits, where their own rounding alone gives 2.1e-4; P in two parts would
+// double the second product). kF32: f32 products (v_mfma_f32_32x32x2_f32, an eighth of the
 // rate). kSplit: each f32 operand as two f16 parts, x = hi + lo to 2^-24, and the three
 // products above 2^-24 of theirs; queries scaled by a power of two per row, keys and values
 // per sixteen tokens, or per token where those are far apart (KeyScale), probabilities by 2^11
@@ -25,7 +27,7 @@
 // Bound: the matrix instructions and the vector instructions beside them (7 to 8 for each;
 // from registers alone 7 leave the card 1278 TFLOP/s of f16 on random values); latency where
 // rows are few. Measured: 16384 tokens, 16 heads of 128, f16, 2048 keys per row 346 us (795
-// TFLOP/s); 2 x 4096, 8 heads of 80, f32, 1024 keys 128 us, on the f32 instructions 298; 8
+// TFLOP/s); 2 x 4096, 8 heads of 80, f32, 1024 keys 131 us, on the f32 instructions 298; 8
 // single tokens, 32 / 8 heads of 128, 2048 of up to 16384 keys 24.7 us. For the first: values
 // read from LDS transposed by ds_read_b64_tr_b16 instead of gathered 1140 -> 473 us; loads
 // without branches and 32-bit offsets 473 -> 375; the maximum's reference moved only when it

@@ -1,12 +1,14 @@
 // Low-rank adapters of many requests beside a shared 1x1 projection:
 //   y = x W^T + bias + residual + scale_s (x A_s^T) B_s^T,  s the row's adapter.
 //
-// The adapters' products are f32 in EXACT and FAST contexts alike: at rank r they are
-// r (c_in + c_out) of the projection's c_in c_out operations. Few rows take two passes of
+// The adapters' products keep f32's accuracy in EXACT and FAST contexts alike: at rank r they
+// are r (c_in + c_out) of the projection's c_in c_out operations. Few rows take two passes of
 // f32 products:
 //   row shrink: t = x A_s^T [rows][rank], a wave per rank of a row;
 //   row project: x W^T in tiles of 16 x 16, finished with bias, residual and scale_s t B_s^T.
-// More rows take the product of lora_gemm.hip behind one pass over x, which forms t as well.
+// More rows take the product of lora_gemm.hip behind one pass over x, which forms t as well:
+// with adapters stored in f16 by f16 products of x and t in two parts, with f32 ones by f32
+// products (and x split in a pass of its own).
 //
 // A tile of 16 rows takes the adapters its rows name one after another, each product
 // over all 16 rows and kept for its own: rows of one image share one, single tokens of
