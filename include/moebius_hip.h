@@ -539,7 +539,8 @@ int32_t mh_block_attention_scratch(MhContext *ctx, uint32_t dtype, const MhBlock
  * blocks are skipped, one listed twice counts once), in one pass with f32 scores and
  * sums; scale > 0; rows of k and of v less than 32 MiB apart. Rows that see no key are
  * zero, rows at or above q_len are left as they were; what lies at keys a row does not
- * see (NaN and infinities among it) does not reach it.
+ * see (NaN and infinities among it) does not reach it. An infinite value at a key that it
+ * does see makes its channel infinite, or NaN where the key's probability rounds to zero.
  * f16 tensors: f16 products, of probabilities that are rounded to f16. f32 tensors: f32
  * products, where keys are read often of operands in two f16 parts (which hold a value to
  * 2^-24 of itself, of a query or key to 2^-33 of the largest of that head of its token, in
