@@ -699,3 +699,35 @@ def test_lists_of_the_same_order_agree_in_bits(ctx, dtype, q_block):
     a = run(ctx, q, k, v, tile([20, 3, 39, 7, -1, -1, -1, -1]), q_block, 16)
     b = run(ctx, q, k, v, tile([-1, 20, 3, 20, 50, 39, 3, 7]), q_block, 16)
     assert np.array_equal(a, b)
+
+
+def test_split_operands_captured_and_replayed(ctx):
+    """Two graphs of f32 calls whose keys are split, lists too, with scratch of their own, replayed among eager
+    calls in the context's workspace."""
+    r = np.random.default_rng(19)
+    blocks = dev(ctx, np.tile(np.arange(20, dtype=np.int32), (1, 2, 1, 1)))
+    calls, wants = [], []
+    for _ in range(2):
+        q, k, v = (heads(ctx, r.standard_normal((1, t, 1, 72)).astype(np.float32)) for t in (128, 640, 640))
+        out = heads(ctx, np.zeros((1, 128, 1, 72), np.float32))
+        scratch = E.DeviceArray(ctx, (block_attention_scratch(q, k, blocks, 64, 32),), np.uint8)
+        assert scratch.nbytes >= 640 * 72 * 8
+        calls.append((q, k, v, out, scratch))
+        block_attention(q, k, v, blocks, out, q_block=64, kv_block=32)
+        wants.append(out.numpy())
+    with pytest.raises(MoebiusError, match="captured call needs scratch"):
+        capture(ctx, lambda: block_attention(*calls[0][:3], blocks, calls[0][3], q_block=64, kv_block=32))
+    graphs = [capture(ctx, lambda c=c: block_attention(*c[:3], blocks, c[3], q_block=64, kv_block=32, scratch=c[4])) for c in calls]
+    eager = heads(ctx, np.zeros((1, 128, 1, 72), np.float32))
+    for turn in range(4):
+        for c in calls:
+            c[3].buf.upload(np.zeros((1, 128, 1, 72), np.float32))
+        for launch, _ in graphs:
+            launch()
+        block_attention(*calls[turn % 2][:3], blocks, eager, q_block=64, kv_block=32)
+        ctx.synchronize()
+        for c, want in zip(calls, wants):
+            assert np.array_equal(c[3].numpy(), want)
+        assert np.array_equal(eager.numpy(), wants[turn % 2])
+    for _, destroy in graphs:
+        destroy()
