@@ -245,10 +245,13 @@ def _own_state(c, d):
         out, st["view"] = outputs(**({"x": E.DeviceArray(ctx, d["x"].shape, "f2" if c["x16"] else "f4")} if c["branch"] else {}),
                                   y=E.DeviceArray(ctx, d["x"].shape, "f2" if c["h16"] else "f4"))
         st.update(x=heads(d["x"][:, :, None]), y=Heads(out["y"], n, rows, 1, ch), x_out=None, branch=None, keep=d["keep"],
-                  post=G.Norm(c["post"], array(d["g_post"]), None, d["eps"]),
-                  pre=G.Norm(c["pre"], array(d["g_pre"]), array(d["b_pre"]), d["eps"]), gate=None, scale=None, shift=None)
+                  post=None, pre=None, gate=None, scale=None, shift=None)
+        if c["pre"] != "none":
+            st["pre"] = G.Norm(c["pre"], array(d["g_pre"]), array(d["b_pre"]), d["eps"])
         if c["branch"]:
             st.update(branch=heads(d["h"][:, :, None]), x_out=Heads(out["x"], n, rows, 1, ch))
+            if c["post"] != "none":
+                st["post"] = G.Norm(c["post"], array(d["g_post"]), None, d["eps"])
         if c["mod"]:
             mod = array(d["mod"])
             st.update({k: Heads(mod, n, 1, 1, ch, ld=3 * ch, offset=i * ch)
