@@ -68,6 +68,11 @@ extern "C" {
 #define MH_ROPE_INTERLEAVED 0u
 #define MH_ROPE_HALVES 1u
 
+/* Norms of a row (MhNorm): none, by the root mean square, LayerNorm. */
+#define MH_NORM_NONE 0u
+#define MH_NORM_RMS 1u
+#define MH_NORM_LAYER 2u
+
 typedef struct MhContext MhContext;
 typedef struct MhEvent MhEvent;
 typedef struct MhUNet MhUNet;
@@ -585,6 +590,109 @@ int32_t mh_conv1x1_lora(MhContext *ctx, const float *x, uint64_t rows, uint32_t 
                         uint32_t weight_dtype, uint32_t c_out, const float *bias, const float *residual,
                         const MhAdapters *adapters, const int32_t *slot, uint64_t rows_per_slot, float *out,
                         void *scratch, uint64_t scratch_bytes);
+
+/* ---- streams of tokens: a cache in 8 bits, attention over it, gated norms ----
+ *
+ * No counterpart in the reference. Heads as above; codes, tables and lengths are device arrays. */
+
+/* Keys and values in 8 bits, in pages of `block` tokens (16, 32, 64 or 128): a code byte b stands
+ * for (b - 128) * scale, with one f32 scale for the keys and one for the values of each page and
+ * head. k [pages][heads][block][dp], v [pages][heads][dp][block] (16-byte aligned, dp = d rounded
+ * up to 16, d <= 256), k_scale, v_scale [pages][heads]: mh_cache8_sizes bytes each. What a page
+ * holds before it is written has no meaning and needs no clearing. */
+typedef struct MhCache8 {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    uint32_t pages, heads, d, block;
+} MhCache8;
+
+/* Token p of item i lies in page pages[i * blocks + p / block], p < blocks * block <= 2^30. An entry
+ * outside 0 .. the cache's pages - 1 (-1 by convention) has no page: its tokens are not written, not
+ * read back and seen by no query, so that pages behind a window can be handed out again. Items may
+ * share pages that are read; a page that a call writes for two items holds either's tokens. */
+typedef struct MhPageTable {
+    const int32_t *pages; /* [n][blocks] */
+    uint32_t n, blocks;
+} MhPageTable;
+
+/* Bytes of k (and of v), and of k_scale (and of v_scale). Host only. */
+int32_t mh_cache8_sizes(uint32_t pages, uint32_t heads, uint32_t d, uint32_t block, uint64_t *code_bytes,
+                        uint64_t *scale_bytes);
+
+/* Token t < len[i] (NULL: tokens) of item i, row i * tokens + t of k and v, is held as token
+ * first[i] + t (NULL: t); first and len are clamped to what the table has. The scale of a block
+ * and head is the f32 value next to a / 127, a the largest finite magnitude among its new tokens;
+ * where the block holds tokens before the first new one it is at least what it was, and if it grows
+ * their codes are rounded to it. Codes are x / scale rounded to the nearest integer, ties to even:
+ * off by at most half a scale for each time that they were rounded. Infinities are held as the
+ * largest value of their sign, NaN and everything at a scale of 0 as 0. Tokens behind the last new
+ * one in its block have no meaning afterwards. */
+int32_t mh_cache8_write(MhContext *ctx, const MhCache8 *cache, const MhPageTable *table, const void *k, uint64_t ld_k,
+                        const void *v, uint64_t ld_v, uint32_t dtype, uint32_t tokens, const int32_t *first,
+                        const int32_t *len);
+
+/* Rows t < len[i] (NULL: tokens) of k and v = code * scale of token first[i] + t (NULL: t), rounded
+ * to dtype. Other rows, and those without a page, are left as they were. */
+int32_t mh_cache8_read(MhContext *ctx, const MhCache8 *cache, const MhPageTable *table, void *k, uint64_t ld_k, void *v,
+                       uint64_t ld_v, uint32_t dtype, uint32_t tokens, const int32_t *first, const int32_t *len);
+
+/* q_tokens queries of heads_q heads for each item of a table (query head h reads key head
+ * h / (heads_q / heads)). Row t < q_len[i] (NULL: q_tokens) stands at position
+ * p = t + kv_len[i] - q_len[i] and sees the tokens j < kv_len[i] (NULL: all of the table's blocks),
+ * causal those with j <= p; window > 0: of these, those with j > p - window or j < sinks. */
+typedef struct MhCacheAttention {
+    uint32_t q_tokens, heads_q;
+    uint32_t causal, window, sinks; /* sinks only with a window */
+    uint32_t reserved;              /* 0 */
+    const int32_t *q_len, *kv_len;  /* [n] or NULL */
+} MhCacheAttention;
+
+/* Scratch of mh_cache8_attention for these shapes on this context (0: none needed). */
+int32_t mh_cache8_attention_scratch(MhContext *ctx, uint32_t dtype, const MhCacheAttention *shape, const MhCache8 *cache,
+                                    const MhPageTable *table, uint64_t *bytes);
+
+/* out [n][q_tokens][heads_q][d] = softmax(scale q . k) v over the tokens that a row sees, k and v
+ * the values that the cache holds, in one pass with f32 scores and sums; scale > 0. Rows that see
+ * no token are zero, rows at or above q_len are left as they were. Codes enter the f16 products
+ * exactly. f16: queries as they are, probabilities rounded to f16. f32: queries (to 2^-24 of
+ * themselves or 2^-39 of the largest of their head, whichever is more) and probabilities in two f16
+ * parts, or on FAST contexts rounded to f16 once. Tokens are split over workgroups where rows are
+ * few, and the parts joined through scratch (mh_cache8_attention_scratch bytes, 16-byte aligned);
+ * NULL takes the context's workspace, which is refused while the stream is being captured into a
+ * graph. out overlaps no input. */
+int32_t mh_cache8_attention(MhContext *ctx, const void *q, uint64_t ld_q, uint32_t dtype, const MhCacheAttention *shape,
+                            const MhCache8 *cache, const MhPageTable *table, float scale, void *out, uint64_t ld_out,
+                            void *scratch, uint64_t scratch_bytes);
+
+/* A norm over the channels of a row: (v - mean) / sqrt(mean((v - mean)^2) + eps) * gamma + beta,
+ * MH_NORM_RMS without the mean; gamma, beta [c] f32 or NULL. */
+typedef struct MhNorm {
+    uint32_t kind; /* MH_NORM_* */
+    float eps;
+    const float *gamma, *beta;
+} MhNorm;
+
+/* Around a block of a transformer, for rows of c <= 32768 channels:
+ *   s = keep * x + gate * post(branch)      (branch NULL: s = x)
+ *   x_out = s,   y = pre(s) * (1 + scale) + shift
+ * in one pass with f32 sums, x_out and y each rounded once (y from s before that). x and x_out are
+ * of x_dtype, branch and y of branch_dtype; x_out or y may be NULL. gate, scale and shift are f32
+ * vectors [items][c], ld elements apart, or NULL (gate 1, scale and shift 0); row r takes those of
+ * item r / rows_per_item. An output may be an input of its type (same pointer and ld); no other
+ * overlap. */
+typedef struct MhGatedNorm {
+    const void *x, *branch;
+    void *x_out, *y;
+    uint64_t ld_x, ld_branch, ld_x_out, ld_y;
+    uint32_t x_dtype, branch_dtype;
+    uint64_t rows, rows_per_item;
+    uint32_t c;
+    float keep;
+    MhNorm post, pre;
+    const float *gate, *scale, *shift;
+    uint64_t ld_gate, ld_scale, ld_shift;
+} MhGatedNorm;
+int32_t mh_gated_norm(MhContext *ctx, const MhGatedNorm *n);
 
 /* ---- UNet (src/unet) ---- */
 

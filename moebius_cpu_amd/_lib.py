@@ -124,6 +124,12 @@ SIGNATURES = {
     "mh_block_attention": (_i32, [_vp, _vp, _u64, _vp, _u64, _vp, _u64, _u32, _vp, _vp, _f32, _vp, _u64, _vp, _u64]),
     "mh_conv1x1_lora_scratch": (_i32, [_vp, _u64, _u32, _u32, _u32, _u32, ctypes.POINTER(_u64)]),
     "mh_conv1x1_lora": (_i32, [_vp, _vp, _u64, _u32, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _u64, _vp, _vp, _u64]),
+    "mh_cache8_sizes": (_i32, [_u32, _u32, _u32, _u32, ctypes.POINTER(_u64), ctypes.POINTER(_u64)]),
+    "mh_cache8_write": (_i32, [_vp, _vp, _vp, _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp]),
+    "mh_cache8_read": (_i32, [_vp, _vp, _vp, _vp, _u64, _vp, _u64, _u32, _u32, _vp, _vp]),
+    "mh_cache8_attention_scratch": (_i32, [_vp, _u32, _vp, _vp, _vp, ctypes.POINTER(_u64)]),
+    "mh_cache8_attention": (_i32, [_vp, _vp, _u64, _u32, _vp, _vp, _vp, _f32, _vp, _u64, _vp, _u64]),
+    "mh_gated_norm": (_i32, [_vp, _vp]),
     "mh_unet_create": (_i32, [_vp, _vp, _u32, ctypes.POINTER(_vp)]),
     "mh_unet_destroy": (None, [_vp]),
     "mh_unet_forward": (_i32, [_vp, _vp, _u32, _u32, _vp]),
@@ -214,6 +220,43 @@ class AdapterSet(ctypes.Structure):
                 ("reserved", ctypes.c_uint32)]
 
 
+class Cache8(ctypes.Structure):
+    """include/moebius_hip.h MhCache8."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("d", ctypes.c_uint32), ("block", ctypes.c_uint32)]
+
+
+class PageTable(ctypes.Structure):
+    """include/moebius_hip.h MhPageTable."""
+    _fields_ = [("pages", ctypes.c_void_p), ("n", ctypes.c_uint32), ("blocks", ctypes.c_uint32)]
+
+
+class CacheAttention(ctypes.Structure):
+    """include/moebius_hip.h MhCacheAttention."""
+    _fields_ = [("q_tokens", ctypes.c_uint32), ("heads_q", ctypes.c_uint32), ("causal", ctypes.c_uint32),
+                ("window", ctypes.c_uint32), ("sinks", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+                ("q_len", ctypes.c_void_p), ("kv_len", ctypes.c_void_p)]
+
+
+class Norm(ctypes.Structure):
+    """include/moebius_hip.h MhNorm."""
+    _fields_ = [("kind", ctypes.c_uint32), ("eps", ctypes.c_float), ("gamma", ctypes.c_void_p),
+                ("beta", ctypes.c_void_p)]
+
+
+class GatedNorm(ctypes.Structure):
+    """include/moebius_hip.h MhGatedNorm."""
+    _fields_ = [("x", ctypes.c_void_p), ("branch", ctypes.c_void_p), ("x_out", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("ld_x", ctypes.c_uint64), ("ld_branch", ctypes.c_uint64),
+                ("ld_x_out", ctypes.c_uint64), ("ld_y", ctypes.c_uint64), ("x_dtype", ctypes.c_uint32),
+                ("branch_dtype", ctypes.c_uint32), ("rows", ctypes.c_uint64), ("rows_per_item", ctypes.c_uint64),
+                ("c", ctypes.c_uint32), ("keep", ctypes.c_float), ("post", Norm), ("pre", Norm),
+                ("gate", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("shift", ctypes.c_void_p),
+                ("ld_gate", ctypes.c_uint64), ("ld_scale", ctypes.c_uint64), ("ld_shift", ctypes.c_uint64)]
+
+
+NORM = {"none": 0, "rms": 1, "layer": 2}
 ROPE_PAIRING = {"interleaved": 0, "halves": 1}
 
 MODEL_UNET = 0

@@ -1,0 +1,64 @@
+// Which variant of the attention over a cache in 8 bits runs, and the scratch its splits
+// join through.
+#include <algorithm>
+
+#include "cache8_attention.hpp"
+
+namespace mh {
+namespace {
+
+// Tiles of 16 channels of the instantiated kernels that hold a head of d channels.
+int head_tiles(int d) {
+    const int t = int(ceil_div(d, 16));
+    return t <= 4 ? 4 : t <= 6 ? t : t <= 8 ? 8 : t <= 10 ? 10 : 16;
+}
+
+struct Plan {
+    int nq, dt, row_tiles, splits;
+    int64_t items;
+    size_t bytes;
+};
+
+// The tokens are split over workgroups where the rows alone leave CUs idle, up to two workgroups
+// per CU and down to 256 tokens, a chunk for each wave.
+Plan plan(const Context &ctx, const Cache8Attention &a) {
+    Plan p;
+    const int64_t rows = int64_t(a.q_tokens) * (a.q.heads / a.c.heads);
+    p.dt = head_tiles(a.c.d);
+    p.nq = rows > 16 && p.dt <= 8 ? 2 : 1;
+    p.row_tiles = int(ceil_div(rows, 16 * p.nq));
+    p.items = int64_t(a.t.n) * a.c.heads * p.row_tiles;
+    int64_t tokens = int64_t(a.t.blocks) << a.c.block_log;
+    if (a.window) tokens = std::min(tokens, int64_t(a.window) + a.sinks + a.q_tokens);
+    p.splits = int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), 2 * int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1))));
+    p.bytes = p.splits > 1 ? size_t(p.items) * p.splits * p.nq * 16 * (p.dt * 16 + 2) * sizeof(float) : 0;
+    return p;
+}
+
+}  // namespace
+
+size_t cache8_attention_scratch(const Context &ctx, const Cache8Attention &a) {
+    if (!a.t.n || !a.q_tokens) return 0;
+    return plan(ctx, a).bytes;
+}
+
+void cache8_attention(Context &ctx, const Cache8Attention &c, void *scratch) {
+    if (!c.t.n || !c.q_tokens) return;
+    const Plan p = plan(ctx, c);
+    MH_REQUIRE(p.items * p.splits < (int64_t(1) << 26), "cache8_attention: too many rows");
+    c8a::Args a{};
+    a.q = c.q.p, a.out = c.out, a.ldq = c.q.ld, a.ldo = c.ld_out;
+    a.k = c.c.k, a.v = c.c.v, a.ks = c.c.k_scale, a.vs = c.c.v_scale;
+    a.table = c.t.table, a.q_len = c.q_len, a.kv_len = c.kv_len;
+    a.part = p.splits > 1 ? static_cast<float *>(scratch) : nullptr;
+    a.c = c.scale * 1.44269504088896340736f;
+    a.n = c.t.n, a.q_tokens = c.q_tokens, a.hk = c.c.heads, a.g = c.q.heads / c.c.heads, a.d = c.c.d, a.dp = c.c.dp();
+    a.blocks = c.t.blocks, a.pages = c.c.pages, a.block_log = c.c.block_log;
+    a.row_tiles = p.row_tiles, a.splits = p.splits, a.work = int(p.items * p.splits);
+    a.causal = c.causal, a.window = c.window, a.sinks = c.sinks;
+    if (c.type == kF16) c8a::launch_f16(ctx, a, p.nq, p.dt);
+    else if (ctx.precision == Precision::Fast) c8a::launch_f32_half(ctx, a, p.nq, p.dt);
+    else c8a::launch_f32(ctx, a, p.nq, p.dt);
+}
+
+}  // namespace mh

@@ -1,0 +1,10 @@
+// The attention over a cache in 8 bits, instantiated.
+#include "cache8_attention.hpp"
+
+namespace mh {
+namespace c8a {
+
+void launch_f32_half(Context &ctx, const Args &a, int nq, int dt) { launch_rows_dt<float, 1>(ctx, a, nq, dt); }
+
+}  // namespace c8a
+}  // namespace mh

@@ -7,59 +7,22 @@
 
 #include "attention.hpp"
 #include "capi_context.hpp"
+#include "capi_rows.hpp"
 
 namespace {
 
+using mh::capi::aligned4;
 using mh::capi::C;
+using mh::capi::check_scratch;
 using mh::capi::dim;
 using mh::capi::guard;
 using mh::capi::need;
+using mh::capi::no_overlap;
+using mh::capi::Rows;
+using mh::capi::rows_of;
+using mh::capi::same_or_apart;
+using mh::capi::size_of;
 using mh::capi::wtype;
-
-size_t size_of(mh::WeightType t) { return t == mh::kF16 ? 2 : 4; }
-
-// A strided tensor of heads: its rows' elements and where they lie.
-struct Rows {
-    const char *p;
-    int64_t rows, ld, cols;
-    size_t size;
-    const char *end() const { return p + (rows ? size_t((rows - 1) * ld + cols) * size : 0); }
-};
-
-Rows rows_of(const void *p, uint64_t rows, uint32_t heads, uint32_t d, uint64_t ld, mh::WeightType t,
-             const char *what) {
-    const std::string name = what;
-    if (heads == 0 || d == 0) mh::fail(mh::kInvalidArgument, name + ": no heads or channels");
-    const uint64_t cols = uint64_t(dim(heads, "heads")) * uint64_t(dim(d, "d"));
-    if (cols > (1u << 30)) mh::fail(mh::kInvalidArgument, name + ": row too large");
-    if (ld < cols) mh::fail(mh::kInvalidArgument, name + ": ld is less than heads * d");
-    if (ld > (uint64_t(1) << 40) || (rows && ld > (uint64_t(1) << 60) / rows))
-        mh::fail(mh::kInvalidArgument, name + ": tensor too large");
-    if (rows) need(p, what);
-    if (reinterpret_cast<uintptr_t>(p) % size_of(t)) mh::fail(mh::kInvalidArgument, name + " is not aligned to its type");
-    return Rows{static_cast<const char *>(p), int64_t(rows), int64_t(ld), int64_t(cols), size_of(t)};
-}
-
-// Whether a and b share elements: ranges that meet, unless their rows step alike and
-// their columns lie apart.
-bool overlap(const Rows &a, const Rows &b) {
-    if (!a.rows || !b.rows || a.p >= b.end() || b.p >= a.end()) return false;
-    if (a.ld != b.ld || a.size != b.size) return true;
-    const int64_t step = a.ld * int64_t(a.size);
-    int64_t off = (b.p - a.p) % step;
-    if (off < 0) off += step;
-    return off < a.cols * int64_t(a.size) || off + b.cols * int64_t(b.size) > step;
-}
-
-void no_overlap(const Rows &a, const Rows &b, const char *what) {
-    if (overlap(a, b)) mh::fail(mh::kInvalidArgument, std::string(what) + " overlap");
-}
-
-// The same place (in place), or apart.
-void same_or_apart(const Rows &in, const Rows &out, const char *what) {
-    if (in.p == out.p && in.ld == out.ld) return;
-    no_overlap(in, out, what);
-}
 
 mh::RopeTable rope_table(const MhRope *r, uint32_t d) {
     need(r, "rope");
@@ -86,12 +49,6 @@ mh::RopeTable rope_table(const MhRope *r, uint32_t d) {
     t.pairing = mh::RopePairing(r->pairing);
     t.inverse = r->inverse != 0;
     return t;
-}
-
-// Arrays of 4-byte elements (NULL counts as aligned).
-void aligned4(const void *p, const char *what) {
-    if (reinterpret_cast<uintptr_t>(p) % 4)
-        mh::fail(mh::kInvalidArgument, std::string(what) + " is not aligned to its type");
 }
 
 void few_rows(uint64_t rows) {
@@ -129,21 +86,6 @@ mh::BlockShape block_shape(const MhBlockShape *s) {
     b.q_len = s->q_len;
     b.kv_len = s->kv_len;
     return b;
-}
-
-// The caller's scratch, or NULL where the context's workspace is to be used.
-void *check_scratch(mh::Context &c, void *scratch, uint64_t bytes, size_t needed) {
-    if (!needed) return nullptr;
-    if (scratch) {
-        if (bytes < needed) mh::fail(mh::kInvalidArgument, "scratch is smaller than this call needs");
-        if (!mh::aligned16(scratch)) mh::fail(mh::kInvalidArgument, "scratch is not 16-byte aligned");
-        return scratch;
-    }
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    HIP_CHECK(hipStreamIsCapturing(c.stream, &st));
-    if (st != hipStreamCaptureStatusNone)
-        mh::fail(mh::kInvalidArgument, "a captured call needs scratch of its own: the context's workspace may move");
-    return nullptr;
 }
 
 }  // namespace
