@@ -221,14 +221,19 @@ def _own_state(c, d):
         return Heads(array(t), t.shape[0], t.shape[1], t.shape[2], t.shape[3])
 
     st = {"op": c["op"], "case": c}
+    def write(k, v, length):
+        k, v, length = heads(k), heads(v), array(length)
+        torch.cuda.synchronize()  # the copies run on torch's stream
+        K.cache_write(st["cache"], st["table"], k, v, length=length)
+        ctx.synchronize()
+
     if c["op"] in ("cache", "attend"):
         st["cache"] = K.Cache8(ctx, d["table"].numel(), c["hk"], c["d"], c["block"])
         st["table"] = array(d["table"])
-    torch.cuda.synchronize()
     if c["op"] == "cache":
         n, rows = c["n"], _rows_back(c)
         if c["hist"]:
-            K.cache_write(st["cache"], st["table"], heads(d["k0"]), heads(d["v0"]), length=array(d["first"]))
+            write(d["k0"], d["v0"], d["first"])
         start = d["first"] // c["block"] * c["block"]
         out, st["view"] = outputs(k=E.DeviceArray(ctx, (n, rows, c["hk"], c["d"]), "f2" if c["f16"] else "f4"),
                                   v=E.DeviceArray(ctx, (n, rows, c["hk"], c["d"]), "f2" if c["f16"] else "f4"))
@@ -236,7 +241,7 @@ def _own_state(c, d):
                   back=array(d["first"] - start + c["tokens"]), k_out=Heads(out["k"], n, rows, c["hk"], c["d"]),
                   v_out=Heads(out["v"], n, rows, c["hk"], c["d"]))
     elif c["op"] == "attend":
-        K.cache_write(st["cache"], st["table"], heads(d["k"]), heads(d["v"]), length=array(d["kv_len"]))
+        write(d["k"], d["v"], d["kv_len"])
         out, st["view"] = outputs(out=E.DeviceArray(ctx, d["q"].shape, "f2" if c["f16"] else "f4"))
         st.update(q=heads(d["q"]), q_len=array(d["q_len"]), kv_len=array(d["kv_len"]), scale=d["scale"],
                   out=Heads(out["out"], c["n"], c["q"], c["hq"], c["d"]))
