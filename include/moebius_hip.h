@@ -621,12 +621,12 @@ int32_t mh_cache8_sizes(uint32_t pages, uint32_t heads, uint32_t d, uint32_t blo
 
 /* Token t < len[i] (NULL: tokens) of item i, row i * tokens + t of k and v, is held as token
  * first[i] + t (NULL: t); first and len are clamped to what the table has. The scale of a block
- * and head is the f32 value next to a / 127, a the largest finite magnitude among its new tokens;
- * where the block holds tokens before the first new one it is at least what it was, and if it grows
- * their codes are rounded to it. Codes are x / scale rounded to the nearest integer, ties to even:
- * off by at most half a scale for each time that they were rounded. Infinities are held as the
- * largest value of their sign, NaN and everything at a scale of 0 as 0. Tokens behind the last new
- * one in its block have no meaning afterwards. */
+ * and head is a * (1 / 127) in f32, a the largest finite magnitude among its new tokens; where the
+ * block holds tokens before the first new one it is at least what it was, and if it grows their
+ * codes are rounded to it. Codes are x / scale rounded to the nearest integer, ties to even: off by
+ * at most half a scale for each time that they were rounded. Infinities are held as the largest
+ * value of their sign, NaN and everything at a scale of 0 as 0. Tokens behind the last new one in
+ * its block have no meaning afterwards. */
 int32_t mh_cache8_write(MhContext *ctx, const MhCache8 *cache, const MhPageTable *table, const void *k, uint64_t ld_k,
                         const void *v, uint64_t ld_v, uint32_t dtype, uint32_t tokens, const int32_t *first,
                         const int32_t *len);

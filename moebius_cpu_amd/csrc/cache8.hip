@@ -2,8 +2,8 @@
 // read back.
 //
 // A block of tokens and a head of it share a scale: with a = max |x| over the block's finite
-// values, s = a / 127 rounded to f32 and the code is x / s rounded to the nearest integer (ties
-// to even), so a value is off by at most s / 2. Where a block holds tokens already, s is the
+// values, s = a (1 / 127) in f32 and the code is x / s rounded to the nearest integer (ties to
+// even), so a value is off by at most s / 2. Where a block holds tokens already, s is the
 // larger of its scale and the new tokens', and the codes it holds are rounded to the new one.
 // The quotient is rounded as if exact: c = rint(x * (1 / s)) is the nearest integer or one
 // beside it, x - c s is exact in f32 (fused; within s of zero, and a multiple of the smaller of
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void cache8_write_kernel(RowArgs a) {
         __syncthreads();
         for (int w = 0; w < nt / 64; ++w) mx = __builtin_fmaxf(mx, wave_max[w]);
     }
-    const float sc = __builtin_fmaxf(s0, mx / 127.0f);
+    const float sc = __builtin_fmaxf(s0, mx * (1.0f / 127.0f));
     const bool grown = held && sc > s0;
     // (the barrier above, or the wave's own order, lies between the reads of s0 and this store)
     if (tid == 0) *scale = sc;

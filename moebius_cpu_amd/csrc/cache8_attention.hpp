@@ -294,7 +294,9 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
                 for (int e = 0; e < 4; ++e) {
                     const float y = __builtin_amdgcn_exp2f(sc[n][t][e] - mu);
                     l[n] += y;
-                    const float z = y * vrel;
+                    float z = y * vrel;
+                    // (both parts are of z rounded to f32; a product fused with its conversion is not)
+                    if constexpr (PARTS == 2) asm("" : "+v"(z));
                     const _Float16 h = static_cast<_Float16>(z);
                     p[n][0][t / 2][(t % 2) * 4 + e] = h;
                     if constexpr (PARTS == 2) p[n][1][t / 2][(t % 2) * 4 + e] = static_cast<_Float16>(z - float(h));

@@ -64,7 +64,7 @@ class Held:
         for h in range(x.shape[1]):
             v = x[:, h].astype(np.float64)
             fine = np.isfinite(v)
-            s = F32(np.abs(v[fine]).max() if fine.any() else 0) / F32(127)
+            s = F32(np.abs(v[fine]).max() if fine.any() else 0) * (F32(1) / F32(127))
             if lo:
                 s0 = self.scale[which, page, h]
                 s = max(s, s0)
@@ -395,6 +395,13 @@ def test_scores_and_values_of_very_different_size(ctx, dtype, q):
     c.held.write(c.table, kv, [0], [512])
     c.run()
     c.check()
+
+
+def test_probabilities_in_two_parts(ctx):
+    """Few keys of nearly equal weight: no term of the bound hides a probability whose parts do not belong together."""
+    c = Case(ctx, F32, n=2, q=256, kv=64, hq=8, hk=4, d=32, block=16, causal=False)
+    c.run(scale=2.0 ** -6)
+    c.check(scale=2.0 ** -6)
 
 
 def test_queries_of_any_size(ctx):
