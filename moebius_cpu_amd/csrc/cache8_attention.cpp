@@ -14,24 +14,28 @@ int head_tiles(int d) {
 }
 
 struct Plan {
-    int nq, dt, row_tiles, splits;
+    int nq, waves, dt, row_tiles, splits;  // waves > 0: of 32 rows that share chunks in LDS, else nq tiles of 16 rows
     int64_t items;
     size_t bytes;
 };
 
-// The tokens are split over workgroups where the rows alone leave CUs idle, up to two workgroups
-// per CU and down to 256 tokens, a chunk for each wave.
 Plan plan(const Context &ctx, const Cache8Attention &a) {
     Plan p;
     const int64_t rows = int64_t(a.q_tokens) * (a.q.heads / a.c.heads);
     p.dt = head_tiles(a.c.d);
     p.nq = rows > 16 && p.dt <= 8 ? 2 : 1;
-    p.row_tiles = int(ceil_div(rows, 16 * p.nq));
+    p.waves = rows > 64 ? (rows > 128 && p.dt <= 8 ? 8 : 4) : 0;
+    const int tile = p.waves ? 32 * p.waves : 16 * p.nq;
+    p.row_tiles = int(ceil_div(rows, tile));
     p.items = int64_t(a.t.n) * a.c.heads * p.row_tiles;
     int64_t tokens = int64_t(a.t.blocks) << a.c.block_log;
     if (a.window) tokens = std::min(tokens, int64_t(a.window) + a.sinks + a.q_tokens);
-    p.splits = int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), 2 * int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1))));
-    p.bytes = p.splits > 1 ? size_t(p.items) * p.splits * p.nq * 16 * (p.dt * 16 + 2) * sizeof(float) : 0;
+    // The tokens are split over workgroups where the rows alone leave CUs idle, up to two workgroups
+    // per CU (one of waves that share) and down to 256 tokens.
+    const int64_t room = (p.waves ? 1 : 2) * int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1);
+    p.splits = int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), room)));
+    const int floats = (p.waves ? (p.dt + 1) / 2 * 32 : p.dt * 16) + 2;
+    p.bytes = p.splits > 1 ? size_t(p.items) * p.splits * tile * floats * sizeof(float) : 0;
     return p;
 }
 
@@ -56,9 +60,11 @@ void cache8_attention(Context &ctx, const Cache8Attention &c, void *scratch) {
     a.blocks = c.t.blocks, a.pages = c.c.pages, a.block_log = c.c.block_log;
     a.row_tiles = p.row_tiles, a.splits = p.splits, a.work = int(p.items * p.splits);
     a.causal = c.causal, a.window = c.window, a.sinks = c.sinks;
-    if (c.type == kF16) c8a::launch_f16(ctx, a, p.nq, p.dt);
-    else if (ctx.precision == Precision::Fast) c8a::launch_f32_half(ctx, a, p.nq, p.dt);
-    else c8a::launch_f32(ctx, a, p.nq, p.dt);
+    const int size = c.type == kF16 ? 2 : 4;
+    a.wide_out = c.c.d % 4 == 0 && c.ld_out % 4 == 0 && reinterpret_cast<uintptr_t>(c.out) % (4 * size) == 0;
+    if (c.type == kF16) c8a::launch_f16(ctx, a, p.nq, p.waves, p.dt);
+    else if (ctx.precision == Precision::Fast) c8a::launch_f32_half(ctx, a, p.nq, p.waves, p.dt);
+    else c8a::launch_f32(ctx, a, p.nq, p.waves, p.dt);
 }
 
 }  // namespace mh

@@ -32,6 +32,7 @@ struct Args {
     float c;      // scale . log2 e
     int n, q_tokens, hk, g, d, dp, blocks, pages, block_log, row_tiles, splits, work;
     int causal, window, sinks;
+    int wide_out;  // rows of out in vectors of four
 };
 
 // Eight codes as f16: a byte b in the low bits of 1024 is 1024 + b.
@@ -368,39 +369,359 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     }
 }
 
-// Joins the splits of a row: a wave per row.
-template <typename T, int DT, int NQ>
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// The value of lane +- 32.
+__device__ __forceinline__ float other_half(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// LDS of one staged chunk: keys [64][KS * 16] and values [KS * 16 rounded up to 32][64] as f16, rows
+// padded by 16 bytes (the rows of a read then lie on distinct banks), and the scales of its four
+// groups of 16 tokens.
+template <int KS>
+struct Stage {
+    static constexpr int kDT = (KS + 1) / 2;                   // tiles of 32 channels
+    static constexpr int kKS = KS * 16 + 8, kVS = kChunk + 8;  // halves of a row
+    static constexpr int kV = kChunk * kKS * 2, kMeta = kV + kDT * 32 * kVS * 2;
+    static constexpr int kBytes = kMeta + 32;
+};
+
+// Many rows per key head: W waves of 32 rows share chunks of 64 tokens, which are turned into f16
+// once, on their way into LDS, two buffers deep.
+//
+// S^T = K . Q^T and O^T = V^T . P^T on 32x32x16 instructions: a lane holds one row's scores (column
+// lane % 32), and with LDS row r of a half chunk holding token 16 (r / 4 % 2) + 4 (r / 8) + r % 4 they
+// are those of the 16 tokens of its half h = lane / 32: one block, one pair of scales, and the B
+// operand of the second product as they stand.
+template <typename T, int PARTS, int KS, int W>
+__global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void cache8_tiles_kernel(Args a) {
+    using L = Stage<KS>;
+    constexpr int DT = L::kDT, NT = 64 * W;
+    constexpr int kLazy = PARTS == 2 ? kLazySplit : kLazyHalf;
+    constexpr int U = (kChunk * KS + NT - 1) / NT;  // 16-byte runs of codes per thread, of keys and of values
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, h = lane >> 5;
+
+    const int per_xcd = (a.work + 7) / 8;
+    int w = int(blockIdx.x % 8) * per_xcd + int(blockIdx.x / 8);
+    if (int(blockIdx.x / 8) >= per_xcd || w >= a.work) return;
+    const int work = w;
+    const int split = w % a.splits;
+    w /= a.splits;
+    const int r0 = w % a.row_tiles * 32 * W;
+    w /= a.row_tiles;
+    const int hk = w % a.hk, item = w / a.hk;
+    const Range rg = range_of(a, item, r0, 32 * W);
+    if (r0 >= rg.rows) return;
+    const int share = (rg.chunks + a.splits - 1) / a.splits;
+    const int c0 = min(split * share, rg.chunks), c1 = min(c0 + share, rg.chunks);
+
+    // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of step c.
+    const int wrow = r0 + wave * 32, row = wrow + col;
+    const bool row_ok = row < rg.rows, rows_here = wrow < rg.rows;
+    const int t = (row_ok ? row : r0) / a.g, qh = hk * a.g + (row_ok ? row : r0) % a.g;
+    const int64_t row_at = int64_t(item) * a.q_tokens + t;
+    const T *qp = static_cast<const T *>(a.q) + row_at * a.ldq + int64_t(qh) * a.d;
+    halfx8 q[PARTS][KS];
+    float cq = a.c;
+    {
+        float x[KS][8];
+        float mx = 0.0f;
+        bool odd = false;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int ch = s * 16 + h * 8 + i;
+                const float v = ch < a.d ? float(qp[ch]) : 0.0f;
+                x[s][i] = v;
+                const bool fine = __builtin_fabsf(v) < __builtin_huge_valf();
+                odd = odd || !fine;
+                mx = fine ? __builtin_fmaxf(mx, __builtin_fabsf(v)) : mx;
+            }
+        int e = 0;
+        if constexpr (sizeof(T) == 4) {  // scaled by a power of two per row, so that no value leaves f16
+            mx = __builtin_fmaxf(mx, other_half(mx));
+            e = mx == 0.0f ? 0 : __builtin_amdgcn_frexp_expf(mx) - 1 - kSplitQ;
+            cq = ldexpf(a.c, e);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = sizeof(T) == 4 ? ldexpf(x[s][i], -e) : x[s][i];
+                q[0][s][i] = static_cast<_Float16>(y);
+                if constexpr (PARTS == 2) q[1][s][i] = static_cast<_Float16>(odd ? 0.0f : y - float(q[0][s][i]));
+            }
+    }
+    // The row sees tokens lo .. hi - 1 and those below min(hi, sinks); all rows of the wave those of
+    // lo_all .. hi_all - 1 and below min(hi_all, sinks), none those at or above hi_any.
+    const int at = t + rg.off, hi = a.causal ? min(rg.kv_len, at + 1) : rg.kv_len;
+    const int lo = a.window ? max(at - a.window + 1, 0) : 0;
+    const int t_first = wrow / a.g, t_last = (min(rg.rows, wrow + 32) - 1) / a.g;
+    const int hi_all = a.causal ? min(rg.kv_len, t_first + rg.off + 1) : rg.kv_len;
+    const int lo_all = a.window ? max(t_last + rg.off - a.window + 1, 0) : 0;
+    const int hi_any = a.causal ? min(rg.kv_len, t_last + rg.off + 1) : rg.kv_len;
+    const int lo_any = a.window ? max(t_first + rg.off - a.window + 1, 0) : 0;
+
+    // Channels behind dp of the staged keys: zeros, which the chunks never overwrite.
+    if (a.dp < KS * 16)
+        for (int i = tid; i < 2 * kChunk * 2; i += NT)
+            for (int ch = a.dp; ch < KS * 16; ch += 16)
+                *reinterpret_cast<uintx4 *>(smem + (i >= 2 * kChunk ? L::kBytes : 0) +
+                                            ((i / 2 % kChunk) * L::kKS + ch + i % 2 * 8) * 2) = uintx4{0, 0, 0, 0};
+
+    const int runs = a.dp / 16;  // 16-byte runs of a token's keys
+    const int64_t tile = int64_t(a.dp) << a.block_log;
+    const int block = 1 << a.block_log;
+    auto page_of = [&](int token, bool &ok) {
+        const int b = token >> a.block_log;
+        const int page = b < a.blocks ? a.table[int64_t(item) * a.blocks + b] : -1;
+        ok = page >= 0 && page < a.pages;
+        return (ok ? int64_t(page) : 0) * a.hk + hk;
+    };
+    uintx4 kr[U], vr[U];
+    float sr = 0.0f;  // threads 0 .. 7: the scales of keys, then of values, of the four groups; -1: no page
+    auto fetch = [&](int chunk) {
+        const int base = chunk * kChunk;
+        bool ok;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = tid + u * NT;
+            if (i < kChunk * runs) {
+                const int tk = i / runs, run = i - tk * runs, token = base + tk;
+                kr[u] = *reinterpret_cast<const uintx4 *>(a.k + page_of(token, ok) * tile + (token & (block - 1)) * a.dp + run * 16);
+                const int ch = i >> 2, tv = base + (i & 3) * 16;
+                vr[u] = *reinterpret_cast<const uintx4 *>(a.v + page_of(tv, ok) * tile + (ch << a.block_log) + (tv & (block - 1)));
+            }
+        }
+        if (tid < 8) {
+            const int tk = base + (tid & 3) * 16;
+            const int64_t p = page_of(tk, ok);
+            sr = ok && tk < rg.kv_len ? (tid < 4 ? a.ks : a.vs)[p] : -1.0f;
+        }
+    };
+    auto stage = [&](char *buf) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = tid + u * NT;
+            if (i < kChunk * runs) {
+                const int tk = i / runs, run = i - tk * runs;
+                const int j = tk & 31, r = (tk & 32) + 4 * (j >> 4) + 8 * ((j & 15) >> 2) + (j & 3);
+                halfx8 *kp = reinterpret_cast<halfx8 *>(buf + (r * L::kKS + run * 16) * 2);
+                kp[0] = halves(kr[u][0], kr[u][1]), kp[1] = halves(kr[u][2], kr[u][3]);
+                halfx8 *vp = reinterpret_cast<halfx8 *>(buf + L::kV + ((i >> 2) * L::kVS + (i & 3) * 16) * 2);
+                vp[0] = halves(vr[u][0], vr[u][1]), vp[1] = halves(vr[u][2], vr[u][3]);
+            }
+        }
+        if (tid < 8) reinterpret_cast<float *>(buf + L::kMeta)[tid] = sr;
+    };
+
+    floatx16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = kNegInf, l = 0.0f;
+    int ve = kNoExp, ve_max = kNoExp;
+
+    if (c0 < c1) {
+        fetch(rg.chunk(c0));
+        stage(smem);
+        if (c0 + 1 < c1) fetch(rg.chunk(c0 + 1));
+    }
+    __syncthreads();
+    for (int i = c0; i < c1; ++i) {
+        const char *const buf = smem + ((i - c0) & 1) * L::kBytes;
+        if (i + 1 < c1) {
+            stage(smem + ((i + 1 - c0) & 1) * L::kBytes);
+            if (i + 2 < c1) fetch(rg.chunk(i + 2));
+        }
+        const int base = rg.chunk(i) * kChunk;
+        if (rows_here && base < hi_any && (base + kChunk > lo_any || base < a.sinks)) {
+            const float *const meta = reinterpret_cast<const float *>(buf + L::kMeta);
+            const floatx4 v4 = *reinterpret_cast<const floatx4 *>(meta + 4);
+            floatx16 sc[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+                const char *p = buf + ((b * 32 + col) * L::kKS + h * 8) * 2;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const halfx8 k = *reinterpret_cast<const halfx8 *>(p + s * 32);
+                    if constexpr (PARTS == 2) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[1][s], sc[b], 0, 0, 0);
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[0][s], sc[b], 0, 0, 0);
+                }
+            }
+            // The sums' exponent follows the blocks' scales of values.
+            const float vmax = __builtin_fmaxf(__builtin_fmaxf(v4[0], v4[1]), __builtin_fmaxf(v4[2], v4[3]));
+            const int tv = __builtin_amdgcn_readfirstlane(vmax > 0.0f ? __builtin_amdgcn_frexp_expf(vmax) : kNoExp);
+            if (tv > ve || (tv > kNoExp && tv < ve - kBelow)) {
+                ve_max = max(ve_max, tv);
+                const int to = max(tv, ve_max - kDeepest);
+                if (to != ve) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[d][e] = ldexpf(o[d][e], ve - to);
+                    ve = to;
+                }
+            }
+            float ks[2], vrel[2];
+            bool there = true;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float v = h ? v4[2 * b + 1] : v4[2 * b];
+                vrel[b] = v > 0.0f ? ldexpf(v, (PARTS == 2 ? kSplitP : 0) - ve) : 0.0f;
+                // (0 times the smallest is 0, and a masked score stays -inf)
+                ks[b] = __builtin_fminf(__builtin_fmaxf(meta[2 * b + h] * cq, 0x1p-126f), 0x1.fffffep127f);
+                there = there && v >= 0.0f;
+            }
+            if (!(base + kChunk <= hi_all && (base >= lo_all || base + kChunk <= a.sinks)) || !__all(there)) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const bool page = (h ? v4[2 * b + 1] : v4[2 * b]) >= 0.0f;
+                    const int t0 = base + b * 32 + h * 16;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (!(page && t0 + e < hi && (t0 + e >= lo || t0 + e < a.sinks))) sc[b][e] = kNegInf;
+                }
+            }
+            float mx = kNegInf;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float x = sc[b][0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) x = __builtin_fmaxf(x, sc[b][e]);
+                mx = __builtin_fmaxf(mx, x * ks[b]);
+            }
+            mx = __builtin_fmaxf(mx, other_half(mx));
+            if (__any(mx > m + float(kLazy))) {
+                const float mn = __builtin_fmaxf(m, mx);
+                const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] *= f;
+                m = mn;
+            }
+            const float mu = m == kNegInf ? 0.0f : m;
+            // The fused exponent is off by half a step of m, which is nothing until scores are so large
+            // that the largest key's power would leave the range: their products are rounded first.
+            if (__any(__builtin_fabsf(mu) > 1048576.0f)) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sc[b][e] *= ks[b];
+                    ks[b] = 1.0f;
+                }
+            }
+            halfx8 p[PARTS][4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], ks[b], -mu));
+                    l += y;
+                    float z = y * vrel[b];
+                    // (both parts are of z rounded to f32; a product fused with its conversion is not)
+                    if constexpr (PARTS == 2) asm("" : "+v"(z));
+                    const _Float16 x = static_cast<_Float16>(z);
+                    p[0][2 * b + e / 8][e % 8] = x;
+                    if constexpr (PARTS == 2) p[1][2 * b + e / 8][e % 8] = static_cast<_Float16>(z - float(x));
+                }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const char *vp = buf + L::kV + (col * L::kVS + (s / 2) * 32 + h * 16 + (s % 2) * 8) * 2;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const halfx8 v = *reinterpret_cast<const halfx8 *>(vp + d * 32 * L::kVS * 2);
+                    if constexpr (PARTS == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[1][s], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[0][s], o[d], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (!row_ok) return;
+    l += other_half(l);
+    const int back = ve == kNoExp ? 0 : ve - (PARTS == 2 ? kSplitP : 0);
+    if (a.part) {
+        float *part = a.part + (int64_t(work) * 32 * W + wave * 32 + col) * (DT * 32 + 2);
+        if (h == 0) part[DT * 32] = m, part[DT * 32 + 1] = l;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) part[d * 32 + 8 * (e / 4) + 4 * h + e % 4] = ldexpf(o[d][e], back);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *op = static_cast<T *>(a.out) + row_at * a.ldo + int64_t(qh) * a.d;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            const int ch = d * 32 + 8 * f + 4 * h;
+            typedef T V4 __attribute__((ext_vector_type(4)));
+            V4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(ldexpf(o[d][4 * f + e], back) * inv);
+            if (a.wide_out) {
+                if (ch < a.d) *reinterpret_cast<V4 *>(op + ch) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (ch + e < a.d) op[ch + e] = v[e];
+            }
+        }
+}
+
+// Joins the splits of a row: a wave per row, TILE rows per workgroup of the split, PF floats of
+// sums each (then the maximum and the sum of the probabilities).
+template <typename T, int TILE, int PF>
 __global__ __launch_bounds__(64) void cache8_join_kernel(Args a) {
-    const int lane = threadIdx.x, col = blockIdx.x % (16 * NQ);
-    const int base = blockIdx.x / (16 * NQ);
+    const int lane = threadIdx.x, col = blockIdx.x % TILE;
+    const int base = blockIdx.x / TILE;
     int w = base;
-    const int r0 = w % a.row_tiles * 16 * NQ;
+    const int r0 = w % a.row_tiles * TILE;
     w /= a.row_tiles;
     const int hk = w % a.hk, item = w / a.hk;
     const int q_len = a.q_len ? min(max(a.q_len[item], 0), a.q_tokens) : a.q_tokens;
     const int row = r0 + col;
     if (row >= q_len * a.g) return;
-    constexpr int PF = DT * 16 + 2;
-    const float *p = a.part + (int64_t(base) * a.splits * NQ * 16 + col) * PF;
-    const int64_t step = int64_t(NQ) * 16 * PF;
+    const float *p = a.part + (int64_t(base) * a.splits * TILE + col) * (PF + 2);
+    const int64_t step = int64_t(TILE) * (PF + 2);
     float m = kNegInf;
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) m = __builtin_fmaxf(m, p[s * step + DT * 16]);
+    for (int s = 0; s < a.splits; ++s) m = __builtin_fmaxf(m, p[s * step + PF]);
     const float mu = m == kNegInf ? 0.0f : m;
-    float l = 0.0f, o[(DT * 16 + 63) / 64] = {};
+    float l = 0.0f, o[(PF + 63) / 64] = {};
 #pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(p[s * step + DT * 16] - mu);
-        l = __builtin_fmaf(p[s * step + DT * 16 + 1], f, l);
+        const float f = __builtin_amdgcn_exp2f(p[s * step + PF] - mu);
+        l = __builtin_fmaf(p[s * step + PF + 1], f, l);
 #pragma unroll
-        for (int i = 0; i < (DT * 16 + 63) / 64; ++i)
+        for (int i = 0; i < (PF + 63) / 64; ++i)
             if (i * 64 + lane < a.d) o[i] = __builtin_fmaf(p[s * step + i * 64 + lane], f, o[i]);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T *op = static_cast<T *>(a.out) + (int64_t(item) * a.q_tokens + row / a.g) * a.ldo + int64_t(hk * a.g + row % a.g) * a.d;
 #pragma unroll
-    for (int i = 0; i < (DT * 16 + 63) / 64; ++i)
+    for (int i = 0; i < (PF + 63) / 64; ++i)
         if (i * 64 + lane < a.d) op[i * 64 + lane] = static_cast<T>(o[i] * inv);
+}
+
+template <typename T, int TILE, int PF>
+void launch_join(Context &ctx, const Args &a) {
+    if (!a.part) return;
+    cache8_join_kernel<T, TILE, PF><<<dim3{uint32_t(a.work / a.splits * TILE)}, dim3{64}, 0, ctx.stream>>>(a);
+    MH_LAUNCH_CHECK();
 }
 
 template <typename T, int PARTS, int DT, int NQ>
@@ -410,30 +731,41 @@ void launch_rows(Context &ctx, const Args &a) {
     if (lds > 48 * 1024) HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
     cache8_rows_kernel<T, PARTS, DT, NQ><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{256}, lds, ctx.stream>>>(a);
     MH_LAUNCH_CHECK();
-    if (a.part) {
-        cache8_join_kernel<T, DT, NQ><<<dim3{uint32_t(a.work / a.splits * 16 * NQ)}, dim3{64}, 0, ctx.stream>>>(a);
-        MH_LAUNCH_CHECK();
-    }
+    launch_join<T, 16 * NQ, DT * 16>(ctx, a);
 }
 
+template <typename T, int PARTS, int KS, int W>
+void launch_tiles(Context &ctx, const Args &a) {
+    const size_t lds = 2 * Stage<KS>::kBytes;
+    const void *fn = reinterpret_cast<const void *>(&cache8_tiles_kernel<T, PARTS, KS, W>);
+    HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+    cache8_tiles_kernel<T, PARTS, KS, W><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{64 * W}, lds, ctx.stream>>>(a);
+    MH_LAUNCH_CHECK();
+    launch_join<T, 32 * W, Stage<KS>::kDT * 32>(ctx, a);
+}
+
+// dt: tiles of 16 channels as chosen by head_tiles; waves > 0: that many of 32 rows share a chunk.
 template <typename T, int PARTS>
-void launch_rows_dt(Context &ctx, const Args &a, int nq, int dt) {
-    auto by_nq = [&](auto n) {
+void launch_all(Context &ctx, const Args &a, int nq, int waves, int dt) {
+    auto by = [&](auto n) {
         constexpr int DT = decltype(n)::value;
-        if (nq == 1) launch_rows<T, PARTS, DT, 1>(ctx, a);
+        if constexpr (DT <= 8)
+            if (waves == 8) return launch_tiles<T, PARTS, DT, 8>(ctx, a);
+        if (waves) launch_tiles<T, PARTS, DT, 4>(ctx, a);
+        else if (nq == 1) launch_rows<T, PARTS, DT, 1>(ctx, a);
         else if constexpr (DT <= 8) launch_rows<T, PARTS, DT, 2>(ctx, a);
     };
-    if (dt == 4) by_nq(std::integral_constant<int, 4>{});
-    else if (dt == 5) by_nq(std::integral_constant<int, 5>{});
-    else if (dt == 6) by_nq(std::integral_constant<int, 6>{});
-    else if (dt == 8) by_nq(std::integral_constant<int, 8>{});
-    else if (dt == 10) by_nq(std::integral_constant<int, 10>{});
-    else by_nq(std::integral_constant<int, 16>{});
+    if (dt == 4) by(std::integral_constant<int, 4>{});
+    else if (dt == 5) by(std::integral_constant<int, 5>{});
+    else if (dt == 6) by(std::integral_constant<int, 6>{});
+    else if (dt == 8) by(std::integral_constant<int, 8>{});
+    else if (dt == 10) by(std::integral_constant<int, 10>{});
+    else by(std::integral_constant<int, 16>{});
 }
 
-void launch_f16(Context &ctx, const Args &a, int nq, int dt);
-void launch_f32(Context &ctx, const Args &a, int nq, int dt);
-void launch_f32_half(Context &ctx, const Args &a, int nq, int dt);
+void launch_f16(Context &ctx, const Args &a, int nq, int waves, int dt);
+void launch_f32(Context &ctx, const Args &a, int nq, int waves, int dt);
+void launch_f32_half(Context &ctx, const Args &a, int nq, int waves, int dt);
 
 }  // namespace c8a
 }  // namespace mh

@@ -4,7 +4,9 @@
 namespace mh {
 namespace c8a {
 
-void launch_f16(Context &ctx, const Args &a, int nq, int dt) { launch_rows_dt<_Float16, 1>(ctx, a, nq, dt); }
+void launch_f16(Context &ctx, const Args &a, int nq, int waves, int dt) {
+    launch_all<_Float16, 1>(ctx, a, nq, waves, dt);
+}
 
 }  // namespace c8a
 }  // namespace mh

@@ -4,7 +4,9 @@
 namespace mh {
 namespace c8a {
 
-void launch_f32(Context &ctx, const Args &a, int nq, int dt) { launch_rows_dt<float, 2>(ctx, a, nq, dt); }
+void launch_f32(Context &ctx, const Args &a, int nq, int waves, int dt) {
+    launch_all<float, 2>(ctx, a, nq, waves, dt);
+}
 
 }  // namespace c8a
 }  // namespace mh
