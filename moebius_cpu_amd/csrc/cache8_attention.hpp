@@ -32,7 +32,7 @@ struct Args {
     float c;      // scale . log2 e
     int n, q_tokens, hk, g, d, dp, blocks, pages, block_log, row_tiles, splits, work;
     int causal, window, sinks;
-    int wide_out;  // rows of out in vectors of four
+    int wide;  // rows of q in vectors of eight, of out in vectors of four
 };
 
 // Eight codes as f16: a byte b in the low bits of 1024 is 1024 + b.
@@ -81,6 +81,28 @@ constexpr int kNoExp = -1000;
 // that follows it down, and how far below the largest seen.
 constexpr int kBelow = 10, kDeepest = 80;
 constexpr int kSplitQ = 14;  // split queries are scaled to a largest value of 2^14 .. 2^15
+
+// Eight channels of a row of queries from ch on, zeros behind d.
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float (&x)[8]) {
+    typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr int kE = 16 / int(sizeof(T));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+    if (wide) {
+        if (ch < d)
+#pragma unroll
+            for (int j = 0; j < 8 / kE; ++j) {
+                const V v = reinterpret_cast<const V *>(p + ch)[j];
+#pragma unroll
+                for (int i = 0; i < kE; ++i) x[j * kE + i] = float(v[i]);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (ch + i < d) x[i] = float(p[ch + i]);
+    }
+}
 
 // Few rows per key head: a wave takes 16 * NQ rows and every fourth chunk of 64 tokens of its
 // workgroup's share, straight from memory into registers.
@@ -135,16 +157,15 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
         float mx = 0.0f;
         bool odd = false;
 #pragma unroll
-        for (int s = 0; s < DC * 2; ++s)
+        for (int s = 0; s < DC * 2; ++s) {
+            load8(qp[n], (s / 2) * 64 + g * 16 + (s % 2) * 8, a.d, a.wide, x[s]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int ch = (s / 2) * 64 + g * 16 + (s % 2) * 8 + i;
-                const float v = ch < a.d ? float(qp[n][ch]) : 0.0f;
-                x[s][i] = v;
-                const bool fine = __builtin_fabsf(v) < __builtin_huge_valf();
-                odd = odd || !fine;
-                mx = fine ? __builtin_fmaxf(mx, __builtin_fabsf(v)) : mx;
+                const float v = __builtin_fabsf(x[s][i]);
+                odd = odd || !(v < __builtin_huge_valf());
+                mx = v < __builtin_huge_valf() ? __builtin_fmaxf(mx, v) : mx;
             }
+        }
         int e = 0;
         if constexpr (sizeof(T) == 4) {  // scaled by a power of two per row, so that no value leaves f16
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
@@ -171,16 +192,20 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     int kch[DC];
 #pragma unroll
     for (int c = 0; c < DC; ++c) kch[c] = c * 64 + g * 16 < a.dp ? c * 64 + g * 16 : 0;
-    auto page_of = [&](int token, bool &ok) {
+    // Pages of the chunk that is loaded next, a chunk ahead of its codes: of the lane's key rows, of its group.
+    int kpage = -1, vpage = -1;
+    auto page_at = [&](int token) {
         const int b = token >> a.block_log;
         const int page = b < a.blocks ? a.table[int64_t(item) * a.blocks + b] : -1;
-        ok = page >= 0 && page < a.pages;
-        return (ok ? int64_t(page) : 0) * a.hk + hk;
+        return page >= 0 && page < a.pages ? page : -1;
+    };
+    auto next_pages = [&](int chunk) {
+        kpage = page_at(chunk * kChunk + 16 * (col >> 2));
+        vpage = page_at(chunk * kChunk + 16 * g);
     };
     auto load_k = [&](int chunk) {
         const int t0 = chunk * kChunk + 16 * (col >> 2);
-        bool ok;
-        const uint8_t *p = a.k + page_of(t0, ok) * tile + ((t0 & (block - 1)) + (col & 3)) * a.dp;
+        const uint8_t *p = a.k + (int64_t(max(kpage, 0)) * a.hk + hk) * tile + ((t0 & (block - 1)) + (col & 3)) * a.dp;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -188,8 +213,8 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     };
     auto load_v = [&](int chunk) {
         const int t0 = chunk * kChunk + 16 * g;
-        const int64_t at = page_of(t0, there);
-        there = there && t0 < rg.kv_len;  // (blocks behind it may never have been written)
+        const int64_t at = int64_t(max(vpage, 0)) * a.hk + hk;
+        there = vpage >= 0 && t0 < rg.kv_len;  // (blocks behind it may never have been written)
         ks = a.ks[at], vs = a.vs[at];
         const uint8_t *p = a.v + at * tile + (t0 & (block - 1)) + (col << a.block_log);
 #pragma unroll
@@ -208,7 +233,11 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     int ve = kNoExp, ve_max = kNoExp;  // the exponent that the sums are scaled by, and the largest seen
 
     int i = c0 + wave;
-    if (i < c1) load_k(rg.chunk(i)), load_v(rg.chunk(i));
+    if (i < c1) {
+        next_pages(rg.chunk(i));
+        load_k(rg.chunk(i)), load_v(rg.chunk(i));
+        next_pages(rg.chunk(i + 4));
+    }
     for (; i < c1; i += 4) {
         const int base = rg.chunk(i) * kChunk;
         floatx4 sc[NQ][4];
@@ -317,7 +346,10 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
                 }
             }
         }
-        if (more) load_v(rg.chunk(i + 4));
+        if (more) {
+            load_v(rg.chunk(i + 4));
+            next_pages(rg.chunk(i + 8));
+        }
     }
 
     // Scales taken back; the waves' sums joined in LDS, each wave then finishing some of them.
@@ -433,16 +465,15 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
         float mx = 0.0f;
         bool odd = false;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s) {
+            load8(qp, s * 16 + h * 8, a.d, a.wide, x[s]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int ch = s * 16 + h * 8 + i;
-                const float v = ch < a.d ? float(qp[ch]) : 0.0f;
-                x[s][i] = v;
-                const bool fine = __builtin_fabsf(v) < __builtin_huge_valf();
-                odd = odd || !fine;
-                mx = fine ? __builtin_fmaxf(mx, __builtin_fabsf(v)) : mx;
+                const float v = __builtin_fabsf(x[s][i]);
+                odd = odd || !(v < __builtin_huge_valf());
+                mx = v < __builtin_huge_valf() ? __builtin_fmaxf(mx, v) : mx;
             }
+        }
         int e = 0;
         if constexpr (sizeof(T) == 4) {  // scaled by a power of two per row, so that no value leaves f16
             mx = __builtin_fmaxf(mx, other_half(mx));
@@ -478,32 +509,27 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     const int runs = a.dp / 16;  // 16-byte runs of a token's keys
     const int64_t tile = int64_t(a.dp) << a.block_log;
     const int block = 1 << a.block_log;
-    auto page_of = [&](int token, bool &ok) {
-        const int b = token >> a.block_log;
+    // The page of group lane % 4 of the chunk that is fetched next, read a chunk ahead of its codes.
+    int pg = -1;
+    auto next_pages = [&](int chunk) {
+        const int b = (chunk * kChunk + (lane & 3) * 16) >> a.block_log;
         const int page = b < a.blocks ? a.table[int64_t(item) * a.blocks + b] : -1;
-        ok = page >= 0 && page < a.pages;
-        return (ok ? int64_t(page) : 0) * a.hk + hk;
+        pg = page >= 0 && page < a.pages ? page : -1;
     };
     uintx4 kr[U], vr[U];
     float sr = 0.0f;  // threads 0 .. 7: the scales of keys, then of values, of the four groups; -1: no page
     auto fetch = [&](int chunk) {
         const int base = chunk * kChunk;
-        bool ok;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = tid + u * NT;
-            if (i < kChunk * runs) {
-                const int tk = i / runs, run = i - tk * runs, token = base + tk;
-                kr[u] = *reinterpret_cast<const uintx4 *>(a.k + page_of(token, ok) * tile + (token & (block - 1)) * a.dp + run * 16);
-                const int ch = i >> 2, tv = base + (i & 3) * 16;
-                vr[u] = *reinterpret_cast<const uintx4 *>(a.v + page_of(tv, ok) * tile + (ch << a.block_log) + (tv & (block - 1)));
-            }
+            const int tk = min(i / runs, kChunk - 1), run = i % runs, tv = (i & 3) * 16, ch = min(i >> 2, a.dp - 1);
+            const int64_t kp = int64_t(max(__shfl(pg, tk >> 4), 0)) * a.hk + hk, vp = int64_t(max(__shfl(pg, i & 3), 0)) * a.hk + hk;
+            kr[u] = *reinterpret_cast<const uintx4 *>(a.k + kp * tile + ((base + tk) & (block - 1)) * a.dp + run * 16);
+            vr[u] = *reinterpret_cast<const uintx4 *>(a.v + vp * tile + (ch << a.block_log) + ((base + tv) & (block - 1)));
         }
-        if (tid < 8) {
-            const int tk = base + (tid & 3) * 16;
-            const int64_t p = page_of(tk, ok);
-            sr = ok && tk < rg.kv_len ? (tid < 4 ? a.ks : a.vs)[p] : -1.0f;
-        }
+        if (tid < 8)
+            sr = pg >= 0 && base + (tid & 3) * 16 < rg.kv_len ? (tid < 4 ? a.ks : a.vs)[int64_t(pg) * a.hk + hk] : -1.0f;
     };
     auto stage = [&](char *buf) {
 #pragma unroll
@@ -530,16 +556,20 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     int ve = kNoExp, ve_max = kNoExp;
 
     if (c0 < c1) {
+        next_pages(rg.chunk(c0));
         fetch(rg.chunk(c0));
+        next_pages(rg.chunk(c0 + 1));
         stage(smem);
-        if (c0 + 1 < c1) fetch(rg.chunk(c0 + 1));
+        fetch(rg.chunk(c0 + 1));
+        next_pages(rg.chunk(c0 + 2));
     }
     __syncthreads();
     for (int i = c0; i < c1; ++i) {
         const char *const buf = smem + ((i - c0) & 1) * L::kBytes;
         if (i + 1 < c1) {
             stage(smem + ((i + 1 - c0) & 1) * L::kBytes);
-            if (i + 2 < c1) fetch(rg.chunk(i + 2));
+            fetch(rg.chunk(i + 2));
+            next_pages(rg.chunk(i + 3));
         }
         const int base = rg.chunk(i) * kChunk;
         if (rows_here && base < hi_any && (base + kChunk > lo_any || base < a.sinks)) {
@@ -672,7 +702,7 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
             V4 v;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(ldexpf(o[d][4 * f + e], back) * inv);
-            if (a.wide_out) {
+            if (a.wide) {
                 if (ch < a.d) *reinterpret_cast<V4 *>(op + ch) = v;
             } else {
 #pragma unroll
