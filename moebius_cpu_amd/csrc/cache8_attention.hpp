@@ -7,6 +7,8 @@
 // instructions and the scales join outside of them: ks in the scores, vs in the probabilities.
 #pragma once
 
+#include <type_traits>
+
 #include "cache8.hpp"
 
 namespace mh {
@@ -80,6 +82,7 @@ constexpr int kNoExp = -1000;
 // How far a block's exponent of values may lie below the one that the sums are scaled by before
 // that follows it down, and how far below the largest seen.
 constexpr int kBelow = 10, kDeepest = 80;
+constexpr int kReadsAhead = 6;  // fragments of 16 bytes per lane on their way from LDS
 constexpr int kSplitQ = 14;  // split queries are scaled to a largest value of 2^14 .. 2^15
 
 // Eight channels of a row of queries from ch on, zeros behind d.
@@ -192,20 +195,20 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     int kch[DC];
 #pragma unroll
     for (int c = 0; c < DC; ++c) kch[c] = c * 64 + g * 16 < a.dp ? c * 64 + g * 16 : 0;
-    // Pages of the chunk that is loaded next, a chunk ahead of its codes: of the lane's key rows, of its group.
+    // Pages of the chunk that is loaded next, a chunk ahead of its codes: of the lane's key rows, of its
+    // group (looked at when they are used, not waited for where they are read).
     int kpage = -1, vpage = -1;
-    auto page_at = [&](int token) {
-        const int b = token >> a.block_log;
-        const int page = b < a.blocks ? a.table[int64_t(item) * a.blocks + b] : -1;
-        return page >= 0 && page < a.pages ? page : -1;
-    };
+    auto page_at = [&](int token) { return a.table[int64_t(item) * a.blocks + min(token >> a.block_log, a.blocks - 1)]; };
     auto next_pages = [&](int chunk) {
         kpage = page_at(chunk * kChunk + 16 * (col >> 2));
         vpage = page_at(chunk * kChunk + 16 * g);
     };
+    auto at_page = [&](int page) {
+        return int64_t(uint32_t(page) < uint32_t(a.pages) ? page : 0) * a.hk + hk;
+    };
     auto load_k = [&](int chunk) {
         const int t0 = chunk * kChunk + 16 * (col >> 2);
-        const uint8_t *p = a.k + (int64_t(max(kpage, 0)) * a.hk + hk) * tile + ((t0 & (block - 1)) + (col & 3)) * a.dp;
+        const uint8_t *p = a.k + at_page(kpage) * tile + ((t0 & (block - 1)) + (col & 3)) * a.dp;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -213,8 +216,8 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     };
     auto load_v = [&](int chunk) {
         const int t0 = chunk * kChunk + 16 * g;
-        const int64_t at = int64_t(max(vpage, 0)) * a.hk + hk;
-        there = vpage >= 0 && t0 < rg.kv_len;  // (blocks behind it may never have been written)
+        const int64_t at = at_page(vpage);
+        there = uint32_t(vpage) < uint32_t(a.pages) && t0 < rg.kv_len;  // (blocks behind it may never have been written)
         ks = a.ks[at], vs = a.vs[at];
         const uint8_t *p = a.v + at * tile + (t0 & (block - 1)) + (col << a.block_log);
 #pragma unroll
@@ -410,27 +413,60 @@ __device__ __forceinline__ float other_half(float x) {
     return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// LDS of one staged chunk: keys [64][KS * 16] and values [KS * 16 rounded up to 32][64] as f16, rows
-// padded by 16 bytes (the rows of a read then lie on distinct banks), and the scales of its four
-// groups of 16 tokens.
-template <int KS>
+// LDS of the staged chunks: keys [64][KS * 16] and values [KS * 16 rounded up to 32][64] as f16, rows
+// padded by 16 bytes (the rows of a read then lie on distinct banks), and the scales of each chunk's
+// four groups of 16 tokens; NB of each but three of the scales.
+template <int KS, int NB>
 struct Stage {
     static constexpr int kDT = (KS + 1) / 2;                   // tiles of 32 channels
     static constexpr int kKS = KS * 16 + 8, kVS = kChunk + 8;  // halves of a row
-    static constexpr int kV = kChunk * kKS * 2, kMeta = kV + kDT * 32 * kVS * 2;
-    static constexpr int kBytes = kMeta + 32;
+    static constexpr int kK = kChunk * kKS * 2, kV = kDT * 32 * kVS * 2;
+    static constexpr int kV0 = NB * kK, kMeta = kV0 + NB * kV, kBytes = kMeta + 3 * 32;
 };
 
+// Orders the MFMAs of a block and the reads from LDS that feed them, one for every PARTS: some reads ahead
+// of the first product, then one beside each (the compiler's own order waits for every second read).
+template <int MFMAS, int PARTS>
+__device__ __forceinline__ void feed() {
+    constexpr int kReads = MFMAS / PARTS, kFirst = kReads < kReadsAhead ? kReads : kReadsAhead;
+    __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0);
+        if (i + kFirst < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
+// Loads that are the same for all lanes, of memory that nothing writes while the kernel runs: through
+// the scalar unit.
+template <typename X>
+__device__ __forceinline__ X scalar_load(const X *p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) X *>(reinterpret_cast<uintptr_t>(p));
+}
+
 // Many rows per key head: W waves of 32 rows share chunks of 64 tokens, which are turned into f16
-// once, on their way into LDS, two buffers deep.
+// once, on their way into LDS.
 //
 // S^T = K . Q^T and O^T = V^T . P^T on 32x32x16 instructions: a lane holds one row's scores (column
 // lane % 32), and with LDS row r of a half chunk holding token 16 (r / 4 % 2) + 4 (r / 8) + r % 4 they
 // are those of the 16 tokens of its half h = lane / 32: one block, one pair of scales, and the B
 // operand of the second product as they stand.
-template <typename T, int PARTS, int KS, int W>
+//
+// A chunk takes two phases with a barrier behind each: the products (O^T of the chunk before, S^T of
+// this one), then the exponentials and the staging of chunks to come. Where W is 8, waves 4 .. 7 are
+// a phase behind, so that of the two waves of a SIMD one feeds the matrix unit while the other takes
+// the vector unit; keys are then staged two chunks ahead and values one, in three buffers, as the
+// waves behind still read one that the others are done with. Else one buffer is enough, and the
+// workgroups of a CU drift apart.
+//
+// WIDE: blocks of 64 or 128 tokens. A chunk then lies in one page and has one scale of keys and one of
+// values, which every wave reads through the scalar unit; else its four groups of 16 tokens have
+// their own, staged beside the codes.
+template <typename T, int PARTS, int KS, int W, bool WIDE>
 __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void cache8_tiles_kernel(Args a) {
-    using L = Stage<KS>;
+    constexpr bool TURNS = W == 8;
+    constexpr int NB = TURNS ? 3 : 1, AHEAD = TURNS ? 1 : 0;  // keys are staged AHEAD + 1 chunks ahead, values AHEAD
+    using L = Stage<KS, NB>;
     constexpr int DT = L::kDT, NT = 64 * W;
     constexpr int kLazy = PARTS == 2 ? kLazySplit : kLazyHalf;
     constexpr int U = (kChunk * KS + NT - 1) / NT;  // 16-byte runs of codes per thread, of keys and of values
@@ -450,11 +486,11 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     const Range rg = range_of(a, item, r0, 32 * W);
     if (r0 >= rg.rows) return;
     const int share = (rg.chunks + a.splits - 1) / a.splits;
-    const int c0 = min(split * share, rg.chunks), c1 = min(c0 + share, rg.chunks);
+    const int c0 = min(split * share, rg.chunks), n = min(c0 + share, rg.chunks) - c0;
 
     // Q^T: this lane's row, channels 16 c + 8 h .. + 7 of step c.
     const int wrow = r0 + wave * 32, row = wrow + col;
-    const bool row_ok = row < rg.rows, rows_here = wrow < rg.rows;
+    const bool row_ok = row < rg.rows;
     const int t = (row_ok ? row : r0) / a.g, qh = hk * a.g + (row_ok ? row : r0) % a.g;
     const int64_t row_at = int64_t(item) * a.q_tokens + t;
     const T *qp = static_cast<const T *>(a.q) + row_at * a.ldq + int64_t(qh) * a.d;
@@ -489,65 +525,105 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
                 if constexpr (PARTS == 2) q[1][s][i] = static_cast<_Float16>(odd ? 0.0f : y - float(q[0][s][i]));
             }
     }
-    // The row sees tokens lo .. hi - 1 and those below min(hi, sinks); all rows of the wave those of
-    // lo_all .. hi_all - 1 and below min(hi_all, sinks), none those at or above hi_any.
+    // The row sees tokens lo .. hi - 1 and those below min(hi, sinks), all rows of the wave those of
+    // lo_all .. hi_all - 1 and below min(hi_all, sinks).
     const int at = t + rg.off, hi = a.causal ? min(rg.kv_len, at + 1) : rg.kv_len;
     const int lo = a.window ? max(at - a.window + 1, 0) : 0;
-    const int t_first = wrow / a.g, t_last = (min(rg.rows, wrow + 32) - 1) / a.g;
+    const int t_first = wrow / a.g, t_last = max(min(rg.rows, wrow + 32) - 1, 0) / a.g;
     const int hi_all = a.causal ? min(rg.kv_len, t_first + rg.off + 1) : rg.kv_len;
     const int lo_all = a.window ? max(t_last + rg.off - a.window + 1, 0) : 0;
-    const int hi_any = a.causal ? min(rg.kv_len, t_last + rg.off + 1) : rg.kv_len;
-    const int lo_any = a.window ? max(t_first + rg.off - a.window + 1, 0) : 0;
 
     // Channels behind dp of the staged keys: zeros, which the chunks never overwrite.
     if (a.dp < KS * 16)
-        for (int i = tid; i < 2 * kChunk * 2; i += NT)
+        for (int i = tid; i < NB * kChunk * 2; i += NT)
             for (int ch = a.dp; ch < KS * 16; ch += 16)
-                *reinterpret_cast<uintx4 *>(smem + (i >= 2 * kChunk ? L::kBytes : 0) +
-                                            ((i / 2 % kChunk) * L::kKS + ch + i % 2 * 8) * 2) = uintx4{0, 0, 0, 0};
+                *reinterpret_cast<uintx4 *>(smem + ((i / 2) * L::kKS + ch + i % 2 * 8) * 2) = uintx4{0, 0, 0, 0};
 
     const int runs = a.dp / 16;  // 16-byte runs of a token's keys
-    const int64_t tile = int64_t(a.dp) << a.block_log;
+    const uint32_t tile = uint32_t(a.dp) << a.block_log;
     const int block = 1 << a.block_log;
-    // The page of group lane % 4 of the chunk that is fetched next, read a chunk ahead of its codes.
-    int pg = -1;
-    auto next_pages = [&](int chunk) {
-        const int b = (chunk * kChunk + (lane & 3) * 16) >> a.block_log;
-        const int page = b < a.blocks ? a.table[int64_t(item) * a.blocks + b] : -1;
-        pg = page >= 0 && page < a.pages ? page : -1;
+    // This thread's runs: token and channel of keys, channel and group of values, and their places in LDS
+    // (threads behind the last run repeat it).
+    int ktk[U], koff[U], kput[U], voff[U], vgrp[U], vput[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = min(tid + u * NT, kChunk * runs - 1);
+        const int tk = i / runs, run = i - tk * runs, j = tk & 31;
+        ktk[u] = tk, koff[u] = WIDE ? tk * a.dp + run * 16 : run * 16;
+        kput[u] = (((tk & 32) + 4 * (j >> 4) + 8 * ((j & 15) >> 2) + (j & 3)) * L::kKS + run * 16) * 2;
+        vgrp[u] = i & 3, voff[u] = ((i >> 2) << a.block_log) + (WIDE ? (i & 3) * 16 : 0);
+        vput[u] = ((i >> 2) * L::kVS + (i & 3) * 16) * 2;
+    }
+    // Pages are read a chunk or more ahead of the codes, and looked at when they are used, so that
+    // nothing waits for them. WIDE: of the chunks i + 1 .. i + AHEAD + 2 behind chunk i; else those of
+    // this thread's runs, and threads 0 .. 7's that of the scales of keys, then of values, of the groups.
+    int page[AHEAD + 2], kpg[U], vpg[U], spg = -1;
+    auto block_of = [&](int i, int group) {
+        return int64_t(item) * a.blocks + min((rg.chunk(c0 + i) * kChunk + group * 16) >> a.block_log, a.blocks - 1);
+    };
+    auto at_page = [&](int pg) {
+        return (uint32_t(pg) < uint32_t(a.pages) ? uint32_t(pg) : 0u) * uint32_t(a.hk) + uint32_t(hk);
+    };
+    auto pages_k = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) kpg[u] = a.table[block_of(i, ktk[u] >> 4)];
+        if (tid < 8) spg = a.table[block_of(i, tid & 3)];
+    };
+    auto pages_v = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) vpg[u] = a.table[block_of(i, vgrp[u])];
     };
     uintx4 kr[U], vr[U];
-    float sr = 0.0f;  // threads 0 .. 7: the scales of keys, then of values, of the four groups; -1: no page
-    auto fetch = [&](int chunk) {
-        const int base = chunk * kChunk;
+    float sr = 0.0f;  // -1: no page
+    auto fetch_k = [&](int i, int pg) {
+        const int base = rg.chunk(c0 + i) * kChunk;
+        if constexpr (WIDE) {
+            const uint8_t *p = a.k + uint64_t(at_page(pg)) * tile + uint32_t((base & (block - 1)) * a.dp);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = tid + u * NT;
-            const int tk = min(i / runs, kChunk - 1), run = i % runs, tv = (i & 3) * 16, ch = min(i >> 2, a.dp - 1);
-            const int64_t kp = int64_t(max(__shfl(pg, tk >> 4), 0)) * a.hk + hk, vp = int64_t(max(__shfl(pg, i & 3), 0)) * a.hk + hk;
-            kr[u] = *reinterpret_cast<const uintx4 *>(a.k + kp * tile + ((base + tk) & (block - 1)) * a.dp + run * 16);
-            vr[u] = *reinterpret_cast<const uintx4 *>(a.v + vp * tile + (ch << a.block_log) + ((base + tv) & (block - 1)));
+            for (int u = 0; u < U; ++u) kr[u] = *reinterpret_cast<const uintx4 *>(p + uint32_t(koff[u]));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                kr[u] = *reinterpret_cast<const uintx4 *>(a.k + uint64_t(at_page(kpg[u])) * tile +
+                                                          uint32_t(((base + ktk[u]) & (block - 1)) * a.dp + koff[u]));
+            if (tid < 8)
+                sr = uint32_t(spg) < uint32_t(a.pages) && base + (tid & 3) * 16 < rg.kv_len
+                         ? (tid < 4 ? a.ks : a.vs)[at_page(spg)] : -1.0f;
         }
-        if (tid < 8)
-            sr = pg >= 0 && base + (tid & 3) * 16 < rg.kv_len ? (tid < 4 ? a.ks : a.vs)[int64_t(pg) * a.hk + hk] : -1.0f;
     };
-    auto stage = [&](char *buf) {
+    auto fetch_v = [&](int i, int pg) {
+        const int base = rg.chunk(c0 + i) * kChunk;
+        if constexpr (WIDE) {
+            const uint8_t *p = a.v + uint64_t(at_page(pg)) * tile + uint32_t(base & (block - 1));
+#pragma unroll
+            for (int u = 0; u < U; ++u) vr[u] = *reinterpret_cast<const uintx4 *>(p + uint32_t(voff[u]));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                vr[u] = *reinterpret_cast<const uintx4 *>(a.v + uint64_t(at_page(vpg[u])) * tile +
+                                                          uint32_t(voff[u] + ((base + vgrp[u] * 16) & (block - 1))));
+        }
+    };
+    auto stage_k = [&](int i) {
+        char *const buf = smem + i % NB * L::kK;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = tid + u * NT;
-            if (i < kChunk * runs) {
-                const int tk = i / runs, run = i - tk * runs;
-                const int j = tk & 31, r = (tk & 32) + 4 * (j >> 4) + 8 * ((j & 15) >> 2) + (j & 3);
-                halfx8 *kp = reinterpret_cast<halfx8 *>(buf + (r * L::kKS + run * 16) * 2);
-                kp[0] = halves(kr[u][0], kr[u][1]), kp[1] = halves(kr[u][2], kr[u][3]);
-                halfx8 *vp = reinterpret_cast<halfx8 *>(buf + L::kV + ((i >> 2) * L::kVS + (i & 3) * 16) * 2);
-                vp[0] = halves(vr[u][0], vr[u][1]), vp[1] = halves(vr[u][2], vr[u][3]);
-            }
+            halfx8 *p = reinterpret_cast<halfx8 *>(buf + kput[u]);
+            p[0] = halves(kr[u][0], kr[u][1]), p[1] = halves(kr[u][2], kr[u][3]);
         }
-        if (tid < 8) reinterpret_cast<float *>(buf + L::kMeta)[tid] = sr;
+        if (!WIDE && tid < 8) reinterpret_cast<float *>(smem + L::kMeta)[i % 3 * 8 + tid] = sr;
+    };
+    auto stage_v = [&](int i) {
+        char *const buf = smem + L::kV0 + i % NB * L::kV;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            halfx8 *p = reinterpret_cast<halfx8 *>(buf + vput[u]);
+            p[0] = halves(vr[u][0], vr[u][1]), p[1] = halves(vr[u][2], vr[u][3]);
+        }
     };
 
-    floatx16 o[DT];
+    floatx16 o[DT], sc[2];
+    halfx8 p[PARTS][4];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -555,130 +631,225 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     float m = kNegInf, l = 0.0f;
     int ve = kNoExp, ve_max = kNoExp;
 
-    if (c0 < c1) {
-        next_pages(rg.chunk(c0));
-        fetch(rg.chunk(c0));
-        next_pages(rg.chunk(c0 + 1));
-        stage(smem);
-        fetch(rg.chunk(c0 + 1));
-        next_pages(rg.chunk(c0 + 2));
-    }
-    __syncthreads();
-    for (int i = c0; i < c1; ++i) {
-        const char *const buf = smem + ((i - c0) & 1) * L::kBytes;
-        if (i + 1 < c1) {
-            stage(smem + ((i + 1 - c0) & 1) * L::kBytes);
-            fetch(rg.chunk(i + 2));
-            next_pages(rg.chunk(i + 3));
+    auto scores = [&](int i) {
+        const char *const kp = smem + i % NB * L::kK + (col * L::kKS + h * 8) * 2;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const halfx8 k = *reinterpret_cast<const halfx8 *>(kp + b * 32 * L::kKS * 2 + s * 32);
+                if constexpr (PARTS == 2) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[1][s], sc[b], 0, 0, 0);
+                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[0][s], sc[b], 0, 0, 0);
+            }
+    };
+    auto values = [&](int i) {
+        const char *const vp = smem + L::kV0 + i % NB * L::kV + (col * L::kVS + h * 16) * 2;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const halfx8 v = *reinterpret_cast<const halfx8 *>(vp + ((s / 2) * 32 + (s % 2) * 8 + d * 32 * L::kVS) * 2);
+                if constexpr (PARTS == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[1][s], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[0][s], o[d], 0, 0, 0);
+            }
+    };
+    // What the chunk's scales make of its scores and probabilities, formed beside the products: the
+    // factor of the scores, the scales of values against the power of two of the sums (PARTS 1: the
+    // logarithm, so that it joins the exponent, and the inverse, which takes it out of the sum).
+    float ks[2], vrel[2], inv[2];
+    int shift = 0;       // how far that power of two moves
+    bool whole = false;  // every row of the wave sees all of the chunk
+    float ks_next = 0.0f, vs_next = 0.0f;  // WIDE: the scales of chunk i + 1
+    bool page_next = false;
+    bool page_here = false;
+    auto follow = [&](int tv) {
+        const bool go = tv > ve || (tv > kNoExp && tv < ve - kBelow);
+        ve_max = go ? max(ve_max, tv) : ve_max;
+        const int to = go ? max(tv, ve_max - kDeepest) : ve;
+        shift = ve - to;
+        ve = to;
+    };
+    auto factors = [&](int b, float k, float v) {
+        // (codes at a scale of 0 are 0: any factor will do)
+        const float x = v > 0.0f ? ldexpf(v, (PARTS == 2 ? kSplitP : 0) - ve) : 1.0f;
+        if constexpr (PARTS == 2) {
+            vrel[b] = x;
+        } else {
+            const float y = __builtin_fmaxf(x, 0x1p-90f);  // (values far below the largest count as nothing)
+            vrel[b] = __builtin_amdgcn_logf(y), inv[b] = __builtin_amdgcn_rcpf(y);
         }
-        const int base = rg.chunk(i) * kChunk;
-        if (rows_here && base < hi_any && (base + kChunk > lo_any || base < a.sinks)) {
-            const float *const meta = reinterpret_cast<const float *>(buf + L::kMeta);
-            const floatx4 v4 = *reinterpret_cast<const floatx4 *>(meta + 4);
-            floatx16 sc[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
-                const char *p = buf + ((b * 32 + col) * L::kKS + h * 8) * 2;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const halfx8 k = *reinterpret_cast<const halfx8 *>(p + s * 32);
-                    if constexpr (PARTS == 2) sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[1][s], sc[b], 0, 0, 0);
-                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[0][s], sc[b], 0, 0, 0);
-                }
-            }
-            // The sums' exponent follows the blocks' scales of values.
+        // (0 times the smallest is 0, and a masked score stays -inf)
+        ks[b] = __builtin_fminf(__builtin_fmaxf(k * cq, 0x1p-126f), 0x1.fffffep127f);
+    };
+    auto prepare = [&](int i) {
+        const int base = rg.chunk(c0 + i) * kChunk;
+        whole = base + kChunk <= hi_all && (base >= lo_all || base + kChunk <= a.sinks);
+        if constexpr (WIDE) {
+            const float v = page_next ? vs_next : 0.0f;
+            // the exponent as frexp gives it; below the normal range as at its end
+            follow(v > 0.0f ? max(int(__builtin_bit_cast(uint32_t, v) >> 23), 1) - 126 : kNoExp);
+            factors(0, ks_next, v);
+            ks[1] = ks[0], vrel[1] = vrel[0], inv[1] = inv[0];
+            page_here = page_next;
+            whole = whole && page_next;
+        } else {
+            const floatx4 *const meta = reinterpret_cast<const floatx4 *>(smem + L::kMeta) + i % 3 * 2;
+            const floatx4 k4 = meta[0], v4 = meta[1];
             const float vmax = __builtin_fmaxf(__builtin_fmaxf(v4[0], v4[1]), __builtin_fmaxf(v4[2], v4[3]));
-            const int tv = __builtin_amdgcn_readfirstlane(vmax > 0.0f ? __builtin_amdgcn_frexp_expf(vmax) : kNoExp);
-            if (tv > ve || (tv > kNoExp && tv < ve - kBelow)) {
-                ve_max = max(ve_max, tv);
-                const int to = max(tv, ve_max - kDeepest);
-                if (to != ve) {
+            const float vmin = __builtin_fminf(__builtin_fminf(v4[0], v4[1]), __builtin_fminf(v4[2], v4[3]));
+            follow(__builtin_amdgcn_readfirstlane(vmax > 0.0f ? __builtin_amdgcn_frexp_expf(vmax) : kNoExp));
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
+            for (int b = 0; b < 2; ++b) factors(b, h ? k4[2 * b + 1] : k4[2 * b], h ? v4[2 * b + 1] : v4[2 * b]);
+            whole = whole && __builtin_amdgcn_readfirstlane(vmin >= 0.0f);
+        }
+    };
+    bool far = false;
+    auto softmax = [&](int i) {
+        if (shift) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[d][e] = ldexpf(o[d][e], ve - to);
-                    ve = to;
-                }
-            }
-            float ks[2], vrel[2];
-            bool there = true;
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const float v = h ? v4[2 * b + 1] : v4[2 * b];
-                vrel[b] = v > 0.0f ? ldexpf(v, (PARTS == 2 ? kSplitP : 0) - ve) : 0.0f;
-                // (0 times the smallest is 0, and a masked score stays -inf)
-                ks[b] = __builtin_fminf(__builtin_fmaxf(meta[2 * b + h] * cq, 0x1p-126f), 0x1.fffffep127f);
-                there = there && v >= 0.0f;
-            }
-            if (!(base + kChunk <= hi_all && (base >= lo_all || base + kChunk <= a.sinks)) || !__all(there)) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const bool page = (h ? v4[2 * b + 1] : v4[2 * b]) >= 0.0f;
-                    const int t0 = base + b * 32 + h * 16;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (!(page && t0 + e < hi && (t0 + e >= lo || t0 + e < a.sinks))) sc[b][e] = kNegInf;
-                }
-            }
-            float mx = kNegInf;
+                for (int e = 0; e < 16; ++e) o[d][e] = ldexpf(o[d][e], shift);
+        }
+        if (!whole) {
+            const int base = rg.chunk(c0 + i) * kChunk;
+            const float *const v4 = reinterpret_cast<const float *>(smem + L::kMeta) + i % 3 * 8 + 4;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                float x = sc[b][0];
+                const bool there = WIDE ? page_here : v4[2 * b + h] >= 0.0f;
+                const int t0 = base + b * 32 + h * 16;
 #pragma unroll
-                for (int e = 1; e < 16; ++e) x = __builtin_fmaxf(x, sc[b][e]);
-                mx = __builtin_fmaxf(mx, x * ks[b]);
+                for (int e = 0; e < 16; ++e)
+                    if (!(there && t0 + e < hi && (t0 + e >= lo || t0 + e < a.sinks))) sc[b][e] = kNegInf;
             }
-            mx = __builtin_fmaxf(mx, other_half(mx));
-            if (__any(mx > m + float(kLazy))) {
-                const float mn = __builtin_fmaxf(m, mx);
-                const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
-                l *= f;
+        }
+        float mx[4];  // (several chains: a dependent instruction waits for twice its issue)
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+        for (int x = 0; x < 4; ++x) {
+            mx[x] = sc[x / 2][x % 2 * 8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[d][e] *= f;
-                m = mn;
-            }
-            const float mu = m == kNegInf ? 0.0f : m;
-            // The fused exponent is off by half a step of m, which is nothing until scores are so large
-            // that the largest key's power would leave the range: their products are rounded first.
-            if (__any(__builtin_fabsf(mu) > 1048576.0f)) {
+            for (int e = 1; e < 8; ++e) mx[x] = __builtin_fmaxf(mx[x], sc[x / 2][x % 2 * 8 + e]);
+        }
+        float top = __builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]) * ks[0], __builtin_fmaxf(mx[2], mx[3]) * ks[1]);
+        top = __builtin_fmaxf(top, other_half(top));
+        if (__any(top > m + float(kLazy))) {
+            const float mn = __builtin_fmaxf(m, top);
+            const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
+            l *= f;
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[b][e] *= ks[b];
-                    ks[b] = 1.0f;
-                }
-            }
-            halfx8 p[PARTS][4];
+                for (int e = 0; e < 16; ++e) o[d][e] *= f;
+            m = mn;
+            far = __any(__builtin_fabsf(m) > 1048576.0f && m != kNegInf);
+        }
+        const float mu = m == kNegInf ? 0.0f : m;
+        // The fused exponent is off by half a step of m, which is nothing until scores are so large
+        // that the largest key's power would leave the range: their products are rounded first.
+        if (far) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][e], ks[b], -mu));
-                    l += y;
-                    float z = y * vrel[b];
-                    // (both parts are of z rounded to f32; a product fused with its conversion is not)
-                    if constexpr (PARTS == 2) asm("" : "+v"(z));
-                    const _Float16 x = static_cast<_Float16>(z);
-                    p[0][2 * b + e / 8][e % 8] = x;
-                    if constexpr (PARTS == 2) p[1][2 * b + e / 8][e % 8] = static_cast<_Float16>(z - float(x));
-                }
+                for (int e = 0; e < 16; ++e) sc[b][e] = sc[b][e] * ks[b] - mu + (PARTS == 2 ? 0.0f : vrel[b]);
+        } else {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const char *vp = buf + L::kV + (col * L::kVS + (s / 2) * 32 + h * 16 + (s % 2) * 8) * 2;
+            for (int b = 0; b < 2; ++b) {
+                const float off = PARTS == 2 ? -mu : vrel[b] - mu;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const halfx8 v = *reinterpret_cast<const halfx8 *>(vp + d * 32 * L::kVS * 2);
-                    if constexpr (PARTS == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[1][s], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[0][s], o[d], 0, 0, 0);
-                }
+                for (int e = 0; e < 16; ++e) sc[b][e] = __builtin_fmaf(sc[b][e], ks[b], off);
             }
         }
+        float sum[4] = {};
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float y = __builtin_amdgcn_exp2f(sc[b][e]);
+                sum[2 * b + e % 2] += y;
+                float z = PARTS == 2 ? y * vrel[b] : y;
+                // (both parts are of z rounded to f32; a product fused with its conversion is not)
+                if constexpr (PARTS == 2) asm("" : "+v"(z));
+                const _Float16 x = static_cast<_Float16>(z);
+                p[0][2 * b + e / 8][e % 8] = x;
+                if constexpr (PARTS == 2) p[1][2 * b + e / 8][e % 8] = static_cast<_Float16>(z - float(x));
+            }
+        if constexpr (PARTS == 2) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        else l = __builtin_fmaf(sum[0] + sum[1], inv[0], __builtin_fmaf(sum[2] + sum[3], inv[1], l));
+    };
+
+    // What chunk i + 1 needs of the scales, and the page of a chunk to come.
+    auto scales = [&]() {
+        ks_next = scalar_load(a.ks + at_page(page[0])), vs_next = scalar_load(a.vs + at_page(page[0]));
+        page_next = uint32_t(page[0]) < uint32_t(a.pages);
+    };
+    if constexpr (WIDE) {
+        page[0] = scalar_load(a.table + block_of(0, 0));
+        scales();
+#pragma unroll
+        for (int x = 0; x < AHEAD + 2; ++x) page[x] = scalar_load(a.table + block_of(x, 0));  // (chunks 0 ..)
+    } else {
+        pages_k(0);
+        pages_v(0);
+    }
+    fetch_k(0, page[0]);
+    fetch_v(0, page[0]);
+    if constexpr (!WIDE) pages_k(1), pages_v(1);
+    stage_k(0);
+    fetch_k(1, page[1]);
+    if constexpr (!WIDE) pages_k(2);
+    if constexpr (TURNS) {
+        stage_v(0);
+        fetch_v(1, page[1]);
+        if constexpr (!WIDE) pages_v(2);
+        stage_k(1);
+        fetch_k(2, page[2]);
+        if constexpr (!WIDE) pages_k(3);
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int x = 0; x < AHEAD + 1; ++x) page[x] = page[x + 1];
+        page[AHEAD + 1] = scalar_load(a.table + block_of(AHEAD + 2, 0));
+    }
+    __syncthreads();
+    if (TURNS && wave >= 4) __syncthreads();
+    if (n > 0) {
+        scores(0);
+        feed<PARTS * 2 * KS, PARTS>();
+        prepare(0);
+    }
+    __syncthreads();
+    for (int i = 0; i < n; ++i) {
+        int page_new = -1;
+        if constexpr (WIDE) {
+            scales();
+            page_new = scalar_load(a.table + block_of(i + AHEAD + 3, 0));
+        }
+        softmax(i);
+        if (i + AHEAD + 1 < n) stage_k(i + AHEAD + 1);
+        if (i + AHEAD < n) stage_v(i + AHEAD);
+        fetch_v(i + AHEAD + 1, page[AHEAD]);
+        if constexpr (!WIDE) pages_v(i + AHEAD + 2);
+        fetch_k(i + AHEAD + 2, page[AHEAD + 1]);
+        if constexpr (!WIDE) pages_k(i + AHEAD + 3);
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int x = 0; x < AHEAD + 1; ++x) page[x] = page[x + 1];
+            page[AHEAD + 1] = page_new;
+        }
+        __syncthreads();
+        __builtin_amdgcn_s_setprio(1);
+        values(i);
+        scores(i + 1);  // (behind the last chunk: of what the buffer holds, and not used)
+        feed<PARTS * (4 * DT + 2 * KS), PARTS>();
+        __builtin_amdgcn_s_setprio(0);
+        if (i + 1 < n) prepare(i + 1);
         __syncthreads();
     }
+    if (TURNS && wave < 4) __syncthreads();
     if (!row_ok) return;
     l += other_half(l);
     const int back = ve == kNoExp ? 0 : ve - (PARTS == 2 ? kSplitP : 0);
@@ -691,7 +862,7 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
             for (int e = 0; e < 16; ++e) part[d * 32 + 8 * (e / 4) + 4 * h + e % 4] = ldexpf(o[d][e], back);
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
     T *op = static_cast<T *>(a.out) + row_at * a.ldo + int64_t(qh) * a.d;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -701,7 +872,7 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
             typedef T V4 __attribute__((ext_vector_type(4)));
             V4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(ldexpf(o[d][4 * f + e], back) * inv);
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(ldexpf(o[d][4 * f + e], back) * by);
             if (a.wide) {
                 if (ch < a.d) *reinterpret_cast<V4 *>(op + ch) = v;
             } else {
@@ -764,14 +935,16 @@ void launch_rows(Context &ctx, const Args &a) {
     launch_join<T, 16 * NQ, DT * 16>(ctx, a);
 }
 
-template <typename T, int PARTS, int KS, int W>
+template <typename T, int PARTS, int KS, int W, bool WIDE>
 void launch_tiles(Context &ctx, const Args &a) {
-    const size_t lds = 2 * Stage<KS>::kBytes;
-    const void *fn = reinterpret_cast<const void *>(&cache8_tiles_kernel<T, PARTS, KS, W>);
+    using L = Stage<KS, W == 8 ? 3 : 1>;
+    const size_t lds = L::kBytes;
+    static_assert(lds <= 160 * 1024, "chunks exceed the LDS");
+    const void *fn = reinterpret_cast<const void *>(&cache8_tiles_kernel<T, PARTS, KS, W, WIDE>);
     HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
-    cache8_tiles_kernel<T, PARTS, KS, W><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{64 * W}, lds, ctx.stream>>>(a);
+    cache8_tiles_kernel<T, PARTS, KS, W, WIDE><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{64 * W}, lds, ctx.stream>>>(a);
     MH_LAUNCH_CHECK();
-    launch_join<T, 32 * W, Stage<KS>::kDT * 32>(ctx, a);
+    launch_join<T, 32 * W, L::kDT * 32>(ctx, a);
 }
 
 // dt: tiles of 16 channels as chosen by head_tiles; waves > 0: that many of 32 rows share a chunk.
@@ -780,8 +953,9 @@ void launch_all(Context &ctx, const Args &a, int nq, int waves, int dt) {
     auto by = [&](auto n) {
         constexpr int DT = decltype(n)::value;
         if constexpr (DT <= 8)
-            if (waves == 8) return launch_tiles<T, PARTS, DT, 8>(ctx, a);
-        if (waves) launch_tiles<T, PARTS, DT, 4>(ctx, a);
+            if (waves == 8)
+                return a.block_log >= 6 ? launch_tiles<T, PARTS, DT, 8, true>(ctx, a) : launch_tiles<T, PARTS, DT, 8, false>(ctx, a);
+        if (waves) a.block_log >= 6 ? launch_tiles<T, PARTS, DT, 4, true>(ctx, a) : launch_tiles<T, PARTS, DT, 4, false>(ctx, a);
         else if (nq == 1) launch_rows<T, PARTS, DT, 1>(ctx, a);
         else if constexpr (DT <= 8) launch_rows<T, PARTS, DT, 2>(ctx, a);
     };

@@ -37,7 +37,7 @@ Held sizes(uint32_t pages, uint32_t heads, uint32_t d, uint32_t block) {
         mh::fail(mh::kInvalidArgument, "cache: block is 16, 32, 64 or 128");
     h.c.pages = dim(pages, "pages");
     h.c.heads = dim(heads, "heads");
-    if (uint64_t(pages) * heads >= (uint64_t(1) << 40)) mh::fail(mh::kInvalidArgument, "cache too large");
+    if (uint64_t(pages) * heads >= (uint64_t(1) << 31)) mh::fail(mh::kInvalidArgument, "cache too large");
     h.c.d = int(d);
     h.c.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
     h.codes = uint64_t(pages) * heads * block * h.c.dp();
