@@ -24,7 +24,7 @@ Plan plan(const Context &ctx, const Cache8Attention &a) {
     const int64_t rows = int64_t(a.q_tokens) * (a.q.heads / a.c.heads);
     p.dt = head_tiles(a.c.d);
     p.nq = rows > 16 && p.dt <= 8 ? 2 : 1;
-    p.waves = rows > 64 ? (rows > 128 && p.dt <= 8 ? 8 : 4) : 0;
+    p.waves = rows > 64 ? (rows > 128 && p.dt > 4 && p.dt <= 8 ? 8 : 4) : 0;
     const int tile = p.waves ? 32 * p.waves : 16 * p.nq;
     p.row_tiles = int(ceil_div(rows, tile));
     p.items = int64_t(a.t.n) * a.c.heads * p.row_tiles;

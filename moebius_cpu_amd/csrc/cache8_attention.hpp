@@ -414,14 +414,13 @@ __device__ __forceinline__ float other_half(float x) {
 }
 
 // LDS of the staged chunks: keys [64][KS * 16] and values [KS * 16 rounded up to 32][64] as f16, rows
-// padded by 16 bytes (the rows of a read then lie on distinct banks), and the scales of each chunk's
-// four groups of 16 tokens; NB of each but three of the scales.
+// padded by 16 bytes (the rows of a read then lie on distinct banks); NB of each.
 template <int KS, int NB>
 struct Stage {
     static constexpr int kDT = (KS + 1) / 2;                   // tiles of 32 channels
     static constexpr int kKS = KS * 16 + 8, kVS = kChunk + 8;  // halves of a row
     static constexpr int kK = kChunk * kKS * 2, kV = kDT * 32 * kVS * 2;
-    static constexpr int kV0 = NB * kK, kMeta = kV0 + NB * kV, kBytes = kMeta + 3 * 32;
+    static constexpr int kV0 = NB * kK, kBytes = kV0 + NB * kV;
 };
 
 // Orders the MFMAs of a block and the reads from LDS that feed them, one for every PARTS: some reads ahead
@@ -459,12 +458,13 @@ __device__ __forceinline__ X scalar_load(const X *p) {
 // waves behind still read one that the others are done with. Else one buffer is enough, and the
 // workgroups of a CU drift apart.
 //
-// WIDE: blocks of 64 or 128 tokens. A chunk then lies in one page and has one scale of keys and one of
-// values, which every wave reads through the scalar unit; else its four groups of 16 tokens have
-// their own, staged beside the codes.
+// WIDE: blocks of 64 or 128 tokens, so that a chunk lies in one page and has one scale of keys and one of
+// values, read through the scalar unit. Else its four groups of 16 tokens have their own: lane l
+// reads the page of group l % 4 and, of keys or (l & 4) of values, its scale.
 template <typename T, int PARTS, int KS, int W, bool WIDE>
-__global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void cache8_tiles_kernel(Args a) {
+__global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void cache8_tiles_kernel(Args a) {
     constexpr bool TURNS = W == 8;
+    constexpr int NP = WIDE ? 1 : 4;  // groups of tokens with a page of their own
     constexpr int NB = TURNS ? 3 : 1, AHEAD = TURNS ? 1 : 0;  // keys are staged AHEAD + 1 chunks ahead, values AHEAD
     using L = Stage<KS, NB>;
     constexpr int DT = L::kDT, NT = 64 * W;
@@ -554,54 +554,41 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
         vgrp[u] = i & 3, voff[u] = ((i >> 2) << a.block_log) + (WIDE ? (i & 3) * 16 : 0);
         vput[u] = ((i >> 2) * L::kVS + (i & 3) * 16) * 2;
     }
-    // Pages are read a chunk or more ahead of the codes, and looked at when they are used, so that
-    // nothing waits for them. WIDE: of the chunks i + 1 .. i + AHEAD + 2 behind chunk i; else those of
-    // this thread's runs, and threads 0 .. 7's that of the scales of keys, then of values, of the groups.
-    int page[AHEAD + 2], kpg[U], vpg[U], spg = -1;
-    auto block_of = [&](int i, int group) {
-        return int64_t(item) * a.blocks + min((rg.chunk(c0 + i) * kChunk + group * 16) >> a.block_log, a.blocks - 1);
+    // Pages of the chunks i + 1 .. i + AHEAD + 2 behind chunk i: read a chunk or more ahead of the codes,
+    // and looked at when they are used, so that nothing waits for them.
+    int page[AHEAD + 2];
+    auto read_page = [&](int i) {
+        const int base = rg.chunk(c0 + i) * kChunk + (WIDE ? 0 : (lane & 3) * 16);
+        const int32_t *p = a.table + int64_t(item) * a.blocks + min(base >> a.block_log, a.blocks - 1);
+        if constexpr (WIDE) return scalar_load(p);
+        else return *p;
     };
-    auto at_page = [&](int pg) {
-        return (uint32_t(pg) < uint32_t(a.pages) ? uint32_t(pg) : 0u) * uint32_t(a.hk) + uint32_t(hk);
-    };
-    auto pages_k = [&](int i) {
+    auto there = [&](int pg) { return uint32_t(pg) < uint32_t(a.pages); };
+    auto at_page = [&](int pg) { return (there(pg) ? uint32_t(pg) : 0u) * uint32_t(a.hk) + uint32_t(hk); };
+    // at_page of a thread's group
+    auto at_group = [&](int pg, int group) {
+        const uint32_t own = at_page(pg);
+        if constexpr (WIDE) return own;
+        uint32_t at = __builtin_amdgcn_readlane(own, 0);
 #pragma unroll
-        for (int u = 0; u < U; ++u) kpg[u] = a.table[block_of(i, ktk[u] >> 4)];
-        if (tid < 8) spg = a.table[block_of(i, tid & 3)];
-    };
-    auto pages_v = [&](int i) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) vpg[u] = a.table[block_of(i, vgrp[u])];
+        for (int x = 1; x < 4; ++x) at = group == x ? uint32_t(__builtin_amdgcn_readlane(own, x)) : at;
+        return at;
     };
     uintx4 kr[U], vr[U];
-    float sr = 0.0f;  // -1: no page
     auto fetch_k = [&](int i, int pg) {
         const int base = rg.chunk(c0 + i) * kChunk;
-        if constexpr (WIDE) {
-            const uint8_t *p = a.k + uint64_t(at_page(pg)) * tile + uint32_t((base & (block - 1)) * a.dp);
 #pragma unroll
-            for (int u = 0; u < U; ++u) kr[u] = *reinterpret_cast<const uintx4 *>(p + uint32_t(koff[u]));
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                kr[u] = *reinterpret_cast<const uintx4 *>(a.k + uint64_t(at_page(kpg[u])) * tile +
-                                                          uint32_t(((base + ktk[u]) & (block - 1)) * a.dp + koff[u]));
-            if (tid < 8)
-                sr = uint32_t(spg) < uint32_t(a.pages) && base + (tid & 3) * 16 < rg.kv_len
-                         ? (tid < 4 ? a.ks : a.vs)[at_page(spg)] : -1.0f;
+        for (int u = 0; u < U; ++u) {
+            const int off = WIDE ? (base & (block - 1)) * a.dp + koff[u] : ((base + ktk[u]) & (block - 1)) * a.dp + koff[u];
+            kr[u] = *reinterpret_cast<const uintx4 *>(a.k + uint64_t(at_group(pg, ktk[u] >> 4)) * tile + uint32_t(off));
         }
     };
     auto fetch_v = [&](int i, int pg) {
         const int base = rg.chunk(c0 + i) * kChunk;
-        if constexpr (WIDE) {
-            const uint8_t *p = a.v + uint64_t(at_page(pg)) * tile + uint32_t(base & (block - 1));
 #pragma unroll
-            for (int u = 0; u < U; ++u) vr[u] = *reinterpret_cast<const uintx4 *>(p + uint32_t(voff[u]));
-        } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                vr[u] = *reinterpret_cast<const uintx4 *>(a.v + uint64_t(at_page(vpg[u])) * tile +
-                                                          uint32_t(voff[u] + ((base + vgrp[u] * 16) & (block - 1))));
+        for (int u = 0; u < U; ++u) {
+            const int off = WIDE ? (base & (block - 1)) + voff[u] : ((base + vgrp[u] * 16) & (block - 1)) + voff[u];
+            vr[u] = *reinterpret_cast<const uintx4 *>(a.v + uint64_t(at_group(pg, vgrp[u])) * tile + uint32_t(off));
         }
     };
     auto stage_k = [&](int i) {
@@ -611,7 +598,6 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
             halfx8 *p = reinterpret_cast<halfx8 *>(buf + kput[u]);
             p[0] = halves(kr[u][0], kr[u][1]), p[1] = halves(kr[u][2], kr[u][3]);
         }
-        if (!WIDE && tid < 8) reinterpret_cast<float *>(smem + L::kMeta)[i % 3 * 8 + tid] = sr;
     };
     auto stage_v = [&](int i) {
         char *const buf = smem + L::kV0 + i % NB * L::kV;
@@ -663,9 +649,10 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     float ks[2], vrel[2], inv[2];
     int shift = 0;       // how far that power of two moves
     bool whole = false;  // every row of the wave sees all of the chunk
-    float ks_next = 0.0f, vs_next = 0.0f;  // WIDE: the scales of chunk i + 1
-    bool page_next = false;
-    bool page_here = false;
+    // The scales of chunk i + 1, and which of its groups have a page; then those of the chunk at hand.
+    float ks_next = 0.0f, vs_next = 0.0f;  // (WIDE alone)
+    float scale_next = 0.0f;               // (else: the lane's)
+    bool ok_next = false, ok[NP];
     auto follow = [&](int tv) {
         const bool go = tv > ve || (tv > kNoExp && tv < ve - kBelow);
         ve_max = go ? max(ve_max, tv) : ve_max;
@@ -688,24 +675,32 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     auto prepare = [&](int i) {
         const int base = rg.chunk(c0 + i) * kChunk;
         whole = base + kChunk <= hi_all && (base >= lo_all || base + kChunk <= a.sinks);
+        int tv = kNoExp;
+        float k[NP], v[NP];
         if constexpr (WIDE) {
-            const float v = page_next ? vs_next : 0.0f;
-            // the exponent as frexp gives it; below the normal range as at its end
-            follow(v > 0.0f ? max(int(__builtin_bit_cast(uint32_t, v) >> 23), 1) - 126 : kNoExp);
-            factors(0, ks_next, v);
-            ks[1] = ks[0], vrel[1] = vrel[0], inv[1] = inv[0];
-            page_here = page_next;
-            whole = whole && page_next;
+            ok[0] = ok_next;
+            k[0] = ok[0] ? ks_next : 0.0f, v[0] = ok[0] ? vs_next : 0.0f;
         } else {
-            const floatx4 *const meta = reinterpret_cast<const floatx4 *>(smem + L::kMeta) + i % 3 * 2;
-            const floatx4 k4 = meta[0], v4 = meta[1];
-            const float vmax = __builtin_fmaxf(__builtin_fmaxf(v4[0], v4[1]), __builtin_fmaxf(v4[2], v4[3]));
-            const float vmin = __builtin_fminf(__builtin_fminf(v4[0], v4[1]), __builtin_fminf(v4[2], v4[3]));
-            follow(__builtin_amdgcn_readfirstlane(vmax > 0.0f ? __builtin_amdgcn_frexp_expf(vmax) : kNoExp));
+            // (blocks behind the last token may never have been written)
+            const float x = ok_next && base + 16 * (lane & 3) < rg.kv_len ? scale_next : -1.0f;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) factors(b, h ? k4[2 * b + 1] : k4[2 * b], h ? v4[2 * b + 1] : v4[2 * b]);
-            whole = whole && __builtin_amdgcn_readfirstlane(vmin >= 0.0f);
+            for (int g = 0; g < NP; ++g) {
+                k[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), g));
+                v[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 4 + g));
+                ok[g] = __builtin_bit_cast(int, v[g]) >= 0;
+            }
         }
+#pragma unroll
+        for (int x = 0; x < NP; ++x) {
+            // the exponent as frexp gives it; below the normal range as at its end
+            const int bits = __builtin_bit_cast(int, v[x]);
+            tv = max(tv, bits > 0 ? max(bits >> 23, 1) - 126 : kNoExp);
+            whole = whole && ok[x];
+        }
+        follow(tv);
+        factors(0, h ? k[1 % NP] : k[0], h ? v[1 % NP] : v[0]);
+        if constexpr (WIDE) ks[1] = ks[0], vrel[1] = vrel[0], inv[1] = inv[0];
+        else factors(1, h ? k[3 % NP] : k[2 % NP], h ? v[3 % NP] : v[2 % NP]);
     };
     bool far = false;
     auto softmax = [&](int i) {
@@ -717,14 +712,13 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
         }
         if (!whole) {
             const int base = rg.chunk(c0 + i) * kChunk;
-            const float *const v4 = reinterpret_cast<const float *>(smem + L::kMeta) + i % 3 * 8 + 4;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const bool there = WIDE ? page_here : v4[2 * b + h] >= 0.0f;
+                const bool seen = h ? ok[(2 * b + 1) % NP] : ok[2 * b % NP];
                 const int t0 = base + b * 32 + h * 16;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (!(there && t0 + e < hi && (t0 + e >= lo || t0 + e < a.sinks))) sc[b][e] = kNegInf;
+                    if (!(seen && t0 + e < hi && (t0 + e >= lo || t0 + e < a.sinks))) sc[b][e] = kNegInf;
             }
         }
         float mx[4];  // (several chains: a dependent instruction waits for twice its issue)
@@ -781,39 +775,31 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
         else l = __builtin_fmaf(sum[0] + sum[1], inv[0], __builtin_fmaf(sum[2] + sum[3], inv[1], l));
     };
 
-    // What chunk i + 1 needs of the scales, and the page of a chunk to come.
-    auto scales = [&]() {
-        ks_next = scalar_load(a.ks + at_page(page[0])), vs_next = scalar_load(a.vs + at_page(page[0]));
-        page_next = uint32_t(page[0]) < uint32_t(a.pages);
+    auto scales = [&]() {  // of the chunk whose page is the first in line
+        const uint32_t at = at_page(page[0]);
+        if constexpr (WIDE) ks_next = scalar_load(a.ks + at), vs_next = scalar_load(a.vs + at);
+        else scale_next = (lane & 4 ? a.vs : a.ks)[at];
+        ok_next = there(page[0]);
     };
-    if constexpr (WIDE) {
-        page[0] = scalar_load(a.table + block_of(0, 0));
-        scales();
+    auto move_up = [&](int pg) {
 #pragma unroll
-        for (int x = 0; x < AHEAD + 2; ++x) page[x] = scalar_load(a.table + block_of(x, 0));  // (chunks 0 ..)
-    } else {
-        pages_k(0);
-        pages_v(0);
-    }
+        for (int j = 0; j < AHEAD + 1; ++j) page[j] = page[j + 1];
+        page[AHEAD + 1] = pg;
+    };
+#pragma unroll
+    for (int x = 0; x < AHEAD + 2; ++x) page[x] = read_page(x);  // (chunks 0 ..)
+    scales();
     fetch_k(0, page[0]);
     fetch_v(0, page[0]);
-    if constexpr (!WIDE) pages_k(1), pages_v(1);
     stage_k(0);
     fetch_k(1, page[1]);
-    if constexpr (!WIDE) pages_k(2);
     if constexpr (TURNS) {
         stage_v(0);
         fetch_v(1, page[1]);
-        if constexpr (!WIDE) pages_v(2);
         stage_k(1);
-        fetch_k(2, page[2]);
-        if constexpr (!WIDE) pages_k(3);
+        fetch_k(2, page[AHEAD + 1]);
     }
-    if constexpr (WIDE) {
-#pragma unroll
-        for (int x = 0; x < AHEAD + 1; ++x) page[x] = page[x + 1];
-        page[AHEAD + 1] = scalar_load(a.table + block_of(AHEAD + 2, 0));
-    }
+    move_up(read_page(AHEAD + 2));
     __syncthreads();
     if (TURNS && wave >= 4) __syncthreads();
     if (n > 0) {
@@ -823,23 +809,14 @@ __global__ __launch_bounds__(64 * W, (KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void
     }
     __syncthreads();
     for (int i = 0; i < n; ++i) {
-        int page_new = -1;
-        if constexpr (WIDE) {
-            scales();
-            page_new = scalar_load(a.table + block_of(i + AHEAD + 3, 0));
-        }
+        scales();
+        const int page_new = read_page(i + AHEAD + 3);
         softmax(i);
         if (i + AHEAD + 1 < n) stage_k(i + AHEAD + 1);
         if (i + AHEAD < n) stage_v(i + AHEAD);
         fetch_v(i + AHEAD + 1, page[AHEAD]);
-        if constexpr (!WIDE) pages_v(i + AHEAD + 2);
         fetch_k(i + AHEAD + 2, page[AHEAD + 1]);
-        if constexpr (!WIDE) pages_k(i + AHEAD + 3);
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int x = 0; x < AHEAD + 1; ++x) page[x] = page[x + 1];
-            page[AHEAD + 1] = page_new;
-        }
+        move_up(page_new);
         __syncthreads();
         __builtin_amdgcn_s_setprio(1);
         values(i);
