@@ -30,10 +30,12 @@ Plan plan(const Context &ctx, const Cache8Attention &a) {
     p.items = int64_t(a.t.n) * a.c.heads * p.row_tiles;
     int64_t tokens = int64_t(a.t.blocks) << a.c.block_log;
     if (a.window) tokens = std::min(tokens, int64_t(a.window) + a.sinks + a.q_tokens);
-    // The tokens are split over workgroups where the rows alone leave CUs idle, up to two workgroups
-    // per CU (one of waves that share) and down to 256 tokens.
-    const int64_t room = (p.waves ? 1 : 2) * int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1);
-    p.splits = int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), room)));
+    // The tokens are split over workgroups where the rows alone leave CUs idle, up to one workgroup per
+    // CU, into shares of 256 tokens or more, where there are more than 512. Single tokens, 32 heads over
+    // 8 of 128, f16, us with this rule and with up to two workgroups per CU: 8 items of 16384 tokens
+    // 52.0, 58.0, of 4096 22.7, 28.1, 1 of 16384 20.4, 29.9; 1 of 300 10.7 whole, 12.0 in two.
+    const int64_t room = int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1);
+    p.splits = tokens > 512 ? int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), room))) : 1;
     const int floats = (p.waves ? (p.dt + 1) / 2 * 32 : p.dt * 16) + 2;
     p.bytes = p.splits > 1 ? size_t(p.items) * p.splits * tile * floats * sizeof(float) : 0;
     return p;

@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
         }
         const float inv = a.part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
         float *part = a.part ? a.part + ((int64_t(work) * NQ + n) * 16 + col) * (DT * 16 + 2) : nullptr;
-        if (part && wave == 0 && g == 0) part[DT * 16] = top, part[DT * 16 + 1] = sum;
+        if (part && row_ok[n] && wave == 0 && g == 0) part[DT * 16] = top, part[DT * 16 + 1] = sum;
         T *op = static_cast<T *>(a.out) + row_at[n] * a.ldo + row_ch[n];
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
@@ -397,8 +397,9 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) y = __builtin_fmaf(joined[(x * kOut + (n * DT + t) * 4 + e) * 64 + lane], mw[x], y);
                 const int ch = t * 16 + 4 * g + e;
+                if (!row_ok[n]) continue;
                 if (part) part[ch] = y;
-                else if (row_ok[n] && ch < a.d) op[ch] = static_cast<T>(y * inv);
+                else if (ch < a.d) op[ch] = static_cast<T>(y * inv);
             }
         }
     }
@@ -860,12 +861,14 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
         }
 }
 
-// Joins the splits of a row: a wave per row, TILE rows per workgroup of the split, PF floats of
-// sums each (then the maximum and the sum of the probabilities).
+// Joins the splits of a row, TILE rows per workgroup of the split, PF floats of sums each (then the
+// maximum and the sum of the probabilities): a workgroup per row, every fourth split to a wave.
 template <typename T, int TILE, int PF>
-__global__ __launch_bounds__(64) void cache8_join_kernel(Args a) {
-    const int lane = threadIdx.x, col = blockIdx.x % TILE;
-    const int base = blockIdx.x / TILE;
+__global__ __launch_bounds__(256) void cache8_join_kernel(Args a) {
+    constexpr int C = (PF + 63) / 64;
+    __shared__ float joined[3][C][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = blockIdx.x % TILE, base = blockIdx.x / TILE;
     int w = base;
     const int r0 = w % a.row_tiles * TILE;
     w /= a.row_tiles;
@@ -876,29 +879,39 @@ __global__ __launch_bounds__(64) void cache8_join_kernel(Args a) {
     const float *p = a.part + (int64_t(base) * a.splits * TILE + col) * (PF + 2);
     const int64_t step = int64_t(TILE) * (PF + 2);
     float m = kNegInf;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) m = __builtin_fmaxf(m, p[s * step + PF]);
-    const float mu = m == kNegInf ? 0.0f : m;
-    float l = 0.0f, o[(PF + 63) / 64] = {};
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) {
-        const float f = __builtin_amdgcn_exp2f(p[s * step + PF] - mu);
-        l = __builtin_fmaf(p[s * step + PF + 1], f, l);
+    for (int s = lane; s < a.splits; s += 64) m = __builtin_fmaxf(m, p[s * step + PF]);
 #pragma unroll
-        for (int i = 0; i < (PF + 63) / 64; ++i)
+    for (int x = 1; x < 64; x *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, x));
+    const float mu = m == kNegInf ? 0.0f : m;
+    float l = 0.0f, o[C] = {};
+    for (int s = lane; s < a.splits; s += 64)
+        l = __builtin_fmaf(p[s * step + PF + 1], __builtin_amdgcn_exp2f(p[s * step + PF] - mu), l);
+#pragma unroll 4
+    for (int s = wave; s < a.splits; s += 4) {
+        const float f = __builtin_amdgcn_exp2f(p[s * step + PF] - mu);
+#pragma unroll
+        for (int i = 0; i < C; ++i)
             if (i * 64 + lane < a.d) o[i] = __builtin_fmaf(p[s * step + i * 64 + lane], f, o[i]);
     }
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+        if (wave) joined[wave - 1][i][lane] = o[i];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T *op = static_cast<T *>(a.out) + (int64_t(item) * a.q_tokens + row / a.g) * a.ldo + int64_t(hk * a.g + row % a.g) * a.d;
 #pragma unroll
-    for (int i = 0; i < (PF + 63) / 64; ++i)
-        if (i * 64 + lane < a.d) op[i * 64 + lane] = static_cast<T>(o[i] * inv);
+    for (int i = 0; i < C; ++i)
+        if (i * 64 + lane < a.d)
+            op[i * 64 + lane] = static_cast<T>((o[i] + joined[0][i][lane] + joined[1][i][lane] + joined[2][i][lane]) * inv);
 }
 
 template <typename T, int TILE, int PF>
 void launch_join(Context &ctx, const Args &a) {
     if (!a.part) return;
-    cache8_join_kernel<T, TILE, PF><<<dim3{uint32_t(a.work / a.splits * TILE)}, dim3{64}, 0, ctx.stream>>>(a);
+    cache8_join_kernel<T, TILE, PF><<<dim3{uint32_t(a.work / a.splits * TILE)}, dim3{256}, 0, ctx.stream>>>(a);
     MH_LAUNCH_CHECK();
 }
 
