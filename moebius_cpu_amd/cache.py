@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 
@@ -21,6 +22,8 @@ from .attention import Heads, _int32, _same
 from .engine import Context, DeviceArray, _ptr
 
 _I32 = np.dtype(np.int32)
+# _lib.PageTable and _lib.CacheAttention, packed: single tokens take no longer on the device than here.
+_TABLE, _SHAPE = struct.Struct("=Q2I").pack, struct.Struct("=6I2Q").pack
 
 
 class Cache8:
@@ -48,7 +51,7 @@ def _table(cache: Cache8, table: DeviceArray, n: int):
         raise MoebiusError(1, "table is int32 [n, blocks]")
     if table.ctx is not cache.ctx:
         raise MoebiusError(1, "table and cache of different contexts")
-    return ctypes.byref(_lib.PageTable(table.ptr, n, table.shape[1]))
+    return _TABLE(table.ptr, n, table.shape[1])
 
 
 def _rows(cache: Cache8, k: Heads, v: Heads):
@@ -90,12 +93,12 @@ def _shape(q: Heads, cache: Cache8, causal, window, sinks, q_len, kv_len):
         raise MoebiusError(1, "q and cache differ in channels")
     if q.ctx is not cache.ctx:
         raise MoebiusError(1, "heads and cache of different contexts")
-    if window < 0 or sinks < 0:
-        raise MoebiusError(1, "window and sinks are not negative")
+    if not (0 <= window < 1 << 32 and 0 <= sinks < 1 << 32):
+        raise MoebiusError(1, "window and sinks are not negative, and below 2^32")
     _int32(q_len, q.n, "q_len")
     _int32(kv_len, q.n, "kv_len")
-    return ctypes.byref(_lib.CacheAttention(q.tokens, q.heads, int(causal), int(window), int(sinks), 0, _ptr(q_len),
-                                            _ptr(kv_len)))
+    return _SHAPE(q.tokens, q.heads, bool(causal), int(window), int(sinks), 0, 0 if q_len is None else q_len.ptr,
+                  0 if kv_len is None else kv_len.ptr)
 
 
 def cache_attention(q: Heads, cache: Cache8, table: DeviceArray, out: Heads, scale: float | None = None,

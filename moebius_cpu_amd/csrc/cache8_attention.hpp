@@ -787,47 +787,49 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
         for (int j = 0; j < AHEAD + 1; ++j) page[j] = page[j + 1];
         page[AHEAD + 1] = pg;
     };
+    if (a.blocks > 0) {  // (without blocks there is no table either)
 #pragma unroll
-    for (int x = 0; x < AHEAD + 2; ++x) page[x] = read_page(x);  // (chunks 0 ..)
-    scales();
-    fetch_k(0, page[0]);
-    fetch_v(0, page[0]);
-    stage_k(0);
-    fetch_k(1, page[1]);
-    if constexpr (TURNS) {
-        stage_v(0);
-        fetch_v(1, page[1]);
-        stage_k(1);
-        fetch_k(2, page[AHEAD + 1]);
-    }
-    move_up(read_page(AHEAD + 2));
-    __syncthreads();
-    if (TURNS && wave >= 4) __syncthreads();
-    if (n > 0) {
-        scores(0);
-        feed<PARTS * 2 * KS, PARTS>();
-        prepare(0);
-    }
-    __syncthreads();
-    for (int i = 0; i < n; ++i) {
+        for (int x = 0; x < AHEAD + 2; ++x) page[x] = read_page(x);  // (chunks 0 ..)
         scales();
-        const int page_new = read_page(i + AHEAD + 3);
-        softmax(i);
-        if (i + AHEAD + 1 < n) stage_k(i + AHEAD + 1);
-        if (i + AHEAD < n) stage_v(i + AHEAD);
-        fetch_v(i + AHEAD + 1, page[AHEAD]);
-        fetch_k(i + AHEAD + 2, page[AHEAD + 1]);
-        move_up(page_new);
+        fetch_k(0, page[0]);
+        fetch_v(0, page[0]);
+        stage_k(0);
+        fetch_k(1, page[1]);
+        if constexpr (TURNS) {
+            stage_v(0);
+            fetch_v(1, page[1]);
+            stage_k(1);
+            fetch_k(2, page[AHEAD + 1]);
+        }
+        move_up(read_page(AHEAD + 2));
         __syncthreads();
-        __builtin_amdgcn_s_setprio(1);
-        values(i);
-        scores(i + 1);  // (behind the last chunk: of what the buffer holds, and not used)
-        feed<PARTS * (4 * DT + 2 * KS), PARTS>();
-        __builtin_amdgcn_s_setprio(0);
-        if (i + 1 < n) prepare(i + 1);
+        if (TURNS && wave >= 4) __syncthreads();
+        if (n > 0) {
+            scores(0);
+            feed<PARTS * 2 * KS, PARTS>();
+            prepare(0);
+        }
         __syncthreads();
+        for (int i = 0; i < n; ++i) {
+            scales();
+            const int page_new = read_page(i + AHEAD + 3);
+            softmax(i);
+            if (i + AHEAD + 1 < n) stage_k(i + AHEAD + 1);
+            if (i + AHEAD < n) stage_v(i + AHEAD);
+            fetch_v(i + AHEAD + 1, page[AHEAD]);
+            fetch_k(i + AHEAD + 2, page[AHEAD + 1]);
+            move_up(page_new);
+            __syncthreads();
+            __builtin_amdgcn_s_setprio(1);
+            values(i);
+            scores(i + 1);  // (behind the last chunk: of what the buffer holds, and not used)
+            feed<PARTS * (4 * DT + 2 * KS), PARTS>();
+            __builtin_amdgcn_s_setprio(0);
+            if (i + 1 < n) prepare(i + 1);
+            __syncthreads();
+        }
+        if (TURNS && wave < 4) __syncthreads();
     }
-    if (TURNS && wave < 4) __syncthreads();
     if (!row_ok) return;
     l += other_half(l);
     const int back = ve == kNoExp ? 0 : ve - (PARTS == 2 ? kSplitP : 0);

@@ -274,7 +274,7 @@ int32_t mh_gated_norm(MhContext *ctx, const MhGatedNorm *n) {
             if (!p) return;
             const Rows r = rows_of(p, count, 1, n->c, ld, mh::kF32, what);
             for (const Rows &o : out)
-                if (o.rows) no_overlap(r, o, (std::string(what) + " and x_out or y").c_str());
+                if (o.rows) no_overlap(r, o, "a vector and x_out or y");
         };
         vectors(n->gate, items, n->ld_gate, "gate");
         vectors(n->scale, items, n->ld_scale, "scale");

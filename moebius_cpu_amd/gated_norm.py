@@ -8,16 +8,18 @@
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import numpy as np
 
 from . import _lib
 from ._lib import MoebiusError, check, lib
 from .attention import Heads
-from .engine import DeviceArray, _ptr
+from .engine import DeviceArray
 
 _F32 = np.dtype(np.float32)
+# _lib.GatedNorm, packed: a call of few rows takes no longer on the device than here.
+_PACK = struct.Struct("=4Q4Q2I2QIfIf2QIf2Q3Q3Q").pack
 
 
 class Norm:
@@ -31,13 +33,10 @@ class Norm:
             if a is not None and a.dtype != _F32:
                 raise MoebiusError(1, "gamma and beta are f32 of the row's channels")
         self.gamma, self.beta = gamma, beta
-        self.c = _lib.Norm(_lib.NORM[kind], float(eps), _ptr(gamma), _ptr(beta))
-
-    def _of(self, c):
-        for a in (self.gamma, self.beta):
-            if a is not None and a.nbytes != 4 * c:
-                raise MoebiusError(1, "gamma and beta are f32 of the row's channels")
-        return self.c
+        self._c = None if gamma is None and beta is None else (gamma if beta is None else beta).nbytes // 4
+        if gamma is not None and beta is not None and gamma.nbytes != beta.nbytes:
+            raise MoebiusError(1, "gamma and beta are f32 of the row's channels")
+        self._args = (_lib.NORM[kind], float(eps), 0 if gamma is None else gamma.ptr, 0 if beta is None else beta.ptr)
 
 
 _NONE = Norm()
@@ -49,30 +48,51 @@ def gated_norm(x: Heads, branch: Heads | None = None, post: Norm | None = None, 
     """s = keep x + gate post(branch) (no branch: s = x), x_out = s, y = pre(s) (1 + scale) + shift, over rows
     of all heads * d channels of x. gate, scale and shift: f32 views of one row [1, c] per item. x_out has
     x's type, y the branch's; an output may be an input of its type."""
-    n, rows, c = x.n, x.rows, x.heads * x.d
-    for a in (branch, x_out, y):
-        if a is None:
-            continue
-        if (a.n, a.tokens, a.heads * a.d) != (n, x.tokens, c):
+    ctx, n, tokens, c = x.ctx, x.n, x.tokens, x.heads * x.d
+    bp = bl = op = ol = yp = yl = gp = gl = sp = sl = hp = hl = 0
+    code = x.code
+    if y is not None:
+        yp, yl, code = y.buf.ptr + y._offset, y.ld, y.code
+        if y.n != n or y.tokens != tokens or y.heads * y.d != c:
             raise MoebiusError(1, "x, branch, x_out and y differ in shape")
-        if a.ctx is not x.ctx:
+        if y.ctx is not ctx:
             raise MoebiusError(1, "rows of different contexts")
-    if x_out is not None and x_out.code != x.code:
-        raise MoebiusError(1, "x and x_out differ in type")
-    if branch is not None and y is not None and branch.code != y.code:
-        raise MoebiusError(1, "branch and y differ in type")
-    for a in (gate, scale, shift):
-        if a is not None and ((a.n, a.tokens, a.heads * a.d) != (n, 1, c) or a.code != _lib.DTYPE_F32):
-            raise MoebiusError(1, "gate, scale and shift are f32 [n, 1, c]")
-    other = branch if branch is not None else y
-
-    def at(a):
-        return (None, 0) if a is None else (a.ptr, a.ld)
-
-    (bp, bl), (xp, xl), (yp, yl) = at(branch), at(x_out), at(y)
-    (gp, gl), (sp, sl), (hp, hl) = at(gate), at(scale), at(shift)
-    st = lib().mh_gated_norm(x.ctx.h, ctypes.byref(_lib.GatedNorm(
-        x.ptr, bp, xp, yp, x.ld, bl, xl, yl, x.code, x.code if other is None else other.code, rows, max(x.tokens, 1), c,
-        float(keep), (post or _NONE)._of(c), (pre or _NONE)._of(c), gp, sp, hp, gl, sl, hl)))
+    if branch is not None:
+        bp, bl = branch.buf.ptr + branch._offset, branch.ld
+        if branch.n != n or branch.tokens != tokens or branch.heads * branch.d != c:
+            raise MoebiusError(1, "x, branch, x_out and y differ in shape")
+        if branch.ctx is not ctx:
+            raise MoebiusError(1, "rows of different contexts")
+        if y is not None and branch.code != code:
+            raise MoebiusError(1, "branch and y differ in type")
+        code = branch.code
+    if x_out is not None:
+        op, ol = x_out.buf.ptr + x_out._offset, x_out.ld
+        if x_out.n != n or x_out.tokens != tokens or x_out.heads * x_out.d != c:
+            raise MoebiusError(1, "x, branch, x_out and y differ in shape")
+        if x_out.ctx is not ctx:
+            raise MoebiusError(1, "rows of different contexts")
+        if x_out.code != x.code:
+            raise MoebiusError(1, "x and x_out differ in type")
+    if gate is not None:
+        gp, gl = _vector(gate, n, c, ctx)
+    if scale is not None:
+        sp, sl = _vector(scale, n, c, ctx)
+    if shift is not None:
+        hp, hl = _vector(shift, n, c, ctx)
+    post = _NONE if post is None else post
+    pre = _NONE if pre is None else pre
+    if (post._c is not None and post._c != c) or (pre._c is not None and pre._c != c):
+        raise MoebiusError(1, "gamma and beta are f32 of the row's channels")
+    st = lib().mh_gated_norm(ctx.h, _PACK(x.buf.ptr + x._offset, bp, op, yp, x.ld, bl, ol, yl, x.code, code, n * tokens,
+                                          tokens or 1, c, keep, *post._args, *pre._args, gp, sp, hp, gl, sl, hl))
     if st:
         check(st)
+
+
+def _vector(a, n, c, ctx):
+    if a.n != n or a.tokens != 1 or a.heads * a.d != c or a.code != _lib.DTYPE_F32:
+        raise MoebiusError(1, "gate, scale and shift are f32 [n, 1, c]")
+    if a.ctx is not ctx:
+        raise MoebiusError(1, "rows of different contexts")
+    return a.buf.ptr + a._offset, a.ld
