@@ -75,6 +75,13 @@ __device__ __forceinline__ Range range_of(const Args &a, int item, int r0, int t
     return r;
 }
 
+// Which of the sixteen tokens from t0 on a row sees that sees lo .. hi - 1 and those below sinks and hi:
+// bits, as branches of every token's own cost more than a chunk's products.
+__device__ __forceinline__ uint32_t seen_bits(int t0, int lo, int hi, int sinks) {
+    auto below = [&](int limit) { return (1u << min(max(limit - t0, 0), 16)) - 1u; };
+    return below(hi) & (~below(lo) | below(sinks));
+}
+
 // Exponents of two by which a row's maximum may pass its reference: probabilities of up to
 // 2^kLazy times a scale below 1 fit f16, split ones with 2^kSplitP more.
 constexpr int kLazyHalf = 8, kLazySplit = 3, kSplitP = 11;
@@ -296,13 +303,11 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sc[n][t][e] *= c;
             if (!__all(whole)) {
+                const uint32_t bits = there_now ? seen_bits(t0, lo[n], hi[n], a.sinks) : 0u;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = t0 + 4 * t + e;
-                        if (!(there_now && j < hi[n] && (j >= lo[n] || j < a.sinks))) sc[n][t][e] = kNegInf;
-                    }
+                    for (int e = 0; e < 4; ++e) sc[n][t][e] = bits & (1u << (4 * t + e)) ? sc[n][t][e] : kNegInf;
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -715,11 +720,10 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
             const int base = rg.chunk(c0 + i) * kChunk;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const bool seen = h ? ok[(2 * b + 1) % NP] : ok[2 * b % NP];
-                const int t0 = base + b * 32 + h * 16;
+                const bool page = h ? ok[(2 * b + 1) % NP] : ok[2 * b % NP];
+                const uint32_t bits = page ? seen_bits(base + b * 32 + h * 16, lo, hi, a.sinks) : 0u;
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!(seen && t0 + e < hi && (t0 + e >= lo || t0 + e < a.sinks))) sc[b][e] = kNegInf;
+                for (int e = 0; e < 16; ++e) sc[b][e] = bits & (1u << e) ? sc[b][e] : kNegInf;
             }
         }
         float mx[4];  // (several chains: a dependent instruction waits for twice its issue)
