@@ -380,6 +380,16 @@ def test_attention_fast(case):
     ctx.close()
 
 
+@pytest.mark.parametrize("n,q,kv_len", [(5, 1, [4000, 0, 1, 700, 3999]), (64, 1, list(range(1, 641, 10))), (65, 1, list(range(0, 650, 10))),
+                                        (3, 3, [2, 1500, 64]), (2, 1, [0, 0]), (33, 2, [2000] + 32 * [5])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (600, 70)])
+def test_lengths_far_apart(ctx, n, q, kv_len, window, sinks):
+    """Single tokens of items whose caches are empty, short and long: shares of very different numbers."""
+    c = Case(ctx, np.float16, n=n, q=q, kv=4096 if n < 64 else 1024, hq=2, hk=1, d=40, block=64, kv_len=kv_len, window=window, sinks=sinks)
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("q", [1, 150])
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 def test_scores_and_values_of_very_different_size(ctx, dtype, q):
