@@ -24,17 +24,25 @@ Plan plan(const Context &ctx, const Cache8Attention &a) {
     const int64_t rows = int64_t(a.q_tokens) * (a.q.heads / a.c.heads);
     p.dt = head_tiles(a.c.d);
     p.nq = rows > 16 && p.dt <= 8 ? 2 : 1;
-    p.waves = rows > 64 ? (rows > 128 && p.dt > 4 && p.dt <= 8 ? 8 : 4) : 0;
+    int64_t tokens = int64_t(a.t.blocks) << a.c.block_log;
+    if (a.window) tokens = std::min(tokens, int64_t(a.window) + a.sinks + a.q_tokens);
+    // Waves that share chunks: eight, or four where there are few rows, heads of 64 (of which a CU then
+    // holds three workgroups) or heads that three buffers of LDS do not hold. They pay where they fill
+    // the card or the tokens are many: 32 heads over 8 of 128, f16, us of both ways: 256 queries over
+    // 2000 tokens 39.6, alone 24.1; 1000 over 1000 68, 53; 8 items of 24 over 16384 107, 118; of 64
+    // over 4000 70, 75.
+    const int waves = rows > 128 && p.dt > 4 && p.dt <= 8 ? 8 : 4;
+    const int64_t fill = int64_t(a.t.n) * a.c.heads * ceil_div(rows, 32 * waves);
+    p.waves = rows > 64 && (4 * fill >= 3 * ctx.cu_count || tokens > 4096) ? waves : 0;
     const int tile = p.waves ? 32 * p.waves : 16 * p.nq;
     p.row_tiles = int(ceil_div(rows, tile));
     p.items = int64_t(a.t.n) * a.c.heads * p.row_tiles;
-    int64_t tokens = int64_t(a.t.blocks) << a.c.block_log;
-    if (a.window) tokens = std::min(tokens, int64_t(a.window) + a.sinks + a.q_tokens);
     // The tokens are split over workgroups where the rows alone leave CUs idle, up to one workgroup per
-    // CU, into shares of 256 tokens or more, where there are more than 512. Single tokens, 32 heads over
-    // 8 of 128, f16, us with this rule and with up to two workgroups per CU: 8 items of 16384 tokens
-    // 52.0, 58.0, of 4096 22.7, 28.1, 1 of 16384 20.4, 29.9; 1 of 300 10.7 whole, 12.0 in two.
-    const int64_t room = int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1);
+    // CU (two of four waves that share), into shares of 256 tokens or more, where there are more than
+    // 512. Single tokens, 32 heads over 8 of 128, f16, us with this rule and with up to two workgroups
+    // per CU: 8 items of 16384 tokens 51.6, 57.4, of 4096 22.7, 28.1; 1 of 300 10.7 whole, 12.0 in two.
+    // 8 items of 24 tokens in workgroups of four waves: 107 with two, 125 with one, 120 with three.
+    const int64_t room = (p.waves == 4 && p.dt <= 8 ? 2 : 1) * int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1);
     p.splits = tokens > 512 ? int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), room))) : 1;
     const int floats = (p.waves ? (p.dt + 1) / 2 * 32 : p.dt * 16) + 2;
     p.bytes = p.splits > 1 ? size_t(p.items) * p.splits * tile * floats * sizeof(float) : 0;

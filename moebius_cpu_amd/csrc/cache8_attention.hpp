@@ -114,7 +114,7 @@ __device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float
     }
 }
 
-// Few rows per key head: a wave takes 16 * NQ rows and every fourth chunk of 64 tokens of its
+// Few rows per key head: a wave takes 16 * NQ rows and every WV-th chunk of 64 tokens of its
 // workgroup's share, straight from memory into registers.
 //
 // S^T = K . Q^T on 16x16x32 instructions: a lane holds row lane % 16 of the queries and, with key
@@ -123,12 +123,12 @@ __device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float
 // stand, and their values one load of 16 bytes from a channel's row; keys are 16 bytes of a
 // token's row as two steps of the instruction. A block holds whole groups of 16 tokens, so page,
 // scales and whether the page is there are the lane's own.
-template <typename T, int PARTS, int DT, int NQ>
-__global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
+template <typename T, int PARTS, int DT, int NQ, int WV>
+__global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) {
     constexpr int DC = (DT + 3) / 4;  // chunks of 64 channels
     constexpr int kLazy = PARTS == 2 ? kLazySplit : kLazyHalf;
     constexpr int kOut = NQ * DT * 4 + NQ * 2;  // floats of a lane's partial: sums, then m and l
-    extern __shared__ float joined[];           // [4][kOut][64]
+    extern __shared__ float joined[];           // [WV][kOut][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
 
@@ -246,9 +246,9 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     if (i < c1) {
         next_pages(rg.chunk(i));
         load_k(rg.chunk(i)), load_v(rg.chunk(i));
-        next_pages(rg.chunk(i + 4));
+        next_pages(rg.chunk(i + WV));
     }
-    for (; i < c1; i += 4) {
+    for (; i < c1; i += WV) {
         const int base = rg.chunk(i) * kChunk;
         floatx4 sc[NQ][4];
 #pragma unroll
@@ -267,10 +267,10 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
                 }
             }
         }
-        const bool more = i + 4 < c1;
+        const bool more = i + WV < c1;
         const float ks_now = ks, vs_now = vs;
         const bool there_now = there;
-        if (more) load_k(rg.chunk(i + 4));
+        if (more) load_k(rg.chunk(i + WV));
 
         // The sums' exponent follows the blocks' scales of values.
         int tv = there_now && vs_now > 0.0f ? __builtin_amdgcn_frexp_expf(vs_now) : kNoExp;
@@ -355,8 +355,8 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
             }
         }
         if (more) {
-            load_v(rg.chunk(i + 4));
-            next_pages(rg.chunk(i + 8));
+            load_v(rg.chunk(i + WV));
+            next_pages(rg.chunk(i + 2 * WV));
         }
     }
 
@@ -377,15 +377,15 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        float mw[4], top = kNegInf, sum = 0.0f;
+        float mw[WV], top = kNegInf, sum = 0.0f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < WV; ++x) {
             mw[x] = joined[(x * kOut + NQ * DT * 4 + 2 * n) * 64 + lane];
             top = __builtin_fmaxf(top, mw[x]);
         }
         const float mu = top == kNegInf ? 0.0f : top;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < WV; ++x) {
             mw[x] = __builtin_amdgcn_exp2f(mw[x] - mu);
             sum = __builtin_fmaf(joined[(x * kOut + NQ * DT * 4 + 2 * n + 1) * 64 + lane], mw[x], sum);
         }
@@ -395,12 +395,12 @@ __global__ __launch_bounds__(256) void cache8_rows_kernel(Args a) {
         T *op = static_cast<T *>(a.out) + row_at[n] * a.ldo + row_ch[n];
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-            if (t % 4 != wave || t * 16 >= a.d) continue;
+            if (t % WV != wave || t * 16 >= a.d) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float y = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) y = __builtin_fmaf(joined[(x * kOut + (n * DT + t) * 4 + e) * 64 + lane], mw[x], y);
+                for (int x = 0; x < WV; ++x) y = __builtin_fmaf(joined[(x * kOut + (n * DT + t) * 4 + e) * 64 + lane], mw[x], y);
                 const int ch = t * 16 + 4 * g + e;
                 if (!row_ok[n]) continue;
                 if (part) part[ch] = y;
@@ -923,10 +923,13 @@ void launch_join(Context &ctx, const Args &a) {
 
 template <typename T, int PARTS, int DT, int NQ>
 void launch_rows(Context &ctx, const Args &a) {
-    const size_t lds = size_t(4) * (NQ * DT * 4 + NQ * 2) * 64 * 4;
-    const void *fn = reinterpret_cast<const void *>(&cache8_rows_kernel<T, PARTS, DT, NQ>);
+    // Two waves per SIMD where 256 registers hold one. Single tokens, 8 items of up to 16384 tokens, 32
+    // heads over 8 of 128: f16 45.8 us with eight, 51.6 with four, f32 48.0, 57.1; of 256: 240, 134.
+    constexpr int WV = DT == 16 || (PARTS == 2 && NQ == 2 && DT == 8) ? 4 : 8;
+    const size_t lds = size_t(WV) * (NQ * DT * 4 + NQ * 2) * 64 * 4;
+    const void *fn = reinterpret_cast<const void *>(&cache8_rows_kernel<T, PARTS, DT, NQ, WV>);
     if (lds > 48 * 1024) HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
-    cache8_rows_kernel<T, PARTS, DT, NQ><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{256}, lds, ctx.stream>>>(a);
+    cache8_rows_kernel<T, PARTS, DT, NQ, WV><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{64 * WV}, lds, ctx.stream>>>(a);
     MH_LAUNCH_CHECK();
     launch_join<T, 16 * NQ, DT * 16>(ctx, a);
 }
