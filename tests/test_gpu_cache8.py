@@ -370,7 +370,32 @@ def test_attention(ctx, dtype, case):
     c.check()
 
 
-@pytest.mark.parametrize("case", CASES[1:5] + CASES[9:11])
+# Rows enough to fill the card, so that waves share chunks: four waves (up to 128 rows of a key head, heads
+# of 64 channels or of more than 128), and eight.
+SHARED = [
+    *(dict(n=64, q=70, kv=80, hq=4, hk=4, d=d, block=b, causal=c) for d, b, c in (
+        (33, 16, True), (64, 64, False), (80, 32, True), (128, 128, True), (160, 16, False), (256, 64, True))),
+    dict(n=64, q=35, kv=200, hq=8, hk=4, d=64, block=32, window=40, sinks=20, q_len=[35, 0, 7, 35] * 16, kv_len=[200, 90, 131, 35] * 16),
+    dict(n=64, q=90, kv=150, hq=4, hk=4, d=96, block=64, window=64, absent=[(3, 1), (5, 0), (5, 1), (5, 2)], pad=8, offset=8),
+    *(dict(n=32, q=130, kv=200, hq=8, hk=8, d=d, block=b, causal=c, window=w, sinks=s) for d, b, c, w, s in (
+        (72, 16, True, 0, 0), (80, 64, True, 100, 9), (96, 32, False, 50, 70), (112, 128, True, 1, 0), (128, 64, True, 0, 0))),
+    dict(n=32, q=70, kv=260, hq=16, hk=8, d=128, block=16, q_len=[70, 1, 33, 70] * 8, kv_len=[260, 1, 200, 70] * 8, absent=[(0, 3), (2, 0)]),
+    dict(n=32, q=140, kv=64, hq=8, hk=8, d=65, block=64, pad=1, offset=1, kv_len=[64, 0, 1, 63] * 8, q_len=[140, 140, 1, 63] * 8),
+    # few rows over many tokens: split
+    dict(n=1, q=80, kv=4200, hq=2, hk=2, d=64, block=64, kv_len=[4001]), dict(n=2, q=90, kv=4500, hq=2, hk=1, d=80, block=32, kv_len=[4500, 333]),
+    dict(n=1, q=200, kv=5000, hq=1, hk=1, d=128, block=128, window=4100, sinks=30), dict(n=2, q=70, kv=4200, hq=1, hk=1, d=200, block=16, kv_len=[700, 0]),
+]
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: "-".join(str(c[k]) for k in ("n", "q", "kv", "hk", "d", "block")))
+def test_attention_of_many_rows(ctx, dtype, case):
+    c = Case(ctx, dtype, **case)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("case", CASES[1:5] + CASES[9:11] + SHARED[1:4] + SHARED[9:12])
 def test_attention_fast(case):
     ctx = E.Context(0)
     ctx.set_precision(True)
@@ -390,12 +415,33 @@ def test_lengths_far_apart(ctx, n, q, kv_len, window, sinks):
     c.check()
 
 
-@pytest.mark.parametrize("q", [1, 150])
+@pytest.mark.parametrize("n,q,d", [(1, 1, 64), (2, 9, 80), (64, 70, 64), (32, 130, 128)])
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
-def test_scores_and_values_of_very_different_size(ctx, dtype, q):
+def test_scores_beyond_any_exponent(ctx, dtype, n, q, d):
+    """Scores of 10^7 and more: each row is the value of its largest key, where the next one is far behind."""
+    h = 1 if n < 32 else 4 if n == 64 else 8
+    c = Case(ctx, dtype, n=n, q=q, kv=200, hq=h, hk=h, d=d, block=64, causal=False)
+    c.run(scale=1e6)
+    got = c.out.numpy().astype(np.float64)
+    checked = 0
+    for i in range(n):
+        k, v = (c.held.values(w, c.table, i, 200)[0] for w in (0, 1))
+        for x in range(h):
+            s = 1e6 * c.qh[i, :, x].astype(np.float64) @ k[:, x].T
+            two = np.sort(s, 1)[:, -2:]
+            far = two[:, 1] - two[:, 0] > 1e-5 * np.abs(s).max(1) + 100  # beyond the f32 sums' own error
+            want = v[s.argmax(1), x]
+            assert np.all(np.abs(got[i, far, x] - want[far]) <= 2.0 ** (-10 if dtype == np.float16 else -20) * np.abs(want[far]) + 1e-7)
+            checked += far.sum()
+    assert checked >= 0.9 * n * q * h
+
+
+@pytest.mark.parametrize("q,cap", [(1, 512), (150, 512), (150, 4200)])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_scores_and_values_of_very_different_size(ctx, dtype, q, cap):
     """Values of blocks 2^20 apart, keys that make the softmax nearly one token, queries with a few large channels."""
     r = np.random.default_rng(5)
-    c = Case(ctx, dtype, n=1, q=q, kv=512, hq=2, hk=2, d=64, block=16)
+    c = Case(ctx, dtype, n=1, q=q, kv=cap, hq=2, hk=2, d=64, block=16, kv_len=[512])
     size = np.exp2(np.where(np.arange(32) % 5 == 1, -14, 0) + np.where(np.arange(32) % 7 == 3, 6, 0))
     kv = [np.repeat(r.choice([0.25, 30.0], 32), 16)[None, :, None, None] * r.standard_normal((1, 512, 2, 64)),
           np.repeat(size, 16)[None, :, None, None] * r.standard_normal((1, 512, 2, 64))]
@@ -414,9 +460,10 @@ def test_probabilities_in_two_parts(ctx):
     c.check(scale=2.0 ** -6)
 
 
-def test_queries_of_any_size(ctx):
+@pytest.mark.parametrize("q,cap", [(8, 200), (80, 4200)])
+def test_queries_of_any_size(ctx, q, cap):
     """f32 queries far outside f16 in both directions, and rows that are not finite beside others."""
-    c = Case(ctx, F32, n=1, q=8, kv=200, hq=1, hk=1, d=64, block=64, causal=False)
+    c = Case(ctx, F32, n=1, q=q, kv=cap, hq=1, hk=1, d=64, block=64, causal=False, kv_len=[200])
     for i, e in enumerate([-126, -60, -20, 0, 10]):
         c.qh[0, i] = (c.qh[0, i].astype(np.float64) * 2.0 ** e).astype(F32)
     c.qh[0, 5] = np.nan
@@ -426,11 +473,12 @@ def test_queries_of_any_size(ctx):
     c.run()
     got = c.out.numpy()
     assert np.isnan(got[0, 5:7]).all()
-    want, tol = attention64(c.qh[:, [0, 1, 2, 3, 4, 7]], c.held, c.table, 0.125, False, 0, 0, [6], [200])
-    assert np.all(np.abs(got[0, [0, 1, 2, 3, 4, 7]] - want[0]) <= tol[0])
+    rows = [i for i in range(q) if i not in (5, 6)]
+    want, tol = attention64(c.qh[:, rows], c.held, c.table, 0.125, False, 0, 0, [len(rows)], [200])
+    assert np.all(np.abs(got[0, rows] - want[0]) <= tol[0])
 
 
-@pytest.mark.parametrize("q,kv", [(1, 3000), (200, 1000)])
+@pytest.mark.parametrize("q,kv", [(1, 3000), (200, 1000), (100, 4300)])
 def test_captured_and_replayed(ctx, q, kv):
     """Two graphs with scratch of their own beside eager calls; a write and the attention over it in each."""
     cases = [Case(ctx, np.float16, n=2, q=q, kv=kv, hq=8, hk=2, d=64, block=32, seed=s) for s in (1, 2)]
