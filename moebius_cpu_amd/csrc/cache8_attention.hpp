@@ -86,8 +86,9 @@ __device__ __forceinline__ uint32_t seen_bits(int t0, int lo, int hi, int sinks)
 // 2^kLazy times a scale below 1 fit f16, split ones with 2^kSplitP more.
 constexpr int kLazyHalf = 8, kLazySplit = 3, kSplitP = 11;
 constexpr int kNoExp = -1000;
-// How far a block's exponent of values may lie below the one that the sums are scaled by before
-// that follows it down, and how far below the largest seen.
+// How far an exponent of a chunk's values may lie below the one that the sums are scaled by before
+// that follows the chunk down, and how far below the largest seen. At 2^-10 the probabilities of a row that sees
+// only such values keep all bits of f16 down to 2^-4 of the largest, and 2^-15 of it below that.
 constexpr int kBelow = 10, kDeepest = 80;
 constexpr int kReadsAhead = 6;  // fragments of 16 bytes per lane on their way from LDS
 constexpr int kSplitQ = 14;  // split queries are scaled to a largest value of 2^14 .. 2^15
@@ -248,8 +249,29 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
         load_k(rg.chunk(i)), load_v(rg.chunk(i));
         next_pages(rg.chunk(i + WV));
     }
-    for (; i < c1; i += WV) {
+    for (int visit = 0; i < c1;) {
         const int base = rg.chunk(i) * kChunk;
+        const float ks_now = ks, vs_now = vs;
+        const int ev = there && vs > 0.0f ? __builtin_amdgcn_frexp_expf(vs) : kNoExp;
+        int tv = max(ev, __shfl_xor(ev, 16));
+        tv = __builtin_amdgcn_readfirstlane(max(tv, __shfl_xor(tv, 32)));
+        int tl = tv;
+        bool there_now = there, last = true;
+        if (a.block_log < 6) {
+            // Groups of tokens whose scales of values are far apart are taken in visits of their own to the
+            // chunk, as a row may see the small ones alone: next to the largest their probabilities would
+            // leave f16.
+            tl = ev == kNoExp ? -kNoExp : ev;
+            tl = min(tl, __shfl_xor(tl, 16));
+            tl = __builtin_amdgcn_readfirstlane(min(tl, __shfl_xor(tl, 32)));
+            if (tv > kNoExp && tv - tl > kBelow) {
+                there_now = there && g == visit;
+                tv = tl = __builtin_amdgcn_readlane(ev, 16 * visit);
+                last = visit == 3;
+            }
+        }
+        visit = last ? 0 : visit + 1;
+        const int next = last ? i + WV : i;
         floatx4 sc[NQ][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -267,16 +289,14 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                 }
             }
         }
-        const bool more = i + WV < c1;
-        const float ks_now = ks, vs_now = vs;
-        const bool there_now = there;
-        if (more) load_k(rg.chunk(i + WV));
+        const bool more = next < c1;
+        if (more) {
+            if (!last) next_pages(rg.chunk(i));
+            load_k(rg.chunk(next));
+        }
 
         // The sums' exponent follows the blocks' scales of values.
-        int tv = there_now && vs_now > 0.0f ? __builtin_amdgcn_frexp_expf(vs_now) : kNoExp;
-        tv = max(tv, __shfl_xor(tv, 16));
-        tv = __builtin_amdgcn_readfirstlane(max(tv, __shfl_xor(tv, 32)));
-        if (tv > ve || (tv > kNoExp && tv < ve - kBelow)) {
+        if (tv > ve || (tv > kNoExp && tl < ve - kBelow)) {
             ve_max = max(ve_max, tv);
             const int to = max(tv, ve_max - kDeepest);
             if (to != ve) {
@@ -355,9 +375,10 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
             }
         }
         if (more) {
-            load_v(rg.chunk(i + WV));
-            next_pages(rg.chunk(i + 2 * WV));
+            load_v(rg.chunk(next));
+            next_pages(rg.chunk(next + WV));
         }
+        i = next;
     }
 
     // Scales taken back; the waves' sums joined in LDS, each wave then finishing some of them.
@@ -659,8 +680,12 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     float ks_next = 0.0f, vs_next = 0.0f;  // (WIDE alone)
     float scale_next = 0.0f;               // (else: the lane's)
     bool ok_next = false, ok[NP];
-    auto follow = [&](int tv) {
-        const bool go = tv > ve || (tv > kNoExp && tv < ve - kBelow);
+    // Groups whose scales of values are far apart are taken in visits of their own to the chunk, as a row
+    // may see the small ones alone: next to the largest their probabilities would leave f16.
+    float k_here[NP], v_here[NP];
+    int visit = 0, visits = 1;
+    auto follow = [&](int tv, int tl) {  // largest and smallest exponent of the chunk's values
+        const bool go = tv > ve || (tv > kNoExp && tl < ve - kBelow);
         ve_max = go ? max(ve_max, tv) : ve_max;
         const int to = go ? max(tv, ve_max - kDeepest) : ve;
         shift = ve - to;
@@ -681,29 +706,47 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     auto prepare = [&](int i) {
         const int base = rg.chunk(c0 + i) * kChunk;
         whole = base + kChunk <= hi_all && (base >= lo_all || base + kChunk <= a.sinks);
-        int tv = kNoExp;
-        float k[NP], v[NP];
+        int ev[NP];
         if constexpr (WIDE) {
             ok[0] = ok_next;
-            k[0] = ok[0] ? ks_next : 0.0f, v[0] = ok[0] ? vs_next : 0.0f;
-        } else {
+            k_here[0] = ok[0] ? ks_next : 0.0f, v_here[0] = ok[0] ? vs_next : 0.0f;
+        } else if (visit == 0) {
             // (blocks behind the last token may never have been written)
             const float x = ok_next && base + 16 * (lane & 3) < rg.kv_len ? scale_next : -1.0f;
 #pragma unroll
             for (int g = 0; g < NP; ++g) {
-                k[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), g));
-                v[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 4 + g));
-                ok[g] = __builtin_bit_cast(int, v[g]) >= 0;
+                k_here[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), g));
+                v_here[g] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 4 + g));
+            }
+        }
+        int tv = kNoExp, tl = -kNoExp;
+        float k[NP], v[NP];
+#pragma unroll
+        for (int x = 0; x < NP; ++x) {
+            k[x] = k_here[x], v[x] = v_here[x];
+            // the exponent as frexp gives it; below the normal range as at its end
+            const int bits = __builtin_bit_cast(int, v[x]);
+            ev[x] = bits > 0 ? max(bits >> 23, 1) - 126 : kNoExp;
+            tv = max(tv, ev[x]);
+            tl = bits > 0 ? min(tl, ev[x]) : tl;
+            if (!WIDE) ok[x] = bits >= 0;
+        }
+        if constexpr (!WIDE) {
+            visits = tv > kNoExp && tv - tl > kBelow ? NP : 1;
+            if (visits > 1) {
+                tv = kNoExp;
+#pragma unroll
+                for (int x = 0; x < NP; ++x) {
+                    ok[x] = ok[x] && x == visit;
+                    v[x] = x == visit ? v[x] : 0.0f;
+                    tv = x == visit ? ev[x] : tv;
+                }
+                tl = tv;
             }
         }
 #pragma unroll
-        for (int x = 0; x < NP; ++x) {
-            // the exponent as frexp gives it; below the normal range as at its end
-            const int bits = __builtin_bit_cast(int, v[x]);
-            tv = max(tv, bits > 0 ? max(bits >> 23, 1) - 126 : kNoExp);
-            whole = whole && ok[x];
-        }
-        follow(tv);
+        for (int x = 0; x < NP; ++x) whole = whole && ok[x];
+        follow(tv, tl);
         factors(0, h ? k[1 % NP] : k[0], h ? v[1 % NP] : v[0]);
         if constexpr (WIDE) ks[1] = ks[0], vrel[1] = vrel[0], inv[1] = inv[0];
         else factors(1, h ? k[3 % NP] : k[2 % NP], h ? v[3 % NP] : v[2 % NP]);
@@ -814,22 +857,28 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
             prepare(0);
         }
         __syncthreads();
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < n;) {
+            const bool first = WIDE || visit == 0, last = WIDE || visit + 1 == visits;
             scales();
             const int page_new = read_page(i + AHEAD + 3);
             softmax(i);
-            if (i + AHEAD + 1 < n) stage_k(i + AHEAD + 1);
-            if (i + AHEAD < n) stage_v(i + AHEAD);
+            if (last && i + AHEAD + 1 < n) stage_k(i + AHEAD + 1);
+            if (first && i + AHEAD < n) stage_v(i + AHEAD);
             fetch_v(i + AHEAD + 1, page[AHEAD]);
-            fetch_k(i + AHEAD + 2, page[AHEAD + 1]);
-            move_up(page_new);
+            if (last) {
+                fetch_k(i + AHEAD + 2, page[AHEAD + 1]);
+                move_up(page_new);
+            }
             __syncthreads();
             __builtin_amdgcn_s_setprio(1);
+            const int next = last ? i + 1 : i;
             values(i);
-            scores(i + 1);  // (behind the last chunk: of what the buffer holds, and not used)
+            scores(next);  // (behind the last chunk: of what the buffer holds, and not used)
             feed<PARTS * (4 * DT + 2 * KS), PARTS>();
             __builtin_amdgcn_s_setprio(0);
-            if (i + 1 < n) prepare(i + 1);
+            visit = last ? 0 : visit + 1;
+            i = next;
+            if (i < n) prepare(i);
             __syncthreads();
         }
         if (TURNS && wave < 4) __syncthreads();

@@ -261,8 +261,9 @@ def visible(ql, kl, causal, window, sinks):
     return seen
 
 
-def attention64(q, held, table, scale, causal, window, sinks, q_len, kv_len, fast=False):
-    """out and the bound on its error, NaN where rows are not there."""
+def attention64(q, held, table, scale, causal, window, sinks, q_len, kv_len, fast=False, below=None):
+    """out and the bound on its error, NaN where rows are not there; below: the sums' exponent is at most that far
+    above those of the values that a row sees."""
     n, qt, hq, d = q.shape
     hk = held.codes.shape[2]
     g, parts2 = hq // hk, q.dtype == F32 and not fast
@@ -294,6 +295,11 @@ def attention64(q, held, table, scale, causal, window, sinks, q_len, kv_len, fas
             size = (p @ np.abs(vh) / np.where(z > 0, z, 1))  # what relative errors of p are of
             err = np.expm1(2 * e)[:, None] * size + (2.0 ** -22 if parts2 else 2.0 ** -11 * 1.001) * size + \
                 kl * (2.0 ** -35 if parts2 else 2.0 ** -24) * big
+            if below is not None:
+                of = np.array([held.scale[1, pg, h // g] if 0 <= pg < held.pages else 0 for pg in table[i, np.arange(kl) // held.block]])
+                big, keys = 127 * np.where(seen, of, 0).max(1) * 2.0 ** below, seen.sum(1)
+                err = np.expm1(2 * e)[:, None] * size + (2.0 ** -22 if parts2 else 2.0 ** -11 * 1.001) * size + \
+                    (keys * (2.0 ** -35 if parts2 else 2.0 ** -24) * big)[:, None]
             if q.dtype == np.float16:
                 err = err + 2.0 ** -11 * (np.abs(o) + err) + 2.0 ** -25
             else:
@@ -451,6 +457,32 @@ def test_scores_and_values_of_very_different_size(ctx, dtype, q, cap):
     c.held.write(c.table, kv, [0], [512])
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("n,q,cap,hk", [(3, 1, 512, 2), (2, 5, 300, 2), (1, 150, 512, 2), (1, 150, 4200, 2), (64, 70, 200, 4), (4, 300, 300, 2)])
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("window", [0, 8])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_rows_that_see_only_small_values(ctx, dtype, window, block, n, q, cap, hk):
+    """Neighbouring blocks of values 2^21 apart, tokens that are alike: rows that see only small ones keep their bits.
+
+    The sums' exponent is at most 2^10 above that of any value that a row sees, if it sees those of one block;
+    the larger ones of others only make the bound's terms larger."""
+    r = np.random.default_rng(cap + q)
+    blocks = -(-cap // block)
+    kv_len = [min(300, cap) - (i * 37) % 150 for i in range(n)]
+    q_len = [min(q, x) for x in kv_len]
+    c = Case(ctx, dtype, n=n, q=q, kv=cap, hq=2 * hk, hk=hk, d=64, block=block, q_len=q_len, kv_len=kv_len, window=window, std=0.25)
+    size = np.repeat(np.exp2(r.choice([9, -2, -12, -12], blocks)), block)[None, :cap, None, None]
+    kv = [0.25 * r.standard_normal((n, cap, hk, 64)), size * r.standard_normal((n, cap, hk, 64))]
+    kv = [x.astype(dtype) for x in kv]
+    c.held.write(c.table, kv, np.zeros(n, int), kv_len)
+    cache_write(c.cache, c.dtable, heads(ctx, kv[0]), heads(ctx, kv[1]), length=lens(ctx, kv_len))
+    c.run()
+    want, tol = attention64(c.qh, c.held, c.table, 0.125, True, window, 0, q_len, kv_len, below=10)
+    there = ~np.isnan(want)
+    off = np.abs(c.out.numpy().astype(np.float64) - want)[there]
+    assert np.all(off <= tol[there]), (off / tol[there]).max()
 
 
 def test_probabilities_in_two_parts(ctx):
