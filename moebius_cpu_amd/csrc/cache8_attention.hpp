@@ -127,7 +127,10 @@ __device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float
 template <typename T, int PARTS, int DT, int NQ, int WV>
 __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) {
     constexpr int DC = (DT + 3) / 4;  // chunks of 64 channels
-    constexpr int kLazy = PARTS == 2 ? kLazySplit : kLazyHalf;
+    // Probabilities of f16 in two parts too: the kernel waits for memory, and single tokens of 8 items take 50.2 us
+    // so and 49.9 rounded once, which alone is 2.4e-4 of an output whose own rounding is 2.1e-4.
+    constexpr int PP = sizeof(T) == 2 ? 2 : PARTS;
+    constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf;
     constexpr int kOut = NQ * DT * 4 + NQ * 2;  // floats of a lane's partial: sums, then m and l
     extern __shared__ float joined[];           // [WV][kOut][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -309,9 +312,9 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                 ve = to;
             }
         }
-        const float vrel = there_now && vs_now > 0.0f ? ldexpf(vs_now, (PARTS == 2 ? kSplitP : 0) - ve) : 0.0f;
+        const float vrel = there_now && vs_now > 0.0f ? ldexpf(vs_now, (PP == 2 ? kSplitP : 0) - ve) : 0.0f;
 
-        halfx8 p[NQ][PARTS][2];
+        halfx8 p[NQ][PP][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             const float c = __builtin_fminf(ks_now * cq[n], 0x1.fffffep127f);  // (0 times it is 0)
@@ -354,10 +357,10 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                     l[n] += y;
                     float z = y * vrel;
                     // (both parts are of z rounded to f32; a product fused with its conversion is not)
-                    if constexpr (PARTS == 2) asm("" : "+v"(z));
+                    if constexpr (PP == 2) asm("" : "+v"(z));
                     const _Float16 h = static_cast<_Float16>(z);
                     p[n][0][t / 2][(t % 2) * 4 + e] = h;
-                    if constexpr (PARTS == 2) p[n][1][t / 2][(t % 2) * 4 + e] = static_cast<_Float16>(z - float(h));
+                    if constexpr (PP == 2) p[n][1][t / 2][(t % 2) * 4 + e] = static_cast<_Float16>(z - float(h));
                 }
         }
 #pragma unroll
@@ -368,7 +371,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                 const halfx8 h = halves(vc[t][2 * s], vc[t][2 * s + 1]);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    if constexpr (PARTS == 2)
+                    if constexpr (PP == 2)
                         o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, p[n][1][s], o[n][t], 0, 0, 0);
                     o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, p[n][0][s], o[n][t], 0, 0, 0);
                 }
@@ -391,7 +394,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 joined[(wave * kOut + (n * DT + t) * 4 + e) * 64 + lane] =
-                    ldexpf(o[n][t][e], ve == kNoExp ? 0 : ve - (PARTS == 2 ? kSplitP : 0));
+                    ldexpf(o[n][t][e], ve == kNoExp ? 0 : ve - (PP == 2 ? kSplitP : 0));
         joined[(wave * kOut + NQ * DT * 4 + 2 * n) * 64 + lane] = m[n];
         joined[(wave * kOut + NQ * DT * 4 + 2 * n + 1) * 64 + lane] = l[n];
     }
