@@ -5,6 +5,12 @@
 //   o = sum p_j vs_j vc_j / sum p_j.
 // Codes are integers of 8 bits and exact in f16, so both products run on the f16 matrix
 // instructions and the scales join outside of them: ks in the scores, vs in the probabilities.
+//
+// The probabilities meet vs in f16, whose range is short, so the sums are held against a power of two
+// near the scales of the values that are being read. It moves when those do, and where the blocks of
+// one chunk differ by more than 2^kBelow their groups are taken one after another.
+//
+// f32 queries and probabilities are two f16 parts, so that a product of f32 costs two of f16.
 #pragma once
 
 #include <type_traits>
@@ -124,6 +130,11 @@ __device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float
 // stand, and their values one load of 16 bytes from a channel's row; keys are 16 bytes of a
 // token's row as two steps of the instruction. A block holds whole groups of 16 tokens, so page,
 // scales and whether the page is there are the lane's own.
+//
+// Bound: memory, and the latency of its loads where the tokens are few. Codes are read once and never
+// shared between rows that are not in one wave, which is why nothing is staged. Single tokens of 8 items with up
+// to 16384 tokens, 32 heads over 8 of 128 (210 MB of codes): 40 us of the call's 50, 5.2 TB/s, the join 5. One token
+// over 300, 8 heads of 80, f32: 9.2 us, one workgroup's chain of lengths, page, codes and products.
 template <typename T, int PARTS, int DT, int NQ, int WV>
 __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) {
     constexpr int DC = (DT + 3) / 4;  // chunks of 64 channels
@@ -487,6 +498,11 @@ __device__ __forceinline__ X scalar_load(const X *p) {
 // the vector unit; keys are then staged two chunks ahead and values one, in three buffers, as the
 // waves behind still read one that the others are done with. Else one buffer is enough, and the
 // workgroups of a CU drift apart.
+//
+// Bound: issue, of matrix and vector instructions that both need about half of a SIMD's cycles (0.49 and
+// 0.56 of them at heads of 128; LDS 0.33), and the clock, which gives way under them. 4096 rows of a prompt of 16384, 32 heads over 8 of 128, f16: 964 to 1032 us with the card's clock
+// (up to 998 TFLOP/s; every wave for itself from memory 2738, shared without turns 1115). 4096 x 13312 of 16
+// heads, not causal: 547 to 577. f32 as two products, 2 x 4096 x 4096 of 8 heads of 80: 176 to 193.
 //
 // WIDE: blocks of 64 or 128 tokens, so that a chunk lies in one page and has one scale of keys and one of
 // values, read through the scalar unit. Else its four groups of 16 tokens have their own: lane l
