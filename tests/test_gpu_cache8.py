@@ -492,6 +492,32 @@ def test_probabilities_in_two_parts(ctx):
     c.check(scale=2.0 ** -6)
 
 
+@pytest.mark.parametrize("n,q,hq,hk,d,kv,window", [(2, 1, 8, 4, 64, 16, 0), (1, 5, 8, 2, 128, 300, 26), (3, 1, 4, 4, 80, 2000, 0), (1, 20, 2, 1, 200, 900, 40)])
+def test_f16_rows_alone_round_once(ctx, n, q, hq, hk, d, kv, window):
+    """f16 calls whose rows share no tokens hold probabilities in two parts: off as f32 ones, and half a step of the output."""
+    c = Case(ctx, np.float16, n=n, q=q, kv=kv, hq=hq, hk=hk, d=d, block=32, window=window)
+    c.run()
+    want, tol = attention64(c.qh.astype(F32), c.held, c.table, 1 / np.sqrt(d), True, window, 0, c.q_len, c.kv_len)
+    off = np.abs(c.out.numpy().astype(np.float64) - want)
+    tol = tol + 2.0 ** -11 * (np.abs(want) + tol) + 2.0 ** -25
+    assert np.all(off <= tol), (off / tol).max()
+
+
+@pytest.mark.parametrize("n,block", [(1, 16), (2, 32)])
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_blocks_of_small_values_in_splits(ctx, dtype, n, block):
+    """Single tokens over a long cache whose shares and blocks of values lie far apart, with a page missing between them."""
+    kv_len = [3900, 2117][:n]
+    c = Case(ctx, dtype, n=n, q=1, kv=4000, hq=4, hk=2, d=80, block=block, kv_len=kv_len, absent=[(0, 61), (0, 62)])
+    r = np.random.default_rng(block)
+    size = np.repeat(np.exp2(r.choice([9, -2, -12], c.blocks)), block)[None, :4000, None, None]
+    kv = [(0.25 * r.standard_normal((n, 4000, 2, 80))).astype(dtype), (size * r.standard_normal((n, 4000, 2, 80))).astype(dtype)]
+    c.held.write(c.table, kv, np.zeros(n, int), kv_len)
+    cache_write(c.cache, c.dtable, heads(ctx, kv[0]), heads(ctx, kv[1]), length=lens(ctx, kv_len))
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("q,cap", [(8, 200), (80, 4200)])
 def test_queries_of_any_size(ctx, q, cap):
     """f32 queries far outside f16 in both directions, and rows that are not finite beside others."""
