@@ -654,9 +654,10 @@ int32_t mh_cache8_attention_scratch(MhContext *ctx, uint32_t dtype, const MhCach
 /* out [n][q_tokens][heads_q][d] = softmax(scale q . k) v over the tokens that a row sees, k and v
  * the values that the cache holds, in one pass with f32 scores and sums; scale > 0. Rows that see
  * no token are zero, rows at or above q_len are left as they were. Codes enter the f16 products
- * exactly. f16: queries as they are, probabilities rounded to f16 where many rows share the tokens,
- * else in two f16 parts. f32: queries (to 2^-24 of themselves or 2^-39 of the largest of their head,
- * whichever is more) and probabilities in two f16 parts, or on FAST contexts rounded to f16 once.
+ * exactly. f16: queries as they are, probabilities in two f16 parts. f32: queries (to 2^-24 of
+ * themselves or 2^-39 of the largest of their head, whichever is more) and probabilities in two f16
+ * parts. FAST contexts round f32 queries and, but for f16 calls whose rows are few, probabilities to
+ * f16 once.
  * Values of any scale keep their bits for the rows that see only them, down to 2^-90 of the largest
  * (a row that sees both keeps what an f32 sum does). Tokens are split over workgroups where rows are few, and the parts joined through scratch (mh_cache8_attention_scratch bytes, 16-byte aligned);
  * NULL takes the context's workspace, which is refused while the stream is being captured into a

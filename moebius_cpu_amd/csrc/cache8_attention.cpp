@@ -73,8 +73,10 @@ void cache8_attention(Context &ctx, const Cache8Attention &c, void *scratch) {
     const int size = c.type == kF16 ? 2 : 4;
     a.wide = c.c.d % 8 == 0 && c.q.ld % (16 / size) == 0 && aligned16(c.q.p) && c.ld_out % 4 == 0 &&
              reinterpret_cast<uintptr_t>(c.out) % (4 * size) == 0;
-    if (c.type == kF16) c8a::launch_f16(ctx, a, p.nq, p.waves, p.dt);
-    else if (ctx.precision == Precision::Fast) c8a::launch_f32_half(ctx, a, p.nq, p.waves, p.dt);
+    const bool fast = ctx.precision == Precision::Fast;
+    if (c.type == kF16 && fast && p.waves) c8a::launch_f16_half(ctx, a, p.waves, p.dt);
+    else if (c.type == kF16) c8a::launch_f16(ctx, a, p.nq, p.waves, p.dt);
+    else if (fast) c8a::launch_f32_half(ctx, a, p.nq, p.waves, p.dt);
     else c8a::launch_f32(ctx, a, p.nq, p.waves, p.dt);
 }
 

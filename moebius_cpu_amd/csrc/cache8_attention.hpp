@@ -10,7 +10,8 @@
 // near the scales of the values that are being read. It moves when those do, and where the blocks of
 // one chunk differ by more than 2^kBelow their groups are taken one after another.
 //
-// f32 queries and probabilities are two f16 parts, so that a product of f32 costs two of f16.
+// f32 queries and all probabilities are two f16 parts, at the cost of a product more: one part alone is off by
+// as much as an f16 output's own rounding. FAST contexts take one of each.
 #pragma once
 
 #include <type_traits>
@@ -138,8 +139,8 @@ __device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float
 template <typename T, int PARTS, int DT, int NQ, int WV>
 __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) {
     constexpr int DC = (DT + 3) / 4;  // chunks of 64 channels
-    // Probabilities of f16 in two parts too: the kernel waits for memory, and single tokens of 8 items take 50.2 us
-    // so and 49.9 rounded once, which alone is 2.4e-4 of an output whose own rounding is 2.1e-4.
+    // Probabilities of f16 in two parts on FAST contexts too: the kernel waits for memory, and single tokens of 8 items
+    // take 50.2 us so and 49.9 rounded once.
     constexpr int PP = sizeof(T) == 2 ? 2 : PARTS;
     constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf;
     constexpr int kOut = NQ * DT * 4 + NQ * 2;  // floats of a lane's partial: sums, then m and l
@@ -464,15 +465,21 @@ struct Stage {
     static constexpr int kV0 = NB * kK, kBytes = kV0 + NB * kV;
 };
 
-// Orders the MFMAs of a block and the reads from LDS that feed them, one for every PARTS: some reads ahead
-// of the first product, then one beside each (the compiler's own order waits for every second read).
-template <int MFMAS, int PARTS>
+// Orders the MFMAs of a block and the reads from LDS that feed them, N1 reads for P1 MFMAs each and then N2
+// for P2: some reads ahead of the first product, then one beside each (the compiler's own order waits for
+// every second read).
+template <int N1, int P1, int N2 = 0, int P2 = 1>
 __device__ __forceinline__ void feed() {
-    constexpr int kReads = MFMAS / PARTS, kFirst = kReads < kReadsAhead ? kReads : kReadsAhead;
+    constexpr int kReads = N1 + N2, kFirst = kReads < kReadsAhead ? kReads : kReadsAhead;
     __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
 #pragma unroll
-    for (int i = 0; i < kReads; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0);
+    for (int i = 0; i < N1; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, P1, 0);
+        if (i + kFirst < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = N1; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, P2, 0);
         if (i + kFirst < kReads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
 }
@@ -499,22 +506,28 @@ __device__ __forceinline__ X scalar_load(const X *p) {
 // waves behind still read one that the others are done with. Else one buffer is enough, and the
 // workgroups of a CU drift apart.
 //
-// Bound: issue, of matrix and vector instructions that both need about half of a SIMD's cycles (0.49 and
-// 0.56 of them at heads of 128; LDS 0.33), and the clock, which gives way under them. 4096 rows of a prompt of 16384, 32 heads over 8 of 128, f16: 964 to 1032 us with the card's clock
-// (up to 998 TFLOP/s; every wave for itself from memory 2738, shared without turns 1115). 4096 x 13312 of 16
-// heads, not causal: 547 to 577. f32 as two products, 2 x 4096 x 4096 of 8 heads of 80: 176 to 193.
+// Bound: issue, of matrix and vector instructions that take turns, and the clock, which gives way under them.
+// 4096 rows of a prompt of 16384, 32 heads over 8 of 128, f16: 1377 us (probabilities in one part, as on FAST
+// contexts, 965 to 1007: 998 TFLOP/s at best; every wave for itself from memory 2738, shared without turns 1115).
+// 4096 x 13312 of 16 heads, not causal: 773, in one part 545 to 565. f32, queries in two parts too, 2 x 4096 x 4096 of
+// 8 heads of 80: 176 to 193.
 //
 // WIDE: blocks of 64 or 128 tokens, so that a chunk lies in one page and has one scale of keys and one of
 // values, read through the scalar unit. Else its four groups of 16 tokens have their own: lane l
 // reads the page of group l % 4 and, of keys or (l & 4) of values, its scale.
-template <typename T, int PARTS, int KS, int W, bool WIDE>
+//
+// PARTS: f16 parts of a query, PP: of a probability.
+template <typename T, int PARTS, int PP, int KS, int W, bool WIDE>
 __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 ? 8 : 10) ? 2 : 1)) void cache8_tiles_kernel(Args a) {
     constexpr bool TURNS = W == 8;
     constexpr int NP = WIDE ? 1 : 4;  // groups of tokens with a page of their own
     constexpr int NB = TURNS ? 3 : 1, AHEAD = TURNS ? 1 : 0;  // keys are staged AHEAD + 1 chunks ahead, values AHEAD
     using L = Stage<KS, NB>;
     constexpr int DT = L::kDT, NT = 64 * W;
-    constexpr int kLazy = PARTS == 2 ? kLazySplit : kLazyHalf;
+    constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf, kUp = PP == 2 ? kSplitP : 0;
+    // Whether scales of values join the exponents: a multiplication less for each probability, at an error of
+    // 2^-20 of it, which is nothing beside f16's but more than f32 calls have.
+    constexpr bool LOGS = sizeof(T) == 2 || PP == 1;
     constexpr int U = (kChunk * KS + NT - 1) / NT;  // 16-byte runs of codes per thread, of keys and of values
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -655,7 +668,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     };
 
     floatx16 o[DT], sc[2];
-    halfx8 p[PARTS][4];
+    halfx8 p[PP][4];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -685,13 +698,13 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const halfx8 v = *reinterpret_cast<const halfx8 *>(vp + ((s / 2) * 32 + (s % 2) * 8 + d * 32 * L::kVS) * 2);
-                if constexpr (PARTS == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[1][s], o[d], 0, 0, 0);
+                if constexpr (PP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[1][s], o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[0][s], o[d], 0, 0, 0);
             }
     };
     // What the chunk's scales make of its scores and probabilities, formed beside the products: the
-    // factor of the scores, the scales of values against the power of two of the sums (PARTS 1: the
-    // logarithm, so that it joins the exponent, and the inverse, which takes it out of the sum).
+    // factor of the scores, the scales of values against the power of two of the sums (LOGS: the
+    // logarithm, and the inverse, which takes it out of the sum).
     float ks[2], vrel[2], inv[2];
     int shift = 0;       // how far that power of two moves
     bool whole = false;  // every row of the wave sees all of the chunk
@@ -712,8 +725,8 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     };
     auto factors = [&](int b, float k, float v) {
         // (codes at a scale of 0 are 0: any factor will do)
-        const float x = v > 0.0f ? ldexpf(v, (PARTS == 2 ? kSplitP : 0) - ve) : 1.0f;
-        if constexpr (PARTS == 2) {
+        const float x = v > 0.0f ? ldexpf(v, kUp - ve) : 1.0f;
+        if constexpr (!LOGS) {
             vrel[b] = x;
         } else {
             const float y = __builtin_fmaxf(x, 0x1p-90f);  // (values far below the largest count as nothing)
@@ -815,11 +828,11 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[b][e] = sc[b][e] * ks[b] - mu + (PARTS == 2 ? 0.0f : vrel[b]);
+                for (int e = 0; e < 16; ++e) sc[b][e] = sc[b][e] * ks[b] - mu + (LOGS ? vrel[b] : 0.0f);
         } else {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                const float off = PARTS == 2 ? -mu : vrel[b] - mu;
+                const float off = LOGS ? vrel[b] - mu : -mu;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[b][e] = __builtin_fmaf(sc[b][e], ks[b], off);
             }
@@ -831,14 +844,14 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
             for (int e = 0; e < 16; ++e) {
                 const float y = __builtin_amdgcn_exp2f(sc[b][e]);
                 sum[2 * b + e % 2] += y;
-                float z = PARTS == 2 ? y * vrel[b] : y;
+                float z = LOGS ? y : y * vrel[b];
                 // (both parts are of z rounded to f32; a product fused with its conversion is not)
-                if constexpr (PARTS == 2) asm("" : "+v"(z));
+                if constexpr (!LOGS) asm("" : "+v"(z));
                 const _Float16 x = static_cast<_Float16>(z);
                 p[0][2 * b + e / 8][e % 8] = x;
-                if constexpr (PARTS == 2) p[1][2 * b + e / 8][e % 8] = static_cast<_Float16>(z - float(x));
+                if constexpr (PP == 2) p[1][2 * b + e / 8][e % 8] = static_cast<_Float16>(z - float(x));
             }
-        if constexpr (PARTS == 2) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if constexpr (!LOGS) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         else l = __builtin_fmaf(sum[0] + sum[1], inv[0], __builtin_fmaf(sum[2] + sum[3], inv[1], l));
     };
 
@@ -872,7 +885,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
         if (TURNS && wave >= 4) __syncthreads();
         if (n > 0) {
             scores(0);
-            feed<PARTS * 2 * KS, PARTS>();
+            feed<2 * KS, PARTS>();
             prepare(0);
         }
         __syncthreads();
@@ -893,7 +906,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
             const int next = last ? i + 1 : i;
             values(i);
             scores(next);  // (behind the last chunk: of what the buffer holds, and not used)
-            feed<PARTS * (4 * DT + 2 * KS), PARTS>();
+            feed<4 * DT, PP, 2 * KS, PARTS>();
             __builtin_amdgcn_s_setprio(0);
             visit = last ? 0 : visit + 1;
             i = next;
@@ -904,7 +917,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     }
     if (!row_ok) return;
     l += other_half(l);
-    const int back = ve == kNoExp ? 0 : ve - (PARTS == 2 ? kSplitP : 0);
+    const int back = ve == kNoExp ? 0 : ve - kUp;
     if (a.part) {
         float *part = a.part + (int64_t(work) * 32 * W + wave * 32 + col) * (DT * 32 + 2);
         if (h == 0) part[DT * 32] = m, part[DT * 32 + 1] = l;
@@ -1002,30 +1015,21 @@ void launch_rows(Context &ctx, const Args &a) {
     launch_join<T, 16 * NQ, DT * 16>(ctx, a);
 }
 
-template <typename T, int PARTS, int KS, int W, bool WIDE>
+template <typename T, int PARTS, int PP, int KS, int W, bool WIDE>
 void launch_tiles(Context &ctx, const Args &a) {
     using L = Stage<KS, W == 8 ? 3 : 1>;
     const size_t lds = L::kBytes;
     static_assert(lds <= 160 * 1024, "chunks exceed the LDS");
-    const void *fn = reinterpret_cast<const void *>(&cache8_tiles_kernel<T, PARTS, KS, W, WIDE>);
+    const void *fn = reinterpret_cast<const void *>(&cache8_tiles_kernel<T, PARTS, PP, KS, W, WIDE>);
     HIP_CHECK(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
-    cache8_tiles_kernel<T, PARTS, KS, W, WIDE><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{64 * W}, lds, ctx.stream>>>(a);
+    cache8_tiles_kernel<T, PARTS, PP, KS, W, WIDE><<<dim3{uint32_t((a.work + 7) / 8 * 8)}, dim3{64 * W}, lds, ctx.stream>>>(a);
     MH_LAUNCH_CHECK();
     launch_join<T, 32 * W, L::kDT * 32>(ctx, a);
 }
 
-// dt: tiles of 16 channels as chosen by head_tiles; waves > 0: that many of 32 rows share a chunk.
-template <typename T, int PARTS>
-void launch_all(Context &ctx, const Args &a, int nq, int waves, int dt) {
-    auto by = [&](auto n) {
-        constexpr int DT = decltype(n)::value;
-        if constexpr (DT <= 8)
-            if (waves == 8)
-                return a.block_log >= 6 ? launch_tiles<T, PARTS, DT, 8, true>(ctx, a) : launch_tiles<T, PARTS, DT, 8, false>(ctx, a);
-        if (waves) a.block_log >= 6 ? launch_tiles<T, PARTS, DT, 4, true>(ctx, a) : launch_tiles<T, PARTS, DT, 4, false>(ctx, a);
-        else if (nq == 1) launch_rows<T, PARTS, DT, 1>(ctx, a);
-        else if constexpr (DT <= 8) launch_rows<T, PARTS, DT, 2>(ctx, a);
-    };
+// by(the constant dt), tiles of 16 channels as chosen by head_tiles.
+template <typename F>
+void by_tiles(int dt, F &&by) {
     if (dt == 4) by(std::integral_constant<int, 4>{});
     else if (dt == 5) by(std::integral_constant<int, 5>{});
     else if (dt == 6) by(std::integral_constant<int, 6>{});
@@ -1034,7 +1038,32 @@ void launch_all(Context &ctx, const Args &a, int nq, int waves, int dt) {
     else by(std::integral_constant<int, 16>{});
 }
 
+// nq tiles of 16 rows for each workgroup.
+template <typename T, int PARTS>
+void rows_alone(Context &ctx, const Args &a, int nq, int dt) {
+    by_tiles(dt, [&](auto n) {
+        constexpr int DT = decltype(n)::value;
+        if (nq == 1) launch_rows<T, PARTS, DT, 1>(ctx, a);
+        else if constexpr (DT <= 8) launch_rows<T, PARTS, DT, 2>(ctx, a);
+    });
+}
+
+// Waves of 32 rows that share a chunk, four or eight.
+template <typename T, int PARTS, int PP>
+void rows_shared(Context &ctx, const Args &a, int waves, int dt) {
+    const bool wide = a.block_log >= 6;
+    by_tiles(dt, [&](auto n) {
+        constexpr int DT = decltype(n)::value;
+        if constexpr (DT <= 8)
+            if (waves == 8) return wide ? launch_tiles<T, PARTS, PP, DT, 8, true>(ctx, a) : launch_tiles<T, PARTS, PP, DT, 8, false>(ctx, a);
+        wide ? launch_tiles<T, PARTS, PP, DT, 4, true>(ctx, a) : launch_tiles<T, PARTS, PP, DT, 4, false>(ctx, a);
+    });
+}
+
+// Rows alone where waves is 0. Halves: probabilities (and f32 queries) rounded to f16 once, as FAST contexts ask for;
+// f16 rows alone have no such form, as theirs costs nothing.
 void launch_f16(Context &ctx, const Args &a, int nq, int waves, int dt);
+void launch_f16_half(Context &ctx, const Args &a, int waves, int dt);
 void launch_f32(Context &ctx, const Args &a, int nq, int waves, int dt);
 void launch_f32_half(Context &ctx, const Args &a, int nq, int waves, int dt);
 

@@ -5,7 +5,8 @@ namespace mh {
 namespace c8a {
 
 void launch_f16(Context &ctx, const Args &a, int nq, int waves, int dt) {
-    launch_all<_Float16, 1>(ctx, a, nq, waves, dt);
+    if (waves) rows_shared<_Float16, 1, 2>(ctx, a, waves, dt);
+    else rows_alone<_Float16, 1>(ctx, a, nq, dt);
 }
 
 }  // namespace c8a

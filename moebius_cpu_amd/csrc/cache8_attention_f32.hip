@@ -5,7 +5,8 @@ namespace mh {
 namespace c8a {
 
 void launch_f32(Context &ctx, const Args &a, int nq, int waves, int dt) {
-    launch_all<float, 2>(ctx, a, nq, waves, dt);
+    if (waves) rows_shared<float, 2, 2>(ctx, a, waves, dt);
+    else rows_alone<float, 2>(ctx, a, nq, dt);
 }
 
 }  // namespace c8a
