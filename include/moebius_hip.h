@@ -658,8 +658,10 @@ int32_t mh_cache8_attention_scratch(MhContext *ctx, uint32_t dtype, const MhCach
  * themselves or 2^-39 of the largest of their head, whichever is more) and probabilities in two f16
  * parts. FAST contexts round f32 queries and, but for f16 calls whose rows are few, probabilities to
  * f16 once.
- * Values of any scale keep their bits for the rows that see only them, down to 2^-90 of the largest
- * (a row that sees both keeps what an f32 sum does). Tokens are split over workgroups where rows are few, and the parts joined through scratch (mh_cache8_attention_scratch bytes, 16-byte aligned);
+ * A probability in two parts is held to 2^-22 of itself or 2^-33 of its row's largest, whichever is
+ * more, in one to 2^-11 or 2^-28, beside values of any scale down to 2^-72 of the largest that a
+ * call reads. Sums are f32. Tokens are split over workgroups where rows are few, and the parts
+ * joined through scratch (mh_cache8_attention_scratch bytes, 16-byte aligned);
  * NULL takes the context's workspace, which is refused while the stream is being captured into a
  * graph. out overlaps no input. */
 int32_t mh_cache8_attention(MhContext *ctx, const void *q, uint64_t ld_q, uint32_t dtype, const MhCacheAttention *shape,

@@ -89,14 +89,19 @@ __device__ __forceinline__ uint32_t seen_bits(int t0, int lo, int hi, int sinks)
     return below(hi) & (~below(lo) | below(sinks));
 }
 
-// Exponents of two by which a row's maximum may pass its reference: probabilities of up to
-// 2^kLazy times a scale below 1 fit f16, split ones with 2^kSplitP more.
-constexpr int kLazyHalf = 8, kLazySplit = 3, kSplitP = 11;
+// Exponents of two by which a row's maximum may pass its reference (in one f16 part, in two), and what the scales
+// of values beside the probabilities are lifted by: 2^kLazy times a scale below 2^kUp fits f16, and the more of its
+// range lies below, the smaller the probabilities that keep their bits. Rescales are rarer where kLazy is larger,
+// which pays where a probability costs least.
+constexpr int kLazyHalf = 8, kUpHalf = 7, kLazySplit = 3, kUpSplit = 12;
 constexpr int kNoExp = -1000;
-// How far an exponent of a chunk's values may lie below the one that the sums are scaled by before
-// that follows the chunk down, and how far below the largest seen. At 2^-10 the probabilities of a row that sees
-// only such values keep all bits of f16 down to 2^-4 of the largest, and 2^-15 of it below that.
-constexpr int kBelow = 10, kDeepest = 80;
+// How far an exponent of a chunk's values may lie below the one that the sums are scaled by before that follows the
+// chunk down: a scale beside a probability is 2^(kUp - 1 - kBelow) or more, so that a probability is held to 2^-25 of
+// that, 2^-28 and 2^-33 of its row's largest, where its own 2^-11 or 2^-22 is less. Rows may see only the small values
+// of a chunk, thousands of them with small probabilities, which then must not round to nothing.
+// kDeepest: how far below the largest seen it goes; 2^72 times the sums of 2^30 keys, 127 2^(kLazy + kUp) each,
+// are below the end of f32.
+constexpr int kBelow = 3, kDeepest = 72;
 constexpr int kReadsAhead = 6;  // fragments of 16 bytes per lane on their way from LDS
 constexpr int kSplitQ = 14;  // split queries are scaled to a largest value of 2^14 .. 2^15
 
@@ -142,7 +147,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
     // Probabilities of f16 in two parts on FAST contexts too: the kernel waits for memory, and single tokens of 8 items
     // take 50.2 us so and 49.9 rounded once.
     constexpr int PP = sizeof(T) == 2 ? 2 : PARTS;
-    constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf;
+    constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf, kUp = PP == 2 ? kUpSplit : kUpHalf;
     constexpr int kOut = NQ * DT * 4 + NQ * 2;  // floats of a lane's partial: sums, then m and l
     extern __shared__ float joined[];           // [WV][kOut][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                 ve = to;
             }
         }
-        const float vrel = there_now && vs_now > 0.0f ? ldexpf(vs_now, (PP == 2 ? kSplitP : 0) - ve) : 0.0f;
+        const float vrel = there_now && vs_now > 0.0f ? ldexpf(vs_now, kUp - ve) : 0.0f;
 
         halfx8 p[NQ][PP][2];
 #pragma unroll
@@ -406,7 +411,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 joined[(wave * kOut + (n * DT + t) * 4 + e) * 64 + lane] =
-                    ldexpf(o[n][t][e], ve == kNoExp ? 0 : ve - (PP == 2 ? kSplitP : 0));
+                    ldexpf(o[n][t][e], ve == kNoExp ? 0 : ve - kUp);
         joined[(wave * kOut + NQ * DT * 4 + 2 * n) * 64 + lane] = m[n];
         joined[(wave * kOut + NQ * DT * 4 + 2 * n + 1) * 64 + lane] = l[n];
     }
@@ -524,7 +529,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     constexpr int NB = TURNS ? 3 : 1, AHEAD = TURNS ? 1 : 0;  // keys are staged AHEAD + 1 chunks ahead, values AHEAD
     using L = Stage<KS, NB>;
     constexpr int DT = L::kDT, NT = 64 * W;
-    constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf, kUp = PP == 2 ? kSplitP : 0;
+    constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf, kUp = PP == 2 ? kUpSplit : kUpHalf;
     // Whether scales of values join the exponents: a multiplication less for each probability, at an error of
     // 2^-20 of it, which is nothing beside f16's but more than f32 calls have.
     constexpr bool LOGS = sizeof(T) == 2 || PP == 1;
