@@ -401,17 +401,19 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
         i = next;
     }
 
-    // Scales taken back; the waves' sums joined in LDS, each wave then finishing some of them.
+    // The waves' means joined in LDS, each wave then finishing some of them. A sum is divided before its power of two
+    // is put back: of values near the end of f32 the mean is finite, the sum is not.
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         l[n] += __shfl_xor(l[n], 16);
         l[n] += __shfl_xor(l[n], 32);
+        const float by = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 joined[(wave * kOut + (n * DT + t) * 4 + e) * 64 + lane] =
-                    ldexpf(o[n][t][e], ve == kNoExp ? 0 : ve - kUp);
+                    ldexpf(o[n][t][e] * by, ve == kNoExp ? 0 : ve - kUp);
         joined[(wave * kOut + NQ * DT * 4 + 2 * n) * 64 + lane] = m[n];
         joined[(wave * kOut + NQ * DT * 4 + 2 * n + 1) * 64 + lane] = l[n];
     }
@@ -427,10 +429,12 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
         const float mu = top == kNegInf ? 0.0f : top;
 #pragma unroll
         for (int x = 0; x < WV; ++x) {
-            mw[x] = __builtin_amdgcn_exp2f(mw[x] - mu);
-            sum = __builtin_fmaf(joined[(x * kOut + NQ * DT * 4 + 2 * n + 1) * 64 + lane], mw[x], sum);
+            mw[x] = joined[(x * kOut + NQ * DT * 4 + 2 * n + 1) * 64 + lane] * __builtin_amdgcn_exp2f(mw[x] - mu);
+            sum += mw[x];
         }
-        const float inv = a.part ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int x = 0; x < WV; ++x) mw[x] *= inv;  // a wave's share of the row's probabilities
         float *part = a.part ? a.part + ((int64_t(work) * NQ + n) * 16 + col) * (DT * 16 + 2) : nullptr;
         if (part && row_ok[n] && wave == 0 && g == 0) part[DT * 16] = top, part[DT * 16 + 1] = sum;
         T *op = static_cast<T *>(a.out) + row_at[n] * a.ldo + row_ch[n];
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                 const int ch = t * 16 + 4 * g + e;
                 if (!row_ok[n]) continue;
                 if (part) part[ch] = y;
-                else if (ch < a.d) op[ch] = static_cast<T>(y * inv);
+                else if (ch < a.d) op[ch] = static_cast<T>(y);
             }
         }
     }
@@ -923,16 +927,16 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
     if (!row_ok) return;
     l += other_half(l);
     const int back = ve == kNoExp ? 0 : ve - kUp;
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;  // (before the power of two is put back, as above)
     if (a.part) {
         float *part = a.part + (int64_t(work) * 32 * W + wave * 32 + col) * (DT * 32 + 2);
         if (h == 0) part[DT * 32] = m, part[DT * 32 + 1] = l;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) part[d * 32 + 8 * (e / 4) + 4 * h + e % 4] = ldexpf(o[d][e], back);
+            for (int e = 0; e < 16; ++e) part[d * 32 + 8 * (e / 4) + 4 * h + e % 4] = ldexpf(o[d][e] * by, back);
         return;
     }
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
     T *op = static_cast<T *>(a.out) + row_at * a.ldo + int64_t(qh) * a.d;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -942,7 +946,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
             typedef T V4 __attribute__((ext_vector_type(4)));
             V4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(ldexpf(o[d][4 * f + e], back) * by);
+            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(ldexpf(o[d][4 * f + e] * by, back));
             if (a.wide) {
                 if (ch < a.d) *reinterpret_cast<V4 *>(op + ch) = v;
             } else {
@@ -953,7 +957,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
         }
 }
 
-// Joins the splits of a row, TILE rows per workgroup of the split, PF floats of sums each (then the
+// Joins the splits of a row, TILE rows per workgroup of the split, PF floats of means each (then the
 // maximum and the sum of the probabilities): a workgroup per row, every fourth split to a wave.
 template <typename T, int TILE, int PF>
 __global__ __launch_bounds__(256) void cache8_join_kernel(Args a) {
@@ -978,9 +982,12 @@ __global__ __launch_bounds__(256) void cache8_join_kernel(Args a) {
     float l = 0.0f, o[C] = {};
     for (int s = lane; s < a.splits; s += 64)
         l = __builtin_fmaf(p[s * step + PF + 1], __builtin_amdgcn_exp2f(p[s * step + PF] - mu), l);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 4
     for (int s = wave; s < a.splits; s += 4) {
-        const float f = __builtin_amdgcn_exp2f(p[s * step + PF] - mu);
+        const float f = p[s * step + PF + 1] * __builtin_amdgcn_exp2f(p[s * step + PF] - mu) * inv;
 #pragma unroll
         for (int i = 0; i < C; ++i)
             if (i * 64 + lane < a.d) o[i] = __builtin_fmaf(p[s * step + i * 64 + lane], f, o[i]);
@@ -990,14 +997,11 @@ __global__ __launch_bounds__(256) void cache8_join_kernel(Args a) {
         if (wave) joined[wave - 1][i][lane] = o[i];
     __syncthreads();
     if (wave) return;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T *op = static_cast<T *>(a.out) + (int64_t(item) * a.q_tokens + row / a.g) * a.ldo + int64_t(hk * a.g + row % a.g) * a.d;
 #pragma unroll
     for (int i = 0; i < C; ++i)
         if (i * 64 + lane < a.d)
-            op[i * 64 + lane] = static_cast<T>((o[i] + joined[0][i][lane] + joined[1][i][lane] + joined[2][i][lane]) * inv);
+            op[i * 64 + lane] = static_cast<T>(o[i] + joined[0][i][lane] + joined[1][i][lane] + joined[2][i][lane]);
 }
 
 template <typename T, int TILE, int PF>

@@ -1,5 +1,5 @@
-"""What the attention over a cache in 8 bits makes of probabilities far below a row's largest, and of
-scales of values far apart.
+"""What the attention over a cache in 8 bits makes of probabilities far below a row's largest, of
+scales of values far apart, and of values near the end of f32.
 
 Bounds, beside those of test_gpu_cache8 (e below, from the f32 sums, exponents and FAST queries), for a
 row with probabilities p_j relative to its largest, z = sum p_j, over values v_j = code_j s_j that it
@@ -201,4 +201,24 @@ def test_windows_of_small_values_in_splits(contexts, dtype, fast, block):
     c.held.write(c.table, x, [0, 0], [kv, kv])
     cache_write(c.cache, c.dtable, heads(ctx, x[0]), heads(ctx, x[1]))
     c.run()
+    check(c, 1 / np.sqrt(d), fast)
+
+
+# ---------------------------------------------------------------- values near the end of f32
+
+@pytest.mark.parametrize("fast", [False, True])
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("n,q,hq,hk,d,kv", [(1, 1, 4, 2, 80, 300), (2, 40, 4, 2, 64, 200), (1, 1, 2, 1, 128, 4000), (64, 70, 4, 4, 64, 300),
+                                            (32, 130, 8, 8, 128, 300), (1, 80, 2, 2, 80, 4300)])
+def test_values_near_the_end_of_the_range(contexts, fast, block, n, q, hq, hk, d, kv):
+    """Means of values of up to 3.4e38 are finite: no sum leaves its power of two before it is divided."""
+    ctx = contexts[fast]
+    c = Case(ctx, F32, n=n, q=q, kv=kv, hq=hq, hk=hk, d=d, block=block, std=0.25)
+    r = np.random.default_rng(kv)
+    x = [r.standard_normal((n, kv, hk, d)).astype(F32), ((0.9 + 0.1 * r.random((n, kv, hk, d))) * np.finfo(F32).max).astype(F32)]
+    c.held.write(c.table, x, np.zeros(n, int), c.kv_len)
+    cache_write(c.cache, c.dtable, heads(ctx, x[0]), heads(ctx, x[1]))
+    c.run()
+    keep = {0, n - 1}
+    c.q_len = np.array([c.q_len[i] if i in keep else 0 for i in range(n)])
     check(c, 1 / np.sqrt(d), fast)
