@@ -29,7 +29,7 @@ struct RowArgs {
     uint8_t *code[2];
     float *scale[2];
     const int32_t *table, *first, *len;
-    int n, tokens, blocks, pages, heads, d, dp, runs, block_log, touched;
+    int tokens, blocks, pages, heads, d, dp, runs, block_log, touched;  // runs of 8 channels: 8 runs <= dp
     uint32_t by_runs;  // 2^16 / runs rounded up: p / runs = p by_runs >> 16 for p < 1024 and runs of at most 32
 };
 
@@ -300,7 +300,6 @@ __global__ __launch_bounds__(256) void cache8_write_kernel(RowArgs a) {
     const int c0 = grown ? 0 : q0, nq = q1 - c0;
     for (int i = tid; i < a.runs * 8 * nq; i += nt) {
         const int ch = i / nq, q = c0 + i % nq;
-        if (ch >= a.dp) break;
         uint32_t *const p = v + ch * (block / 4) + q;
         const int lo = max(s.lo - 4 * q, 0), hi = min(s.hi - 4 * q, 4);  // the new tokens of these four
         const uint32_t word = lo < hi ? turned[ch * ldt + q] : 0u;
@@ -344,8 +343,7 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(RowArgs a) {
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int ch = min(run * 8 + i, a.dp - 1);
-                const uint32_t w = *reinterpret_cast<const uint32_t *>(code + ch * block + q * 4);
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(code + (run * 8 + i) * block + q * 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[e].set(i, float(int((w >> (8 * e)) & 255) - 128) * sc);
             }
@@ -366,7 +364,7 @@ RowArgs row_args(const Cache8 &c, const PageTable &t, HeadRows k, HeadRows v, in
     a.ld[0] = k.ld, a.ld[1] = v.ld;
     a.code[0] = c.k, a.code[1] = c.v, a.scale[0] = c.k_scale, a.scale[1] = c.v_scale;
     a.table = t.table, a.first = first, a.len = len;
-    a.n = t.n, a.tokens = tokens, a.blocks = t.blocks, a.pages = c.pages, a.heads = c.heads;
+    a.tokens = tokens, a.blocks = t.blocks, a.pages = c.pages, a.heads = c.heads;
     a.d = c.d, a.dp = c.dp(), a.runs = int(ceil_div(c.d, 8)), a.by_runs = uint32_t((65536 + a.runs - 1) / a.runs), a.block_log = c.block_log;
     // blocks that a run of tokens from anywhere (first NULL: from 0) lies in
     a.touched = int(std::min<int64_t>(t.blocks, (int64_t(tokens) + (first ? c.block() - 1 : 0) + c.block() - 1) >> c.block_log));
@@ -377,8 +375,8 @@ bool wide(HeadRows x, int d, int size) {
     return d % 8 == 0 && x.ld % (16 / size) == 0 && aligned16(x.p);
 }
 
-uint32_t grid_of(const RowArgs &a) {
-    const int64_t g = int64_t(a.n) * a.heads * 2 * a.touched;
+uint32_t grid_of(const RowArgs &a, int n) {
+    const int64_t g = int64_t(n) * a.heads * 2 * a.touched;
     MH_REQUIRE(g < (int64_t(1) << 31), "cache8: too many blocks of tokens");
     return uint32_t(g);
 }
@@ -400,7 +398,7 @@ void cache8_write(Context &ctx, const Cache8 &c, const PageTable &t, HeadRows k,
     const int patches = most_patches(a, first != nullptr && tokens > 1);
     const int pu = int(ceil_div(patches, 256)), nt = int(ceil_div(patches, pu * 64) * 64);
     const size_t lds = size_t(a.dp) * (c.block() / 4 + 1) * 4;
-    const dim3 grid{grid_of(a)}, threads{uint32_t(nt)};
+    const dim3 grid{grid_of(a, t.n)}, threads{uint32_t(nt)};
     auto go = [&](auto kernel) { kernel<<<grid, threads, lds, ctx.stream>>>(a); };
     auto by_size = [&](auto zero, auto vecs) {
         using T = decltype(zero);
@@ -426,7 +424,7 @@ void cache8_read(Context &ctx, const Cache8 &c, const PageTable &t, HeadRows k, 
     const int size = type == kF16 ? 2 : 4;
     const bool vec = wide(k, c.d, size) && wide(v, c.d, size);
     const int patches = most_patches(a, first != nullptr && tokens > 1);
-    const dim3 grid{grid_of(a)}, threads{uint32_t(patches <= 64 ? 64 : patches <= 128 ? 128 : 256)};
+    const dim3 grid{grid_of(a, t.n)}, threads{uint32_t(patches <= 64 ? 64 : patches <= 128 ? 128 : 256)};
     if (type == kF16) {
         if (vec) cache8_read_kernel<_Float16, true><<<grid, threads, 0, ctx.stream>>>(a);
         else cache8_read_kernel<_Float16, false><<<grid, threads, 0, ctx.stream>>>(a);

@@ -66,7 +66,7 @@ void cache8_attention(Context &ctx, const Cache8Attention &c, void *scratch) {
     a.table = c.t.table, a.q_len = c.q_len, a.kv_len = c.kv_len;
     a.part = p.splits > 1 ? static_cast<float *>(scratch) : nullptr;
     a.c = c.scale * 1.44269504088896340736f;
-    a.n = c.t.n, a.q_tokens = c.q_tokens, a.hk = c.c.heads, a.g = c.q.heads / c.c.heads, a.d = c.c.d, a.dp = c.c.dp();
+    a.q_tokens = c.q_tokens, a.hk = c.c.heads, a.g = c.q.heads / c.c.heads, a.d = c.c.d, a.dp = c.c.dp();
     a.blocks = c.t.blocks, a.pages = c.c.pages, a.block_log = c.c.block_log;
     a.row_tiles = p.row_tiles, a.splits = p.splits, a.work = int(p.items * p.splits);
     a.causal = c.causal, a.window = c.window, a.sinks = c.sinks;

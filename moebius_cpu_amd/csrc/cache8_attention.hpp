@@ -40,7 +40,7 @@ struct Args {
     const int32_t *table, *q_len, *kv_len;
     float *part;  // split partials, NULL: none
     float c;      // scale . log2 e
-    int n, q_tokens, hk, g, d, dp, blocks, pages, block_log, row_tiles, splits, work;
+    int q_tokens, hk, g, d, dp, blocks, pages, block_log, row_tiles, splits, work;
     int causal, window, sinks;
     int wide;  // rows of q in vectors of eight, of out in vectors of four
 };
