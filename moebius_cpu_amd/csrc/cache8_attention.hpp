@@ -356,7 +356,7 @@ __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) 
                 for (int e = 0; e < 4; ++e) mx = __builtin_fmaxf(mx, sc[n][t][e]);
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
-            if (__any(mx > m[n] + float(kLazy))) {
+            if (__any(mx - m[n] > float(kLazy))) {  // (a sum of both would round past it where scores are large)
                 const float mn = __builtin_fmaxf(m[n], mx);
                 const float f = __builtin_amdgcn_exp2f(m[n] - (mn == kNegInf ? 0.0f : mn));
                 l[n] *= f;
@@ -820,7 +820,7 @@ __global__ __launch_bounds__(64 * W, (W == 4 && KS <= 4 ? 3 : KS <= (PARTS == 2 
         }
         float top = __builtin_fmaxf(__builtin_fmaxf(mx[0], mx[1]) * ks[0], __builtin_fmaxf(mx[2], mx[3]) * ks[1]);
         top = __builtin_fmaxf(top, other_half(top));
-        if (__any(top > m + float(kLazy))) {
+        if (__any(top - m > float(kLazy))) {  // (as above)
             const float mn = __builtin_fmaxf(m, top);
             const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));
             l *= f;

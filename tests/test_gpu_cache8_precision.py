@@ -222,3 +222,32 @@ def test_values_near_the_end_of_the_range(contexts, fast, block, n, q, hq, hk, d
     keep = {0, n - 1}
     c.q_len = np.array([c.q_len[i] if i in keep else 0 for i in range(n)])
     check(c, 1 / np.sqrt(d), fast)
+
+
+# ---------------------------------------------------------------- scores whose steps are coarse
+
+@pytest.mark.parametrize("dtype,fast", KINDS, ids=NAMES)
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("factor", [8, 32])
+@pytest.mark.parametrize("n,q,hk", [(1, 2, 1), (64, 70, 4), (32, 130, 8)])
+def test_maxima_that_grow_by_steps_of_large_scores(contexts, dtype, fast, block, factor, n, q, hk):
+    """Scores of 2^26 and 2^28 whose maximum grows by a step or two of f32 from chunk to chunk: probabilities stay within f16.
+    All values are the same, and so is their mean, whatever the weights."""
+    ctx, kv, d = contexts[fast], 640, 64 if hk < 8 else 128
+    c = Case(ctx, dtype, n=n, q=q, kv=kv, hq=hk, hk=hk, d=d, block=block, causal=False)
+    c.table[:] = c.table[:1]
+    c.dtable = dev(ctx, c.table)
+    k = np.zeros((1, kv, hk, d))
+    k[..., 0], k[..., 1] = 127, (np.arange(kv) // 64)[None, :, None]
+    v = np.full((1, kv, hk, d), 127 * (1 - 2.0 ** -10))  # a scale just below a power of two
+    x = [k.astype(dtype), v.astype(dtype)]
+    cache_write(c.cache, dev(ctx, c.table[:1]), heads(ctx, x[0]), heads(ctx, x[1]))
+    c.qh[:] = 0
+    c.qh[..., 0], c.qh[..., 1] = 65504, 0.5
+    c.q = heads(ctx, c.qh)
+    c.run(scale=factor / 1.4426950408889634)
+    want = float(x[1].flat[0])
+    # f32 sums of kv products and of the probabilities, the codes' scale, and the output's rounding
+    tol = want * ((2.0 ** -11 * 1.001 if fast else 2.0 ** -22) + 2 * (kv + 16) * U + (2.0 ** -11 if dtype == F16 else U))
+    got = c.out.numpy().astype(np.float64)
+    assert np.isfinite(got).all() and np.all(np.abs(got - want) <= tol), np.abs(got - want).max() / tol
