@@ -510,8 +510,9 @@ __global__ __launch_bounds__(256, (occupancy(MODE, DT, WR))) void block_attentio
             for (int i = 0; i < 16; ++i) mx = __builtin_fmaxf(mx, sc[b][i]);
         mx = __builtin_fmaxf(mx, other_half(mx)) * c;
         // The reference m follows the maximum only when that has grown by 2^kLazy: probabilities
-        // stay below 2^kLazy and most tiles leave the sums as they are. top follows tv alike.
-        if (__any(mx > m + float(kLazy) || (SPLIT && tv > top + kLazyV))) {
+        // stay below 2^kLazy and most tiles leave the sums as they are. top follows tv alike. (By the
+        // difference: a sum of m and kLazy would round past it where scores are 2^25 and more.)
+        if (__any(mx - m > float(kLazy) || (SPLIT && tv > top + kLazyV))) {
             const float mn = __builtin_fmaxf(m, mx);
             const float f = __builtin_amdgcn_exp2f(m - (mn == kNegInf ? 0.0f : mn));  // 0 before the first key
             const int tn = max(top, tv);
