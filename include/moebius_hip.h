@@ -609,7 +609,8 @@ typedef struct MhCache8 {
 /* Token p of item i lies in page pages[i * blocks + p / block], p < blocks * block <= 2^30. An entry
  * outside 0 .. the cache's pages - 1 (-1 by convention) has no page: its tokens are not written, not
  * read back and seen by no query, so that pages behind a window can be handed out again. Items may
- * share pages that are read; a page that one call writes for two items has no meaning afterwards. */
+ * share pages that are read; a page that one call writes for two items, or for two blocks of one, has
+ * no meaning afterwards. */
 typedef struct MhPageTable {
     const int32_t *pages; /* [n][blocks] */
     uint32_t n, blocks;
@@ -626,7 +627,9 @@ int32_t mh_cache8_sizes(uint32_t pages, uint32_t heads, uint32_t d, uint32_t blo
  * codes are rounded to it. Codes are x / scale rounded to the nearest integer, ties to even: off by
  * at most half a scale for each time that they were rounded. Infinities are held as the largest
  * value of their sign, NaN and everything at a scale of 0 as 0. Tokens behind the last new one in
- * its block have no meaning afterwards. */
+ * its block have no meaning afterwards. A block whose first new token is not its first is taken to
+ * hold those before it: one that was never written has no scale, and a stream that begins inside of
+ * it none either, so streams begin where a block does. */
 int32_t mh_cache8_write(MhContext *ctx, const MhCache8 *cache, const MhPageTable *table, const void *k, uint64_t ld_k,
                         const void *v, uint64_t ld_v, uint32_t dtype, uint32_t tokens, const int32_t *first,
                         const int32_t *len);
@@ -660,10 +663,12 @@ int32_t mh_cache8_attention_scratch(MhContext *ctx, uint32_t dtype, const MhCach
  * f16 once.
  * A probability in two parts is held to 2^-22 of itself or 2^-33 of its row's largest, whichever is
  * more, in one to 2^-11 or 2^-28, beside values of any scale down to 2^-72 of the largest that a
- * call reads. Sums are f32. Tokens are split over workgroups where rows are few, and the parts
- * joined through scratch (mh_cache8_attention_scratch bytes, 16-byte aligned);
- * NULL takes the context's workspace, which is refused while the stream is being captured into a
- * graph. out overlaps no input. */
+ * call reads. Sums are f32, and means of values up to the end of f32 finite (but for those within
+ * 2^-10 of it). Tokens are split over workgroups where rows are few, and the parts joined through
+ * scratch (mh_cache8_attention_scratch bytes, 16-byte aligned); NULL takes the context's workspace,
+ * which is refused while the stream is being captured into a graph. Whether and how is decided by the
+ * table's length, as lengths are on the device: short streams under a long table may take twice as
+ * long as under one of their own. out overlaps no input. */
 int32_t mh_cache8_attention(MhContext *ctx, const void *q, uint64_t ld_q, uint32_t dtype, const MhCacheAttention *shape,
                             const MhCache8 *cache, const MhPageTable *table, float scale, void *out, uint64_t ld_out,
                             void *scratch, uint64_t scratch_bytes);

@@ -28,9 +28,14 @@ Plan plan(const Context &ctx, const Cache8Attention &a) {
     if (a.window) tokens = std::min(tokens, int64_t(a.window) + a.sinks + a.q_tokens);
     // Waves that share chunks: eight, or four where there are few rows, heads of 64 (of which a CU then
     // holds three workgroups) or heads that three buffers of LDS do not hold. They pay where they fill
-    // the card or the tokens are many: 32 heads over 8 of 128, f16, us of both ways: 256 queries over
-    // 2000 tokens 39.6, alone 24.1; 1000 over 1000 68, 53; 8 items of 24 over 16384 107, 118; of 64
-    // over 4000 70, 75.
+    // the card or the tokens are many. us shared (the better of four and eight waves), alone:
+    //                                   32 heads over 8 of 128   16 over 4 of 64   8 of 80   f32: of 128   of 64
+    //   1 item, 256 queries, 2000 tokens        45, 29                24, 20        22, 18     52, 38    26, 23
+    //   1, 1000, 1000                           75, 59                40, 22        33, 15     85, 74    44, 25
+    //   8, 24, 16384                            126, 150              48, 59        87, 44     159, 237  55, 64
+    //   8, 64, 4000                             84, 90                42, 29        38, 31     102, 128  45, 32
+    //   4, 200, 4000                            133, 167              62, 56        45, 35     157, 243  68, 62
+    // A few hundred rows of large heads over a few thousand tokens are where the rule leaves most behind.
     const int waves = rows > 128 && p.dt > 4 && p.dt <= 8 ? 8 : 4;
     const int64_t fill = int64_t(a.t.n) * a.c.heads * ceil_div(rows, 32 * waves);
     p.waves = rows > 64 && (4 * fill >= 3 * ctx.cu_count || tokens > 4096) ? waves : 0;
@@ -40,8 +45,11 @@ Plan plan(const Context &ctx, const Cache8Attention &a) {
     // The tokens are split over workgroups where the rows alone leave CUs idle, up to one workgroup per
     // CU (two of four waves that share), into shares of 256 tokens or more, where there are more than
     // 512. Single tokens, 32 heads over 8 of 128, f16, us with this rule and with up to two workgroups
-    // per CU: 8 items of 16384 tokens 51.6, 57.4, of 4096 22.7, 28.1; 1 of 300 10.7 whole, 12.0 in two.
-    // 8 items of 24 tokens in workgroups of four waves: 107 with two, 125 with one, 120 with three.
+    // per CU: 8 items of 16384 tokens 49, 55, of 4096 21, 27 (16 over 4 of 64, 16384: 19, 21; 8 of 80:
+    // 34, 39); 1 of 300 9.4 whole, 11.7 in two. 8 items of 24 queries over 16384 in workgroups of four
+    // waves: 127 with two, 146 with one, 143 with three (heads of 64: 48, 65, 49).
+    // Tokens are the table's, as lengths are on the device: one query over 300 tokens takes 15.8 under a
+    // table for 16384 and 9.5 under one of its own.
     const int64_t room = (p.waves == 4 && p.dt <= 8 ? 2 : 1) * int64_t(ctx.cu_count) / std::max<int64_t>(p.items, 1);
     p.splits = tokens > 512 ? int(std::max<int64_t>(1, std::min(ceil_div(tokens, 256), room))) : 1;
     const int floats = (p.waves ? (p.dt + 1) / 2 * 32 : p.dt * 16) + 2;

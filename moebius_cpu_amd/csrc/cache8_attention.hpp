@@ -140,13 +140,12 @@ __device__ __forceinline__ void load8(const T *p, int ch, int d, int wide, float
 //
 // Bound: memory, and the latency of its loads where the tokens are few. Codes are read once and never
 // shared between rows that are not in one wave, which is why nothing is staged. Single tokens of 8 items with up
-// to 16384 tokens, 32 heads over 8 of 128 (210 MB of codes): 40 us of the call's 50, 5.2 TB/s, the join 5. One token
-// over 300, 8 heads of 80, f32: 9.2 us, one workgroup's chain of lengths, page, codes and products.
+// to 16384 tokens, 32 heads over 8 of 128 (210 MB of codes): 42 us of the call's 51, 5 TB/s, the join 5. One token
+// over 300, 8 heads of 80, f32: 9.1 us, one workgroup's chain of lengths, page, codes and products.
 template <typename T, int PARTS, int DT, int NQ, int WV>
 __global__ __launch_bounds__(64 * WV, (WV / 4)) void cache8_rows_kernel(Args a) {
     constexpr int DC = (DT + 3) / 4;  // chunks of 64 channels
-    // Probabilities of f16 in two parts on FAST contexts too: the kernel waits for memory, and single tokens of 8 items
-    // take 50.2 us so and 49.9 rounded once.
+    // Probabilities of f16 in two parts on FAST contexts too: the kernel waits for memory, and takes 0.3 us more of 50.
     constexpr int PP = sizeof(T) == 2 ? 2 : PARTS;
     constexpr int kLazy = PP == 2 ? kLazySplit : kLazyHalf, kUp = PP == 2 ? kUpSplit : kUpHalf;
     constexpr int kOut = NQ * DT * 4 + NQ * 2;  // floats of a lane's partial: sums, then m and l
@@ -516,11 +515,12 @@ __device__ __forceinline__ X scalar_load(const X *p) {
 // waves behind still read one that the others are done with. Else one buffer is enough, and the
 // workgroups of a CU drift apart.
 //
-// Bound: issue, of matrix and vector instructions that take turns, and the clock, which gives way under them.
-// 4096 rows of a prompt of 16384, 32 heads over 8 of 128, f16: 1377 us (probabilities in one part, as on FAST
-// contexts, 965 to 1007: 998 TFLOP/s at best; every wave for itself from memory 2738, shared without turns 1115).
-// 4096 x 13312 of 16 heads, not causal: 773, in one part 545 to 565. f32, queries in two parts too, 2 x 4096 x 4096 of
-// 8 heads of 80: 176 to 193.
+// Bound: issue, of matrix and vector instructions that take turns (0.61 and 0.58 of a SIMD's cycles at heads of 128,
+// LDS 0.28), and the clock, which gives way under them. 4096 rows of a prompt of 16384, 32 heads over 8 of 128, f16:
+// 1252 to 1305 us with the card's clock, three products where a plain one has two (up to 1150 TFLOP/s of them);
+// probabilities in one part, as on FAST contexts, 965 to 1007 (every wave for itself from memory 2738, shared without
+// turns 1115). 4096 x 13312 of 16 heads, not causal: 715 to 727, in one part 545 to 564. f32, queries in two parts too,
+// 2 x 4096 x 4096 of 8 heads of 80: 174 to 179, FAST 120.
 //
 // WIDE: blocks of 64 or 128 tokens, so that a chunk lies in one page and has one scale of keys and one of
 // values, read through the scalar unit. Else its four groups of 16 tokens have their own: lane l
@@ -1031,8 +1031,8 @@ void launch_join(Context &ctx, const Args &a) {
 
 template <typename T, int PARTS, int DT, int NQ>
 void launch_rows(Context &ctx, const Args &a) {
-    // Two waves per SIMD where 256 registers hold one. Single tokens, 8 items of up to 16384 tokens, 32
-    // heads over 8 of 128: f16 45.8 us with eight, 51.6 with four, f32 48.0, 57.1; of 256: 240, 134.
+    // Two waves per SIMD where 256 registers hold one. Single tokens, 8 items of 16384 tokens, 32 heads over 8 of 128, us
+    // with eight and with four: f16 49, 57, f32 49, 57; of 256: 185, 107 and 242, 106; five f32 queries of 128: 140, 76.
     constexpr int WV = DT == 16 || (PARTS == 2 && NQ == 2 && DT == 8) ? 4 : 8;
     const size_t lds = size_t(WV) * (NQ * DT * 4 + NQ * 2) * 64 * 4;
     const void *fn = reinterpret_cast<const void *>(&cache8_rows_kernel<T, PARTS, DT, NQ, WV>);
